@@ -1,0 +1,855 @@
+// Selective state space scan: every channel d carries S states that decay and take input at rates that
+// the input sets,
+//   dt = softplus(delta + delta_bias) (or their sum),  a = exp(dt A[d,s]),
+//   h[t] = a h[t-1] + dt x B[t,g,s],  y = (sum_s C[t,g,s] h[t] + D x) silu(z),
+// g the group of channels d belongs to, and its backward pass, walking down with
+// q = dy silu(z), ypre the bracket above, G[T-1] the gradient of the last state:
+//   g[t] = q C + G[t],  G[t-1] = a g[t],  w = G[t-1] h[t-1],
+//   dC = sum_d q h[t],  dB = sum_d g dt x,  du = sum_s g B,  ddt = x du + sum_s A w,  dA = sum_tn dt w,
+//   dx = dt du + D q,  ddelta = ddt sigmoid(delta + delta_bias),  dz = dy ypre silu'(z),  dD = sum q x.
+//
+// Bound: the vector ALUs.  A state's step is four operations and an exp2 forward (fourteen and the sums
+// over channels backward), at 16 states a channel several times what moving the channel's few bytes
+// takes.  A lane keeps four states of one channel in registers, LANES lanes make up the channel, and a
+// workgroup of four wavefronts takes 256 / LANES channels of a batch row through time in tiles of 16
+// steps: what there is once per channel (softplus, products, the gate) is computed by one thread for
+// every element of a tile and handed over through LDS, B and C are read from there by all channels.
+//
+// The time axis is cut into chunks where there are too few rows and channels to fill the chip: a first
+// pass finds what each chunk adds to a state of zero and sum dt, by which it decays what it is given
+// (exp(A sum dt)), the states at the chunks' starts follow one from the other, and the second pass runs all
+// chunks at once.  The same backwards with G.
+#include <type_traits>
+
+#include "sequence.h"
+
+namespace haste_hip {
+namespace {
+
+constexpr int TS = 16;           // steps of a tile; a training pass keeps the states at every tile's start
+constexpr int K = 4;             // states of a lane
+constexpr int kMaxStates = 64;
+constexpr float kLog2e = 1.44269504088896341f;
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+struct ScanShape {
+  int T, N, D, S, G;
+  int share;         // channels of a group, D / G
+  int blocks_group;  // workgroups of a group
+  int chunk, chunks; // steps of a chunk (a multiple of TS)
+  int softplus;
+};
+
+template <typename T>
+struct ScanInputs {
+  Rows<const T> x, delta, B, C, z;  // z.p may be null
+  const float *A, *skip, *bias;     // skip (D), bias may be null
+  const long long* lengths;
+};
+
+// log(1 + e) for 0 <= e <= 1, exact to a few ulp however small e is: log(w) has the error of w = 1 + e,
+// and e / (w - 1) takes it back out.
+__device__ __forceinline__ float log1p_of(float e) {
+  const float w = 1.0f + e, d = w - 1.0f;
+  const float l = __builtin_amdgcn_logf(w) * 0.693147180559945309f;
+  return d == 0.f ? e : l * (e * __builtin_amdgcn_rcpf(d));
+}
+__device__ __forceinline__ float softplus_of(float v) { return fmaxf(v, 0.f) + log1p_of(exp_of(-fabsf(v))); }
+__device__ __forceinline__ float step_size(float raw, int softplus) { return softplus ? softplus_of(raw) : raw; }
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kRor4 = 0x124, kRor8 = 0x128;
+
+// A lane's place in a wavefront: the states are told apart by the highest of the low four bits of the
+// lane (sums over them rotate rows of 16 lanes), the channels by the rest (sums over them swap halves
+// of the wavefront, which adds two values in one go).
+template <int LANES>
+struct Place {
+  static constexpr int kChannels = 64 / LANES;  // of a wavefront
+  static constexpr int kLow = 16 / LANES;       // of them in a row of 16 lanes
+  static constexpr int kBlock = 4 * kChannels;  // of a workgroup
+  static __device__ __forceinline__ int states(int lane) { return (lane & 15) / kLow; }
+  static __device__ __forceinline__ int channel(int lane) { return (lane >> 4) * kLow + (lane & (kLow - 1)); }
+};
+
+// Sum over the lanes of a channel, in each of them.
+template <int LANES>
+__device__ __forceinline__ float sum_states(float v) {
+  if (LANES >= 2) v += dpp<kRor8>(v);
+  if (LANES >= 4) v += dpp<kRor4>(v);
+  if (LANES >= 8) v += dpp<kXor2>(v);
+  if (LANES >= 16) v += dpp<kXor1>(v);
+  return v;
+}
+
+__device__ __forceinline__ float swap_add_halves(float a, float b) {  // lower half: a's sum, upper: b's
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap_add_rows(float a, float b) {  // even rows: a's sum, odd: b's
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Sums of a lane's four values over the channels of the wavefront: row r of 16 lanes gets that of
+// value kSummed(r).
+template <int LANES>
+__device__ __forceinline__ float sum_channels(const float (&v)[K]) {
+  float s = swap_add_rows(swap_add_halves(v[0], v[1]), swap_add_halves(v[2], v[3]));
+  if (LANES <= 8) s += dpp<kXor1>(s);
+  if (LANES <= 4) s += dpp<kXor2>(s);
+  if (LANES <= 2) s += dpp<kHalfMirror>(s);
+  return s;
+}
+__device__ __forceinline__ int summed_value(int lane) {
+  const int r = lane >> 4;
+  return (r & 1) << 1 | r >> 1;  // 0, 2, 1, 3
+}
+
+// A channel's states [S] of float, this lane's four of them; those beyond S are 0.
+__device__ __forceinline__ void load_states(const float* p, int s0, int S, float (&h)[K]) {
+  load_channels<K>(p, s0, S, h);
+}
+__device__ __forceinline__ void store_states(float* p, int s0, int S, const float (&h)[K]) {
+  store_channels<K>(p, s0, S, h);
+}
+
+// Which row and channels a workgroup works on.
+template <int LANES>
+struct Block {
+  int n, g, c0, c_end;  // channels c0 .. of a group that ends at c_end
+  __device__ __forceinline__ Block(const ScanShape& s, unsigned block) {
+    const unsigned per_row = s.G * s.blocks_group;
+    n = block / per_row;
+    const unsigned rest = block % per_row;
+    g = rest / s.blocks_group;
+    c0 = g * s.share + (int)(rest % s.blocks_group) * Place<LANES>::kBlock;
+    c_end = (g + 1) * s.share;
+  }
+};
+
+// A tile's elements as the threads of a workgroup share them: WIDTH channels of ITEMS rows each.
+template <int LANES>
+struct Tile {
+  static constexpr int kBlock = Place<LANES>::kBlock;
+  static constexpr int kEach = TS * kBlock / 256;
+  static constexpr int WIDTH = kEach < 4 ? kEach : 4;
+  static constexpr int ITEMS = kEach / WIDTH;
+  static constexpr int kPerRow = kBlock / WIDTH;     // threads of a row
+  static constexpr int kRowStep = 256 / kPerRow;     // rows between a thread's items
+  static constexpr int kShared = (TS * LANES * K + 255) / 256;  // elements of B (of C) a thread loads
+  static __device__ __forceinline__ int row(int i) { return i * kRowStep + threadIdx.x / kPerRow; }
+  static __device__ __forceinline__ int column() { return (threadIdx.x % kPerRow) * WIDTH; }
+};
+
+// The elements of one tensor's tile, in the tensor's own type (half the registers of float, while the
+// tile before is worked on).
+template <typename T, int LANES>
+struct Held {
+  typedef Tile<LANES> L;
+  T v[L::ITEMS][L::WIDTH];
+  __device__ __forceinline__ void load(const Rows<const T>& rows, int t0, int end, const Block<LANES>& b) {
+#pragma unroll
+    for (int i = 0; i < L::ITEMS; ++i) {
+      const int t = t0 + L::row(i), c = b.c0 + L::column();
+      if (t < end && c + L::WIDTH <= b.c_end) {
+        const typename Wide<T, L::WIDTH>::type w = *reinterpret_cast<const typename Wide<T, L::WIDTH>::type*>(rows.at(t, b.n) + c);
+#pragma unroll
+        for (int e = 0; e < L::WIDTH; ++e) v[i][e] = w[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < L::WIDTH; ++e) v[i][e] = t < end && c + e < b.c_end ? rows.at(t, b.n)[c + e] : (T)0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int i, int e) const { return (float)v[i][e]; }
+};
+
+// The tile of B or C: [TS][LANES * K], states beyond S and steps beyond the row's end 0.
+template <typename T, int LANES>
+struct HeldShared {
+  T v[Tile<LANES>::kShared];
+  __device__ __forceinline__ void load(const Rows<const T>& rows, int t0, int end, const Block<LANES>& b, int S) {
+#pragma unroll
+    for (int i = 0; i < Tile<LANES>::kShared; ++i) {
+      const int e = i * 256 + threadIdx.x, t = t0 + e / (LANES * K), s = e % (LANES * K);
+      v[i] = e < TS * LANES * K && t < end && s < S ? rows.at(t, b.n)[(size_t)b.g * S + s] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ void put(float* lds) const {
+#pragma unroll
+    for (int i = 0; i < Tile<LANES>::kShared; ++i) {
+      const int e = i * 256 + threadIdx.x;
+      if (e < TS * LANES * K) lds[e] = (float)v[i];
+    }
+  }
+};
+
+// Forward pass over a chunk.  LOCAL: only what the chunk adds to a state of zero, and the sum of dt.
+// starts: the states at the chunks' starts [chunks][N][D][S] (LOCAL: out, what each adds), null when
+// there is one chunk; kept: the states at the tiles' starts [tiles][N][D][S], or null.
+template <typename T, int LANES, bool LOCAL>
+__global__ __launch_bounds__(256)
+void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ h0, float* __restrict__ starts,
+                                   float* __restrict__ sum_dt, float* __restrict__ kept, T* __restrict__ y,
+                                   float* __restrict__ h_last) {
+  typedef Place<LANES> P;
+  typedef Tile<LANES> L;
+  __shared__ float2_t step_lds[TS][P::kBlock];  // dt, dt x
+  __shared__ float4_t B_lds[TS * LANES], C_lds[LOCAL ? 1 : TS * LANES];
+  __shared__ float y_lds[LOCAL ? 1 : TS][P::kBlock];
+
+  const Block<LANES> b(s, blockIdx.x);
+  const int t0 = blockIdx.y * s.chunk, t1 = min(s.T, t0 + s.chunk);
+  const Extent extent = extent_of(in.lengths, b.n, s.T);
+  const int end = min(t1, extent.steps);
+  const int lane = threadIdx.x & 63, s0 = P::states(lane) * K;
+  const int mine = (threadIdx.x >> 6) * P::kChannels + P::channel(lane);  // this lane's channel in the block
+  const int d = b.c0 + mine;
+  const bool live = d < b.c_end;
+  const size_t state = ((size_t)b.n * s.D + d) * s.S, states = (size_t)s.N * s.D * s.S;
+
+  float A2[K], h[K], dt_sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < K; ++r) A2[r] = h[r] = 0.f;
+  if (live) {
+    load_states(in.A + (size_t)d * s.S, s0, s.S, A2);
+#pragma unroll
+    for (int r = 0; r < K; ++r) A2[r] *= kLog2e;
+    if (!LOCAL) {
+      if (blockIdx.y > 0) load_states(starts + blockIdx.y * states + state, s0, s.S, h);
+      else if (h0 != nullptr) load_states(h0 + state, s0, s.S, h);
+    }
+  }
+  float bias[L::WIDTH], skip[L::WIDTH];
+#pragma unroll
+  for (int e = 0; e < L::WIDTH; ++e) bias[e] = skip[e] = 0.f;
+  if (in.bias != nullptr) load_channels<L::WIDTH>(in.bias, b.c0 + L::column(), b.c_end, bias);
+  if (!LOCAL && in.skip != nullptr) load_channels<L::WIDTH>(in.skip, b.c0 + L::column(), b.c_end, skip);
+
+  Held<T, LANES> x, delta, z;
+  HeldShared<T, LANES> Bt, Ct;
+  auto fetch = [&](int t) {
+    x.load(in.x, t, end, b);
+    delta.load(in.delta, t, end, b);
+    if (!LOCAL && in.z.p != nullptr) z.load(in.z, t, end, b);
+    Bt.load(in.B, t, end, b, s.S);
+    if (!LOCAL) Ct.load(in.C, t, end, b, s.S);
+  };
+  if (t0 < end) fetch(t0);
+  for (int t = t0; t < end; t += TS) {
+    float xs[L::ITEMS][L::WIDTH], gate[L::ITEMS][L::WIDTH];
+#pragma unroll
+    for (int i = 0; i < L::ITEMS; ++i) {
+      const bool inside = t + L::row(i) < end;
+#pragma unroll
+      for (int e = 0; e < L::WIDTH; ++e) {
+        xs[i][e] = x.get(i, e);
+        const float dt = inside ? step_size(delta.get(i, e) + bias[e], s.softplus) : 0.f;
+        step_lds[L::row(i)][L::column() + e] = float2_t{dt, dt * xs[i][e]};
+        if (!LOCAL) {
+          gate[i][e] = 1.f;
+          if (in.z.p != nullptr) gate[i][e] = z.get(i, e) * sigmoid_of(z.get(i, e));
+        }
+      }
+    }
+    Bt.put(reinterpret_cast<float*>(B_lds));
+    if (!LOCAL) Ct.put(reinterpret_cast<float*>(C_lds));
+    if (t + TS < end) fetch(t + TS);
+    __syncthreads();
+
+    if (!LOCAL && kept != nullptr && live) store_states(kept + (size_t)(t / TS) * states + state, s0, s.S, h);
+#pragma unroll 4
+    for (int j = 0; j < TS; ++j) {
+      const float2_t dt_u = step_lds[j][mine];
+      const float4_t Bv = B_lds[j * LANES + s0 / K];
+      float ys = 0.f;
+      float4_t Cv;
+      if (!LOCAL) Cv = C_lds[j * LANES + s0 / K];
+#pragma unroll
+      for (int r = 0; r < K; ++r) {
+        const float a = __builtin_amdgcn_exp2f(dt_u.x * A2[r]);
+        h[r] = a * h[r] + dt_u.y * Bv[r];
+        if (!LOCAL) ys += h[r] * Cv[r];
+      }
+      if (LOCAL) {
+        dt_sum += dt_u.x;
+      } else {
+        ys = sum_states<LANES>(ys);
+        if (s0 == 0) y_lds[j][mine] = ys;
+      }
+    }
+    __syncthreads();
+
+    if (!LOCAL) {
+#pragma unroll
+      for (int i = 0; i < L::ITEMS; ++i) {
+        if (t + L::row(i) >= end) continue;
+        float o[L::WIDTH];
+#pragma unroll
+        for (int e = 0; e < L::WIDTH; ++e)
+          o[e] = (y_lds[L::row(i)][L::column() + e] + skip[e] * xs[i][e]) * gate[i][e];
+        store_channels<L::WIDTH>(y + ((size_t)(t + L::row(i)) * s.N + b.n) * s.D, b.c0 + L::column(), b.c_end, o);
+      }
+    }
+  }
+
+  if (LOCAL) {
+    if (live) {
+      store_states(starts + blockIdx.y * states + state, s0, s.S, h);
+      if (s0 == 0) sum_dt[((size_t)blockIdx.y * s.N + b.n) * s.D + d] = dt_sum;
+    }
+    return;
+  }
+  float fill[L::WIDTH];
+#pragma unroll
+  for (int e = 0; e < L::WIDTH; ++e) fill[e] = extent.fill;
+  for (int t = max(t0, end) + (int)threadIdx.x / L::kPerRow; t < t1; t += L::kRowStep)
+    store_channels<L::WIDTH>(y + ((size_t)t * s.N + b.n) * s.D, b.c0 + L::column(), b.c_end, fill);
+  if (blockIdx.y + 1 == (unsigned)s.chunks && live && h_last != nullptr) {
+    if (extent.fill != 0.f) {  // NaN
+#pragma unroll
+      for (int r = 0; r < K; ++r) h[r] = extent.fill;
+    }
+    store_states(h_last + state, s0, s.S, h);
+  }
+}
+
+// The chunks one after the other, in place: at[c] is what chunk c adds to a state of zero, and becomes
+// what it is given.  Forward from `first` at chunk 0, backward (REVERSE) from it at the last chunk.
+template <bool REVERSE>
+__global__ __launch_bounds__(256)
+void scan_chunks_kernel(ScanShape s, const float* __restrict__ A, const float* __restrict__ first,
+                        const float* __restrict__ sum_dt, float* __restrict__ at) {
+  const size_t states = (size_t)s.N * s.D * s.S, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= states) return;
+  const size_t channel = i / s.S;
+  const float A2 = A[channel % s.D * s.S + i % s.S] * kLog2e;
+  float h = first != nullptr ? first[i] : 0.f;
+  for (int k = 0; k < s.chunks; ++k) {
+    const int c = REVERSE ? s.chunks - 1 - k : k;
+    const float decay = __builtin_amdgcn_exp2f(A2 * sum_dt[(size_t)c * s.N * s.D + channel]);
+    const float added = at[c * states + i];
+    at[c * states + i] = h;
+    h = h == 0.f ? added : decay * h + added;  // (0 times a product of growth beyond float's range is 0, not NaN)
+  }
+}
+
+// What a backward pass writes besides dB and dC.
+template <typename T>
+struct ScanGradients {
+  T *dx, *ddelta, *dz;  // [T,N,D]; dz null without z
+  float* dh0;           // or null
+  float* partial;       // [chunks * N][D * S + 2 D]: dA, dD, d delta_bias
+  float *dB, *dC;       // [blocks of a group][T][N][G][S]
+};
+
+// Backward pass over a chunk.  LOCAL: only G at the chunk's start for a gradient of zero at its end, and
+// the sum of dt.  ends: [chunks][N][D][S], the gradients at the chunks' ends
+// (LOCAL: out), null when there is one chunk.
+template <typename T, int LANES, bool LOCAL>
+__global__ __launch_bounds__(256, 2)
+void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ kept, Rows<const T> dy,
+                                    const float* __restrict__ dh_last, float* __restrict__ ends, float* __restrict__ sum_dt,
+                                    ScanGradients<T> out) {
+  typedef Place<LANES> P;
+  typedef Tile<LANES> L;
+  __shared__ float2_t step_lds[TS][P::kBlock];  // dt, dt x
+  __shared__ float q_lds[TS][P::kBlock];        // dy silu(z)
+  __shared__ float4_t C_lds[TS * LANES], B_lds[LOCAL ? 1 : TS * LANES];
+  __shared__ float ypre_lds[LOCAL ? 1 : TS][P::kBlock], du_lds[LOCAL ? 1 : TS][P::kBlock], Aw_lds[LOCAL ? 1 : TS][P::kBlock];
+  __shared__ float dB_lds[LOCAL ? 1 : 4][TS * LANES * K], dC_lds[LOCAL ? 1 : 4][TS * LANES * K];  // of each wavefront
+
+  const Block<LANES> b(s, blockIdx.x);
+  const int t0 = blockIdx.y * s.chunk, t1 = min(s.T, t0 + s.chunk);
+  const Extent extent = extent_of(in.lengths, b.n, s.T);
+  const int end = min(t1, extent.steps);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s0 = P::states(lane) * K;
+  const int mine = wave * P::kChannels + P::channel(lane);
+  const int d = b.c0 + mine;
+  const bool live = d < b.c_end;
+  const size_t state = ((size_t)b.n * s.D + d) * s.S, states = (size_t)s.N * s.D * s.S;
+  const size_t shared_row = (size_t)s.G * s.S;  // of dB, dC
+
+  float A[K], A2[K], G[K], dA[K], dt_sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < K; ++r) A[r] = G[r] = dA[r] = 0.f;
+  if (live) {
+    load_states(in.A + (size_t)d * s.S, s0, s.S, A);
+    if (blockIdx.y + 1 == (unsigned)s.chunks) {
+      if (dh_last != nullptr && !LOCAL) load_states(dh_last + state, s0, s.S, G);
+    } else if (!LOCAL) {
+      load_states(ends + blockIdx.y * states + state, s0, s.S, G);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < K; ++r) A2[r] = A[r] * kLog2e;
+  const int column = L::column();
+  float bias[L::WIDTH], skip[L::WIDTH], dskip[L::WIDTH], dbias[L::WIDTH];
+#pragma unroll
+  for (int e = 0; e < L::WIDTH; ++e) bias[e] = skip[e] = dskip[e] = dbias[e] = 0.f;
+  if (in.bias != nullptr) load_channels<L::WIDTH>(in.bias, b.c0 + column, b.c_end, bias);
+  if (!LOCAL && in.skip != nullptr) load_channels<L::WIDTH>(in.skip, b.c0 + column, b.c_end, skip);
+
+  if (!LOCAL) {
+    float fill[L::WIDTH];
+#pragma unroll
+    for (int e = 0; e < L::WIDTH; ++e) fill[e] = extent.fill;
+    for (int t = max(t0, end) + (int)threadIdx.x / L::kPerRow; t < t1; t += L::kRowStep) {
+      const size_t at = ((size_t)t * s.N + b.n) * s.D;
+      store_channels<L::WIDTH>(out.dx + at, b.c0 + column, b.c_end, fill);
+      store_channels<L::WIDTH>(out.ddelta + at, b.c0 + column, b.c_end, fill);
+      if (out.dz != nullptr) store_channels<L::WIDTH>(out.dz + at, b.c0 + column, b.c_end, fill);
+    }
+    const size_t part = (size_t)(blockIdx.x % s.blocks_group) * s.T;
+    for (int e = threadIdx.x; e < (t1 - max(t0, end)) * s.S; e += 256) {
+      const size_t at = ((part + max(t0, end) + e / s.S) * s.N + b.n) * shared_row + (size_t)b.g * s.S + e % s.S;
+      out.dB[at] = out.dC[at] = extent.fill;
+    }
+  }
+
+  Held<T, LANES> x, delta, z, up;
+  HeldShared<T, LANES> Bt, Ct;
+  float start[K], start_next[K];
+  auto fetch = [&](int t) {
+    if (!LOCAL) x.load(in.x, t, end, b);
+    delta.load(in.delta, t, end, b);
+    if (in.z.p != nullptr) z.load(in.z, t, end, b);
+    up.load(dy, t, end, b);
+    Ct.load(in.C, t, end, b, s.S);
+    if (!LOCAL) {
+      Bt.load(in.B, t, end, b, s.S);
+      if (live) load_states(kept + (size_t)(t / TS) * states + state, s0, s.S, start_next);
+    }
+  };
+#pragma unroll
+  for (int r = 0; r < K; ++r) start[r] = start_next[r] = 0.f;
+  const int last = t0 < end ? t0 + (end - 1 - t0) / TS * TS : t0 - TS;  // the last tile
+  if (last >= t0) fetch(last);
+  for (int t = last; t >= t0; t -= TS) {
+    Held<T, LANES> x_now = x, delta_now = delta, z_now = z, up_now = up;
+#pragma unroll
+    for (int i = 0; i < L::ITEMS; ++i) {
+      const bool inside = t + L::row(i) < end;
+#pragma unroll
+      for (int e = 0; e < L::WIDTH; ++e) {
+        const float dt = inside ? step_size(delta.get(i, e) + bias[e], s.softplus) : 0.f;
+        step_lds[L::row(i)][column + e] = float2_t{dt, LOCAL ? 0.f : dt * x.get(i, e)};
+        float q = up.get(i, e);
+        if (in.z.p != nullptr) q *= z.get(i, e) * sigmoid_of(z.get(i, e));
+        q_lds[L::row(i)][column + e] = q;
+      }
+    }
+    Ct.put(reinterpret_cast<float*>(C_lds));
+    if (!LOCAL) Bt.put(reinterpret_cast<float*>(B_lds));
+#pragma unroll
+    for (int r = 0; r < K; ++r) start[r] = start_next[r];
+    if (t - TS >= t0) fetch(t - TS);
+    __syncthreads();
+
+    if (LOCAL) {
+#pragma unroll 4
+      for (int j = TS - 1; j >= 0; --j) {
+        const float dt = step_lds[j][mine].x, q = q_lds[j][mine];
+        const float4_t Cv = C_lds[j * LANES + s0 / K];
+        dt_sum += dt;
+#pragma unroll
+        for (int r = 0; r < K; ++r) G[r] = __builtin_amdgcn_exp2f(dt * A2[r]) * (q * Cv[r] + G[r]);
+      }
+      __syncthreads();
+      continue;
+    }
+
+    float a[TS][K], before[TS][K];  // the decays and the states before the steps
+#pragma unroll
+    for (int j = 0; j < TS; ++j) {
+      const float2_t dt_u = step_lds[j][mine];
+      const float q = q_lds[j][mine];
+      const float4_t Bv = B_lds[j * LANES + s0 / K], Cv = C_lds[j * LANES + s0 / K];
+      float ypre = 0.f, dCv[K];
+#pragma unroll
+      for (int r = 0; r < K; ++r) {
+        a[j][r] = __builtin_amdgcn_exp2f(dt_u.x * A2[r]);
+        before[j][r] = start[r];
+        start[r] = a[j][r] * start[r] + dt_u.y * Bv[r];
+        ypre += start[r] * Cv[r];
+        dCv[r] = q * start[r];
+      }
+      ypre = sum_states<LANES>(ypre);
+      if (s0 == 0) ypre_lds[j][mine] = ypre;
+      const float sum = sum_channels<LANES>(dCv);
+      if ((lane & (P::kLow - 1)) == 0) dC_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum;
+      __builtin_amdgcn_sched_barrier(0);  // a step's operands are not fetched steps ahead: they would take the registers
+    }
+#pragma unroll
+    for (int j = TS - 1; j >= 0; --j) {
+      const float2_t dt_u = step_lds[j][mine];
+      const float q = q_lds[j][mine];
+      const float4_t Bv = B_lds[j * LANES + s0 / K], Cv = C_lds[j * LANES + s0 / K];
+      float du = 0.f, Aw = 0.f, dBv[K];
+#pragma unroll
+      for (int r = 0; r < K; ++r) {
+        const float g = q * Cv[r] + G[r];
+        dBv[r] = g * dt_u.y;
+        du += g * Bv[r];
+        G[r] = g * a[j][r];
+        const float w = G[r] * before[j][r];
+        Aw += w * A[r];
+        dA[r] += w * dt_u.x;
+      }
+      du = sum_states<LANES>(du);
+      Aw = sum_states<LANES>(Aw);
+      if (s0 == 0) {
+        du_lds[j][mine] = du;
+        Aw_lds[j][mine] = Aw;
+      }
+      const float sum = sum_channels<LANES>(dBv);
+      if ((lane & (P::kLow - 1)) == 0) dB_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+
+#pragma unroll
+    for (int i = 0; i < L::ITEMS; ++i) {
+      const int row = L::row(i);
+      if (t + row >= end) continue;
+      float dxo[L::WIDTH], ddo[L::WIDTH], dzo[L::WIDTH];
+#pragma unroll
+      for (int e = 0; e < L::WIDTH; ++e) {
+        const float xv = x_now.get(i, e), raw = delta_now.get(i, e) + bias[e], upv = up_now.get(i, e);
+        const float dt = step_lds[row][column + e].x, q = q_lds[row][column + e], du = du_lds[row][column + e];
+        dxo[e] = dt * du + skip[e] * q;
+        ddo[e] = xv * du + Aw_lds[row][column + e];
+        if (s.softplus) ddo[e] *= sigmoid_of(raw);
+        dskip[e] += q * xv;
+        dbias[e] += ddo[e];
+        if (in.z.p != nullptr) {
+          const float zv = z_now.get(i, e);
+          dzo[e] = upv * (ypre_lds[row][column + e] + skip[e] * xv) * silu_slope(zv, sigmoid_of(zv));
+        }
+      }
+      const size_t at = ((size_t)(t + row) * s.N + b.n) * s.D;
+      store_channels<L::WIDTH>(out.dx + at, b.c0 + column, b.c_end, dxo);
+      store_channels<L::WIDTH>(out.ddelta + at, b.c0 + column, b.c_end, ddo);
+      if (out.dz != nullptr) store_channels<L::WIDTH>(out.dz + at, b.c0 + column, b.c_end, dzo);
+    }
+    const size_t part = (size_t)(blockIdx.x % s.blocks_group) * s.T;
+    for (int e = threadIdx.x; e < TS * LANES * K; e += 256) {
+      const int j = e / (LANES * K), st = e % (LANES * K);
+      if (t + j >= end || st >= s.S) continue;
+      const size_t at = ((part + t + j) * s.N + b.n) * shared_row + (size_t)b.g * s.S + st;
+      out.dB[at] = (dB_lds[0][e] + dB_lds[1][e]) + (dB_lds[2][e] + dB_lds[3][e]);
+      out.dC[at] = (dC_lds[0][e] + dC_lds[1][e]) + (dC_lds[2][e] + dC_lds[3][e]);
+    }
+    __syncthreads();
+  }
+
+  if (LOCAL) {
+    if (live) {
+      store_states(ends + blockIdx.y * states + state, s0, s.S, G);
+      if (s0 == 0) sum_dt[((size_t)blockIdx.y * s.N + b.n) * s.D + d] = dt_sum;
+    }
+    return;
+  }
+  float* partial = out.partial + ((size_t)blockIdx.y * s.N + b.n) * ((size_t)s.D * (s.S + 2));
+  if (live) {
+    if (blockIdx.y == 0 && out.dh0 != nullptr) {
+      if (extent.fill != 0.f) {  // NaN
+#pragma unroll
+        for (int r = 0; r < K; ++r) G[r] = extent.fill;
+      }
+      store_states(out.dh0 + state, s0, s.S, G);
+    }
+    store_states(partial + (size_t)d * s.S, s0, s.S, dA);
+  }
+  // the threads of a column add theirs in order
+  static_assert(256 * L::WIDTH <= TS * P::kBlock, "a row a thread of the column fits q_lds, and step_lds");
+  float(*skip_sums)[P::kBlock] = q_lds;
+  float(*bias_sums)[P::kBlock] = reinterpret_cast<float(*)[P::kBlock]>(&step_lds[0][0]);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < L::WIDTH; ++e) {
+    skip_sums[threadIdx.x / L::kPerRow][column + e] = dskip[e];
+    bias_sums[threadIdx.x / L::kPerRow][column + e] = dbias[e];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < P::kBlock; e += 256) {
+    if (b.c0 + e >= b.c_end) continue;
+    float ds = 0.f, db = 0.f;
+    for (int r = 0; r < L::kRowStep; ++r) {
+      ds += skip_sums[r][e];
+      db += bias_sums[r][e];
+    }
+    partial[(size_t)s.D * s.S + b.c0 + e] = ds;
+    partial[(size_t)s.D * (s.S + 1) + b.c0 + e] = db;
+  }
+}
+
+// dB, dC = the sums of the blocks' parts, rounded.
+template <typename T>
+__global__ __launch_bounds__(256)
+void scan_shared_kernel(int parts, size_t count, const float* __restrict__ dB_parts, const float* __restrict__ dC_parts,
+                        T* __restrict__ dB, T* __restrict__ dC) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  const float* from = blockIdx.y == 0 ? dB_parts : dC_parts;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) sum += from[p * count + i];
+  (blockIdx.y == 0 ? dB : dC)[i] = (T)sum;
+}
+
+// A single step: LANES neighbouring lanes a channel, its states in and out as whole lines.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256)
+void selective_scan_step_kernel(ScanShape s, ScanInputs<T> in, const float* h, float* h_out, T* __restrict__ y) {
+  const unsigned i = blockIdx.x * 256 + threadIdx.x, channel = i / LANES, s0 = i % LANES * K;
+  const unsigned n = channel / s.D;
+  if (n >= (unsigned)s.N) return;
+  const unsigned d = channel % s.D, g = d / s.share;
+  const size_t state = (size_t)channel * s.S;
+  float A[K], hs[K], Bv[K], Cv[K];
+  load_states(h + state, s0, s.S, hs);
+  load_states(in.A + (size_t)d * s.S, s0, s.S, A);
+  load_channels<K>(in.B.at(0, n) + (size_t)g * s.S, s0, s.S, Bv);
+  load_channels<K>(in.C.at(0, n) + (size_t)g * s.S, s0, s.S, Cv);
+  const float x = (float)in.x.at(0, n)[d];
+  const float dt = step_size((float)in.delta.at(0, n)[d] + (in.bias != nullptr ? in.bias[d] : 0.f), s.softplus);
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < K; ++r) {
+    hs[r] = exp_of(dt * A[r]) * hs[r] + dt * x * Bv[r];
+    sum += hs[r] * Cv[r];
+  }
+  store_states(h_out + state, s0, s.S, hs);
+  if (LANES >= 2) sum += dpp<kXor1>(sum);
+  if (LANES >= 4) sum += dpp<kXor2>(sum);
+  if (LANES >= 8) sum += dpp<kHalfMirror>(sum);
+  if (LANES >= 16) sum += dpp<kRor8>(sum);
+  if (s0 != 0) return;
+  if (in.skip != nullptr) sum += in.skip[d] * x;
+  if (in.z.p != nullptr) {
+    const float zv = (float)in.z.at(0, n)[d];
+    sum *= zv * sigmoid_of(zv);
+  }
+  y[channel] = (T)sum;
+}
+
+int lanes_for(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
+
+template <typename F>
+int with_lanes(int S, F&& f) {
+  switch (lanes_for(S)) {
+    case 2: return f(std::integral_constant<int, 2>());
+    case 4: return f(std::integral_constant<int, 4>());
+    case 8: return f(std::integral_constant<int, 8>());
+    default: return f(std::integral_constant<int, 16>());
+  }
+}
+
+// Cuts the time axis so that `waves` wavefronts a SIMD have work, in chunks of no fewer than 4 tiles.
+ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, int waves) {
+  ScanShape s = {T, N, D, S, G, D / G, 0, 0, 0, softplus};
+  const int block = 256 / lanes_for(S);
+  s.blocks_group = (s.share + block - 1) / block;
+  const size_t blocks = (size_t)N * G * s.blocks_group, wanted = (size_t)device_cu_count() * waves;
+  const size_t tiles = (T + TS - 1) / TS;
+  size_t chunks = blocks >= wanted ? 1 : (wanted + blocks - 1) / blocks;
+  const size_t most = tiles / 4 > 0 ? tiles / 4 : 1;
+  chunks = chunks < most ? chunks : most;
+  s.chunk = (int)((tiles + chunks - 1) / chunks) * TS;
+  s.chunks = (T + s.chunk - 1) / s.chunk;
+  return s;
+}
+ScanShape forward_shape(int T, int N, int D, int S, int G, int softplus) { return shape_of(T, N, D, S, G, softplus, 2); }
+ScanShape backward_shape(int T, int N, int D, int S, int G, int softplus) { return shape_of(T, N, D, S, G, softplus, 2); }
+
+// Floats of workspace, in the order they lie there.
+struct ScanWorkspace {
+  size_t at_chunks, sum_dt, partial, sums, dB, dC, total;
+};
+ScanWorkspace forward_workspace(const ScanShape& s) {
+  ScanWorkspace w = {};
+  if (s.chunks > 1) {
+    w.sum_dt = (size_t)s.chunks * s.N * s.D * s.S;
+    w.total = w.sum_dt + (size_t)s.chunks * s.N * s.D;
+  }
+  return w;
+}
+ScanWorkspace backward_workspace(const ScanShape& s) {
+  ScanWorkspace w = forward_workspace(s);
+  const size_t parts = (size_t)s.chunks * s.N, columns = (size_t)s.D * (s.S + 2);
+  w.partial = w.total;
+  w.sums = w.partial + parts * columns;
+  w.dB = w.sums + column_sums_scratch((int)parts, columns);
+  w.dC = w.dB + (size_t)s.blocks_group * s.T * s.N * s.G * s.S;
+  w.total = w.dC + (w.dC - w.dB);
+  return w;
+}
+
+template <typename T>
+int forward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, const float* h0, T* y, float* h_last, float* kept,
+            float* workspace, size_t workspace_bytes) {
+  const size_t blocks = (size_t)s.N * s.G * s.blocks_group, states = (size_t)s.N * s.D * s.S;
+  const ScanWorkspace w = forward_workspace(s);
+  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ || (states + 255) / 256 > kGridLimit)
+    return too_large("selective_scan: too many rows of channels");
+  if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_forward: the workspace is too small");
+  HASTE_HIP_REQUIRE(workspace != nullptr || w.total == 0);
+  float *starts = workspace, *sum_dt = s.chunks > 1 ? workspace + w.sum_dt : nullptr;
+  return with_lanes(s.S, [&](auto lanes) {
+    dim3 grid((unsigned)blocks, s.chunks);
+    if (s.chunks > 1) {
+      ScopedKernelTimer timer("selective_scan_chunks", stream);
+      selective_scan_forward_kernel<T, lanes(), true><<<grid, 256, 0, stream>>>(s, in, nullptr, starts, sum_dt, nullptr, nullptr, nullptr);
+      HASTE_HIP_TRY(hipGetLastError());
+      scan_chunks_kernel<false><<<(unsigned)((states + 255) / 256), 256, 0, stream>>>(s, in.A, h0, sum_dt, starts);
+      HASTE_HIP_TRY(hipGetLastError());
+    }
+    ScopedKernelTimer timer("selective_scan_forward", stream);
+    selective_scan_forward_kernel<T, lanes(), false><<<grid, 256, 0, stream>>>(s, in, h0, starts, nullptr, kept, y, h_last);
+    HASTE_HIP_TRY(hipGetLastError());
+    return HASTE_HIP_OK;
+  });
+}
+
+template <typename T>
+int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, const float* kept, const Rows<const T>& dy,
+             const float* dh_last, T* dx, T* ddelta, float* dA, T* dB, T* dC, float* dskip, T* dz, float* dbias, float* dh0,
+             float* workspace, size_t workspace_bytes) {
+  const size_t blocks = (size_t)s.N * s.G * s.blocks_group, states = (size_t)s.N * s.D * s.S;
+  const size_t shared = (size_t)s.T * s.N * s.G * s.S, columns = (size_t)s.D * (s.S + 2);
+  const ScanWorkspace w = backward_workspace(s);
+  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ || (states + 255) / 256 > kGridLimit || (shared + 255) / 256 > kGridLimit)
+    return too_large("selective_scan: too many rows of channels");
+  if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_backward: the workspace is too small");
+  float *ends = workspace + w.at_chunks, *sum_dt = workspace + w.sum_dt;
+  const ScanGradients<T> out = {dx, ddelta, dz, dh0, workspace + w.partial, workspace + w.dB, workspace + w.dC};
+  HASTE_HIP_PROPAGATE(with_lanes(s.S, [&](auto lanes) {
+    dim3 grid((unsigned)blocks, s.chunks);
+    if (s.chunks > 1) {
+      ScopedKernelTimer timer("selective_scan_chunks", stream);
+      selective_scan_backward_kernel<T, lanes(), true><<<grid, 256, 0, stream>>>(s, in, nullptr, dy, dh_last, ends, sum_dt, out);
+      HASTE_HIP_TRY(hipGetLastError());
+      scan_chunks_kernel<true><<<(unsigned)((states + 255) / 256), 256, 0, stream>>>(s, in.A, dh_last, sum_dt, ends);
+      HASTE_HIP_TRY(hipGetLastError());
+    }
+    ScopedKernelTimer timer("selective_scan_backward", stream);
+    selective_scan_backward_kernel<T, lanes(), false><<<grid, 256, 0, stream>>>(s, in, kept, dy, dh_last, ends, sum_dt, out);
+    HASTE_HIP_TRY(hipGetLastError());
+    return HASTE_HIP_OK;
+  }));
+  {
+    ScopedKernelTimer timer("selective_scan_shared", stream);
+    scan_shared_kernel<T><<<dim3((unsigned)((shared + 255) / 256), 2), 256, 0, stream>>>(s.blocks_group, shared, out.dB, out.dC, dB, dC);
+    HASTE_HIP_TRY(hipGetLastError());
+  }
+  const size_t first = (size_t)s.D * s.S;
+  const ColumnOutputs to = {{dA, dskip, dbias, nullptr}, {first, first + s.D, columns, columns}};
+  return column_sums(stream, s.chunks * s.N, columns, out.partial, workspace + w.sums, to);
+}
+
+int check_sizes(int T, int N, int D, int S, int G) {
+  HASTE_HIP_REQUIRE(T > 0 && N > 0 && D > 0 && S > 0 && G > 0 && D % G == 0);
+  if (S > kMaxStates) return too_large("selective_scan: up to 64 states a channel are implemented");
+  if (T > kSizeLimit || N > kSizeLimit || D > kSizeLimit / (kMaxStates + 2)) return too_large("selective_scan: sizes beyond 2^30");
+  return HASTE_HIP_OK;
+}
+
+template <typename T>
+ScanInputs<T> inputs_of(const void* x, size_t x_step, size_t x_row, const void* delta, size_t delta_step, size_t delta_row,
+                        const float* A, const void* B, size_t B_step, size_t B_row, const void* C, size_t C_step, size_t C_row,
+                        const float* D, const void* z, size_t z_step, size_t z_row, const float* delta_bias,
+                        const void* lengths) {
+  return {{static_cast<const T*>(x), x_step, x_row}, {static_cast<const T*>(delta), delta_step, delta_row},
+          {static_cast<const T*>(B), B_step, B_row}, {static_cast<const T*>(C), C_step, C_row},
+          {static_cast<const T*>(z), z_step, z_row}, A, D, delta_bias, static_cast<const long long*>(lengths)};
+}
+
+template <typename T>
+int step(hipStream_t stream, int N, int D, int S, int G, int softplus, const ScanInputs<T>& in, const float* h, T* y,
+         float* h_out) {
+  const ScanShape s = {1, N, D, S, G, D / G, 0, TS, 1, softplus};
+  return with_lanes(S, [&](auto lanes) {
+    const size_t blocks = ((size_t)N * D * lanes() + 255) / 256;
+    if (blocks > kGridLimit) return too_large("selective_scan: too many rows of channels");
+    ScopedKernelTimer timer("selective_scan_iterate", stream);
+    selective_scan_step_kernel<T, lanes()><<<(unsigned)blocks, 256, 0, stream>>>(s, in, h, h_out, y);
+    HASTE_HIP_TRY(hipGetLastError());
+    return HASTE_HIP_OK;
+  });
+}
+
+}  // namespace
+}  // namespace haste_hip
+
+extern "C" {
+
+using namespace haste_hip;
+
+size_t haste_hip_selective_scan_workspace_bytes(int backward, int steps, int batch_size, int channels, int states, int groups) {
+  if (check_sizes(steps, batch_size, channels, states, groups) != HASTE_HIP_OK) return 0;
+  const size_t floats = backward ? backward_workspace(backward_shape(steps, batch_size, channels, states, groups, 0)).total
+                                 : forward_workspace(forward_shape(steps, batch_size, channels, states, groups, 0)).total;
+  return floats * sizeof(float);
+}
+
+size_t haste_hip_selective_scan_kept_bytes(int steps, int batch_size, int channels, int states) {
+  if (check_sizes(steps, batch_size, channels, states, 1) != HASTE_HIP_OK) return 0;
+  return (size_t)((steps + TS - 1) / TS) * batch_size * channels * states * sizeof(float);
+}
+
+#define HASTE_HIP_SCAN_INPUTS                                                                                          \
+  const void *x, size_t x_step, size_t x_row, const void *delta, size_t delta_step, size_t delta_row, const float *A,  \
+      const void *B, size_t B_step, size_t B_row, const void *C, size_t C_step, size_t C_row, const float *D,          \
+      const void *z, size_t z_step, size_t z_row, const float *delta_bias, int delta_softplus
+
+#define HASTE_HIP_SELECTIVE_SCAN(SUFFIX, T)                                                                            \
+  int haste_hip_selective_scan_forward_##SUFFIX(int steps, int batch_size, int channels, int states, int groups,       \
+                                                HASTE_HIP_SCAN_INPUTS, const float* h0, const void* lengths, void* y,  \
+                                                float* h_last, float* kept, void* workspace, size_t workspace_bytes,   \
+                                                void* stream) {                                                        \
+    HASTE_HIP_PROPAGATE(check_sizes(steps, batch_size, channels, states, groups));                                     \
+    HASTE_HIP_REQUIRE(x && delta && A && B && C && y);                                                                 \
+    return forward<T>(as_stream(stream), forward_shape(steps, batch_size, channels, states, groups, delta_softplus),   \
+                      inputs_of<T>(x, x_step, x_row, delta, delta_step, delta_row, A, B, B_step, B_row, C, C_step,     \
+                                   C_row, D, z, z_step, z_row, delta_bias, lengths),                                   \
+                      h0, static_cast<T*>(y), h_last, kept, static_cast<float*>(workspace), workspace_bytes);          \
+  }                                                                                                                    \
+  int haste_hip_selective_scan_backward_##SUFFIX(                                                                      \
+      int steps, int batch_size, int channels, int states, int groups, HASTE_HIP_SCAN_INPUTS, const void* lengths,     \
+      const float* kept, const void* dy, size_t dy_step, size_t dy_row, const float* dh_last, void* dx, void* ddelta,  \
+      float* dA, void* dB, void* dC, float* dD, void* dz, float* ddelta_bias, float* dh0, void* workspace,             \
+      size_t workspace_bytes, void* stream) {                                                                          \
+    HASTE_HIP_PROPAGATE(check_sizes(steps, batch_size, channels, states, groups));                                     \
+    HASTE_HIP_REQUIRE(x && delta && A && B && C && kept && dy && dx && ddelta && dA && dB && dC && workspace);         \
+    HASTE_HIP_REQUIRE((z == nullptr) == (dz == nullptr));                                                              \
+    return backward<T>(as_stream(stream), backward_shape(steps, batch_size, channels, states, groups, delta_softplus), \
+                       inputs_of<T>(x, x_step, x_row, delta, delta_step, delta_row, A, B, B_step, B_row, C, C_step,    \
+                                    C_row, D, z, z_step, z_row, delta_bias, lengths),                                  \
+                       kept, {static_cast<const T*>(dy), dy_step, dy_row}, dh_last, static_cast<T*>(dx),               \
+                       static_cast<T*>(ddelta), dA, static_cast<T*>(dB), static_cast<T*>(dC), dD, static_cast<T*>(dz), \
+                       ddelta_bias, dh0, static_cast<float*>(workspace), workspace_bytes);                             \
+  }                                                                                                                    \
+  int haste_hip_selective_scan_iterate_##SUFFIX(                                                                       \
+      int batch_size, int channels, int states, int groups, const void* x, size_t x_row, const void* delta,            \
+      size_t delta_row, const float* A, const void* B, size_t B_row, const void* C, size_t C_row, const float* D,      \
+      const void* z, size_t z_row, const float* delta_bias, int delta_softplus, const float* h, void* y, float* h_out, \
+      void* stream) {                                                                                                  \
+    HASTE_HIP_PROPAGATE(check_sizes(1, batch_size, channels, states, groups));                                         \
+    HASTE_HIP_REQUIRE(x && delta && A && B && C && h && y && h_out);                                                   \
+    return step<T>(as_stream(stream), batch_size, channels, states, groups, delta_softplus,                            \
+                   inputs_of<T>(x, 0, x_row, delta, 0, delta_row, A, B, 0, B_row, C, 0, C_row, D, z, 0, z_row,         \
+                                delta_bias, nullptr),                                                                  \
+                   h, static_cast<T*>(y), h_out);                                                                      \
+  }
+
+HASTE_HIP_SELECTIVE_SCAN(f32, float)
+HASTE_HIP_SELECTIVE_SCAN(f16, _Float16)
+HASTE_HIP_SELECTIVE_SCAN(bf16, __bf16)
+
+}  // extern "C"

@@ -15,6 +15,9 @@ Differences, on purpose:
   * DropConnect of LSTM and GRU is applied inside the recurrence kernel while it loads the
     recurrent matrix (the mask is drawn here and handed over), instead of materialising a
     dropped-out copy of the matrix first (frameworks/pytorch/lstm.py:252).
+
+CausalConv, SelectiveScan and ResidualNorm, at the end, are the layers of a state space block; the reference has
+none of them.
 """
 import torch
 import torch.nn as nn
@@ -22,7 +25,8 @@ import torch.nn.functional as F
 
 from . import ops
 
-__all__ = ["LSTM", "GRU", "IndRNN", "LayerNormLSTM", "LayerNormGRU", "LayerNormIndRNN"]
+__all__ = ["LSTM", "GRU", "IndRNN", "LayerNormLSTM", "LayerNormGRU", "LayerNormIndRNN",
+           "CausalConv", "SelectiveScan", "ResidualNorm"]
 
 
 def _t(w):
@@ -746,3 +750,289 @@ class LayerNormGRU(_RNNBase):
         h = _eager_gru(self.training, self.zoneout, x, h0, self.kernel, R, self.bias,
                        self.recurrent_bias, zmask, gamma=self.gamma)
         return self._time_major(h[1:]), self._final_state(h, lengths)
+
+
+# ---- the layers of a state space block ---------------------------------------------------
+# Projections between them are the caller's.  Parameters are handed over in float32 whatever they are kept in (their
+# gradients come back in the type they have); activations keep theirs.
+class _CausalConvFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, kernel, bias, silu, state, lengths):
+        ctx.save_for_backward(x, kernel, bias, state, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return ops.causal_conv_forward(x, kernel, bias, silu, state, lengths)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dstate_out):
+        x, kernel, bias, state, lengths = ctx.saved_tensors
+        dx, dkernel, dbias, dstate = ops.causal_conv_backward(x, kernel, bias, ctx.silu, state, lengths, dy, dstate_out)
+        return dx, dkernel, dbias, None, dstate, None
+
+
+class _SelectiveScanFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, training, x, delta, A, B, C, D, z, delta_bias, delta_softplus, h0, lengths):
+        y, h_last, cache = ops.selective_scan_forward(training and any(ctx.needs_input_grad), x, delta, A, B, C, D, z, delta_bias,
+                                                      delta_softplus, h0, lengths)
+        ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, lengths, cache)
+        ctx.delta_softplus, ctx.has_h0 = delta_softplus, h0 is not None
+        ctx.set_materialize_grads(False)
+        return y, h_last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh_last):
+        x, delta, A, B, C, D, z, delta_bias, lengths, cache = ctx.saved_tensors
+        dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0 = ops.selective_scan_backward(
+            x, delta, A, B, C, D, z, delta_bias, ctx.delta_softplus, None, lengths, cache, dy, dh_last)
+        return None, dx, ddelta, dA, dB, dC, dD, dz, dbias, None, dh0 if ctx.has_h0 else None, None
+
+
+class _ResidualNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, update, residual, gate, scale, after_weight, before_weight, before_bias, centered, eps):
+        out, normed, stats = ops.residual_norm_forward(update, residual, gate, scale, after_weight, before_weight, before_bias,
+                                                       centered, eps)
+        ctx.save_for_backward(update, residual, gate, scale, after_weight, before_weight, before_bias, stats)
+        ctx.centered = centered
+        ctx.set_materialize_grads(False)
+        return out, normed
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dnormed):
+        return (*ops.residual_norm_backward(*ctx.saved_tensors, dout, dnormed, centered=ctx.centered), None, None)
+
+
+def _wide(*tensors):
+    """Half types as float32; what the plain forms compute in."""
+    return tuple(t if t is None or t.dtype in (torch.float32, torch.float64) else t.float() for t in tensors)
+
+
+def _inside(lengths, T, N, like):
+    """[T,N]: the steps that belong to the rows' sequences."""
+    steps = torch.arange(T, device=like.device)[:, None]
+    return steps < (torch.full((N,), T, device=like.device) if lengths is None else torch.where(lengths < 0, lengths + T + 1, lengths))
+
+
+def _eager_causal_conv(x, kernel, bias, silu, state, lengths):
+    dtype, (T, N, D), W = x.dtype, x.shape, kernel.shape[0]
+    x, kernel, bias, state = _wide(x, kernel, bias, state)
+    inside = _inside(lengths, T, N, x)
+    x = torch.where(inside[..., None], x, 0.0)
+    padded = torch.cat([x.new_zeros(W - 1, N, D) if state is None else state, x])
+    pre = sum(kernel[k] * padded[k:k + T] for k in range(W))
+    pre = pre if bias is None else pre + bias
+    y = torch.where(inside[..., None], F.silu(pre) if silu else pre, 0.0)
+    rows = inside.sum(0) + torch.arange(W - 1, device=x.device)[:, None]
+    return y.to(dtype), padded[rows, torch.arange(N, device=x.device)].to(dtype)
+
+
+def _eager_selective_scan(x, delta, A, B, C, D, z, delta_bias, delta_softplus, h0, lengths):
+    dtype, (T, N, channels) = x.dtype, x.shape
+    x, delta, A, B, C, D, z, delta_bias, h = _wide(x, delta, A, B, C, D, z, delta_bias, h0)
+    inside = _inside(lengths, T, N, x)
+    x, delta, z = (t if t is None else torch.where(inside[..., None], t, 0.0) for t in (x, delta, z))
+    B, C = (torch.where(inside[..., None, None], t if t.dim() == 4 else t.unsqueeze(2), 0.0) for t in (B, C))
+    share = channels // B.shape[2]
+    dt = delta if delta_bias is None else delta + delta_bias
+    dt = F.softplus(dt, threshold=50.0) if delta_softplus else dt
+    h = x.new_zeros(N, channels, A.shape[1]) if h is None else h
+    ys = []
+    for t in range(T):
+        new = torch.exp(dt[t, :, :, None] * A) * h + (dt[t] * x[t])[..., None] * B[t].repeat_interleave(share, 1)
+        y = (new * C[t].repeat_interleave(share, 1)).sum(-1)
+        h = torch.where(inside[t][:, None, None], new, h)
+        ys.append(y if D is None else y + D * x[t])
+    y = torch.stack(ys)
+    y = y if z is None else y * F.silu(z)
+    return torch.where(inside[..., None], y, 0.0).to(dtype), h
+
+
+def _eager_residual_norm(update, residual, gate, scale, after_weight, before_weight, before_bias, centered, eps):
+    dtype = update.dtype
+    v, residual, gate, scale, after, before, bias = _wide(update, residual, gate, scale, after_weight, before_weight, before_bias)
+
+    def norm(v):
+        v = v - v.mean(-1, keepdim=True) if centered else v
+        return v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps)
+
+    v = v if after is None else norm(v) * after
+    v = v if gate is None else v * F.silu(gate)
+    v = v if scale is None else v * scale
+    v = v if residual is None else v + residual
+    n = None if before is None else norm(v) * before
+    n = n if bias is None else n + bias
+    return v.to(dtype), None if n is None else n.to(dtype)
+
+
+class _BlockLayer(nn.Module):
+    """What the layers of a state space block share."""
+    _name = "layer"
+
+    def _fused(self, x):
+        """Whether the fused ops run, decided and checked as the recurrent layers do."""
+        fused = _RNNBase._is_cuda(self)
+        if fused and not x.is_cuda:
+            raise RuntimeError("%s: the parameters are GPU tensors, the input must be one too" % self._name)
+        if fused and x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise RuntimeError("%s: the input must be float32, float16 or bfloat16" % self._name)
+        return fused
+
+    def _rows(self, t):
+        return t.transpose(0, 1) if t is not None and getattr(self, "batch_first", False) else t
+
+    def _lengths(self, lengths, x):
+        """int64 [N] on the input's device.  Lengths beyond x are an error where the host knows them; on the GPU they give NaNs."""
+        if lengths is None:
+            return None
+        lengths = torch.as_tensor(lengths, dtype=torch.long)
+        steps = x.shape[0]
+        if not lengths.is_cuda and lengths.numel():
+            for length in lengths.aminmax():
+                if not -steps - 1 <= length <= steps:
+                    raise IndexError("length %d is out of bounds for sequences of %d steps" % (length, steps))
+        if tuple(lengths.shape) != (x.shape[1],):
+            raise ValueError("%s: lengths must be [%d], got %s" % (self._name, x.shape[1], list(lengths.shape)))
+        return lengths.to(x.device).contiguous()
+
+
+def _as_float(p):
+    return p if p is None or p.dtype == torch.float32 else p.float()
+
+
+class CausalConv(_BlockLayer):
+    """Short causal convolution over time, one filter per channel: y[t] = act(bias + sum_k kernel[k] x[t-width+1+k]),
+    act(v) = v sigmoid(v) with silu.  Parameters: kernel [width, channels], bias [channels] (uniform in
+    +-width^-0.5).  width of 1 to 8."""
+    _name = "CausalConv"
+
+    def __init__(self, channels, width=4, bias=True, silu=True, batch_first=False):
+        super().__init__()
+        if not 1 <= width <= 8:
+            raise ValueError("%s: width must be in [1, 8]" % self._name)
+        self.channels, self.width, self.silu, self.batch_first = channels, width, silu, batch_first
+        self.kernel = nn.Parameter(torch.empty(width, channels))
+        self.bias = nn.Parameter(torch.empty(channels)) if bias else None
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            for p in self.parameters():
+                p.uniform_(-self.width ** -0.5, self.width ** -0.5)
+
+    def forward(self, input, state=None, lengths=None):
+        """input [T,N,channels] ([N,T,channels] if batch_first) -> (output, state): state [width-1,N,channels] holds the
+        inputs before the first step (None: zeros), and is returned for the step behind the last (of the row's
+        length).  Outputs behind a row's length are 0."""
+        x = self._rows(input)
+        lengths = self._lengths(lengths, x)
+        if self._fused(x):
+            y, state = _CausalConvFunction.apply(x, _as_float(self.kernel), _as_float(self.bias), self.silu, state, lengths)
+        else:
+            y, state = _eager_causal_conv(x, self.kernel, self.bias, self.silu, state, lengths)
+        return self._rows(y), state
+
+    def step(self, input, state):
+        """One step without gradients: input [N,channels] -> (output, state)."""
+        with torch.no_grad():
+            if self._fused(input):
+                return ops.causal_conv_iterate(input, state, _as_float(self.kernel), _as_float(self.bias), self.silu)
+            y, state = _eager_causal_conv(input.unsqueeze(0), self.kernel, self.bias, self.silu, state, None)
+            return y[0], state
+
+
+class SelectiveScan(_BlockLayer):
+    """Selective state space recurrence: with A = -exp(log_decay) and dt = softplus(delta + delta_bias),
+    h[t] = exp(dt A) h[t-1] + dt x B, y = (sum_s C h + skip x) silu(z).  Parameters: log_decay [channels, state_size]
+    (logarithms of 1 .. state_size), skip [channels] (ones), delta_bias [channels] (step sizes of 0.001 to 0.1).  `groups`
+    groups of channels share B and C; state_size of 1 to 64."""
+    _name = "SelectiveScan"
+
+    def __init__(self, channels, state_size=16, groups=1, batch_first=False):
+        super().__init__()
+        if not 1 <= state_size <= 64:
+            raise ValueError("%s: state_size must be in [1, 64]" % self._name)
+        if groups < 1 or channels % groups:
+            raise ValueError("%s: %d channels cannot be shared by %d groups" % (self._name, channels, groups))
+        self.channels, self.state_size, self.groups, self.batch_first = channels, state_size, groups, batch_first
+        self.log_decay = nn.Parameter(torch.empty(channels, state_size))
+        self.skip = nn.Parameter(torch.empty(channels))
+        self.delta_bias = nn.Parameter(torch.empty(channels))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            self.log_decay.copy_(torch.log(torch.arange(1.0, self.state_size + 1)).expand_as(self.log_decay))
+            self.skip.fill_(1.0)
+            dt = torch.exp(torch.empty_like(self.delta_bias, dtype=torch.float32).uniform_(-6.907755, -2.302585))
+            self.delta_bias.copy_(dt + torch.log(-torch.expm1(-dt)))
+
+    def _decay(self):
+        return -torch.exp(_as_float(self.log_decay) if self.log_decay.dtype != torch.float64 else self.log_decay)
+
+    def _grouped(self, t):
+        return t.unflatten(-1, (self.groups, self.state_size))
+
+    def forward(self, x, delta, B, C, z=None, state=None, lengths=None):
+        """x, delta, z [T,N,channels], B, C [T,N,groups*state_size] ([N,T,*] if batch_first) -> (output, state): state
+        [N,channels,state_size], float32, before the first step (None: zeros) and after the last (of the row's length).
+        Outputs behind a row's length are 0."""
+        x, delta, B, C, z = (self._rows(t) for t in (x, delta, B, C, z))
+        lengths = self._lengths(lengths, x)
+        arguments = x, delta, self._decay(), self._grouped(B), self._grouped(C)
+        if self._fused(x):
+            y, state = _SelectiveScanFunction.apply(torch.is_grad_enabled(), *arguments, _as_float(self.skip), z,
+                                                    _as_float(self.delta_bias), True, state, lengths)
+        else:
+            y, state = _eager_selective_scan(*arguments, self.skip, z, self.delta_bias, True, state, lengths)
+        return self._rows(y), state
+
+    def step(self, x, delta, B, C, z=None, state=None):
+        """One step without gradients: x, delta, z [N,channels], B, C [N,groups*state_size] -> (output, state)."""
+        with torch.no_grad():
+            if state is None:
+                state = torch.zeros(x.shape[0], self.channels, self.state_size, device=x.device,
+                                    dtype=x.dtype if x.dtype == torch.float64 else torch.float32)
+            arguments = x, delta, self._decay(), self._grouped(B), self._grouped(C)
+            if self._fused(x):
+                return ops.selective_scan_iterate(*arguments, state, _as_float(self.skip), z, _as_float(self.delta_bias), True)
+            x, delta, A, B, C = (t if t is arguments[2] else t.unsqueeze(0) for t in arguments)
+            y, state = _eager_selective_scan(x, delta, A, B, C, self.skip, None if z is None else z.unsqueeze(0),
+                                             self.delta_bias, True, state, None)
+            return y[0], state
+
+
+class ResidualNorm(_BlockLayer):
+    """The norms around a block, its gate and its residual scale: out = residual + scale norm(update) after_weight silu(gate),
+    normed = norm(out) before_weight + before_bias, of which `out` leaves the block and `normed` enters the next one.  norm is
+    the root mean square norm, or layer norm (centered).  Parameters, each [channels]: after_weight (ones; absent unless
+    norm_after), scale (`scale`; absent if None), before_weight (ones; absent unless norm_before), before_bias (zeros; centered
+    only).  At most 8192 channels."""
+    _name = "ResidualNorm"
+
+    def __init__(self, channels, centered=False, norm_after=True, norm_before=True, scale=1.0, eps=1e-5):
+        super().__init__()
+        self.channels, self.centered, self.eps, self.initial_scale = channels, centered, eps, scale
+        make = lambda wanted: nn.Parameter(torch.empty(channels)) if wanted else None  # noqa: E731
+        self.after_weight = make(norm_after)
+        self.scale = make(scale is not None)
+        self.before_weight = make(norm_before)
+        self.before_bias = make(norm_before and centered)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            for p, value in ((self.after_weight, 1.0), (self.scale, self.initial_scale), (self.before_weight, 1.0),
+                             (self.before_bias, 0.0)):
+                if p is not None:
+                    p.fill_(value)
+
+    def forward(self, update, residual=None, gate=None):
+        """Tensors [T,N,channels] (in whatever order, or [N,channels]) -> (out, normed); normed is None unless norm_before."""
+        weights = self.scale, self.after_weight, self.before_weight, self.before_bias
+        if self._fused(update) or update.is_cuda and not list(self.parameters()):
+            return _ResidualNormFunction.apply(update, residual, gate, *map(_as_float, weights), self.centered, self.eps)
+        return _eager_residual_norm(update, residual, gate, *weights, self.centered, self.eps)

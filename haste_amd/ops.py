@@ -5,7 +5,13 @@ with the same argument order, allocation protocol and return tuples, implemented
 calls into libhaste_hip.so.  Tensors are float32 or float64, for the GRU also float16 (all tensors of a call alike),
 contiguous, on the GPU; torch is used only to allocate device memory and to name the
 current stream.
+
+The operators of a state space block (causal_conv_*, selective_scan_*, residual_norm_*, at the end) have rules of
+their own: see the comment before them.
 """
+import ctypes
+import functools
+
 import torch
 
 from . import lib
@@ -57,7 +63,6 @@ def stream_status(stream=None):
     lib.HasteHipError when a persistent kernel launched on it gave up a bounded wait (its
     outputs, and those of library kernels queued behind it, are invalid); see
     haste_hip_stream_status in include/haste_hip.h."""
-    import ctypes
     handle = lib.load()
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
@@ -70,7 +75,6 @@ def stream_status(stream=None):
 def workspace_bytes(time_steps, batch_size, input_size, hidden_size, half_gru=False):
     """Upper bound of the scratch memory any cell needs for these sizes on the current device
     (half_gru: the GRU on half tensors, which also stages fp32 copies of its tensors there)."""
-    import ctypes
     handle = lib.load()
     fn = handle.haste_hip_gru_half_workspace_bytes if half_gru else handle.haste_hip_workspace_bytes
     fn.restype = ctypes.c_size_t
@@ -83,7 +87,6 @@ def set_workspace(buffer, stream=None):
     caller keeps alive and leaves alone) as the scratch memory of `stream` (default: the current
     stream); None takes it back.  With a lent buffer the ops allocate, free and synchronize
     nothing themselves, so they can be recorded into a HIP graph."""
-    import ctypes
     handle = lib.load()
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
@@ -103,7 +106,6 @@ def set_workspace(buffer, stream=None):
 def workspace_high_water(stream=None):
     """Bytes of scratch memory the calls made on `stream` so far have needed (what to lend for
     a replay of the same calls)."""
-    import ctypes
     handle = lib.load()
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
@@ -585,3 +587,339 @@ def layer_norm_gru_backward(x_t, kernel_t, recurrent_kernel_t, bias, recurrent_b
              act_Wx, gamma[0], dgamma[0], act_Rh, gamma[1], dgamma[1], act_Rh_norm_cache,
              _mask_or_none(has_zoneout, zoneout_mask))
     return dx, dh, dW, dR, dbx, dbr, dgamma
+
+
+# ---- The operators of a state space block ---------------------------------------------
+# The short causal convolution, the selective scan, and the norms around the block.  They have no
+# counterpart in the reference.  Activations are float32, float16 or bfloat16, all of a call alike;
+# parameters, recurrent states (h) and statistics are float32 whatever the activations are; the
+# convolution's state holds inputs and has their type.  Inputs may have any strides (they are copied where
+# channels are not contiguous), outputs are contiguous.  lengths[N] (int64, on the GPU): steps at and behind a row's
+# length are not read, their outputs and gradients are 0, and the row's state is that of its last step; -1 counts as T, and a
+# length that names no step gives NaNs for its row.  Scratch memory comes from torch's allocator, so calls may be
+# recorded into a graph, and run on several streams at once.
+_ACTIVATIONS = {torch.float32: "_f32", torch.float16: "_f16", torch.bfloat16: "_bf16"}
+
+
+def _described(t):
+    return "%s %s on %s" % (t.dtype, list(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__
+
+
+def _activation(what, t, shape, like):
+    if not torch.is_tensor(t) or t.shape != shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError("%s must be %s %s on %s, got %s" % (what, like.dtype, list(shape), like.device, _described(t)))
+
+
+def _float(what, t, shape, like):
+    """A parameter, state or statistic, contiguous."""
+    if not torch.is_tensor(t) or t.shape != shape or t.dtype != torch.float32 or t.device != like.device:
+        raise ValueError("%s must be float32 %s on %s, got %s" % (what, list(shape), like.device, _described(t)))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _activation_suffix(x):
+    suffix = _ACTIVATIONS.get(x.dtype)
+    if suffix is None:
+        raise ValueError("activations must be float32, float16 or bfloat16, got %s" % x.dtype)
+    if not x.is_cuda:
+        raise ValueError("tensor must be a GPU tensor")
+    return suffix
+
+
+def _packed_rows(t, shared=False):
+    """`t` with contiguous channels (shared: groups and states): itself, or a copy."""
+    if t.stride(-1) != 1 and t.size(-1) != 1 or shared and t.stride(-2) != t.size(-1) and t.size(-2) != 1:
+        return t.contiguous()
+    return t
+
+
+def _strided(t):
+    """The three arguments an entry point takes for a tensor [T,N,...]."""
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on_device_of(index, name):
+    """Runs an operator on the device of its argument `name`, number `index` (the current device needs nothing)."""
+    def decorate(op):
+        @functools.wraps(op)
+        def on_device(*args, **kwargs):
+            like = args[index] if len(args) > index else kwargs.get(name)
+            if torch.is_tensor(like) and like.is_cuda and like.device.index != torch.cuda.current_device():
+                with torch.cuda.device(like.device):
+                    return op(*args, **kwargs)
+            return op(*args, **kwargs)
+        return on_device
+    return decorate
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(entry, device, *sizes):
+    """What a *_bytes entry point says for these sizes (all ints) on the current device, which `device` is."""
+    fn = lib.load()[entry]
+    fn.restype = ctypes.c_size_t
+    fn.argtypes = [ctypes.c_int] * len(sizes)
+    return int(fn(*sizes))
+
+
+def _scratch(entry, like, *sizes):
+    if max(sizes) >= 2 ** 31:
+        raise ValueError("sizes beyond 2^31 are not implemented, got %s" % (sizes,))
+    return torch.empty(max(1, _scratch_bytes(entry, like.device, *sizes)), device=like.device, dtype=torch.uint8)
+
+
+def _zero_rows(T, N, D, like):
+    return torch.zeros(1, 1, D, device=like.device, dtype=like.dtype).expand(T, N, D)
+
+
+def _invoke(name, *values):
+    lib.invoke(name, lib.entry(name), list(values))
+
+
+def _conv_arguments(x, kernel, bias, state, lengths, steps=True):
+    dims = 3 if steps else 2
+    if not torch.is_tensor(x) or x.dim() != dims or not torch.is_tensor(kernel) or kernel.dim() != 2 or 0 in x.shape:
+        raise ValueError("x must be [%s], of no size 0, and kernel [W,D], got %s and %s"
+                         % ("T,N,D" if steps else "N,D", _described(x), _described(kernel)))
+    N, D = x.shape[-2:]
+    W = kernel.shape[0]
+    if not 1 <= W <= 8:
+        raise ValueError("kernels of 1 to 8 steps are implemented, got %d" % W)
+    kernel = _float("kernel", kernel, (W, D), x)
+    if bias is not None:
+        bias = _float("bias", bias, (D,), x)
+    if state is not None:
+        _activation("state", state, (W - 1, N, D), x)
+        state = state.contiguous()
+    if lengths is not None:
+        _check_lengths(lengths, x)
+    return _packed_rows(x), kernel, bias, state, _activation_suffix(x)
+
+
+@_on_device_of(0, "x")
+def causal_conv_forward(x, kernel, bias=None, silu=False, state=None, lengths=None):
+    """x[T,N,D], kernel[W,D] -> y[T,N,D], state_out[W-1,N,D]: y[t] = act(bias + sum_k kernel[k] X[t+k]) with
+    X = [state; x] (state None: zeros), act(v) = v sigmoid(v) with silu; state_out: the inputs before the next step."""
+    x, kernel, bias, state, suffix = _conv_arguments(x, kernel, bias, state, lengths)
+    (T, N, D), W = x.shape, kernel.shape[0]
+    y = torch.empty(T, N, D, device=x.device, dtype=x.dtype)
+    state_out = torch.empty(W - 1, N, D, device=x.device, dtype=x.dtype)
+    _invoke("haste_hip_causal_conv_forward" + suffix, T, N, D, W, *_strided(x), kernel.data_ptr(), _address(bias), bool(silu),
+            _address(state), _address(lengths), y.data_ptr(), state_out.data_ptr())
+    return y, state_out
+
+
+@_on_device_of(0, "x")
+def causal_conv_backward(x, kernel, bias, silu, state, lengths, dy, dstate_out=None):
+    """Gradients (dx, dkernel, dbias, dstate) from those of y (None: zeros) and of state_out; dbias and dstate are None
+    where there is no bias or state."""
+    like = x
+    x, kernel, bias, state, suffix = _conv_arguments(x, kernel, bias, state, lengths)
+    (T, N, D), W = x.shape, kernel.shape[0]
+    dy = _zero_rows(T, N, D, x) if dy is None else dy
+    _activation("dy", dy, like.shape, x)
+    dy = _packed_rows(dy)
+    if dstate_out is not None:
+        _activation("dstate_out", dstate_out, (W - 1, N, D), x)
+        dstate_out = dstate_out.contiguous()
+    dx = torch.empty(T, N, D, device=x.device, dtype=x.dtype)
+    dkernel, dbias = torch.empty_like(kernel), None if bias is None else torch.empty_like(bias)
+    dstate = None if state is None else torch.empty_like(state)
+    scratch = _scratch("haste_hip_causal_conv_workspace_bytes", x, T, N, D, W)
+    _invoke("haste_hip_causal_conv_backward" + suffix, T, N, D, W, *_strided(x), kernel.data_ptr(), _address(bias), bool(silu),
+            _address(state), _address(lengths), *_strided(dy), _address(dstate_out), dx.data_ptr(), dkernel.data_ptr(),
+            _address(dbias), _address(dstate), scratch.data_ptr(), scratch.numel())
+    return dx, dkernel, dbias, dstate
+
+
+@_on_device_of(0, "x")
+def causal_conv_iterate(x, state, kernel, bias=None, silu=False, state_out=None):
+    """One step: x[N,D], state[W-1,N,D] -> y[N,D], state_out (which may be given, and may be state)."""
+    x, kernel, bias, read, suffix = _conv_arguments(x, kernel, bias, state, None, steps=False)
+    (N, D), W = x.shape, kernel.shape[0]
+    if read is None:
+        raise ValueError("state must be %s %s on %s, got None" % (x.dtype, [W - 1, N, D], x.device))
+    y = torch.empty(N, D, device=x.device, dtype=x.dtype)
+    if state_out is None:
+        state_out = torch.empty(W - 1, N, D, device=x.device, dtype=x.dtype)
+    else:
+        _output("state_out", state_out, (W - 1, N, D), x.dtype, x)
+    _invoke("haste_hip_causal_conv_forward" + suffix, 1, N, D, W, x.data_ptr(), 0, x.stride(0), kernel.data_ptr(),
+            _address(bias), bool(silu), read.data_ptr(), None, y.data_ptr(), state_out.data_ptr())
+    return y, state_out
+
+
+def _output(what, t, shape, dtype, like):
+    if not torch.is_tensor(t) or t.shape != shape or t.dtype != dtype or t.device != like.device or not t.is_contiguous():
+        raise ValueError("%s must be %s %s on %s, contiguous, got %s" % (what, dtype, list(shape), like.device, _described(t)))
+
+
+def _scan_arguments(x, delta, A, B, C, D, z, delta_bias, steps=True):
+    """The arguments checked: (x, delta, A, B, C, D, z, delta_bias) as the entry points take them, S, G and the suffix."""
+    dims = 3 if steps else 2
+    if not torch.is_tensor(x) or x.dim() != dims or 0 in x.shape:
+        raise ValueError("x must be [%s], of no size 0, got %s" % ("T,N,D" if steps else "N,D", _described(x)))
+    if not torch.is_tensor(A) or A.dim() != 2 or not 1 <= A.shape[1] <= 64:
+        raise ValueError("A must be float32 [D,S], S of 1 to 64, got %s" % _described(A))
+    channels, S = x.shape[-1], A.shape[1]
+    if not torch.is_tensor(B) or B.dim() not in (dims, dims + 1):
+        raise ValueError("B must be [%s,G,S] or [%s,S], got %s" % ((("T,N", "T,N") if steps else ("N", "N")) + (_described(B),)))
+    G = B.shape[-2] if B.dim() == dims + 1 else 1
+    if G < 1 or channels % G:
+        raise ValueError("%d channels cannot be shared by %d groups" % (channels, G))
+    _activation("delta", delta, x.shape, x)
+    A = _float("A", A, (channels, S), x)
+    shape = x.shape[:-1] + ((G, S) if B.dim() == dims + 1 else (S,))
+    _activation("B", B, shape, x)
+    _activation("C", C, shape, x)
+    shared = B.dim() == dims + 1
+    if D is not None:
+        D = _float("D", D, (channels,), x)
+    if z is not None:
+        _activation("z", z, x.shape, x)
+        z = _packed_rows(z)
+    if delta_bias is not None:
+        delta_bias = _float("delta_bias", delta_bias, (channels,), x)
+    return (_packed_rows(x), _packed_rows(delta), A, _packed_rows(B, shared), _packed_rows(C, shared), D, z, delta_bias, S, G,
+            _activation_suffix(x))
+
+
+@_on_device_of(1, "x")
+def selective_scan_forward(training, x, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False, h0=None,
+                           lengths=None):
+    """x, delta, z[T,N,D], A[D,S], B, C[T,N,G,S] ([T,N,S]: one group), D, delta_bias[D], h0[N,D,S]
+    -> y[T,N,D], h_last[N,D,S], cache (what the backward pass needs; None unless training):
+    dt = delta + delta_bias, of which delta_softplus takes the softplus; h[t] = exp(dt A) h[t-1] + dt x B;
+    y = (sum_s C h + D x) z sigmoid(z).  Parts that are None are left out."""
+    x, delta, A, B, C, D, z, delta_bias, S, G, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias)
+    T, N, channels = x.shape
+    if h0 is not None:
+        h0 = _float("h0", h0, (N, channels, S), x)
+    if lengths is not None:
+        _check_lengths(lengths, x)
+    y = torch.empty(T, N, channels, device=x.device, dtype=x.dtype)
+    h_last = torch.empty(N, channels, S, device=x.device)
+    cache = None
+    if training:
+        cache = _scratch("haste_hip_selective_scan_kept_bytes", x, T, N, channels, S)
+    scratch = _scratch("haste_hip_selective_scan_workspace_bytes", x, 0, T, N, channels, S, G)
+    _invoke("haste_hip_selective_scan_forward" + suffix, T, N, channels, S, G, *_strided(x), *_strided(delta), A.data_ptr(),
+            *_strided(B), *_strided(C), _address(D), *_strided(z), _address(delta_bias), bool(delta_softplus), _address(h0),
+            _address(lengths), y.data_ptr(), h_last.data_ptr(), _address(cache), scratch.data_ptr(), scratch.numel())
+    return y, h_last, cache
+
+
+@_on_device_of(0, "x")
+def selective_scan_backward(x, delta, A, B, C, D, z, delta_bias, delta_softplus, h0, lengths, cache, dy, dh_last=None):
+    """Gradients (dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dh0) from those of y (None: zeros) and h_last, and the cache of
+    the forward pass of the same arguments; those of arguments that are None are None (dh0 is always given)."""
+    dims_B = B.shape if torch.is_tensor(B) else None
+    x, delta, A, B, C, D, z, delta_bias, S, G, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias)
+    T, N, channels = x.shape
+    if lengths is not None:
+        _check_lengths(lengths, x)
+    kept = _scratch_bytes("haste_hip_selective_scan_kept_bytes", x.device, T, N, channels, S)
+    if not torch.is_tensor(cache) or cache.dtype != torch.uint8 or cache.numel() != kept or cache.device != x.device:
+        raise ValueError("the cache must be that of a forward pass in training over the same arguments")
+    dy = _zero_rows(T, N, channels, x) if dy is None else dy
+    _activation("dy", dy, x.shape, x)
+    dy = _packed_rows(dy)
+    if dh_last is not None:
+        dh_last = _float("dh_last", dh_last, (N, channels, S), x)
+    like = dict(device=x.device, dtype=x.dtype)
+    dx, ddelta = torch.empty(T, N, channels, **like), torch.empty(T, N, channels, **like)
+    dz = None if z is None else torch.empty(T, N, channels, **like)
+    dB, dC = torch.empty(dims_B, **like), torch.empty(dims_B, **like)
+    dA, dh0 = torch.empty_like(A), torch.empty(N, channels, S, device=x.device)
+    dD = None if D is None else torch.empty_like(D)
+    dbias = None if delta_bias is None else torch.empty_like(delta_bias)
+    scratch = _scratch("haste_hip_selective_scan_workspace_bytes", x, 1, T, N, channels, S, G)
+    _invoke("haste_hip_selective_scan_backward" + suffix, T, N, channels, S, G, *_strided(x), *_strided(delta), A.data_ptr(),
+            *_strided(B), *_strided(C), _address(D), *_strided(z), _address(delta_bias), bool(delta_softplus),
+            _address(lengths), cache.data_ptr(), *_strided(dy), _address(dh_last), dx.data_ptr(), ddelta.data_ptr(),
+            dA.data_ptr(), dB.data_ptr(), dC.data_ptr(), _address(dD), _address(dz), _address(dbias), dh0.data_ptr(),
+            scratch.data_ptr(), scratch.numel())
+    return dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0
+
+
+@_on_device_of(0, "x")
+def selective_scan_iterate(x, delta, A, B, C, h, D=None, z=None, delta_bias=None, delta_softplus=False, h_out=None):
+    """One step: x, delta, z[N,D], B, C[N,G,S] ([N,S]), h[N,D,S] -> y[N,D], h_out (which may be given, and may be h)."""
+    x, delta, A, B, C, D, z, delta_bias, S, G, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias, steps=False)
+    N, channels = x.shape
+    h = _float("h", h, (N, channels, S), x)
+    y = torch.empty(N, channels, device=x.device, dtype=x.dtype)
+    if h_out is None:
+        h_out = torch.empty(N, channels, S, device=x.device)
+    else:
+        _output("h_out", h_out, (N, channels, S), torch.float32, x)
+    _invoke("haste_hip_selective_scan_iterate" + suffix, N, channels, S, G, x.data_ptr(), x.stride(0), delta.data_ptr(),
+            delta.stride(0), A.data_ptr(), B.data_ptr(), B.stride(0), C.data_ptr(), C.stride(0), _address(D), _address(z),
+            0 if z is None else z.stride(0), _address(delta_bias), bool(delta_softplus), h.data_ptr(), y.data_ptr(),
+            h_out.data_ptr())
+    return y, h_out
+
+
+def _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias):
+    """The arguments checked, activations as [T,N,D]."""
+    if not torch.is_tensor(update) or update.dim() not in (2, 3) or 0 in update.shape:
+        raise ValueError("update must be [T,N,D] or [N,D], of no size 0, got %s" % _described(update))
+    D = update.shape[-1]
+    if D > 8192:
+        raise ValueError("rows of up to 8192 channels are implemented, got %d" % D)
+    for what, t in (("residual", residual), ("gate", gate)):
+        if t is not None:
+            _activation(what, t, update.shape, update)
+    if before_weight is None and before_bias is not None:
+        raise ValueError("before_bias needs before_weight")
+    weights = [None if w is None else _float(what, w, (D,), update) for what, w in
+               (("scale", scale), ("after_weight", after_weight), ("before_weight", before_weight), ("before_bias", before_bias))]
+    return [_norm_rows(t) for t in (update, residual, gate)], weights, _activation_suffix(update)
+
+
+def _norm_rows(t):
+    return t if t is None else _packed_rows(t if t.dim() == 3 else t.unsqueeze(0))
+
+
+@_on_device_of(0, "update")
+def residual_norm_forward(update, residual=None, gate=None, scale=None, after_weight=None, before_weight=None, before_bias=None,
+                          centered=False, eps=1e-5):
+    """update, residual, gate[T,N,D] (or [N,D]), weights[D] -> out, normed (None without before_weight), stats:
+    out = residual + scale norm(update) after_weight gate sigmoid(gate), normed = norm(out) before_weight + before_bias,
+    norm(v) = v / sqrt(mean v^2 + eps), centered: of v - mean v.  Parts that are None are left out (update is not normed without
+    after_weight); stats is what the backward pass needs."""
+    rows, weights, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
+    T, N, D = rows[0].shape
+    out = torch.empty(update.shape, device=update.device, dtype=update.dtype)
+    normed = None if before_weight is None else torch.empty_like(out)
+    stats = torch.empty(T, N, 4, device=update.device)
+    _invoke("haste_hip_residual_norm_forward" + suffix, T, N, D, *_strided(rows[0]), *_strided(rows[1]), *_strided(rows[2]),
+            *map(_address, weights), bool(centered), float(eps), out.data_ptr(), _address(normed), stats.data_ptr())
+    return out, normed, stats
+
+
+@_on_device_of(0, "update")
+def residual_norm_backward(update, residual, gate, scale, after_weight, before_weight, before_bias, stats, dout, dnormed,
+                           centered=False):
+    """Gradients (dupdate, dresidual, dgate, dscale, dafter_weight, dbefore_weight, dbefore_bias) from those of out and normed
+    (either may be None: zeros); those of arguments that are None are None."""
+    rows, weights, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
+    T, N, D = rows[0].shape
+    stats = _float("stats", stats, (T, N, 4), update)
+    if dnormed is not None and before_weight is None:
+        raise ValueError("dnormed needs before_weight")
+    for what, t in (("dout", dout), ("dnormed", dnormed)):
+        if t is not None:
+            _activation(what, t, update.shape, update)
+    grads = [None if t is None else torch.empty(update.shape, device=update.device, dtype=update.dtype)
+             for t in (update, residual, gate)]
+    sums = [None if w is None else torch.empty_like(w) for w in weights]
+    scratch = _scratch("haste_hip_residual_norm_workspace_bytes", update, T, N, D)
+    dout, dnormed = _norm_rows(dout), _norm_rows(dnormed)
+    _invoke("haste_hip_residual_norm_backward" + suffix, T, N, D, *_strided(rows[0]), *_strided(rows[1]), *_strided(rows[2]),
+            *map(_address, weights[:3]), bool(centered), stats.data_ptr(), *_strided(dout), *_strided(dnormed),
+            *map(_address, grads), *map(_address, sums), scratch.data_ptr(), scratch.numel())
+    return (*grads, *sums)

@@ -642,6 +642,164 @@ int haste_hip_gru_backward_iterate_f16(int batch_size, int input_size, int hidde
                                        void* dbr, void* dh, void* dp, void* dq,
                                        const void* zoneout_mask, void* stream);
 
+/* ---- The operators of a state space block -------------------------------------------------
+ * A short causal convolution, the selective scan, and the norms around the block; no counterpart in
+ * the reference, whose recurrences they stand beside.  Suffixes _f32, _f16 and _bf16 name the type of the activations
+ * (passed as const void* there is one declaration for all three); parameters, recurrent states and
+ * statistics are float whatever the activations are, sums are float, and a result is rounded once.
+ * Activations that are read may have any strides: `name_step` and `name_row` are the elements between
+ * steps and between batch rows, channels are contiguous; what is written is packed, [T,N,D].
+ * lengths: NULL, or N 64-bit integers on the device: the row's steps are those before its length
+ * (counted from the end when negative, -1 being T); steps behind them are not read, their outputs and
+ * gradients are 0 and the row's last state is that of its last step.  A length that names no step of 0 .. T gives NaNs for
+ * what is computed of the row itself.  Nothing is accumulated into: every output is assigned.
+ * Scratch memory is the caller's: `workspace` holds what the operator's *_workspace_bytes says for the
+ * current device (0 for sizes the call refuses); nothing is allocated, no call synchronizes, every sum
+ * is added in an order that depends on the sizes only.
+ *
+ * Causal convolution over time, X = [state; x], y[t] = act(bias + sum_k kernel[k] X[t+k]):
+ * x,y[T,N,D] kernel[W,D] bias[D] or NULL, W of 1 .. 8; silu != 0: act(v) = v sigmoid(v), else v;
+ * state[W-1,N,D], the inputs before the first (NULL: zeros); state_out[W-1,N,D], those before the
+ * next (may be `state`; NULL: not wanted).  A single step is the call with steps = 1.  Backward: dstate_out, the gradient
+ * of state_out, or NULL; dbias, dstate may be NULL. */
+size_t haste_hip_causal_conv_workspace_bytes(int steps, int batch_size, int channels, int width);
+int haste_hip_causal_conv_forward_f32(int steps, int batch_size, int channels, int width, const void* x,
+    size_t x_step, size_t x_row, const float* kernel, const float* bias, int silu, const void* state,
+    const void* lengths, void* y, void* state_out, void* stream);
+int haste_hip_causal_conv_backward_f32(int steps, int batch_size, int channels, int width, const void* x,
+    size_t x_step, size_t x_row, const float* kernel, const float* bias, int silu, const void* state,
+    const void* lengths, const void* dy, size_t dy_step, size_t dy_row, const void* dstate_out, void* dx,
+    float* dkernel, float* dbias, void* dstate, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_causal_conv_forward_f16(int steps, int batch_size, int channels, int width, const void* x,
+    size_t x_step, size_t x_row, const float* kernel, const float* bias, int silu, const void* state,
+    const void* lengths, void* y, void* state_out, void* stream);
+int haste_hip_causal_conv_backward_f16(int steps, int batch_size, int channels, int width, const void* x,
+    size_t x_step, size_t x_row, const float* kernel, const float* bias, int silu, const void* state,
+    const void* lengths, const void* dy, size_t dy_step, size_t dy_row, const void* dstate_out, void* dx,
+    float* dkernel, float* dbias, void* dstate, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_causal_conv_forward_bf16(int steps, int batch_size, int channels, int width, const void* x,
+    size_t x_step, size_t x_row, const float* kernel, const float* bias, int silu, const void* state,
+    const void* lengths, void* y, void* state_out, void* stream);
+int haste_hip_causal_conv_backward_bf16(int steps, int batch_size, int channels, int width, const void* x,
+    size_t x_step, size_t x_row, const float* kernel, const float* bias, int silu, const void* state,
+    const void* lengths, const void* dy, size_t dy_step, size_t dy_row, const void* dstate_out, void* dx,
+    float* dkernel, float* dbias, void* dstate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Selective state space scan (S states a channel, at most 64; G groups of D / G channels share B, C):
+ *   dt = softplus(delta + delta_bias) (delta_softplus 0: delta + delta_bias),
+ *   h[t] = exp(dt A) h[t-1] + dt x B,  y = (sum_s C h[t] + D x) silu(z)
+ * x,delta,z,y[T,N,D] B,C[T,N,G,S] (the G*S of a step contiguous) A,h0,h_last: [D,S], [N,D,S] twice;
+ * D[D], z, delta_bias[D], h0, h_last may be NULL.  kept: NULL, or haste_hip_selective_scan_kept_bytes of memory for
+ * what the backward pass needs of the states.  Backward: dh_last[N,D,S], the gradient of h_last, or
+ * NULL; dz NULL without z; dD, ddelta_bias, dh0 may be NULL.  iterate: one step, tensors without the
+ * step axis, h_out may be h. */
+size_t haste_hip_selective_scan_workspace_bytes(int backward, int steps, int batch_size, int channels, int states,
+                                                int groups);
+size_t haste_hip_selective_scan_kept_bytes(int steps, int batch_size, int channels, int states);
+int haste_hip_selective_scan_forward_f32(int steps, int batch_size, int channels, int states, int groups,
+    const void* x, size_t x_step, size_t x_row,
+    const void* delta, size_t delta_step, size_t delta_row, const float* A, const void* B, size_t B_step,
+    size_t B_row, const void* C, size_t C_step, size_t C_row, const float* D, const void* z, size_t z_step,
+    size_t z_row, const float* delta_bias, int delta_softplus, const float* h0,
+    const void* lengths, void* y, float* h_last, float* kept, void* workspace, size_t workspace_bytes,
+    void* stream);
+int haste_hip_selective_scan_backward_f32(int steps, int batch_size, int channels, int states, int groups,
+    const void* x, size_t x_step, size_t x_row,
+    const void* delta, size_t delta_step, size_t delta_row, const float* A, const void* B, size_t B_step,
+    size_t B_row, const void* C, size_t C_step, size_t C_row, const float* D, const void* z, size_t z_step,
+    size_t z_row, const float* delta_bias, int delta_softplus, const void* lengths,
+    const float* kept, const void* dy, size_t dy_step, size_t dy_row, const float* dh_last, void* dx,
+    void* ddelta, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddelta_bias, float* dh0,
+    void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_selective_scan_iterate_f32(int batch_size, int channels, int states, int groups, const void* x,
+    size_t x_row, const void* delta, size_t delta_row, const float* A, const void* B, size_t B_row,
+    const void* C, size_t C_row, const float* D, const void* z, size_t z_row, const float* delta_bias,
+    int delta_softplus, const float* h, void* y, float* h_out, void* stream);
+int haste_hip_selective_scan_forward_f16(int steps, int batch_size, int channels, int states, int groups,
+    const void* x, size_t x_step, size_t x_row,
+    const void* delta, size_t delta_step, size_t delta_row, const float* A, const void* B, size_t B_step,
+    size_t B_row, const void* C, size_t C_step, size_t C_row, const float* D, const void* z, size_t z_step,
+    size_t z_row, const float* delta_bias, int delta_softplus, const float* h0,
+    const void* lengths, void* y, float* h_last, float* kept, void* workspace, size_t workspace_bytes,
+    void* stream);
+int haste_hip_selective_scan_backward_f16(int steps, int batch_size, int channels, int states, int groups,
+    const void* x, size_t x_step, size_t x_row,
+    const void* delta, size_t delta_step, size_t delta_row, const float* A, const void* B, size_t B_step,
+    size_t B_row, const void* C, size_t C_step, size_t C_row, const float* D, const void* z, size_t z_step,
+    size_t z_row, const float* delta_bias, int delta_softplus, const void* lengths,
+    const float* kept, const void* dy, size_t dy_step, size_t dy_row, const float* dh_last, void* dx,
+    void* ddelta, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddelta_bias, float* dh0,
+    void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_selective_scan_iterate_f16(int batch_size, int channels, int states, int groups, const void* x,
+    size_t x_row, const void* delta, size_t delta_row, const float* A, const void* B, size_t B_row,
+    const void* C, size_t C_row, const float* D, const void* z, size_t z_row, const float* delta_bias,
+    int delta_softplus, const float* h, void* y, float* h_out, void* stream);
+int haste_hip_selective_scan_forward_bf16(int steps, int batch_size, int channels, int states, int groups,
+    const void* x, size_t x_step, size_t x_row,
+    const void* delta, size_t delta_step, size_t delta_row, const float* A, const void* B, size_t B_step,
+    size_t B_row, const void* C, size_t C_step, size_t C_row, const float* D, const void* z, size_t z_step,
+    size_t z_row, const float* delta_bias, int delta_softplus, const float* h0,
+    const void* lengths, void* y, float* h_last, float* kept, void* workspace, size_t workspace_bytes,
+    void* stream);
+int haste_hip_selective_scan_backward_bf16(int steps, int batch_size, int channels, int states, int groups,
+    const void* x, size_t x_step, size_t x_row,
+    const void* delta, size_t delta_step, size_t delta_row, const float* A, const void* B, size_t B_step,
+    size_t B_row, const void* C, size_t C_step, size_t C_row, const float* D, const void* z, size_t z_step,
+    size_t z_row, const float* delta_bias, int delta_softplus, const void* lengths,
+    const float* kept, const void* dy, size_t dy_step, size_t dy_row, const float* dh_last, void* dx,
+    void* ddelta, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddelta_bias, float* dh0,
+    void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_selective_scan_iterate_bf16(int batch_size, int channels, int states, int groups, const void* x,
+    size_t x_row, const void* delta, size_t delta_row, const float* A, const void* B, size_t B_row,
+    const void* C, size_t C_row, const float* D, const void* z, size_t z_row, const float* delta_bias,
+    int delta_softplus, const float* h, void* y, float* h_out, void* stream);
+
+/* The norms around a block with its gate and residual scale:
+ *   out = residual + scale norm(update) after_weight silu(gate),
+ *   normed = norm(out) before_weight + before_bias
+ * update,residual,gate,out,normed[T,N,D] weights [D], D at most 8192; norm(v) = v / sqrt(mean v^2 + eps), of
+ * v - mean v where centered != 0.  residual, gate, scale NULL: left out; after_weight NULL: update is
+ * not normed; before_weight and normed NULL: there is no second norm.  stats[T,N,4]: what the backward pass
+ * needs (NULL: not wanted).  Backward: dout, dnormed may be NULL (zeros); dresidual, dgate and the
+ * weights' gradients may be NULL (not wanted). */
+size_t haste_hip_residual_norm_workspace_bytes(int steps, int batch_size, int channels);
+int haste_hip_residual_norm_forward_f32(int steps, int batch_size, int channels, const void* update,
+    size_t update_step, size_t update_row, const void* residual, size_t residual_step, size_t residual_row,
+    const void* gate, size_t gate_step, size_t gate_row, const float* scale, const float* after_weight,
+    const float* before_weight, const float* before_bias, int centered, float eps, void* out,
+    void* normed, float* stats, void* stream);
+int haste_hip_residual_norm_backward_f32(int steps, int batch_size, int channels, const void* update,
+    size_t update_step, size_t update_row, const void* residual, size_t residual_step, size_t residual_row,
+    const void* gate, size_t gate_step, size_t gate_row, const float* scale, const float* after_weight,
+    const float* before_weight, int centered, const float* stats, const void* dout,
+    size_t dout_step, size_t dout_row, const void* dnormed, size_t dnormed_step, size_t dnormed_row,
+    void* dupdate, void* dresidual, void* dgate, float* dscale, float* dafter_weight, float* dbefore_weight,
+    float* dbefore_bias, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_residual_norm_forward_f16(int steps, int batch_size, int channels, const void* update,
+    size_t update_step, size_t update_row, const void* residual, size_t residual_step, size_t residual_row,
+    const void* gate, size_t gate_step, size_t gate_row, const float* scale, const float* after_weight,
+    const float* before_weight, const float* before_bias, int centered, float eps, void* out,
+    void* normed, float* stats, void* stream);
+int haste_hip_residual_norm_backward_f16(int steps, int batch_size, int channels, const void* update,
+    size_t update_step, size_t update_row, const void* residual, size_t residual_step, size_t residual_row,
+    const void* gate, size_t gate_step, size_t gate_row, const float* scale, const float* after_weight,
+    const float* before_weight, int centered, const float* stats, const void* dout,
+    size_t dout_step, size_t dout_row, const void* dnormed, size_t dnormed_step, size_t dnormed_row,
+    void* dupdate, void* dresidual, void* dgate, float* dscale, float* dafter_weight, float* dbefore_weight,
+    float* dbefore_bias, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_residual_norm_forward_bf16(int steps, int batch_size, int channels, const void* update,
+    size_t update_step, size_t update_row, const void* residual, size_t residual_step, size_t residual_row,
+    const void* gate, size_t gate_step, size_t gate_row, const float* scale, const float* after_weight,
+    const float* before_weight, const float* before_bias, int centered, float eps, void* out,
+    void* normed, float* stats, void* stream);
+int haste_hip_residual_norm_backward_bf16(int steps, int batch_size, int channels, const void* update,
+    size_t update_step, size_t update_row, const void* residual, size_t residual_step, size_t residual_row,
+    const void* gate, size_t gate_step, size_t gate_row, const float* scale, const float* after_weight,
+    const float* before_weight, int centered, const float* stats, const void* dout,
+    size_t dout_step, size_t dout_row, const void* dnormed, size_t dnormed_step, size_t dnormed_row,
+    void* dupdate, void* dresidual, void* dgate, float* dscale, float* dafter_weight, float* dbefore_weight,
+    float* dbefore_bias, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
