@@ -146,24 +146,25 @@ struct Tile {
   static __device__ __forceinline__ int column() { return (threadIdx.x % kPerRow) * WIDTH; }
 };
 
-// The elements of one tensor's tile, in the tensor's own type (half the registers of float, while the
-// tile before is worked on).
+// The elements of one tensor's tile, packed in the tensor's own type while the tile before is worked on.
 template <typename T, int LANES>
 struct Held {
   typedef Tile<LANES> L;
-  T v[L::ITEMS][L::WIDTH];
+  typedef T packed_t __attribute__((ext_vector_type(L::WIDTH)));
+  packed_t v[L::ITEMS];
   __device__ __forceinline__ void load(const Rows<const T>& rows, int t0, int end, const Block<LANES>& b) {
 #pragma unroll
     for (int i = 0; i < L::ITEMS; ++i) {
       const int t = t0 + L::row(i), c = b.c0 + L::column();
+      packed_t w = {};
       if (t < end && c + L::WIDTH <= b.c_end) {
-        const typename Wide<T, L::WIDTH>::type w = *reinterpret_cast<const typename Wide<T, L::WIDTH>::type*>(rows.at(t, b.n) + c);
+        w = *reinterpret_cast<const typename Wide<T, L::WIDTH>::type*>(rows.at(t, b.n) + c);
+      } else if (t < end) {
 #pragma unroll
-        for (int e = 0; e < L::WIDTH; ++e) v[i][e] = w[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < L::WIDTH; ++e) v[i][e] = t < end && c + e < b.c_end ? rows.at(t, b.n)[c + e] : (T)0.f;
+        for (int e = 0; e < L::WIDTH; ++e)
+          if (c + e < b.c_end) w[e] = rows.at(t, b.n)[c + e];
       }
+      v[i] = w;
     }
   }
   __device__ __forceinline__ float get(int i, int e) const { return (float)v[i][e]; }
@@ -263,25 +264,34 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
     __syncthreads();
 
     if (!LOCAL && kept != nullptr && live) store_states(kept + (size_t)(t / TS) * states + state, s0, s.S, h);
-#pragma unroll 4
-    for (int j = 0; j < TS; ++j) {
-      const float2_t dt_u = step_lds[j][mine];
-      const float4_t Bv = B_lds[j * LANES + s0 / K];
-      float ys = 0.f;
-      float4_t Cv;
-      if (!LOCAL) Cv = C_lds[j * LANES + s0 / K];
+    // a pair of steps' operands are read from LDS while the pair before is computed
+    struct { float2_t dt_u[2]; float4_t B[2], C[2]; } now, next;
+    auto read = [&](auto& to, int j) {
 #pragma unroll
-      for (int r = 0; r < K; ++r) {
-        const float a = __builtin_amdgcn_exp2f(dt_u.x * A2[r]);
-        h[r] = a * h[r] + dt_u.y * Bv[r];
-        if (!LOCAL) ys += h[r] * Cv[r];
+      for (int i = 0; i < 2; ++i) {
+        to.dt_u[i] = step_lds[j + i][mine];
+        to.B[i] = B_lds[(j + i) * LANES + s0 / K];
+        if (!LOCAL) to.C[i] = C_lds[(j + i) * LANES + s0 / K];
       }
-      if (LOCAL) {
-        dt_sum += dt_u.x;
-      } else {
-        ys = sum_states<LANES>(ys);
-        if (s0 == 0) y_lds[j][mine] = ys;
+    };
+    read(now, 0);
+#pragma unroll
+    for (int j = 0; j < TS; j += 2) {
+      if (j + 2 < TS) read(next, j + 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float ys = 0.f;
+#pragma unroll
+        for (int r = 0; r < K; ++r) {
+          const float a = __builtin_amdgcn_exp2f(now.dt_u[i].x * A2[r]);
+          h[r] = a * h[r] + now.dt_u[i].y * now.B[i][r];
+          if (!LOCAL) ys += h[r] * now.C[i][r];
+        }
+        if (LOCAL) dt_sum += now.dt_u[i].x;
+        else y_lds[j + i][mine] = sum_states<LANES>(ys);  // (the lanes of a channel write the same)
       }
+      __builtin_amdgcn_sched_barrier(0);
+      now = next;
     }
     __syncthreads();
 
@@ -358,10 +368,10 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
                                     ScanGradients<T> out) {
   typedef Place<LANES> P;
   typedef Tile<LANES> L;
-  __shared__ float2_t step_lds[TS][P::kBlock];  // dt, dt x
-  __shared__ float q_lds[TS][P::kBlock];        // dy silu(z)
+  __shared__ float4_t step_lds[TS][P::kBlock];  // dt, dt x, q = dy silu(z)
   __shared__ float4_t C_lds[TS * LANES], B_lds[LOCAL ? 1 : TS * LANES];
-  __shared__ float ypre_lds[LOCAL ? 1 : TS][P::kBlock], du_lds[LOCAL ? 1 : TS][P::kBlock], Aw_lds[LOCAL ? 1 : TS][P::kBlock];
+  __shared__ float ypre_lds[LOCAL ? 1 : TS][P::kBlock];
+  __shared__ float2_t du_Aw_lds[LOCAL ? 1 : TS][P::kBlock];
   __shared__ float dB_lds[LOCAL ? 1 : 4][TS * LANES * K], dC_lds[LOCAL ? 1 : 4][TS * LANES * K];  // of each wavefront
 
   const Block<LANES> b(s, blockIdx.x);
@@ -438,10 +448,9 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
 #pragma unroll
       for (int e = 0; e < L::WIDTH; ++e) {
         const float dt = inside ? step_size(delta.get(i, e) + bias[e], s.softplus) : 0.f;
-        step_lds[L::row(i)][column + e] = float2_t{dt, LOCAL ? 0.f : dt * x.get(i, e)};
         float q = up.get(i, e);
         if (in.z.p != nullptr) q *= z.get(i, e) * sigmoid_of(z.get(i, e));
-        q_lds[L::row(i)][column + e] = q;
+        step_lds[L::row(i)][column + e] = float4_t{dt, LOCAL ? 0.f : dt * x.get(i, e), q, 0.f};
       }
     }
     Ct.put(reinterpret_cast<float*>(C_lds));
@@ -454,7 +463,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
     if (LOCAL) {
 #pragma unroll 4
       for (int j = TS - 1; j >= 0; --j) {
-        const float dt = step_lds[j][mine].x, q = q_lds[j][mine];
+        const float dt = step_lds[j][mine].x, q = step_lds[j][mine].z;
         const float4_t Cv = C_lds[j * LANES + s0 / K];
         dt_sum += dt;
 #pragma unroll
@@ -464,52 +473,51 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
       continue;
     }
 
+    // A step's operands are read from LDS while the step before is computed, and not earlier: the registers are
+    // taken by the tile's decays and states.
+    struct { float4_t dt_u_q, B, C; } now, next;
+    auto read = [&](auto& to, int j) {
+      to.dt_u_q = step_lds[j][mine];
+      to.B = B_lds[j * LANES + s0 / K];
+      to.C = C_lds[j * LANES + s0 / K];
+    };
     float a[TS][K], before[TS][K];  // the decays and the states before the steps
+    read(now, 0);
 #pragma unroll
     for (int j = 0; j < TS; ++j) {
-      const float2_t dt_u = step_lds[j][mine];
-      const float q = q_lds[j][mine];
-      const float4_t Bv = B_lds[j * LANES + s0 / K], Cv = C_lds[j * LANES + s0 / K];
+      read(next, j + 1 < TS ? j + 1 : j);
       float ypre = 0.f, dCv[K];
 #pragma unroll
       for (int r = 0; r < K; ++r) {
-        a[j][r] = __builtin_amdgcn_exp2f(dt_u.x * A2[r]);
+        a[j][r] = __builtin_amdgcn_exp2f(now.dt_u_q.x * A2[r]);
         before[j][r] = start[r];
-        start[r] = a[j][r] * start[r] + dt_u.y * Bv[r];
-        ypre += start[r] * Cv[r];
-        dCv[r] = q * start[r];
+        start[r] = a[j][r] * start[r] + now.dt_u_q.y * now.B[r];
+        ypre += start[r] * now.C[r];
+        dCv[r] = now.dt_u_q.z * start[r];
       }
-      ypre = sum_states<LANES>(ypre);
-      if (s0 == 0) ypre_lds[j][mine] = ypre;
-      const float sum = sum_channels<LANES>(dCv);
-      if ((lane & (P::kLow - 1)) == 0) dC_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum;
-      __builtin_amdgcn_sched_barrier(0);  // a step's operands are not fetched steps ahead: they would take the registers
+      ypre_lds[j][mine] = sum_states<LANES>(ypre);  // (the lanes of a channel write the same, as do those of a state below)
+      dC_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum_channels<LANES>(dCv);
+      __builtin_amdgcn_sched_barrier(0);
+      now = next;
     }
 #pragma unroll
     for (int j = TS - 1; j >= 0; --j) {
-      const float2_t dt_u = step_lds[j][mine];
-      const float q = q_lds[j][mine];
-      const float4_t Bv = B_lds[j * LANES + s0 / K], Cv = C_lds[j * LANES + s0 / K];
+      if (j > 0) read(next, j - 1);
       float du = 0.f, Aw = 0.f, dBv[K];
 #pragma unroll
       for (int r = 0; r < K; ++r) {
-        const float g = q * Cv[r] + G[r];
-        dBv[r] = g * dt_u.y;
-        du += g * Bv[r];
+        const float g = now.dt_u_q.z * now.C[r] + G[r];
+        dBv[r] = g * now.dt_u_q.y;
+        du += g * now.B[r];
         G[r] = g * a[j][r];
         const float w = G[r] * before[j][r];
         Aw += w * A[r];
-        dA[r] += w * dt_u.x;
+        dA[r] += w * now.dt_u_q.x;
       }
-      du = sum_states<LANES>(du);
-      Aw = sum_states<LANES>(Aw);
-      if (s0 == 0) {
-        du_lds[j][mine] = du;
-        Aw_lds[j][mine] = Aw;
-      }
-      const float sum = sum_channels<LANES>(dBv);
-      if ((lane & (P::kLow - 1)) == 0) dB_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum;
+      du_Aw_lds[j][mine] = float2_t{sum_states<LANES>(du), sum_states<LANES>(Aw)};
+      dB_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum_channels<LANES>(dBv);
       __builtin_amdgcn_sched_barrier(0);
+      now = next;
     }
     __syncthreads();
 
@@ -521,9 +529,9 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
 #pragma unroll
       for (int e = 0; e < L::WIDTH; ++e) {
         const float xv = x_now.get(i, e), raw = delta_now.get(i, e) + bias[e], upv = up_now.get(i, e);
-        const float dt = step_lds[row][column + e].x, q = q_lds[row][column + e], du = du_lds[row][column + e];
+        const float dt = step_lds[row][column + e].x, q = step_lds[row][column + e].z, du = du_Aw_lds[row][column + e].x;
         dxo[e] = dt * du + skip[e] * q;
-        ddo[e] = xv * du + Aw_lds[row][column + e];
+        ddo[e] = xv * du + du_Aw_lds[row][column + e].y;
         if (s.softplus) ddo[e] *= sigmoid_of(raw);
         dskip[e] += q * xv;
         dbias[e] += ddo[e];
@@ -567,9 +575,9 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
     store_states(partial + (size_t)d * s.S, s0, s.S, dA);
   }
   // the threads of a column add theirs in order
-  static_assert(256 * L::WIDTH <= TS * P::kBlock, "a row a thread of the column fits q_lds, and step_lds");
-  float(*skip_sums)[P::kBlock] = q_lds;
-  float(*bias_sums)[P::kBlock] = reinterpret_cast<float(*)[P::kBlock]>(&step_lds[0][0]);
+  static_assert(256 * L::WIDTH <= TS * P::kBlock, "a row a thread of the column fits ypre_lds, and du_Aw_lds");
+  float(*skip_sums)[P::kBlock] = ypre_lds;
+  float(*bias_sums)[P::kBlock] = reinterpret_cast<float(*)[P::kBlock]>(&du_Aw_lds[0][0]);
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < L::WIDTH; ++e) {
