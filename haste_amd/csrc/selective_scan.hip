@@ -56,7 +56,22 @@ __device__ __forceinline__ float log1p_of(float e) {
   return d == 0.f ? e : l * (e * __builtin_amdgcn_rcpf(d));
 }
 __device__ __forceinline__ float softplus_of(float v) { return fmaxf(v, 0.f) + log1p_of(exp_of(-fabsf(v))); }
-__device__ __forceinline__ float step_size(float raw, int softplus) { return softplus ? softplus_of(raw) : raw; }
+// The same with its derivative, sigmoid(v).
+__device__ __forceinline__ float softplus_of(float v, float* slope) {
+  const float e = exp_of(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
+  *slope = v >= 0.f ? r : e * r;
+  return fmaxf(v, 0.f) + log1p_of(e);
+}
+// Chosen, not branched to, like everything between the steps of a scan: a branch would part it from them.
+__device__ __forceinline__ float step_size(float raw, int softplus, bool inside) {
+  const float soft = softplus_of(raw), dt = softplus ? soft : raw;
+  return inside ? dt : 0.f;
+}
+__device__ __forceinline__ float step_size(float raw, int softplus, bool inside, float* slope) {
+  const float soft = softplus_of(raw, slope), dt = softplus ? soft : raw;
+  *slope = softplus ? *slope : 1.0f;
+  return inside ? dt : 0.f;
+}
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
@@ -146,47 +161,92 @@ struct Tile {
   static __device__ __forceinline__ int column() { return (threadIdx.x % kPerRow) * WIDTH; }
 };
 
-// The elements of one tensor's tile, packed in the tensor's own type while the tile before is worked on.
+// The elements of one tensor's tile, packed in the tensor's own type until they are worked on.
 template <typename T, int LANES>
 struct Held {
   typedef Tile<LANES> L;
   typedef T packed_t __attribute__((ext_vector_type(L::WIDTH)));
   packed_t v[L::ITEMS];
-  __device__ __forceinline__ void load(const Rows<const T>& rows, int t0, int end, const Block<LANES>& b) {
+  __device__ __forceinline__ float get(int i, int e) const { return (float)v[i][e]; }
+};
+
+// This thread's way through a tensor, tile by tile.
+template <typename T, int LANES>
+struct Walk {
+  typedef Tile<LANES> L;
+  T* p;         // of the tile's first row here
+  size_t step;  // elements between steps
+  __device__ __forceinline__ Walk(const Rows<T>& rows, int t0, const Block<LANES>& b)
+      : p(rows.p == nullptr ? nullptr : rows.at(t0, b.n) + (size_t)L::row(0) * rows.step + b.c0 + L::column()), step(rows.step) {}
+  __device__ __forceinline__ void forth() { p += TS * step; }
+  __device__ __forceinline__ void back() { p -= TS * step; }
+  // `rows` of the tile belong to the sequence; whole: all of them do, and all channels to the group
+  template <typename U>
+  __device__ __forceinline__ void load(Held<U, LANES>& to, bool whole, int rows, const Block<LANES>& b) const {
+    typedef typename Wide<U, L::WIDTH>::type wide_t;
 #pragma unroll
     for (int i = 0; i < L::ITEMS; ++i) {
-      const int t = t0 + L::row(i), c = b.c0 + L::column();
-      packed_t w = {};
-      if (t < end && c + L::WIDTH <= b.c_end) {
-        w = *reinterpret_cast<const typename Wide<T, L::WIDTH>::type*>(rows.at(t, b.n) + c);
-      } else if (t < end) {
+      const T* from = p + (size_t)(i * L::kRowStep) * step;
+      if (whole) {
+        to.v[i] = *reinterpret_cast<const wide_t*>(from);
+      } else {
+        typename Held<U, LANES>::packed_t w = {};
+        if (L::row(i) < rows) {
 #pragma unroll
-        for (int e = 0; e < L::WIDTH; ++e)
-          if (c + e < b.c_end) w[e] = rows.at(t, b.n)[c + e];
+          for (int e = 0; e < L::WIDTH; ++e)
+            if (b.c0 + L::column() + e < b.c_end) w[e] = from[e];
+        }
+        to.v[i] = w;
       }
-      v[i] = w;
     }
   }
-  __device__ __forceinline__ float get(int i, int e) const { return (float)v[i][e]; }
+  __device__ __forceinline__ void store(const float (&f)[L::ITEMS][L::WIDTH], bool whole, int rows, const Block<LANES>& b) const {
+    typedef typename Wide<T, L::WIDTH>::type wide_t;
+#pragma unroll
+    for (int i = 0; i < L::ITEMS; ++i) {
+      T* to = p + (size_t)(i * L::kRowStep) * step;
+      if (whole) {
+        wide_t w;
+#pragma unroll
+        for (int e = 0; e < L::WIDTH; ++e) w[e] = (T)f[i][e];
+        *reinterpret_cast<wide_t*>(to) = w;
+      } else if (L::row(i) < rows) {
+#pragma unroll
+        for (int e = 0; e < L::WIDTH; ++e)
+          if (b.c0 + L::column() + e < b.c_end) to[e] = (T)f[i][e];
+      }
+    }
+  }
 };
 
 // The tile of B or C: [TS][LANES * K], states beyond S and steps beyond the row's end 0.
 template <typename T, int LANES>
 struct HeldShared {
-  T v[Tile<LANES>::kShared];
-  __device__ __forceinline__ void load(const Rows<const T>& rows, int t0, int end, const Block<LANES>& b, int S) {
+  typedef Tile<LANES> L;
+  T v[L::kShared];
+  static __device__ __forceinline__ int row(int i) { return (i * 256 + threadIdx.x) / (LANES * K); }
+  static __device__ __forceinline__ int state() { return threadIdx.x % (LANES * K); }  // of every i: 256 is a multiple
+  __device__ __forceinline__ void put(float4_t* lds) const {
 #pragma unroll
-    for (int i = 0; i < Tile<LANES>::kShared; ++i) {
-      const int e = i * 256 + threadIdx.x, t = t0 + e / (LANES * K), s = e % (LANES * K);
-      v[i] = e < TS * LANES * K && t < end && s < S ? rows.at(t, b.n)[(size_t)b.g * S + s] : (T)0.f;
-    }
+    for (int i = 0; i < L::kShared; ++i)
+      if (L::kShared * 256 == TS * LANES * K || i * 256 + (int)threadIdx.x < TS * LANES * K)
+        reinterpret_cast<float*>(lds)[i * 256 + threadIdx.x] = (float)v[i];
   }
-  __device__ __forceinline__ void put(float* lds) const {
+};
+template <typename T, int LANES>
+struct WalkShared {
+  typedef HeldShared<T, LANES> H;
+  const T* p;
+  size_t step;
+  int S;
+  __device__ __forceinline__ WalkShared(const Rows<const T>& rows, int t0, const Block<LANES>& b, int S)
+      : p(rows.at(t0, b.n) + (size_t)H::row(0) * rows.step + (size_t)b.g * S + H::state()), step(rows.step), S(S) {}
+  __device__ __forceinline__ void forth() { p += TS * step; }
+  __device__ __forceinline__ void back() { p -= TS * step; }
+  __device__ __forceinline__ void load(H& to, int rows) const {
 #pragma unroll
-    for (int i = 0; i < Tile<LANES>::kShared; ++i) {
-      const int e = i * 256 + threadIdx.x;
-      if (e < TS * LANES * K) lds[e] = (float)v[i];
-    }
+    for (int i = 0; i < H::L::kShared; ++i)
+      to.v[i] = H::row(i) < (rows < TS ? rows : TS) && H::state() < S ? p[(size_t)(i * 256 / (LANES * K)) * step] : (T)0.f;
   }
 };
 
@@ -200,9 +260,9 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
                                    float* __restrict__ h_last) {
   typedef Place<LANES> P;
   typedef Tile<LANES> L;
-  __shared__ float2_t step_lds[TS][P::kBlock];  // dt, dt x
-  __shared__ float4_t B_lds[TS * LANES], C_lds[LOCAL ? 1 : TS * LANES];
-  __shared__ float y_lds[LOCAL ? 1 : TS][P::kBlock];
+  __shared__ float2_t step_lds[2][TS][P::kBlock];  // dt, dt x
+  __shared__ float4_t B_lds[2][TS * LANES], C_lds[2][LOCAL ? 1 : TS * LANES];
+  __shared__ float y_lds[2][LOCAL ? 1 : TS][P::kBlock];
 
   const Block<LANES> b(s, blockIdx.x);
   const int t0 = blockIdx.y * s.chunk, t1 = min(s.T, t0 + s.chunk);
@@ -232,46 +292,81 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
   if (in.bias != nullptr) load_channels<L::WIDTH>(in.bias, b.c0 + L::column(), b.c_end, bias);
   if (!LOCAL && in.skip != nullptr) load_channels<L::WIDTH>(in.skip, b.c0 + L::column(), b.c_end, skip);
 
-  Held<T, LANES> x, delta, z;
-  HeldShared<T, LANES> Bt, Ct;
-  auto fetch = [&](int t) {
-    x.load(in.x, t, end, b);
-    delta.load(in.delta, t, end, b);
-    if (!LOCAL && in.z.p != nullptr) z.load(in.z, t, end, b);
-    Bt.load(in.B, t, end, b, s.S);
-    if (!LOCAL) Ct.load(in.C, t, end, b, s.S);
+  // While a tile is scanned, the next one's elements are worked out between its steps, into the other half of LDS, and the one
+  // after that is on its way from memory.
+  struct Raw {
+    Held<T, LANES> x, delta, z;
+    HeldShared<T, LANES> B, C;
+  } raw = {}, coming = {};
+  Walk<const T, LANES> x_walk(in.x, t0, b), delta_walk(in.delta, t0, b), z_walk(in.z, t0, b);
+  WalkShared<T, LANES> B_walk(in.B, t0, b, s.S), C_walk(in.C, t0, b, s.S);
+  Walk<T, LANES> y_walk(packed_rows(y, s.N, s.D), t0, b);
+  const bool all_channels = b.c0 + P::kBlock <= b.c_end, gated = !LOCAL && in.z.p != nullptr;
+  auto fetch = [&](Raw& to, int t) {  // the next tile of every walk, which starts at t
+    const int rows = end - t;
+    if (rows <= 0) return;
+    const bool whole = all_channels && rows >= TS;
+    x_walk.load(to.x, whole, rows, b);
+    delta_walk.load(to.delta, whole, rows, b);
+    if (gated) z_walk.load(to.z, whole, rows, b);
+    B_walk.load(to.B, rows);
+    if (!LOCAL) C_walk.load(to.C, rows);
+    x_walk.forth();
+    delta_walk.forth();
+    if (gated) z_walk.forth();
+    B_walk.forth();
+    if (!LOCAL) C_walk.forth();
   };
-  if (t0 < end) fetch(t0);
-  for (int t = t0; t < end; t += TS) {
-    float xs[L::ITEMS][L::WIDTH], gate[L::ITEMS][L::WIDTH];
+  struct Rest {  // what the outputs need besides the states
+    float skipped[L::ITEMS][L::WIDTH], gate[L::ITEMS][L::WIDTH];
+  } before, rest, rest_next;  // of the tile before, this one and the next
+  constexpr int kEach = L::ITEMS * L::WIDTH;
+  auto work_out = [&](const Raw& from, int t, int half, int element, Rest& to) {
+    const int i = element / L::WIDTH, e = element % L::WIDTH;
+    const float xv = from.x.get(i, e);
+    const float dt = step_size(from.delta.get(i, e) + bias[e], s.softplus, t + L::row(i) < end);
+    step_lds[half][L::row(i)][L::column() + e] = float2_t{dt, dt * xv};
+    if (LOCAL) return;
+    to.skipped[i][e] = skip[e] * xv;
+    const float zv = from.z.get(i, e), silu = zv * sigmoid_of(zv);
+    to.gate[i][e] = gated ? silu : 1.f;
+  };
+  auto put_out = [&](int half, bool whole, int rows) {
+    float o[L::ITEMS][L::WIDTH];
 #pragma unroll
-    for (int i = 0; i < L::ITEMS; ++i) {
-      const bool inside = t + L::row(i) < end;
+    for (int i = 0; i < L::ITEMS; ++i)
 #pragma unroll
-      for (int e = 0; e < L::WIDTH; ++e) {
-        xs[i][e] = x.get(i, e);
-        const float dt = inside ? step_size(delta.get(i, e) + bias[e], s.softplus) : 0.f;
-        step_lds[L::row(i)][L::column() + e] = float2_t{dt, dt * xs[i][e]};
-        if (!LOCAL) {
-          gate[i][e] = 1.f;
-          if (in.z.p != nullptr) gate[i][e] = z.get(i, e) * sigmoid_of(z.get(i, e));
-        }
-      }
-    }
-    Bt.put(reinterpret_cast<float*>(B_lds));
-    if (!LOCAL) Ct.put(reinterpret_cast<float*>(C_lds));
-    if (t + TS < end) fetch(t + TS);
-    __syncthreads();
+      for (int e = 0; e < L::WIDTH; ++e)
+        o[i][e] = (y_lds[half][L::row(i)][L::column() + e] + before.skipped[i][e]) * before.gate[i][e];
+    y_walk.store(o, whole, rows, b);
+  };
 
+  if (t0 < end) {
+    fetch(raw, t0);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) work_out(raw, t0, 0, e, rest);
+    raw.B.put(B_lds[0]);
+    if (!LOCAL) raw.C.put(C_lds[0]);
+    fetch(raw, t0 + TS);
+  }
+  int half = 0;
+  for (int t = t0; t < end; t += TS, half ^= 1) {
+    fetch(coming, t + 2 * TS);
+    __syncthreads();
+    if (!LOCAL && t > t0) {  // the tile before
+      put_out(half ^ 1, all_channels, TS);
+      y_walk.forth();
+    }
+    before = rest;
     if (!LOCAL && kept != nullptr && live) store_states(kept + (size_t)(t / TS) * states + state, s0, s.S, h);
     // a pair of steps' operands are read from LDS while the pair before is computed
     struct { float2_t dt_u[2]; float4_t B[2], C[2]; } now, next;
     auto read = [&](auto& to, int j) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        to.dt_u[i] = step_lds[j + i][mine];
-        to.B[i] = B_lds[(j + i) * LANES + s0 / K];
-        if (!LOCAL) to.C[i] = C_lds[(j + i) * LANES + s0 / K];
+        to.dt_u[i] = step_lds[half][j + i][mine];
+        to.B[i] = B_lds[half][(j + i) * LANES + s0 / K];
+        if (!LOCAL) to.C[i] = C_lds[half][(j + i) * LANES + s0 / K];
       }
     };
     read(now, 0);
@@ -288,24 +383,22 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
           if (!LOCAL) ys += h[r] * now.C[i][r];
         }
         if (LOCAL) dt_sum += now.dt_u[i].x;
-        else y_lds[j + i][mine] = sum_states<LANES>(ys);  // (the lanes of a channel write the same)
+        else y_lds[half][j + i][mine] = sum_states<LANES>(ys);  // (the lanes of a channel write the same)
       }
+#pragma unroll
+      for (int e = j * kEach / TS; e < (j + 2) * kEach / TS; ++e) work_out(raw, t + TS, half ^ 1, e, rest_next);
       __builtin_amdgcn_sched_barrier(0);
       now = next;
     }
+    raw.B.put(B_lds[half ^ 1]);
+    if (!LOCAL) raw.C.put(C_lds[half ^ 1]);
+    raw = coming;
+    rest = rest_next;
+  }
+  if (!LOCAL && t0 < end) {
     __syncthreads();
-
-    if (!LOCAL) {
-#pragma unroll
-      for (int i = 0; i < L::ITEMS; ++i) {
-        if (t + L::row(i) >= end) continue;
-        float o[L::WIDTH];
-#pragma unroll
-        for (int e = 0; e < L::WIDTH; ++e)
-          o[e] = (y_lds[L::row(i)][L::column() + e] + skip[e] * xs[i][e]) * gate[i][e];
-        store_channels<L::WIDTH>(y + ((size_t)(t + L::row(i)) * s.N + b.n) * s.D, b.c0 + L::column(), b.c_end, o);
-      }
-    }
+    const int rows = (end - t0 - 1) % TS + 1;
+    put_out(half ^ 1, all_channels && rows == TS, rows);
   }
 
   if (LOCAL) {
@@ -368,7 +461,8 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
                                     ScanGradients<T> out) {
   typedef Place<LANES> P;
   typedef Tile<LANES> L;
-  __shared__ float4_t step_lds[TS][P::kBlock];  // dt, dt x, q = dy silu(z)
+  __shared__ float4_t step_lds[TS][P::kBlock];                // dt, dt x, q = dy silu(z), d dt / d delta
+  __shared__ float2_t rest_lds[LOCAL ? 1 : TS][P::kBlock];    // x, dy silu'(z)
   __shared__ float4_t C_lds[TS * LANES], B_lds[LOCAL ? 1 : TS * LANES];
   __shared__ float ypre_lds[LOCAL ? 1 : TS][P::kBlock];
   __shared__ float2_t du_Aw_lds[LOCAL ? 1 : TS][P::kBlock];
@@ -422,39 +516,58 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
     }
   }
 
-  Held<T, LANES> x, delta, z, up;
+  const int last = t0 < end ? t0 + (end - 1 - t0) / TS * TS : t0 - TS;  // the last tile
+  Held<T, LANES> x = {}, delta = {}, z = {}, up = {};
   HeldShared<T, LANES> Bt, Ct;
+  const int from = max(last, t0);
+  Walk<const T, LANES> x_walk(in.x, from, b), delta_walk(in.delta, from, b), z_walk(in.z, from, b), up_walk(dy, from, b);
+  WalkShared<T, LANES> B_walk(in.B, from, b, s.S), C_walk(in.C, from, b, s.S);
+  Walk<T, LANES> dx_walk(packed_rows(out.dx, s.N, s.D), from, b), ddelta_walk(packed_rows(out.ddelta, s.N, s.D), from, b);
+  Walk<T, LANES> dz_walk(packed_rows(out.dz, s.N, s.D), from, b);
+  const bool all_channels = b.c0 + P::kBlock <= b.c_end, gated = in.z.p != nullptr;
   float start[K], start_next[K];
-  auto fetch = [&](int t) {
-    if (!LOCAL) x.load(in.x, t, end, b);
-    delta.load(in.delta, t, end, b);
-    if (in.z.p != nullptr) z.load(in.z, t, end, b);
-    up.load(dy, t, end, b);
-    Ct.load(in.C, t, end, b, s.S);
+  auto fetch = [&](int t) {  // the tile of every walk, which starts at t
+    const int rows = end - t;
+    const bool whole = all_channels && rows >= TS;
     if (!LOCAL) {
-      Bt.load(in.B, t, end, b, s.S);
+      x_walk.load(x, whole, rows, b);
+      x_walk.back();
+    }
+    delta_walk.load(delta, whole, rows, b);
+    delta_walk.back();
+    if (gated) {
+      z_walk.load(z, whole, rows, b);
+      z_walk.back();
+    }
+    up_walk.load(up, whole, rows, b);
+    up_walk.back();
+    C_walk.load(Ct, rows);
+    C_walk.back();
+    if (!LOCAL) {
+      B_walk.load(Bt, rows);
+      B_walk.back();
       if (live) load_states(kept + (size_t)(t / TS) * states + state, s0, s.S, start_next);
     }
   };
 #pragma unroll
   for (int r = 0; r < K; ++r) start[r] = start_next[r] = 0.f;
-  const int last = t0 < end ? t0 + (end - 1 - t0) / TS * TS : t0 - TS;  // the last tile
   if (last >= t0) fetch(last);
   for (int t = last; t >= t0; t -= TS) {
-    Held<T, LANES> x_now = x, delta_now = delta, z_now = z, up_now = up;
 #pragma unroll
     for (int i = 0; i < L::ITEMS; ++i) {
       const bool inside = t + L::row(i) < end;
 #pragma unroll
       for (int e = 0; e < L::WIDTH; ++e) {
-        const float dt = inside ? step_size(delta.get(i, e) + bias[e], s.softplus) : 0.f;
-        float q = up.get(i, e);
-        if (in.z.p != nullptr) q *= z.get(i, e) * sigmoid_of(z.get(i, e));
-        step_lds[L::row(i)][column + e] = float4_t{dt, LOCAL ? 0.f : dt * x.get(i, e), q, 0.f};
+        const float xv = x.get(i, e), zv = z.get(i, e), upv = up.get(i, e), sz = sigmoid_of(zv);
+        float slope;
+        const float dt = step_size(delta.get(i, e) + bias[e], s.softplus, inside, &slope);
+        const float q = gated ? upv * (zv * sz) : upv;
+        step_lds[L::row(i)][column + e] = float4_t{dt, dt * xv, q, slope};
+        if (!LOCAL) rest_lds[L::row(i)][column + e] = float2_t{xv, upv * silu_slope(zv, sz)};
       }
     }
-    Ct.put(reinterpret_cast<float*>(C_lds));
-    if (!LOCAL) Bt.put(reinterpret_cast<float*>(B_lds));
+    Ct.put(C_lds);
+    if (!LOCAL) Bt.put(B_lds);
 #pragma unroll
     for (int r = 0; r < K; ++r) start[r] = start_next[r];
     if (t - TS >= t0) fetch(t - TS);
@@ -521,30 +634,29 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
     }
     __syncthreads();
 
+    float dxo[L::ITEMS][L::WIDTH], ddo[L::ITEMS][L::WIDTH], dzo[L::ITEMS][L::WIDTH];
 #pragma unroll
     for (int i = 0; i < L::ITEMS; ++i) {
       const int row = L::row(i);
-      if (t + row >= end) continue;
-      float dxo[L::WIDTH], ddo[L::WIDTH], dzo[L::WIDTH];
 #pragma unroll
       for (int e = 0; e < L::WIDTH; ++e) {
-        const float xv = x_now.get(i, e), raw = delta_now.get(i, e) + bias[e], upv = up_now.get(i, e);
-        const float dt = step_lds[row][column + e].x, q = step_lds[row][column + e].z, du = du_Aw_lds[row][column + e].x;
-        dxo[e] = dt * du + skip[e] * q;
-        ddo[e] = xv * du + du_Aw_lds[row][column + e].y;
-        if (s.softplus) ddo[e] *= sigmoid_of(raw);
-        dskip[e] += q * xv;
-        dbias[e] += ddo[e];
-        if (in.z.p != nullptr) {
-          const float zv = z_now.get(i, e);
-          dzo[e] = upv * (ypre_lds[row][column + e] + skip[e] * xv) * silu_slope(zv, sigmoid_of(zv));
-        }
+        const float4_t st = step_lds[row][column + e];
+        const float2_t rest = rest_lds[row][column + e], du_Aw = du_Aw_lds[row][column + e];
+        // (behind the row's end dt, x and q are 0: nothing is added to the sums)
+        dxo[i][e] = st.x * du_Aw.x + skip[e] * st.z;
+        ddo[i][e] = (rest.x * du_Aw.x + du_Aw.y) * st.w;
+        dzo[i][e] = rest.y * (ypre_lds[row][column + e] + skip[e] * rest.x);
+        dskip[e] += st.z * rest.x;
+        dbias[e] += t + row < end ? ddo[i][e] : 0.f;
       }
-      const size_t at = ((size_t)(t + row) * s.N + b.n) * s.D;
-      store_channels<L::WIDTH>(out.dx + at, b.c0 + column, b.c_end, dxo);
-      store_channels<L::WIDTH>(out.ddelta + at, b.c0 + column, b.c_end, ddo);
-      if (out.dz != nullptr) store_channels<L::WIDTH>(out.dz + at, b.c0 + column, b.c_end, dzo);
     }
+    const bool whole = all_channels && end - t >= TS;
+    dx_walk.store(dxo, whole, end - t, b);
+    ddelta_walk.store(ddo, whole, end - t, b);
+    if (gated) dz_walk.store(dzo, whole, end - t, b);
+    dx_walk.back();
+    ddelta_walk.back();
+    dz_walk.back();
     const size_t part = (size_t)(blockIdx.x % s.blocks_group) * s.T;
     for (int e = threadIdx.x; e < TS * LANES * K; e += 256) {
       const int j = e / (LANES * K), st = e % (LANES * K);
@@ -626,7 +738,7 @@ void selective_scan_step_kernel(ScanShape s, ScanInputs<T> in, const float* h, f
   load_channels<K>(in.B.at(0, n) + (size_t)g * s.S, s0, s.S, Bv);
   load_channels<K>(in.C.at(0, n) + (size_t)g * s.S, s0, s.S, Cv);
   const float x = (float)in.x.at(0, n)[d];
-  const float dt = step_size((float)in.delta.at(0, n)[d] + (in.bias != nullptr ? in.bias[d] : 0.f), s.softplus);
+  const float dt = step_size((float)in.delta.at(0, n)[d] + (in.bias != nullptr ? in.bias[d] : 0.f), s.softplus, true);
   float sum = 0.f;
 #pragma unroll
   for (int r = 0; r < K; ++r) {
