@@ -42,25 +42,32 @@ struct Share {
   static constexpr int V = 16 / sizeof(T) < EACH ? 16 / sizeof(T) : EACH;
   static constexpr int kPieces = EACH / V;
   static __device__ __forceinline__ int column(int piece, int thread) { return (piece * THREADS + thread) * V; }
+  static __device__ __forceinline__ int column_of(int i, int thread) { return column(i / V, thread) + i % V; }
 };
 
-template <typename T, int THREADS, typename U>
-__device__ __forceinline__ void load_share(const U* row, int thread, int D, float (&f)[EACH]) {
+// They in the tensor's own type, as they are fetched a row ahead; those beyond the row 0.
+template <typename T, int THREADS>
+struct Held {
   typedef Share<T, THREADS> S;
+  typedef T packed_t __attribute__((ext_vector_type(S::V)));
+  packed_t v[S::kPieces];
+  __device__ __forceinline__ void load(const T* row, int thread, int D) {
 #pragma unroll
-  for (int p = 0; p < S::kPieces; ++p) {
-    float v[S::V];
-    const int c = S::column(p, thread);
-    if (c < D) {
-      load_channels<S::V>(row, c, D, v);
-    } else {
+    for (int p = 0; p < S::kPieces; ++p) {
+      const int c = S::column(p, thread);
+      packed_t w = {};
+      if (c + S::V <= D) {
+        w = *reinterpret_cast<const typename Wide<T, S::V>::type*>(row + c);
+      } else {
 #pragma unroll
-      for (int i = 0; i < S::V; ++i) v[i] = 0.f;
+        for (int i = 0; i < S::V; ++i)
+          if (c + i < D) w[i] = row[c + i];
+      }
+      v[p] = w;
     }
-#pragma unroll
-    for (int i = 0; i < S::V; ++i) f[p * S::V + i] = v[i];
   }
-}
+  __device__ __forceinline__ float get(int i) const { return (float)v[i / S::V][i % S::V]; }
+};
 
 template <typename T, int THREADS, typename U>
 __device__ __forceinline__ void store_share(U* row, int thread, int D, const float (&f)[EACH]) {
@@ -75,23 +82,13 @@ __device__ __forceinline__ void store_share(U* row, int thread, int D, const flo
   }
 }
 
+// A weight's elements, 0 beyond the row; a weight that is absent is `otherwise` everywhere.
 template <typename T, int THREADS>
 __device__ __forceinline__ void load_or(const float* weights, float otherwise, int thread, int D, float (&f)[EACH]) {
-  if (weights != nullptr) {
-    load_share<T, THREADS>(weights, thread, D, f);
-  } else {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) f[i] = otherwise;
-  }
-}
-
-template <int THREADS, typename T>
-__device__ __forceinline__ void load_or_zero(const Rows<const T>& rows, int t, int n, int thread, int D, float (&f)[EACH]) {
-  if (rows.p != nullptr) {
-    load_share<T, THREADS>(rows.at(t, n), thread, D, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) f[i] = 0.f;
+  for (int i = 0; i < EACH; ++i) {
+    const int c = Share<T, THREADS>::column_of(i, thread);
+    f[i] = weights == nullptr ? otherwise : c < D ? weights[c] : 0.f;
   }
 }
 
@@ -125,7 +122,7 @@ template <typename T, int THREADS>
 __device__ __forceinline__ float2 statistics(RowSums<THREADS>& sums, const float (&v)[EACH], const NormShape& s, int thread) {
   typedef Share<T, THREADS> S;
   float mean = 0.f, unused = 0.f;
-  auto inside = [&](int i) { return S::column(i / S::V, thread) + i % S::V < s.D; };
+  auto inside = [&](int i) { return S::column_of(i, thread) < s.D; };
   if (s.centered) {
 #pragma unroll
     for (int i = 0; i < EACH; ++i) mean += inside(i) ? v[i] : 0.f;
@@ -163,22 +160,36 @@ void residual_norm_forward_kernel(NormShape s, NormInputs<T> in, T* __restrict__
   load_or<T, THREADS>(in.before, 1.f, thread, s.D, before);
   load_or<T, THREADS>(in.before_bias, 0.f, thread, s.D, before_bias);
 
+  struct Raw {
+    Held<T, THREADS> update, gate, residual;
+  } coming = {};
+  const bool gated = in.gate.p != nullptr, added = in.residual.p != nullptr;
+  const size_t stride = (size_t)gridDim.x * L::kRows;
+  auto fetch = [&](size_t row) {
+    if (row >= rows) return;
+    const int t = (int)((unsigned)row / (unsigned)s.N), n = (int)((unsigned)row % (unsigned)s.N);
+    coming.update.load(in.update.at(t, n), thread, s.D);
+    if (gated) coming.gate.load(in.gate.at(t, n), thread, s.D);
+    if (added) coming.residual.load(in.residual.at(t, n), thread, s.D);
+  };
+  fetch((size_t)blockIdx.x * L::kRows + group);
   // every thread of the workgroup takes part in all turns: there are barriers in them
-  for (size_t first = (size_t)blockIdx.x * L::kRows; first < rows; first += (size_t)gridDim.x * L::kRows) {
+  for (size_t first = (size_t)blockIdx.x * L::kRows; first < rows; first += stride) {
     const size_t row = first + group;
     const bool live = row < rows;
-    const int t = live ? (int)(row / s.N) : 0, n = live ? (int)(row % s.N) : 0;
-    float v[EACH], gate[EACH], o[EACH];
-    load_share<T, THREADS>(in.update.at(t, n), thread, s.D, v);
-    if (in.gate.p != nullptr) load_share<T, THREADS>(in.gate.at(t, n), thread, s.D, gate);
-    if (in.residual.p != nullptr) load_share<T, THREADS>(in.residual.at(t, n), thread, s.D, o);
+    float v[EACH], o[EACH];
+    const Raw now = coming;
+    fetch(row + stride);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) v[i] = now.update.get(i);
     float2 first_stats = make_float2(0.f, 1.f), second_stats = make_float2(0.f, 1.f);
     if (in.after != nullptr) first_stats = statistics<T, THREADS>(sums, v, s, thread);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       float p = (v[i] - first_stats.x) * first_stats.y * after[i] * scale[i];
-      if (in.gate.p != nullptr) p *= gate[i] * sigmoid_of(gate[i]);
-      o[i] = in.residual.p != nullptr ? o[i] + p : p;
+      const float gate = now.gate.get(i), silu = gate * sigmoid_of(gate);
+      p = gated ? p * silu : p;
+      o[i] = added ? now.residual.get(i) + p : p;
     }
     if (live) store_share<T, THREADS>(out + row * s.D, thread, s.D, o);
     if (in.before != nullptr) {
@@ -195,10 +206,11 @@ void residual_norm_forward_kernel(NormShape s, NormInputs<T> in, T* __restrict__
 template <typename T>
 struct NormGradients {
   T *update, *residual, *gate;  // the latter two may be null
-  float* partial;               // [groups of rows][kSums][D]
+  float* partial;               // [groups of rows][kSums, or kSums - 1 without dbias][D]
 };
 
-template <typename T, int THREADS>
+// BIAS: whether the gradient of before_bias is wanted; its sums would take registers.
+template <typename T, int THREADS, bool BIAS>
 __global__ __launch_bounds__(Launch<THREADS>::kBlock)
 void residual_norm_backward_kernel(NormShape s, NormInputs<T> in, const float* __restrict__ stats, Rows<const T> dout,
                                    Rows<const T> dnormed, NormGradients<T> to) {
@@ -208,64 +220,87 @@ void residual_norm_backward_kernel(NormShape s, NormInputs<T> in, const float* _
   const int thread = threadIdx.x % THREADS, group = threadIdx.x / THREADS;
   RowSums<THREADS> sums = {lds[group], 0};
   const size_t rows = (size_t)s.T * s.N;
+  // A workgroup of 1024 threads has 128 registers a thread: the sums over its rows lie in LDS, and rows are not fetched ahead.
+  constexpr bool kAhead = THREADS < 1024;
+  constexpr int kWanted = BIAS ? kSums : kSums - 1;
+  __shared__ float sums_lds[kAhead ? 1 : kWanted][kAhead ? 1 : EACH][kAhead ? 1 : THREADS];
   float scale[EACH], after[EACH], before[EACH];
   load_or<T, THREADS>(in.scale, 1.f, thread, s.D, scale);
   load_or<T, THREADS>(in.after, 1.f, thread, s.D, after);
   load_or<T, THREADS>(in.before, 1.f, thread, s.D, before);
-  float dscale[EACH], dafter[EACH], dbefore[EACH], dbias[EACH];
+  float over_rows[kAhead ? kWanted : 1][EACH];  // dscale, dafter, dbefore, dbias
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) dscale[i] = dafter[i] = dbefore[i] = dbias[i] = 0.f;
+  for (int k = 0; k < kWanted; ++k)
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (kAhead) over_rows[kAhead ? k : 0][i] = 0.f;
+      else sums_lds[kAhead ? 0 : k][kAhead ? 0 : i][kAhead ? 0 : thread] = 0.f;
+    }
+  auto add = [&](int k, int i, float v) {
+    if (kAhead) over_rows[kAhead ? k : 0][i] += v;
+    else sums_lds[kAhead ? 0 : k][kAhead ? 0 : i][kAhead ? 0 : thread] += v;
+  };
 
-  for (size_t first = (size_t)blockIdx.x * L::kRows; first < rows; first += (size_t)gridDim.x * L::kRows) {
+  struct Raw {
+    Held<T, THREADS> update, gate, residual, dout, dnormed;
+    float4 stats;
+  } coming = {};
+  const bool gated = in.gate.p != nullptr, second = in.before != nullptr;
+  const size_t stride = (size_t)gridDim.x * L::kRows;
+  auto fetch = [&](size_t row) {
+    if (row >= rows) {  // a turn whose row is not there adds nothing
+      coming = {};
+      return;
+    }
+    const int t = (int)((unsigned)row / (unsigned)s.N), n = (int)((unsigned)row % (unsigned)s.N);
+    coming.update.load(in.update.at(t, n), thread, s.D);
+    if (gated) coming.gate.load(in.gate.at(t, n), thread, s.D);
+    if (in.residual.p != nullptr) coming.residual.load(in.residual.at(t, n), thread, s.D);
+    if (dout.p != nullptr) coming.dout.load(dout.at(t, n), thread, s.D);
+    if (dnormed.p != nullptr) coming.dnormed.load(dnormed.at(t, n), thread, s.D);
+    coming.stats = reinterpret_cast<const float4*>(stats)[row];
+  };
+  if (kAhead) fetch((size_t)blockIdx.x * L::kRows + group);
+  for (size_t first = (size_t)blockIdx.x * L::kRows; first < rows; first += stride) {
     const size_t row = first + group;
     const bool live = row < rows;
-    const int t = live ? (int)(row / s.N) : 0, n = live ? (int)(row % s.N) : 0;
-    float u[EACH], gate[EACH], o[EACH], d[EACH], e[EACH];
-    load_share<T, THREADS>(in.update.at(t, n), thread, s.D, u);
-    if (in.gate.p != nullptr) load_share<T, THREADS>(in.gate.at(t, n), thread, s.D, gate);
-    load_or_zero<THREADS>(in.residual, t, n, thread, s.D, o);
-    load_or_zero<THREADS>(dout, t, n, thread, s.D, d);
-    load_or_zero<THREADS>(dnormed, t, n, thread, s.D, e);
-    const float4 st = live ? reinterpret_cast<const float4*>(stats)[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!live) {
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) u[i] = o[i] = d[i] = e[i] = 0.f;
-    }
-    float silu[EACH];
+    if (!kAhead) fetch(row);
+    const Raw now = coming;
+    if (kAhead) fetch(row + stride);
+    float u[EACH], sigmoid[EACH], o[EACH], d[EACH];
     float along = 0.f, mean = 0.f;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      silu[i] = in.gate.p != nullptr ? gate[i] * sigmoid_of(gate[i]) : 1.f;
-      u[i] = (u[i] - st.x) * st.y;
-      if (in.before != nullptr) {
-        o[i] = (o[i] + scale[i] * (u[i] * after[i] * silu[i]) - st.z) * st.w;
-        dbefore[i] += e[i] * o[i];
-        dbias[i] += e[i];
-        e[i] *= before[i];
-        along += e[i] * o[i];
-        mean += e[i];
-      }
+      const float gate = now.gate.get(i);
+      sigmoid[i] = sigmoid_of(gate);
+      u[i] = (now.update.get(i) - now.stats.x) * now.stats.y;
+      d[i] = now.dout.get(i);
+      const float p = scale[i] * (u[i] * after[i]), e = now.dnormed.get(i);
+      o[i] = (now.residual.get(i) + (gated ? p * (gate * sigmoid[i]) : p) - now.stats.z) * now.stats.w;
+      add(2, i, e * o[i]);
+      if (BIAS) add(3, i, e);
+      along += e * before[i] * o[i];
+      mean += e * before[i];
     }
-    if (in.before != nullptr) {
+    if (second) {
       sums(along, mean);
       along /= s.D;
       mean = s.centered ? mean / s.D : 0.f;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) d[i] += (e[i] - o[i] * along - mean) * st.w;
+      for (int i = 0; i < EACH; ++i) d[i] += (now.dnormed.get(i) * before[i] - o[i] * along - mean) * now.stats.w;
     }
     if (live && to.residual != nullptr) store_share<T, THREADS>(to.residual + row * s.D, thread, s.D, d);
     along = mean = 0.f;
     float dgate[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      const bool inside = S::column(i / S::V, thread) + i % S::V < s.D;
-      const float n_i = u[i] * after[i];
-      dscale[i] += d[i] * (n_i * silu[i]);
+      const float gate = now.gate.get(i), silu = gated ? gate * sigmoid[i] : 1.f, n_i = u[i] * after[i];
+      add(0, i, d[i] * (n_i * silu));
       const float ds = d[i] * scale[i];
-      if (in.gate.p != nullptr) dgate[i] = ds * n_i * silu_slope(gate[i], sigmoid_of(gate[i]));
-      const float dn = ds * silu[i];
-      dafter[i] += dn * u[i];
-      d[i] = inside ? dn * after[i] : 0.f;
+      dgate[i] = ds * n_i * silu_slope(gate, sigmoid[i]);
+      const float dn = ds * silu;
+      add(1, i, dn * u[i]);
+      d[i] = S::column_of(i, thread) < s.D ? dn * after[i] : 0.f;
       along += d[i] * u[i];
       mean += d[i];
     }
@@ -275,15 +310,18 @@ void residual_norm_backward_kernel(NormShape s, NormInputs<T> in, const float* _
       along /= s.D;
       mean = s.centered ? mean / s.D : 0.f;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) d[i] = (d[i] - u[i] * along - mean) * st.y;
+      for (int i = 0; i < EACH; ++i) d[i] = (d[i] - u[i] * along - mean) * now.stats.y;
     }
     if (live) store_share<T, THREADS>(to.update + row * s.D, thread, s.D, d);
   }
-  float* partial = to.partial + ((size_t)blockIdx.x * L::kRows + group) * kSums * s.D;
-  store_share<T, THREADS>(partial, thread, s.D, dscale);
-  store_share<T, THREADS>(partial + s.D, thread, s.D, dafter);
-  store_share<T, THREADS>(partial + 2 * (size_t)s.D, thread, s.D, dbefore);
-  store_share<T, THREADS>(partial + 3 * (size_t)s.D, thread, s.D, dbias);
+  float* partial = to.partial + ((size_t)blockIdx.x * L::kRows + group) * kWanted * s.D;
+#pragma unroll
+  for (int k = 0; k < kWanted; ++k) {
+    float sum[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) sum[i] = kAhead ? over_rows[kAhead ? k : 0][i] : sums_lds[kAhead ? 0 : k][kAhead ? 0 : i][kAhead ? 0 : thread];
+    store_share<T, THREADS>(partial + (size_t)k * s.D, thread, s.D, sum);
+  }
 }
 
 // Threads of a row of D: the least power of two that holds it, a wavefront or more.
@@ -311,7 +349,7 @@ int workgroups(size_t rows, int D, int waves) {
   const size_t most = (rows + block / threads - 1) / (block / threads);
   return (int)(wanted > 0 && wanted < most ? wanted : most < kGridLimit ? most : kGridLimit);
 }
-constexpr int kForwardWaves = 8, kBackwardWaves = 4;
+constexpr int kForwardWaves = 4, kBackwardWaves = 2;
 
 struct NormPartials {
   int parts;
@@ -363,15 +401,18 @@ int backward_entry(int steps, int batch_size, int channels, const NormInputs<T>&
   {
     ScopedKernelTimer timer("residual_norm_backward", as_stream(stream));
     HASTE_HIP_PROPAGATE(with_threads(channels, [&](auto threads) {
-      residual_norm_backward_kernel<T, threads()><<<workgroups((size_t)steps * batch_size, channels, kBackwardWaves),
-                                                    Launch<threads()>::kBlock, 0, as_stream(stream)>>>(s, in, stats, dout, dnormed, grads);
+      const dim3 grid(workgroups((size_t)steps * batch_size, channels, kBackwardWaves)), block(Launch<threads()>::kBlock);
+      if (dbias != nullptr)
+        residual_norm_backward_kernel<T, threads(), true><<<grid, block, 0, as_stream(stream)>>>(s, in, stats, dout, dnormed, grads);
+      else
+        residual_norm_backward_kernel<T, threads(), false><<<grid, block, 0, as_stream(stream)>>>(s, in, stats, dout, dnormed, grads);
       HASTE_HIP_TRY(hipGetLastError());
       return HASTE_HIP_OK;
     }));
   }
   const size_t D = channels;
   const ColumnOutputs sums = {{dscale, dafter, dbefore, dbias}, {D, 2 * D, 3 * D, 4 * D}};
-  return column_sums(as_stream(stream), p.parts, p.columns, grads.partial, grads.partial + p.floats, sums);
+  return column_sums(as_stream(stream), p.parts, (dbias != nullptr ? kSums : kSums - 1) * D, grads.partial, grads.partial + p.floats, sums);
 }
 
 }  // namespace

@@ -73,12 +73,6 @@ __device__ __forceinline__ float step_size(float raw, int softplus, bool inside,
   return inside ? dt : 0.f;
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kRor4 = 0x124, kRor8 = 0x128;
-
 // A lane's place in a wavefront: the states are told apart by the highest of the low four bits of the
 // lane (sums over them rotate rows of 16 lanes), the channels by the rest (sums over them swap halves
 // of the wavefront, which adds two values in one go).
@@ -99,15 +93,6 @@ __device__ __forceinline__ float sum_states(float v) {
   if (LANES >= 8) v += dpp<kXor2>(v);
   if (LANES >= 16) v += dpp<kXor1>(v);
   return v;
-}
-
-__device__ __forceinline__ float swap_add_halves(float a, float b) {  // lower half: a's sum, upper: b's
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float swap_add_rows(float a, float b) {  // even rows: a's sum, odd: b's
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Sums of a lane's four values over the channels of the wavefront: row r of 16 lanes gets that of

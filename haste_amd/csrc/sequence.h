@@ -76,11 +76,28 @@ __device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_r
 // d/dx (x sigmoid(x)), s = sigmoid(x).
 __device__ __forceinline__ float silu_slope(float x, float s) { return s * (1.0f + x * (1.0f - s)); }
 
+// Adding across lanes: within rows of 16 by the data path's own permutations, across them by swaps.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kRor4 = 0x124, kRor8 = 0x128;
+__device__ __forceinline__ float swap_add_halves(float a, float b) {  // lower half: a's sum, upper: b's
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap_add_rows(float a, float b) {  // even rows: a's sum, odd: b's
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 // Sum over all 64 lanes, in every lane.
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+  v += dpp<kXor1>(v);
+  v += dpp<kXor2>(v);
+  v += dpp<kHalfMirror>(v);
+  v += dpp<kRor8>(v);
+  v = swap_add_rows(v, v);
+  return swap_add_halves(v, v);
 }
 
 // Sums over p < parts of partial[p][columns]: partials of many workgroups, added in an order that depends
