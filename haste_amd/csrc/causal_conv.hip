@@ -6,7 +6,7 @@
 //   dkernel[k] = sum_{t,n} dpre[t] X[t+k],  dbias = sum dpre.
 //
 // Bound: HBM (forward 2, backward 3 values moved for about 2W and 6W operations).  A thread owns V
-// channels of a batch row (16 bytes a load) and walks a run of `chunk` steps with the last W inputs in
+// channels of a batch row and walks a run of `chunk` steps with the last W inputs in
 // registers, so that every input is read once, but for the W-1 before (backward: after) a run.
 #include <type_traits>
 
@@ -15,13 +15,21 @@
 namespace haste_hip {
 namespace {
 
+// Channels a thread owns.  Of half tensors that is a load of 8 bytes, where 16 would take so many registers that a SIMD
+// has room for two wavefronts instead of four: T=1024 N=8 D=1024 W=4 bf16 27 us backward instead of 23, and 14 forward either way.
+constexpr int V = 4;
+
+// Steps whose elements a thread fetches while those before them are computed.  Two backward, where they are of two tensors:
+// with four a SIMD has room for three wavefronts instead of four (T=2048 N=8 D=4096 W=4 bf16: 126 us instead of 104).
+constexpr int kForwardAhead = 4, kBackwardAhead = 2;
+
 struct ConvShape {
   int T, N, D, chunk;
   int silu;
 };
 
 // X[p] for p >= 0: the state's rows, then the sequence.
-template <int V, typename T>
+template <typename T>
 __device__ __forceinline__ void load_padded(const Rows<const T>& x, const T* state, int W, int p, int n, int c,
                                             int N, int D, float (&f)[V]) {
   if (p >= W - 1) {
@@ -34,7 +42,34 @@ __device__ __forceinline__ void load_padded(const Rows<const T>& x, const T* sta
   }
 }
 
-template <typename T, int W, int V>
+// V channels of U steps, packed in the tensor's own type until they are worked on.
+template <typename T, int U>
+struct HeldSteps {
+  typedef T packed_t __attribute__((ext_vector_type(V)));
+  packed_t v[U];
+  __device__ __forceinline__ void load(const Rows<const T>& rows, int t, int end, int n, int c, int D) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      packed_t w = {};
+      if (t + u < end) {
+        const T* from = rows.at(t + u, n) + c;
+        if (c + V <= D) {
+          w = *reinterpret_cast<const typename Wide<T, V>::type*>(from);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (c + i < D) w[i] = from[i];
+        }
+      }
+      v[u] = w;
+    }
+  }
+  __device__ __forceinline__ void get(int u, float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = (float)v[u][i];
+  }
+};
+template <typename T, int W>
 __global__ __launch_bounds__(256)
 void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __restrict__ kernel,
                                 const float* __restrict__ bias, const T* state, const long long* __restrict__ lengths,
@@ -52,14 +87,14 @@ void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __res
   float win[W][V];  // X[t .. t+W-1], the last of them filled in by every step
   if (t0 < end) {
 #pragma unroll
-    for (int j = 0; j + 1 < W; ++j) load_padded<V>(x, state, W, t0 + j, n, c, N, D, win[j]);
+    for (int j = 0; j + 1 < W; ++j) load_padded(x, state, W, t0 + j, n, c, N, D, win[j]);
   }
   if (blockIdx.y == 0 && state_out != nullptr) {
     // read before any of it is written: state_out may be state (no other thread reads these: a run
     // that is not the first starts W-1 steps or more behind the state)
     float last[W > 1 ? W - 1 : 1][V];
 #pragma unroll
-    for (int j = 0; j + 1 < W; ++j) load_padded<V>(x, state, W, e.steps + j, n, c, N, D, last[j]);
+    for (int j = 0; j + 1 < W; ++j) load_padded(x, state, W, e.steps + j, n, c, N, D, last[j]);
 #pragma unroll
     for (int j = 0; j + 1 < W; ++j) {
       if (e.fill != 0.f) {  // NaN
@@ -91,22 +126,17 @@ void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __res
 #pragma unroll
         for (int v = 0; v < V; ++v) win[k][v] = win[k + 1][v];
     };
-    constexpr int U = 4;
-    int t = t0;
-    for (; t + U <= end; t += U) {
-      float in[U][V];
-#pragma unroll
-      for (int u = 0; u < U; ++u) load_channels<V>(x.at(t + u, n), c, D, in[u]);
+    constexpr int U = kForwardAhead;
+    HeldSteps<T, U> coming;
+    coming.load(x, t0, end, n, c, D);
+    for (int t = t0; t < end; t += U) {
+      const HeldSteps<T, U> now = coming;
+      if (t + U < end) coming.load(x, t + U, end, n, c, D);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) win[W - 1][v] = in[u][v];
-        step(t + u);
+        now.get(u, win[W - 1]);
+        if (t + u < end) step(t + u);
       }
-    }
-    for (; t < end; ++t) {
-      load_channels<V>(x.at(t, n), c, D, win[W - 1]);
-      step(t);
     }
   }
   float fill[V];
@@ -117,7 +147,7 @@ void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __res
 
 // A run computes dX for the steps t0 .. t1-1 of x (the first also for the state): dpre of step t goes
 // into dX[t .. t+W-1], so it needs dpre of W-1 steps behind the run too.  Step t finishes dX[t].
-template <typename T, int W, int V>
+template <typename T, int W>
 __global__ __launch_bounds__(256)
 void causal_conv_backward_kernel(ConvShape s, Rows<const T> x, const float* __restrict__ kernel,
                                  const float* __restrict__ bias, const T* __restrict__ state,
@@ -153,7 +183,7 @@ void causal_conv_backward_kernel(ConvShape s, Rows<const T> x, const float* __re
     for (int v = 0; v < V; ++v) win[k][v] = acc[k][v] = 0.f;
   if (t0 < given) {
 #pragma unroll
-    for (int j = 0; j + 1 < W; ++j) load_padded<V>(x, state, W, t0 + j, n, c, N, D, win[j]);
+    for (int j = 0; j + 1 < W; ++j) load_padded(x, state, W, t0 + j, n, c, N, D, win[j]);
   }
   auto emit = [&](int t) {  // dX[t] is complete: row t of the state, or step t-(W-1) of x
     float o[V];
@@ -203,24 +233,26 @@ void causal_conv_backward_kernel(ConvShape s, Rows<const T> x, const float* __re
     emit(t);
     shift();
   };
-  constexpr int U = 4;
+  constexpr int U = kBackwardAhead;
+  HeldSteps<T, U> x_coming, dy_coming;
+  x_coming.load(x, t0, given, n, c, D);
+  dy_coming.load(dy, t0, given, n, c, D);
   int t = t0;
-  for (; t + U <= given; t += U) {
-    float in[U][V], g[U][V];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      load_channels<V>(x.at(t + u, n), c, D, in[u]);
-      load_channels<V>(dy.at(t + u, n), c, D, g[u]);
+  for (; t < given; t += U) {
+    const HeldSteps<T, U> x_now = x_coming, dy_now = dy_coming;
+    if (t + U < given) {
+      x_coming.load(x, t + U, given, n, c, D);
+      dy_coming.load(dy, t + U, given, n, c, D);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) step(t + u, in[u], g[u]);
+    for (int u = 0; u < U; ++u) {
+      float in[V], g[V];
+      x_now.get(u, in);
+      dy_now.get(u, g);
+      if (t + u < given) step(t + u, in, g);
+    }
   }
-  for (; t < given; ++t) {
-    float in[V], g[V];
-    load_channels<V>(x.at(t, n), c, D, in);
-    load_channels<V>(dy.at(t, n), c, D, g);
-    step(t, in, g);
-  }
+  t = max(t0, given);
   for (; t < t1 + W - 1; ++t) {
     emit(t);
     shift();
@@ -231,11 +263,6 @@ void causal_conv_backward_kernel(ConvShape s, Rows<const T> x, const float* __re
   for (int k = 0; k < W; ++k) store_channels<V>(mine + (size_t)k * D, c, D, dw[k]);
   store_channels<V>(mine + (size_t)W * D, c, D, db);
 }
-
-// Channels a thread owns: 16 bytes of them, and half of that where more than four taps would not fit
-// the registers.
-template <typename T, int W>
-constexpr int channels_per_thread() { return (int)(16 / sizeof(T)) / (W > 4 && sizeof(T) < 4 ? 2 : 1); }
 
 // Steps in a run: 64, and down to 8 (the W-1 steps read twice must stay few) where that leaves fewer
 // than two wavefronts a SIMD.
@@ -251,7 +278,7 @@ struct ConvPartials {
   int parts;
   size_t columns, floats, total;
 };
-ConvPartials partials_of(int T, int N, int D, int W, int V) {
+ConvPartials partials_of(int T, int N, int D, int W) {
   ConvPartials p;
   const size_t chunk = run_length(T, (size_t)N * ((D + V - 1) / V));
   p.parts = (int)((T + chunk - 1) / chunk * N);
@@ -264,13 +291,12 @@ ConvPartials partials_of(int T, int N, int D, int W, int V) {
 template <typename T, int W>
 int forward(hipStream_t stream, ConvShape s, const Rows<const T>& x, const float* kernel, const float* bias, const T* state,
             const long long* lengths, T* y, T* state_out) {
-  constexpr int V = channels_per_thread<T, W>();
   const size_t items = (size_t)s.N * ((s.D + V - 1) / V), blocks = (items + 255) / 256;
   if (blocks > kGridLimit) return too_large("causal_conv: too many rows of channels");
   s.chunk = run_length(s.T, items);
   ScopedKernelTimer timer("causal_conv_forward", stream);
   dim3 grid((unsigned)blocks, (s.T + s.chunk - 1) / s.chunk);
-  causal_conv_forward_kernel<T, W, V><<<grid, 256, 0, stream>>>(s, x, kernel, bias, state, lengths, y, state_out);
+  causal_conv_forward_kernel<T, W><<<grid, 256, 0, stream>>>(s, x, kernel, bias, state, lengths, y, state_out);
   HASTE_HIP_TRY(hipGetLastError());
   return HASTE_HIP_OK;
 }
@@ -279,16 +305,15 @@ template <typename T, int W>
 int backward(hipStream_t stream, ConvShape s, const Rows<const T>& x, const float* kernel, const float* bias, const T* state,
              const long long* lengths, const Rows<const T>& dy, const T* dstate_out, T* dx, float* dkernel,
              float* dbias, T* dstate, float* workspace, size_t workspace_bytes) {
-  constexpr int V = channels_per_thread<T, W>();
   const size_t items = (size_t)s.N * ((s.D + V - 1) / V), blocks = (items + 255) / 256;
   if (blocks > kGridLimit) return too_large("causal_conv: too many rows of channels");
   s.chunk = run_length(s.T, items);
-  const ConvPartials p = partials_of(s.T, s.N, s.D, W, V);
+  const ConvPartials p = partials_of(s.T, s.N, s.D, W);
   if (workspace_bytes < p.total * sizeof(float)) return too_large("causal_conv_backward: the workspace is too small");
   {
     ScopedKernelTimer timer("causal_conv_backward", stream);
     dim3 grid((unsigned)blocks, (s.T + s.chunk - 1) / s.chunk);
-    causal_conv_backward_kernel<T, W, V><<<grid, 256, 0, stream>>>(s, x, kernel, bias, state, lengths, dy, dstate_out, dx,
+    causal_conv_backward_kernel<T, W><<<grid, 256, 0, stream>>>(s, x, kernel, bias, state, lengths, dy, dstate_out, dx,
                                                                    dstate, workspace);
     HASTE_HIP_TRY(hipGetLastError());
   }
@@ -356,12 +381,7 @@ using namespace haste_hip;
 
 size_t haste_hip_causal_conv_workspace_bytes(int steps, int batch_size, int channels, int width) {
   if (!sizes_ok(steps, batch_size, channels, width) || !sizes_small(steps, batch_size, channels) || width > kMaxWidth) return 0;
-  size_t most = 0;
-  for (int V = 4; V <= 8; V *= 2) {  // whatever the type
-    const size_t total = partials_of(steps, batch_size, channels, width, V).total;
-    most = most > total ? most : total;
-  }
-  return most * sizeof(float);
+  return partials_of(steps, batch_size, channels, width).total * sizeof(float);
 }
 
 #define HASTE_HIP_CAUSAL_CONV(SUFFIX, T)                                                                               \
