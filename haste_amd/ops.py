@@ -601,20 +601,42 @@ def layer_norm_gru_backward(x_t, kernel_t, recurrent_kernel_t, bias, recurrent_b
 _ACTIVATIONS = {torch.float32: "_f32", torch.float16: "_f16", torch.bfloat16: "_bf16"}
 
 
+# The checks below are written for few look-ups: a single step's call costs more on the host than on the GPU.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _described(t):
     return "%s %s on %s" % (t.dtype, list(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__
 
 
+def _is(t, shape, dtype, device):
+    """device: what get_device() gives, -1 on the CPU."""
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device
+
+
+def _alike(dtype, device, *tensors):
+    """Whether all that are not None are tensors of that type on that device."""
+    for t in tensors:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != device):
+            return False
+    return True
+
+
 def _activation(what, t, shape, like):
-    if not torch.is_tensor(t) or t.shape != shape or t.dtype != like.dtype or t.device != like.device:
+    if not _is(t, shape, like.dtype, like.get_device()):
         raise ValueError("%s must be %s %s on %s, got %s" % (what, like.dtype, list(shape), like.device, _described(t)))
 
 
 def _float(what, t, shape, like):
     """A parameter, state or statistic, contiguous."""
-    if not torch.is_tensor(t) or t.shape != shape or t.dtype != torch.float32 or t.device != like.device:
+    if not _is(t, shape, torch.float32, like.get_device()):
         raise ValueError("%s must be float32 %s on %s, got %s" % (what, list(shape), like.device, _described(t)))
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _output(what, t, shape, dtype, like):
+    if not _is(t, shape, dtype, like.get_device()) or not t.is_contiguous():
+        raise ValueError("%s must be %s %s on %s, contiguous, got %s" % (what, dtype, list(shape), like.device, _described(t)))
 
 
 def _activation_suffix(x):
@@ -623,19 +645,31 @@ def _activation_suffix(x):
         raise ValueError("activations must be float32, float16 or bfloat16, got %s" % x.dtype)
     if not x.is_cuda:
         raise ValueError("tensor must be a GPU tensor")
+    if x.numel() >= 2 ** 31 and max(x.shape) >= 2 ** 31:  # the entry points count in 32 bits
+        raise ValueError("sizes beyond 2^31 are not implemented, got %s" % list(x.shape))
     return suffix
 
 
-def _packed_rows(t, shared=False):
-    """`t` with contiguous channels (shared: groups and states): itself, or a copy."""
-    if t.stride(-1) != 1 and t.size(-1) != 1 or shared and t.stride(-2) != t.size(-1) and t.size(-2) != 1:
+def _contiguous(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _packed_rows(t):
+    """`t` with contiguous channels: itself, or a copy."""
+    return t if t.stride()[-1] == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _packed_groups(t):
+    """`t`, [...,G,S], with the states of all groups contiguous."""
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] != 1 or strides[-2] != t.shape[-1] and t.shape[-2] != 1:
         return t.contiguous()
     return t
 
 
 def _strided(t):
     """The three arguments an entry point takes for a tensor [T,N,...]."""
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+    return (None, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:2])
 
 
 def _address(t):
@@ -648,7 +682,7 @@ def _on_device_of(index, name):
         @functools.wraps(op)
         def on_device(*args, **kwargs):
             like = args[index] if len(args) > index else kwargs.get(name)
-            if torch.is_tensor(like) and like.is_cuda and like.device.index != torch.cuda.current_device():
+            if isinstance(like, torch.Tensor) and like.is_cuda and like.get_device() != _current_device():
                 with torch.cuda.device(like.device):
                     return op(*args, **kwargs)
             return op(*args, **kwargs)
@@ -666,8 +700,6 @@ def _scratch_bytes(entry, device, *sizes):
 
 
 def _scratch(entry, like, *sizes):
-    if max(sizes) >= 2 ** 31:
-        raise ValueError("sizes beyond 2^31 are not implemented, got %s" % (sizes,))
     return torch.empty(max(1, _scratch_bytes(entry, like.device, *sizes)), device=like.device, dtype=torch.uint8)
 
 
@@ -676,24 +708,29 @@ def _zero_rows(T, N, D, like):
 
 
 def _invoke(name, *values):
-    lib.invoke(name, lib.entry(name), list(values))
+    """Calls entry point `name` on the current stream of the current device, which is the tensors'."""
+    stream = None if lib._raw_stream is None else lib._raw_stream(_current_device())
+    lib.invoke(name, lib.entry(name), list(values), stream)
 
 
 def _conv_arguments(x, kernel, bias, state, lengths, steps=True):
     dims = 3 if steps else 2
-    if not torch.is_tensor(x) or x.dim() != dims or not torch.is_tensor(kernel) or kernel.dim() != 2 or 0 in x.shape:
+    if not isinstance(x, torch.Tensor) or x.dim() != dims or not isinstance(kernel, torch.Tensor) or kernel.dim() != 2 \
+            or not x.numel():
         raise ValueError("x must be [%s], of no size 0, and kernel [W,D], got %s and %s"
                          % ("T,N,D" if steps else "N,D", _described(x), _described(kernel)))
     N, D = x.shape[-2:]
     W = kernel.shape[0]
     if not 1 <= W <= 8:
         raise ValueError("kernels of 1 to 8 steps are implemented, got %d" % W)
-    kernel = _float("kernel", kernel, (W, D), x)
-    if bias is not None:
-        bias = _float("bias", bias, (D,), x)
-    if state is not None:
+    device = x.get_device()
+    if not (_alike(torch.float32, device, kernel, bias) and _alike(x.dtype, device, state) and kernel.shape[1] == D
+            and (bias is None or bias.shape == (D,)) and (state is None or state.shape == (W - 1, N, D))):
+        _float("kernel", kernel, (W, D), x)  # one of these says what is wrong
+        if bias is not None:
+            _float("bias", bias, (D,), x)
         _activation("state", state, (W - 1, N, D), x)
-        state = state.contiguous()
+    kernel, bias, state = _contiguous(kernel), _contiguous(bias), _contiguous(state)
     if lengths is not None:
         _check_lengths(lengths, x)
     return _packed_rows(x), kernel, bias, state, _activation_suffix(x)
@@ -742,9 +779,9 @@ def causal_conv_iterate(x, state, kernel, bias=None, silu=False, state_out=None)
     (N, D), W = x.shape, kernel.shape[0]
     if read is None:
         raise ValueError("state must be %s %s on %s, got None" % (x.dtype, [W - 1, N, D], x.device))
-    y = torch.empty(N, D, device=x.device, dtype=x.dtype)
+    y = x.new_empty((N, D))
     if state_out is None:
-        state_out = torch.empty(W - 1, N, D, device=x.device, dtype=x.dtype)
+        state_out = torch.empty_like(read)
     else:
         _output("state_out", state_out, (W - 1, N, D), x.dtype, x)
     _invoke("haste_hip_causal_conv_forward" + suffix, 1, N, D, W, x.data_ptr(), 0, x.stride(0), kernel.data_ptr(),
@@ -752,39 +789,37 @@ def causal_conv_iterate(x, state, kernel, bias=None, silu=False, state_out=None)
     return y, state_out
 
 
-def _output(what, t, shape, dtype, like):
-    if not torch.is_tensor(t) or t.shape != shape or t.dtype != dtype or t.device != like.device or not t.is_contiguous():
-        raise ValueError("%s must be %s %s on %s, contiguous, got %s" % (what, dtype, list(shape), like.device, _described(t)))
-
-
 def _scan_arguments(x, delta, A, B, C, D, z, delta_bias, steps=True):
     """The arguments checked: (x, delta, A, B, C, D, z, delta_bias) as the entry points take them, S, G and the suffix."""
     dims = 3 if steps else 2
-    if not torch.is_tensor(x) or x.dim() != dims or 0 in x.shape:
+    if not isinstance(x, torch.Tensor) or x.dim() != dims or not x.numel():
         raise ValueError("x must be [%s], of no size 0, got %s" % ("T,N,D" if steps else "N,D", _described(x)))
-    if not torch.is_tensor(A) or A.dim() != 2 or not 1 <= A.shape[1] <= 64:
+    if not isinstance(A, torch.Tensor) or A.dim() != 2 or not 1 <= A.shape[1] <= 64:
         raise ValueError("A must be float32 [D,S], S of 1 to 64, got %s" % _described(A))
-    channels, S = x.shape[-1], A.shape[1]
-    if not torch.is_tensor(B) or B.dim() not in (dims, dims + 1):
+    full = x.shape
+    channels, S = full[-1], A.shape[1]
+    if not isinstance(B, torch.Tensor) or B.dim() not in (dims, dims + 1):
         raise ValueError("B must be [%s,G,S] or [%s,S], got %s" % ((("T,N", "T,N") if steps else ("N", "N")) + (_described(B),)))
-    G = B.shape[-2] if B.dim() == dims + 1 else 1
+    grouped = B.dim() == dims + 1
+    G = B.shape[-2] if grouped else 1
     if G < 1 or channels % G:
         raise ValueError("%d channels cannot be shared by %d groups" % (channels, G))
-    _activation("delta", delta, x.shape, x)
-    A = _float("A", A, (channels, S), x)
-    shape = x.shape[:-1] + ((G, S) if B.dim() == dims + 1 else (S,))
-    _activation("B", B, shape, x)
-    _activation("C", C, shape, x)
-    shared = B.dim() == dims + 1
-    if D is not None:
-        D = _float("D", D, (channels,), x)
-    if z is not None:
-        _activation("z", z, x.shape, x)
-        z = _packed_rows(z)
-    if delta_bias is not None:
-        delta_bias = _float("delta_bias", delta_bias, (channels,), x)
-    return (_packed_rows(x), _packed_rows(delta), A, _packed_rows(B, shared), _packed_rows(C, shared), D, z, delta_bias, S, G,
-            _activation_suffix(x))
+    shape, device, width = (*full[:-1], G, S) if grouped else (*full[:-1], S), x.get_device(), (channels,)
+    if not (_alike(x.dtype, device, delta, B, C, z) and _alike(torch.float32, device, A, D, delta_bias)
+            and delta is not None and C is not None and delta.shape == full and B.shape == shape and C.shape == shape
+            and A.shape[0] == channels and (z is None or z.shape == full) and (D is None or D.shape == width)
+            and (delta_bias is None or delta_bias.shape == width)):
+        _activation("delta", delta, full, x)  # one of these says what is wrong
+        _float("A", A, (channels, S), x)
+        _activation("B", B, shape, x)
+        _activation("C", C, shape, x)
+        for what, t in (("D", D), ("delta_bias", delta_bias)):
+            if t is not None:
+                _float(what, t, width, x)
+        _activation("z", z, full, x)
+    A, D, delta_bias, z = _contiguous(A), _contiguous(D), _contiguous(delta_bias), z if z is None else _packed_rows(z)
+    packed = _packed_groups if grouped else _packed_rows
+    return _packed_rows(x), _packed_rows(delta), A, packed(B), packed(C), D, z, delta_bias, S, G, _activation_suffix(x)
 
 
 @_on_device_of(1, "x")
@@ -851,9 +886,9 @@ def selective_scan_iterate(x, delta, A, B, C, h, D=None, z=None, delta_bias=None
     x, delta, A, B, C, D, z, delta_bias, S, G, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias, steps=False)
     N, channels = x.shape
     h = _float("h", h, (N, channels, S), x)
-    y = torch.empty(N, channels, device=x.device, dtype=x.dtype)
+    y = x.new_empty((N, channels))
     if h_out is None:
-        h_out = torch.empty(N, channels, S, device=x.device)
+        h_out = torch.empty_like(h)
     else:
         _output("h_out", h_out, (N, channels, S), torch.float32, x)
     _invoke("haste_hip_selective_scan_iterate" + suffix, N, channels, S, G, x.data_ptr(), x.stride(0), delta.data_ptr(),
@@ -865,23 +900,40 @@ def selective_scan_iterate(x, delta, A, B, C, h, D=None, z=None, delta_bias=None
 
 def _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias):
     """The arguments checked, activations as [T,N,D]."""
-    if not torch.is_tensor(update) or update.dim() not in (2, 3) or 0 in update.shape:
+    if not isinstance(update, torch.Tensor) or update.dim() not in (2, 3) or not update.numel():
         raise ValueError("update must be [T,N,D] or [N,D], of no size 0, got %s" % _described(update))
     D = update.shape[-1]
     if D > 8192:
         raise ValueError("rows of up to 8192 channels are implemented, got %d" % D)
-    for what, t in (("residual", residual), ("gate", gate)):
-        if t is not None:
-            _activation(what, t, update.shape, update)
     if before_weight is None and before_bias is not None:
         raise ValueError("before_bias needs before_weight")
-    weights = [None if w is None else _float(what, w, (D,), update) for what, w in
-               (("scale", scale), ("after_weight", after_weight), ("before_weight", before_weight), ("before_bias", before_bias))]
-    return [_norm_rows(t) for t in (update, residual, gate)], weights, _activation_suffix(update)
+    full, device, width = update.shape, update.get_device(), (D,)
+    if not (_alike(update.dtype, device, residual, gate)
+            and _alike(torch.float32, device, scale, after_weight, before_weight, before_bias)
+            and (residual is None or residual.shape == full) and (gate is None or gate.shape == full)
+            and (scale is None or scale.shape == width) and (after_weight is None or after_weight.shape == width)
+            and (before_weight is None or before_weight.shape == width) and (before_bias is None or before_bias.shape == width)):
+        for what, t in (("residual", residual), ("gate", gate)):  # one of these says what is wrong
+            if t is not None:
+                _activation(what, t, full, update)
+        for what, t in (("scale", scale), ("after_weight", after_weight), ("before_weight", before_weight),
+                        ("before_bias", before_bias)):
+            if t is not None:
+                _float(what, t, width, update)
+    weights = _contiguous(scale), _contiguous(after_weight), _contiguous(before_weight), _contiguous(before_bias)
+    return (_packed(update), _packed(residual), _packed(gate)), weights, _activation_suffix(update)
+
+
+def _packed(t):
+    return t if t is None else _packed_rows(t)
 
 
 def _norm_rows(t):
-    return t if t is None else _packed_rows(t if t.dim() == 3 else t.unsqueeze(0))
+    """As _strided, of [T,N,D] or [N,D]."""
+    if t is None:
+        return None, 0, 0
+    strides = t.stride()
+    return (t.data_ptr(), strides[0], strides[1]) if len(strides) == 3 else (t.data_ptr(), 0, strides[0])
 
 
 @_on_device_of(0, "update")
@@ -892,11 +944,11 @@ def residual_norm_forward(update, residual=None, gate=None, scale=None, after_we
     norm(v) = v / sqrt(mean v^2 + eps), centered: of v - mean v.  Parts that are None are left out (update is not normed without
     after_weight); stats is what the backward pass needs."""
     rows, weights, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
-    T, N, D = rows[0].shape
-    out = torch.empty(update.shape, device=update.device, dtype=update.dtype)
+    T, N, D = update.shape if update.dim() == 3 else (1, *update.shape)
+    out = update.new_empty(update.shape)
     normed = None if before_weight is None else torch.empty_like(out)
-    stats = torch.empty(T, N, 4, device=update.device)
-    _invoke("haste_hip_residual_norm_forward" + suffix, T, N, D, *_strided(rows[0]), *_strided(rows[1]), *_strided(rows[2]),
+    stats = torch.empty((T, N, 4), device=update.device)
+    _invoke("haste_hip_residual_norm_forward" + suffix, T, N, D, *_norm_rows(rows[0]), *_norm_rows(rows[1]), *_norm_rows(rows[2]),
             *map(_address, weights), bool(centered), float(eps), out.data_ptr(), _address(normed), stats.data_ptr())
     return out, normed, stats
 
@@ -907,7 +959,7 @@ def residual_norm_backward(update, residual, gate, scale, after_weight, before_w
     """Gradients (dupdate, dresidual, dgate, dscale, dafter_weight, dbefore_weight, dbefore_bias) from those of out and normed
     (either may be None: zeros); those of arguments that are None are None."""
     rows, weights, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
-    T, N, D = rows[0].shape
+    T, N, D = update.shape if update.dim() == 3 else (1, *update.shape)
     stats = _float("stats", stats, (T, N, 4), update)
     if dnormed is not None and before_weight is None:
         raise ValueError("dnormed needs before_weight")
@@ -918,8 +970,8 @@ def residual_norm_backward(update, residual, gate, scale, after_weight, before_w
              for t in (update, residual, gate)]
     sums = [None if w is None else torch.empty_like(w) for w in weights]
     scratch = _scratch("haste_hip_residual_norm_workspace_bytes", update, T, N, D)
-    dout, dnormed = _norm_rows(dout), _norm_rows(dnormed)
-    _invoke("haste_hip_residual_norm_backward" + suffix, T, N, D, *_strided(rows[0]), *_strided(rows[1]), *_strided(rows[2]),
-            *map(_address, weights[:3]), bool(centered), stats.data_ptr(), *_strided(dout), *_strided(dnormed),
+    dout, dnormed = _packed(dout), _packed(dnormed)
+    _invoke("haste_hip_residual_norm_backward" + suffix, T, N, D, *_norm_rows(rows[0]), *_norm_rows(rows[1]), *_norm_rows(rows[2]),
+            *map(_address, weights[:3]), bool(centered), stats.data_ptr(), *_norm_rows(dout), *_norm_rows(dnormed),
             *map(_address, grads), *map(_address, sums), scratch.data_ptr(), scratch.numel())
     return (*grads, *sums)
