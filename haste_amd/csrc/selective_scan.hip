@@ -236,7 +236,7 @@ struct WalkShared {
 };
 
 // Forward pass over a chunk.  LOCAL: only what the chunk adds to a state of zero, and the sum of dt.
-// starts: the states at the chunks' starts [chunks][N][D][S] (LOCAL: out, what each adds), null when
+// starts: the states at the chunks' starts [chunks][N][D][S] (LOCAL: out, what each but the last adds), null when
 // there is one chunk; kept: the states at the tiles' starts [tiles][N][D][S], or null.
 template <typename T, int LANES, bool LOCAL>
 __global__ __launch_bounds__(256)
@@ -418,12 +418,22 @@ void scan_chunks_kernel(ScanShape s, const float* __restrict__ A, const float* _
   const size_t channel = i / s.S;
   const float A2 = A[channel % s.D * s.S + i % s.S] * kLog2e;
   float h = first != nullptr ? first[i] : 0.f;
-  for (int k = 0; k < s.chunks; ++k) {
-    const int c = REVERSE ? s.chunks - 1 - k : k;
-    const float decay = __builtin_amdgcn_exp2f(A2 * sum_dt[(size_t)c * s.N * s.D + channel]);
-    const float added = at[c * states + i];
-    at[c * states + i] = h;
-    h = h == 0.f ? added : decay * h + added;  // (0 times a product of growth beyond float's range is 0, not NaN)
+  constexpr int AHEAD = 8;  // chunks read at once: only the products follow one from the other
+  for (int k0 = 0; k0 < s.chunks; k0 += AHEAD) {
+    float added[AHEAD], decay[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j, c = REVERSE ? s.chunks - 1 - k : k;
+      const bool follows = k + 1 < s.chunks;  // behind the last nothing does, and what it adds was not computed
+      added[j] = follows ? at[c * states + i] : 0.f;
+      decay[j] = follows ? __builtin_amdgcn_exp2f(A2 * sum_dt[(size_t)c * s.N * s.D + channel]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j, c = REVERSE ? s.chunks - 1 - k : k;
+      if (k < s.chunks) at[c * states + i] = h;
+      h = h == 0.f ? added[j] : decay[j] * h + added[j];  // (0 times a product of growth beyond float's range is 0, not NaN)
+    }
   }
 }
 
@@ -438,7 +448,7 @@ struct ScanGradients {
 
 // Backward pass over a chunk.  LOCAL: only G at the chunk's start for a gradient of zero at its end, and
 // the sum of dt.  ends: [chunks][N][D][S], the gradients at the chunks' ends
-// (LOCAL: out), null when there is one chunk.
+// (LOCAL: out, but for the first chunk), null when there is one chunk.
 template <typename T, int LANES, bool LOCAL>
 __global__ __launch_bounds__(256, 2)
 void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ kept, Rows<const T> dy,
@@ -454,7 +464,8 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   __shared__ float dB_lds[LOCAL ? 1 : 4][TS * LANES * K], dC_lds[LOCAL ? 1 : 4][TS * LANES * K];  // of each wavefront
 
   const Block<LANES> b(s, blockIdx.x);
-  const int t0 = blockIdx.y * s.chunk, t1 = min(s.T, t0 + s.chunk);
+  const unsigned chunk = blockIdx.y + (LOCAL ? 1 : 0);  // what goes out of the first chunk is found by the second pass
+  const int t0 = chunk * s.chunk, t1 = min(s.T, t0 + s.chunk);
   const Extent extent = extent_of(in.lengths, b.n, s.T);
   const int end = min(t1, extent.steps);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s0 = P::states(lane) * K;
@@ -469,10 +480,10 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   for (int r = 0; r < K; ++r) A[r] = G[r] = dA[r] = 0.f;
   if (live) {
     load_states(in.A + (size_t)d * s.S, s0, s.S, A);
-    if (blockIdx.y + 1 == (unsigned)s.chunks) {
+    if (chunk + 1 == (unsigned)s.chunks) {
       if (dh_last != nullptr && !LOCAL) load_states(dh_last + state, s0, s.S, G);
     } else if (!LOCAL) {
-      load_states(ends + blockIdx.y * states + state, s0, s.S, G);
+      load_states(ends + chunk * states + state, s0, s.S, G);
     }
   }
 #pragma unroll
@@ -655,14 +666,14 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
 
   if (LOCAL) {
     if (live) {
-      store_states(ends + blockIdx.y * states + state, s0, s.S, G);
-      if (s0 == 0) sum_dt[((size_t)blockIdx.y * s.N + b.n) * s.D + d] = dt_sum;
+      store_states(ends + chunk * states + state, s0, s.S, G);
+      if (s0 == 0) sum_dt[((size_t)chunk * s.N + b.n) * s.D + d] = dt_sum;
     }
     return;
   }
-  float* partial = out.partial + ((size_t)blockIdx.y * s.N + b.n) * ((size_t)s.D * (s.S + 2));
+  float* partial = out.partial + ((size_t)chunk * s.N + b.n) * ((size_t)s.D * (s.S + 2));
   if (live) {
-    if (blockIdx.y == 0 && out.dh0 != nullptr) {
+    if (chunk == 0 && out.dh0 != nullptr) {
       if (extent.fill != 0.f) {  // NaN
 #pragma unroll
         for (int r = 0; r < K; ++r) G[r] = extent.fill;
@@ -756,22 +767,22 @@ int with_lanes(int S, F&& f) {
   }
 }
 
-// Cuts the time axis so that `waves` wavefronts a SIMD have work, in chunks of no fewer than 4 tiles.
-ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, int waves) {
+// The time axis is cut where a batch row's channels and the rows make less than a workgroup a CU, into chunks that make about
+// two, of no fewer than 4 tiles.  The first of the two passes costs four fifths of the second, so that at a workgroup a CU or
+// more it is not won back: forward and backward with T=2048, D=4096, S=16 bf16, in two chunks and in one: N=4 (256 workgroups) 826 and
+// 949 us, N=5 1277 and 1253, N=7 1417 and 1237; T=128 N=32 D=512 (256) 81 and 72, T=256 N=12 D=2048 (384) 180 and 166.
+ScanShape shape_of(int T, int N, int D, int S, int G, int softplus) {
   ScanShape s = {T, N, D, S, G, D / G, 0, 0, 0, softplus};
   const int block = 256 / lanes_for(S);
   s.blocks_group = (s.share + block - 1) / block;
-  const size_t blocks = (size_t)N * G * s.blocks_group, wanted = (size_t)device_cu_count() * waves;
-  const size_t tiles = (T + TS - 1) / TS;
-  size_t chunks = blocks >= wanted ? 1 : (wanted + blocks - 1) / blocks;
-  const size_t most = tiles / 4 > 0 ? tiles / 4 : 1;
+  const size_t blocks = (size_t)N * G * s.blocks_group, cus = (size_t)device_cu_count();
+  const size_t tiles = ((size_t)T + TS - 1) / TS, most = tiles / 4 > 0 ? tiles / 4 : 1;
+  size_t chunks = blocks >= cus ? 1 : 2 * cus / blocks;
   chunks = chunks < most ? chunks : most;
   s.chunk = (int)((tiles + chunks - 1) / chunks) * TS;
-  s.chunks = (T + s.chunk - 1) / s.chunk;
+  s.chunks = (int)(((size_t)T + s.chunk - 1) / s.chunk);
   return s;
 }
-ScanShape forward_shape(int T, int N, int D, int S, int G, int softplus) { return shape_of(T, N, D, S, G, softplus, 2); }
-ScanShape backward_shape(int T, int N, int D, int S, int G, int softplus) { return shape_of(T, N, D, S, G, softplus, 2); }
 
 // Floats of workspace, in the order they lie there.
 struct ScanWorkspace {
@@ -810,7 +821,7 @@ int forward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, con
     dim3 grid((unsigned)blocks, s.chunks);
     if (s.chunks > 1) {
       ScopedKernelTimer timer("selective_scan_chunks", stream);
-      selective_scan_forward_kernel<T, lanes(), true><<<grid, 256, 0, stream>>>(s, in, nullptr, starts, sum_dt, nullptr, nullptr, nullptr);
+      selective_scan_forward_kernel<T, lanes(), true><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, starts, sum_dt, nullptr, nullptr, nullptr);
       HASTE_HIP_TRY(hipGetLastError());
       scan_chunks_kernel<false><<<(unsigned)((states + 255) / 256), 256, 0, stream>>>(s, in.A, h0, sum_dt, starts);
       HASTE_HIP_TRY(hipGetLastError());
@@ -838,7 +849,7 @@ int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, co
     dim3 grid((unsigned)blocks, s.chunks);
     if (s.chunks > 1) {
       ScopedKernelTimer timer("selective_scan_chunks", stream);
-      selective_scan_backward_kernel<T, lanes(), true><<<grid, 256, 0, stream>>>(s, in, nullptr, dy, dh_last, ends, sum_dt, out);
+      selective_scan_backward_kernel<T, lanes(), true><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, dy, dh_last, ends, sum_dt, out);
       HASTE_HIP_TRY(hipGetLastError());
       scan_chunks_kernel<true><<<(unsigned)((states + 255) / 256), 256, 0, stream>>>(s, in.A, dh_last, sum_dt, ends);
       HASTE_HIP_TRY(hipGetLastError());
@@ -898,8 +909,8 @@ using namespace haste_hip;
 
 size_t haste_hip_selective_scan_workspace_bytes(int backward, int steps, int batch_size, int channels, int states, int groups) {
   if (check_sizes(steps, batch_size, channels, states, groups) != HASTE_HIP_OK) return 0;
-  const size_t floats = backward ? backward_workspace(backward_shape(steps, batch_size, channels, states, groups, 0)).total
-                                 : forward_workspace(forward_shape(steps, batch_size, channels, states, groups, 0)).total;
+  const size_t floats = backward ? backward_workspace(shape_of(steps, batch_size, channels, states, groups, 0)).total
+                                 : forward_workspace(shape_of(steps, batch_size, channels, states, groups, 0)).total;
   return floats * sizeof(float);
 }
 
@@ -920,7 +931,7 @@ size_t haste_hip_selective_scan_kept_bytes(int steps, int batch_size, int channe
                                                 void* stream) {                                                        \
     HASTE_HIP_PROPAGATE(check_sizes(steps, batch_size, channels, states, groups));                                     \
     HASTE_HIP_REQUIRE(x && delta && A && B && C && y);                                                                 \
-    return forward<T>(as_stream(stream), forward_shape(steps, batch_size, channels, states, groups, delta_softplus),   \
+    return forward<T>(as_stream(stream), shape_of(steps, batch_size, channels, states, groups, delta_softplus),   \
                       inputs_of<T>(x, x_step, x_row, delta, delta_step, delta_row, A, B, B_step, B_row, C, C_step,     \
                                    C_row, D, z, z_step, z_row, delta_bias, lengths),                                   \
                       h0, static_cast<T*>(y), h_last, kept, static_cast<float*>(workspace), workspace_bytes);          \
@@ -933,7 +944,7 @@ size_t haste_hip_selective_scan_kept_bytes(int steps, int batch_size, int channe
     HASTE_HIP_PROPAGATE(check_sizes(steps, batch_size, channels, states, groups));                                     \
     HASTE_HIP_REQUIRE(x && delta && A && B && C && kept && dy && dx && ddelta && dA && dB && dC && workspace);         \
     HASTE_HIP_REQUIRE((z == nullptr) == (dz == nullptr));                                                              \
-    return backward<T>(as_stream(stream), backward_shape(steps, batch_size, channels, states, groups, delta_softplus), \
+    return backward<T>(as_stream(stream), shape_of(steps, batch_size, channels, states, groups, delta_softplus), \
                        inputs_of<T>(x, x_step, x_row, delta, delta_step, delta_row, A, B, B_step, B_row, C, C_step,    \
                                     C_row, D, z, z_step, z_row, delta_bias, lengths),                                  \
                        kept, {static_cast<const T*>(dy), dy_step, dy_row}, dh_last, static_cast<T*>(dx),               \
