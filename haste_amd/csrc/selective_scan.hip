@@ -661,7 +661,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
       out.dB[at] = (dB_lds[0][e] + dB_lds[1][e]) + (dB_lds[2][e] + dB_lds[3][e]);
       out.dC[at] = (dC_lds[0][e] + dC_lds[1][e]) + (dC_lds[2][e] + dC_lds[3][e]);
     }
-    __syncthreads();
+    // No barrier: until the next one a thread overwrites only elements that it alone reads here, and B and C, which nobody does.
   }
 
   if (LOCAL) {

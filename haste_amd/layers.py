@@ -935,9 +935,11 @@ class CausalConv(_BlockLayer):
             y, state = _eager_causal_conv(x, self.kernel, self.bias, self.silu, state, lengths)
         return self._rows(y), state
 
-    def step(self, input, state):
+    def step(self, input, state=None):
         """One step without gradients: input [N,channels] -> (output, state)."""
         with torch.no_grad():
+            if state is None:
+                state = input.new_zeros((self.width - 1, *input.shape))
             if self._fused(input):
                 return ops.causal_conv_iterate(input, state, _as_float(self.kernel), _as_float(self.bias), self.silu)
             y, state = _eager_causal_conv(input.unsqueeze(0), self.kernel, self.bias, self.silu, state, None)

@@ -494,3 +494,54 @@ def test_inference_keeps_nothing_for_a_backward_pass():
     assert cache is None
     full = run_scan(g)
     assert torch.equal(y, full["y"]) and torch.equal(h, full["h_last"])
+
+
+# ---- what stays apart, what may be repeated -----------------------------------------------------
+def test_a_bad_value_stays_in_its_channel_and_row():
+    c, s, n = conv_problem(3, torch.float32, 150, 3, 40, 4), scan_problem(3, torch.float32, 150, 3, 40, 16), norm_problem(3, torch.float32, (150, 3, 40), True)
+    for run, q, name in ((run_conv, c, "x"), (run_scan, s, "x"), (lambda g: run_norm(g, True), n, "update")):
+        good = run(q.g)
+        for bad in (float("nan"), float("inf")):
+            t = q.g[name].clone()
+            t[70, 1, 5] = bad
+            got = run(dict(q.g, **{name: t}))
+            for k in got:
+                if got[k] is None or got[k].dim() < 3 or k == "dstate" or k == "state":
+                    continue
+                rows = got[k] if got[k].shape[1] == 3 else got[k].transpose(0, 1)
+                want = good[k] if got[k].shape[1] == 3 else good[k].transpose(0, 1)
+                others = [0, 2]
+                assert torch.equal(rows[:, others], want[:, others]), (k, bad)
+                if name == "x" and k in ("y", "dx", "ddelta", "dz"):  # (a norm's row is one)
+                    keep = [d for d in range(40) if d != 5]
+                    assert torch.equal(rows[:, 1][:, keep], want[:, 1][:, keep]), (k, bad)
+            if name == "x":
+                assert not got["y"][70, 1, 5].isfinite() and torch.equal(got["y"][:70, 1, 5], good["y"][:70, 1, 5])
+
+
+def test_backward_twice_and_refused_second_derivatives():
+    torch.manual_seed(5)
+    conv, scan, norm = haste_amd.CausalConv(24).cuda(), haste_amd.SelectiveScan(24, 8).cuda(), haste_amd.ResidualNorm(24).cuda()
+    x, delta, B, C, z = (torch.randn(40, 2, k, device="cuda", requires_grad=True) for k in (24, 24, 8, 8, 24))
+    y, _ = scan(conv(x)[0], delta, B, C, z)
+    out, normed = norm(y, x, z)
+    loss = (out * normed).sum()
+    leaves = [x, delta, B, C, z, *conv.parameters(), *scan.parameters(), *norm.parameters()]
+    first = torch.autograd.grad(loss, leaves, retain_graph=True)
+    second = torch.autograd.grad(loss, leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with pytest.raises(RuntimeError):
+        second[0].sum().backward()
+
+
+def test_steps_from_no_state():
+    torch.manual_seed(6)
+    conv, scan = haste_amd.CausalConv(24).cuda(), haste_amd.SelectiveScan(24, 8).cuda()
+    x, delta, B, C, z = (torch.randn(1, 2, k, device="cuda") for k in (24, 24, 8, 8, 24))
+    with torch.no_grad():
+        y, state = conv(x)
+        y1, state1 = conv.step(x[0])
+        assert torch.equal(y[0], y1) and torch.equal(state, state1)
+        y, h = scan(x, delta, B, C, z)
+        y1, h1 = scan.step(x[0], delta[0], B[0], C[0], z[0])
+        assert (y[0] - y1).abs().max() <= 1e-5 and (h - h1).abs().max() <= 1e-5
