@@ -719,40 +719,53 @@ void scan_shared_kernel(int parts, size_t count, const float* __restrict__ dB_pa
   (blockIdx.y == 0 ? dB : dC)[i] = (T)sum;
 }
 
-// A single step: LANES neighbouring lanes a channel, its states in and out as whole lines.
+// A single step: LANES neighbouring lanes a channel, its states in and out as whole lines.  Bound by those lines' bytes, or by
+// latency.  What is the channel's (A and the like) is read once for the rows a workgroup goes through, and a row's elements
+// are on their way while the row before is computed: N=128 D=4096 S=16 bf16, 72 MB, 19.1 us with a thread a row.
 template <typename T, int LANES>
 __global__ __launch_bounds__(256)
 void selective_scan_step_kernel(ScanShape s, ScanInputs<T> in, const float* h, float* h_out, T* __restrict__ y) {
-  const unsigned i = blockIdx.x * 256 + threadIdx.x, channel = i / LANES, s0 = i % LANES * K;
-  const unsigned n = channel / s.D;
-  if (n >= (unsigned)s.N) return;
-  const unsigned d = channel % s.D, g = d / s.share;
-  const size_t state = (size_t)channel * s.S;
-  float A[K], hs[K], Bv[K], Cv[K];
-  load_states(h + state, s0, s.S, hs);
-  load_states(in.A + (size_t)d * s.S, s0, s.S, A);
-  load_channels<K>(in.B.at(0, n) + (size_t)g * s.S, s0, s.S, Bv);
-  load_channels<K>(in.C.at(0, n) + (size_t)g * s.S, s0, s.S, Cv);
-  const float x = (float)in.x.at(0, n)[d];
-  const float dt = step_size((float)in.delta.at(0, n)[d] + (in.bias != nullptr ? in.bias[d] : 0.f), s.softplus, true);
-  float sum = 0.f;
+  const unsigned i = blockIdx.x * 256 + threadIdx.x, d = i / LANES, s0 = i % LANES * K;
+  if (d >= (unsigned)s.D) return;  // (the lanes of a channel together)
+  const size_t shared = (size_t)(d / s.share) * s.S;
+  float A2[K];
+  load_states(in.A + (size_t)d * s.S, s0, s.S, A2);
 #pragma unroll
-  for (int r = 0; r < K; ++r) {
-    hs[r] = exp_of(dt * A[r]) * hs[r] + dt * x * Bv[r];
-    sum += hs[r] * Cv[r];
+  for (int r = 0; r < K; ++r) A2[r] *= kLog2e;
+  const float bias = in.bias != nullptr ? in.bias[d] : 0.f, skip = in.skip != nullptr ? in.skip[d] : 0.f;
+  const bool gated = in.z.p != nullptr;
+
+  struct Row {
+    float h[K], B[K], C[K], x, delta, z;
+  } coming;
+  auto fetch = [&](int n) {
+    load_states(h + ((size_t)n * s.D + d) * s.S, s0, s.S, coming.h);
+    load_channels<K>(in.B.at(0, n) + shared, s0, s.S, coming.B);
+    load_channels<K>(in.C.at(0, n) + shared, s0, s.S, coming.C);
+    coming.x = (float)in.x.at(0, n)[d];
+    coming.delta = (float)in.delta.at(0, n)[d];
+    coming.z = gated ? (float)in.z.at(0, n)[d] : 0.f;
+  };
+  fetch(blockIdx.y);
+  for (int n = blockIdx.y; n < s.N; n += gridDim.y) {
+    Row now = coming;
+    if (n + (int)gridDim.y < s.N) fetch(n + gridDim.y);
+    const float dt = step_size(now.delta + bias, s.softplus, true), u = dt * now.x;
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+      now.h[r] = __builtin_amdgcn_exp2f(dt * A2[r]) * now.h[r] + u * now.B[r];
+      sum += now.h[r] * now.C[r];
+    }
+    store_states(h_out + ((size_t)n * s.D + d) * s.S, s0, s.S, now.h);
+    if (LANES >= 2) sum += dpp<kXor1>(sum);
+    if (LANES >= 4) sum += dpp<kXor2>(sum);
+    if (LANES >= 8) sum += dpp<kHalfMirror>(sum);
+    if (LANES >= 16) sum += dpp<kRor8>(sum);
+    sum += skip * now.x;
+    sum = gated ? sum * (now.z * sigmoid_of(now.z)) : sum;
+    if (s0 == 0) y[(size_t)n * s.D + d] = (T)sum;
   }
-  store_states(h_out + state, s0, s.S, hs);
-  if (LANES >= 2) sum += dpp<kXor1>(sum);
-  if (LANES >= 4) sum += dpp<kXor2>(sum);
-  if (LANES >= 8) sum += dpp<kHalfMirror>(sum);
-  if (LANES >= 16) sum += dpp<kRor8>(sum);
-  if (s0 != 0) return;
-  if (in.skip != nullptr) sum += in.skip[d] * x;
-  if (in.z.p != nullptr) {
-    const float zv = (float)in.z.at(0, n)[d];
-    sum *= zv * sigmoid_of(zv);
-  }
-  y[channel] = (T)sum;
 }
 
 int lanes_for(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
@@ -891,10 +904,12 @@ int step(hipStream_t stream, int N, int D, int S, int G, int softplus, const Sca
          float* h_out) {
   const ScanShape s = {1, N, D, S, G, D / G, 0, TS, 1, softplus};
   return with_lanes(S, [&](auto lanes) {
-    const size_t blocks = ((size_t)N * D * lanes() + 255) / 256;
-    if (blocks > kGridLimit) return too_large("selective_scan: too many rows of channels");
+    const size_t across = ((size_t)D * lanes() + 255) / 256;  // at most 2^22: D is at most 2^30 / 66
+    if (across > kGridLimit) return too_large("selective_scan: too many channels");
+    const size_t wanted = (size_t)device_cu_count() * 8 / across;  // workgroups that fill the chip, per 256 lanes
+    const size_t down = wanted < 1 ? 1 : wanted < (size_t)N ? wanted : (size_t)N;
     ScopedKernelTimer timer("selective_scan_iterate", stream);
-    selective_scan_step_kernel<T, lanes()><<<(unsigned)blocks, 256, 0, stream>>>(s, in, h, h_out, y);
+    selective_scan_step_kernel<T, lanes()><<<dim3((unsigned)across, (unsigned)down), 256, 0, stream>>>(s, in, h, h_out, y);
     HASTE_HIP_TRY(hipGetLastError());
     return HASTE_HIP_OK;
   });
