@@ -84,6 +84,15 @@ void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __res
   const int end = min(t1, e.steps);
   const Rows<T> out = packed_rows(y, N, D);
 
+  // Everything the run starts from is requested before the first use of any of it.
+  float w[W][V], b[V];
+#pragma unroll
+  for (int k = 0; k < W; ++k) load_channels<V>(kernel + (size_t)k * D, c, D, w[k]);
+#pragma unroll
+  for (int v = 0; v < V; ++v) b[v] = 0.f;
+  if (bias != nullptr) load_channels<V>(bias, c, D, b);
+  HeldSteps<T, kForwardAhead> coming;
+  coming.load(x, t0, end, n, c, D);
   float win[W][V];  // X[t .. t+W-1], the last of them filled in by every step
   if (t0 < end) {
 #pragma unroll
@@ -105,12 +114,6 @@ void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __res
     }
   }
   if (t0 < end) {
-    float w[W][V], b[V];
-#pragma unroll
-    for (int k = 0; k < W; ++k) load_channels<V>(kernel + (size_t)k * D, c, D, w[k]);
-#pragma unroll
-    for (int v = 0; v < V; ++v) b[v] = 0.f;
-    if (bias != nullptr) load_channels<V>(bias, c, D, b);
     auto step = [&](int t) {
       float o[V];
 #pragma unroll
@@ -127,8 +130,6 @@ void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __res
         for (int v = 0; v < V; ++v) win[k][v] = win[k + 1][v];
     };
     constexpr int U = kForwardAhead;
-    HeldSteps<T, U> coming;
-    coming.load(x, t0, end, n, c, D);
     for (int t = t0; t < end; t += U) {
       const HeldSteps<T, U> now = coming;
       if (t + U < end) coming.load(x, t + U, end, n, c, D);
