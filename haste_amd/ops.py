@@ -654,49 +654,47 @@ def _contiguous(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _packed_rows(t):
-    """`t` with contiguous channels: itself, or a copy."""
-    return t if t.stride()[-1] == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _packed_groups(t):
-    """`t`, [...,G,S], with the states of all groups contiguous."""
+def _place(values, kept, t, axes, groups=False):
+    """Appends what an entry point takes for a tensor: its address and the strides of its first `axes` axes.  Channels (groups:
+    the states of all groups) must be contiguous; where they are not it is a copy that is placed, and kept."""
+    if t is None:
+        values += (None, 0, 0)[:axes + 1]
+        return
     strides = t.stride()
-    if strides[-1] != 1 and t.shape[-1] != 1 or strides[-2] != t.shape[-1] and t.shape[-2] != 1:
-        return t.contiguous()
-    return t
-
-
-def _strided(t):
-    """The three arguments an entry point takes for a tensor [T,N,...]."""
-    return (None, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:2])
+    if strides[-1] != 1 and t.shape[-1] != 1 or groups and strides[-2] != t.shape[-1] and t.shape[-2] != 1:
+        t = t.contiguous()
+        kept.append(t)
+        strides = t.stride()
+    values.append(t.data_ptr())
+    values += strides[:axes]
 
 
 def _address(t):
     return None if t is None else t.data_ptr()
 
 
-def _on_device_of(index, name):
-    """Runs an operator on the device of its argument `name`, number `index` (the current device needs nothing)."""
-    def decorate(op):
-        @functools.wraps(op)
-        def on_device(*args, **kwargs):
-            like = args[index] if len(args) > index else kwargs.get(name)
-            if isinstance(like, torch.Tensor) and like.is_cuda and like.get_device() != _current_device():
-                with torch.cuda.device(like.device):
-                    return op(*args, **kwargs)
-            return op(*args, **kwargs)
-        return on_device
-    return decorate
+def _apart(what, out, same, *others):
+    """An output that the caller gives may lie where `same` does, and nowhere else among the inputs."""
+    def span(t):
+        first = t.data_ptr()
+        return first, first + (sum((n - 1) * step for n, step in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    begin, end = span(out)
+    for t in (same, *others):
+        if t is not None and t.numel() and (t is not same or t.data_ptr() != begin):
+            first, last = span(t)
+            if first < end and begin < last:
+                raise ValueError("%s overlaps an input of the call" % what)
 
 
 @functools.lru_cache(maxsize=4096)
 def _scratch_bytes(entry, device, *sizes):
-    """What a *_bytes entry point says for these sizes (all ints) on the current device, which `device` is."""
+    """What a *_bytes entry point says for these sizes (all ints) on `device`."""
     fn = lib.load()[entry]
     fn.restype = ctypes.c_size_t
     fn.argtypes = [ctypes.c_int] * len(sizes)
-    return int(fn(*sizes))
+    with torch.cuda.device(device):
+        return int(fn(*sizes))
 
 
 def _scratch(entry, like, *sizes):
@@ -707,13 +705,17 @@ def _zero_rows(T, N, D, like):
     return torch.zeros(1, 1, D, device=like.device, dtype=like.dtype).expand(T, N, D)
 
 
-def _invoke(name, *values):
-    """Calls entry point `name` on the current stream of the current device, which is the tensors'."""
-    stream = None if lib._raw_stream is None else lib._raw_stream(_current_device())
-    lib.invoke(name, lib.entry(name), list(values), stream)
+def _invoke(device, name, values):
+    """Calls entry point `name` on the current stream of the tensors' device, whichever is the current one."""
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _invoke(device, name, values)
+    lib.invoke(name, lib.entry(name), values, None if lib._raw_stream is None else lib._raw_stream(device))
 
 
-def _conv_arguments(x, kernel, bias, state, lengths, steps=True):
+def _conv_arguments(x, kernel, bias, silu, state, lengths, steps=True):
+    """The arguments checked: what the entry points take up to the lengths, the tensors (kernel, bias, state, ...) to keep
+    until the call, the device and the suffix."""
     dims = 3 if steps else 2
     if not isinstance(x, torch.Tensor) or x.dim() != dims or not isinstance(kernel, torch.Tensor) or kernel.dim() != 2 \
             or not x.numel():
@@ -733,64 +735,66 @@ def _conv_arguments(x, kernel, bias, state, lengths, steps=True):
     kernel, bias, state = _contiguous(kernel), _contiguous(bias), _contiguous(state)
     if lengths is not None:
         _check_lengths(lengths, x)
-    return _packed_rows(x), kernel, bias, state, _activation_suffix(x)
+    suffix, values, kept = _activation_suffix(x), [N, D, W] if not steps else [x.shape[0], N, D, W], [kernel, bias, state]
+    if steps:
+        _place(values, kept, x, 2)
+    else:  # the forward pass over one step
+        values.insert(0, 1)
+        _place(values, kept, x, 1)
+        values.insert(5, 0)
+    values += (kernel.data_ptr(), _address(bias), bool(silu), _address(state), _address(lengths))
+    return values, kept, device, suffix
 
 
-@_on_device_of(0, "x")
 def causal_conv_forward(x, kernel, bias=None, silu=False, state=None, lengths=None):
     """x[T,N,D], kernel[W,D] -> y[T,N,D], state_out[W-1,N,D]: y[t] = act(bias + sum_k kernel[k] X[t+k]) with
     X = [state; x] (state None: zeros), act(v) = v sigmoid(v) with silu; state_out: the inputs before the next step."""
-    x, kernel, bias, state, suffix = _conv_arguments(x, kernel, bias, state, lengths)
-    (T, N, D), W = x.shape, kernel.shape[0]
-    y = torch.empty(T, N, D, device=x.device, dtype=x.dtype)
-    state_out = torch.empty(W - 1, N, D, device=x.device, dtype=x.dtype)
-    _invoke("haste_hip_causal_conv_forward" + suffix, T, N, D, W, *_strided(x), kernel.data_ptr(), _address(bias), bool(silu),
-            _address(state), _address(lengths), y.data_ptr(), state_out.data_ptr())
+    values, kept, device, suffix = _conv_arguments(x, kernel, bias, silu, state, lengths)
+    y, state_out = x.new_empty(x.shape), x.new_empty((kernel.shape[0] - 1, *x.shape[1:]))
+    values += (y.data_ptr(), state_out.data_ptr())
+    _invoke(device, "haste_hip_causal_conv_forward" + suffix, values)
     return y, state_out
 
 
-@_on_device_of(0, "x")
 def causal_conv_backward(x, kernel, bias, silu, state, lengths, dy, dstate_out=None):
     """Gradients (dx, dkernel, dbias, dstate) from those of y (None: zeros) and of state_out; dbias and dstate are None
     where there is no bias or state."""
-    like = x
-    x, kernel, bias, state, suffix = _conv_arguments(x, kernel, bias, state, lengths)
+    values, kept, device, suffix = _conv_arguments(x, kernel, bias, silu, state, lengths)
     (T, N, D), W = x.shape, kernel.shape[0]
     dy = _zero_rows(T, N, D, x) if dy is None else dy
-    _activation("dy", dy, like.shape, x)
-    dy = _packed_rows(dy)
+    _activation("dy", dy, x.shape, x)
     if dstate_out is not None:
         _activation("dstate_out", dstate_out, (W - 1, N, D), x)
         dstate_out = dstate_out.contiguous()
-    dx = torch.empty(T, N, D, device=x.device, dtype=x.dtype)
-    dkernel, dbias = torch.empty_like(kernel), None if bias is None else torch.empty_like(bias)
-    dstate = None if state is None else torch.empty_like(state)
+    dx, dkernel = x.new_empty(x.shape), torch.empty_like(kept[0])
+    dbias, dstate = (None if t is None else torch.empty_like(t) for t in kept[1:3])
     scratch = _scratch("haste_hip_causal_conv_workspace_bytes", x, T, N, D, W)
-    _invoke("haste_hip_causal_conv_backward" + suffix, T, N, D, W, *_strided(x), kernel.data_ptr(), _address(bias), bool(silu),
-            _address(state), _address(lengths), *_strided(dy), _address(dstate_out), dx.data_ptr(), dkernel.data_ptr(),
-            _address(dbias), _address(dstate), scratch.data_ptr(), scratch.numel())
+    _place(values, kept, dy, 2)
+    values += (_address(dstate_out), dx.data_ptr(), dkernel.data_ptr(), _address(dbias), _address(dstate), scratch.data_ptr(),
+               scratch.numel())
+    _invoke(device, "haste_hip_causal_conv_backward" + suffix, values)
     return dx, dkernel, dbias, dstate
 
 
-@_on_device_of(0, "x")
 def causal_conv_iterate(x, state, kernel, bias=None, silu=False, state_out=None):
     """One step: x[N,D], state[W-1,N,D] -> y[N,D], state_out (which may be given, and may be state)."""
-    x, kernel, bias, read, suffix = _conv_arguments(x, kernel, bias, state, None, steps=False)
-    (N, D), W = x.shape, kernel.shape[0]
-    if read is None:
-        raise ValueError("state must be %s %s on %s, got None" % (x.dtype, [W - 1, N, D], x.device))
-    y = x.new_empty((N, D))
+    values, kept, device, suffix = _conv_arguments(x, kernel, bias, silu, state, None, steps=False)
+    if state is None:
+        raise ValueError("state must be %s %s on %s, got None" % (x.dtype, [kernel.shape[0] - 1, *x.shape], x.device))
+    y = x.new_empty(x.shape)
     if state_out is None:
-        state_out = torch.empty_like(read)
+        state_out = torch.empty_like(kept[2])
     else:
-        _output("state_out", state_out, (W - 1, N, D), x.dtype, x)
-    _invoke("haste_hip_causal_conv_forward" + suffix, 1, N, D, W, x.data_ptr(), 0, x.stride(0), kernel.data_ptr(),
-            _address(bias), bool(silu), read.data_ptr(), None, y.data_ptr(), state_out.data_ptr())
+        _output("state_out", state_out, state.shape, x.dtype, x)
+        _apart("state_out", state_out, state, x, kernel, bias)
+    values += (y.data_ptr(), state_out.data_ptr())
+    _invoke(device, "haste_hip_causal_conv_forward" + suffix, values)
     return y, state_out
 
 
-def _scan_arguments(x, delta, A, B, C, D, z, delta_bias, steps=True):
-    """The arguments checked: (x, delta, A, B, C, D, z, delta_bias) as the entry points take them, S, G and the suffix."""
+def _scan_arguments(x, delta, A, B, C, D, z, delta_bias, softplus, steps=True):
+    """The arguments checked: the inputs as the entry points take them, the tensors (A, D, delta_bias, ...) to keep until the
+    call, S, G, the device and the suffix."""
     dims = 3 if steps else 2
     if not isinstance(x, torch.Tensor) or x.dim() != dims or not x.numel():
         raise ValueError("x must be [%s], of no size 0, got %s" % ("T,N,D" if steps else "N,D", _described(x)))
@@ -817,89 +821,88 @@ def _scan_arguments(x, delta, A, B, C, D, z, delta_bias, steps=True):
             if t is not None:
                 _float(what, t, width, x)
         _activation("z", z, full, x)
-    A, D, delta_bias, z = _contiguous(A), _contiguous(D), _contiguous(delta_bias), z if z is None else _packed_rows(z)
-    packed = _packed_groups if grouped else _packed_rows
-    return _packed_rows(x), _packed_rows(delta), A, packed(B), packed(C), D, z, delta_bias, S, G, _activation_suffix(x)
+    A, D, delta_bias = _contiguous(A), _contiguous(D), _contiguous(delta_bias)
+    suffix, axes, values, kept = _activation_suffix(x), dims - 1, [], [A, D, delta_bias]
+    _place(values, kept, x, axes)
+    _place(values, kept, delta, axes)
+    values.append(A.data_ptr())
+    _place(values, kept, B, axes, grouped)
+    _place(values, kept, C, axes, grouped)
+    values.append(_address(D))
+    _place(values, kept, z, axes)
+    values += (_address(delta_bias), bool(softplus))
+    return values, kept, S, G, device, suffix
 
 
-@_on_device_of(1, "x")
 def selective_scan_forward(training, x, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False, h0=None,
                            lengths=None):
     """x, delta, z[T,N,D], A[D,S], B, C[T,N,G,S] ([T,N,S]: one group), D, delta_bias[D], h0[N,D,S]
     -> y[T,N,D], h_last[N,D,S], cache (what the backward pass needs; None unless training):
     dt = delta + delta_bias, of which delta_softplus takes the softplus; h[t] = exp(dt A) h[t-1] + dt x B;
     y = (sum_s C h + D x) z sigmoid(z).  Parts that are None are left out."""
-    x, delta, A, B, C, D, z, delta_bias, S, G, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias)
+    values, kept, S, G, device, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias, delta_softplus)
     T, N, channels = x.shape
     if h0 is not None:
         h0 = _float("h0", h0, (N, channels, S), x)
     if lengths is not None:
         _check_lengths(lengths, x)
-    y = torch.empty(T, N, channels, device=x.device, dtype=x.dtype)
-    h_last = torch.empty(N, channels, S, device=x.device)
+    y, h_last = x.new_empty(x.shape), torch.empty((N, channels, S), device=x.device)
     cache = None
     if training:
         cache = _scratch("haste_hip_selective_scan_kept_bytes", x, T, N, channels, S)
     scratch = _scratch("haste_hip_selective_scan_workspace_bytes", x, 0, T, N, channels, S, G)
-    _invoke("haste_hip_selective_scan_forward" + suffix, T, N, channels, S, G, *_strided(x), *_strided(delta), A.data_ptr(),
-            *_strided(B), *_strided(C), _address(D), *_strided(z), _address(delta_bias), bool(delta_softplus), _address(h0),
-            _address(lengths), y.data_ptr(), h_last.data_ptr(), _address(cache), scratch.data_ptr(), scratch.numel())
+    _invoke(device, "haste_hip_selective_scan_forward" + suffix,
+            [T, N, channels, S, G, *values, _address(h0), _address(lengths), y.data_ptr(), h_last.data_ptr(), _address(cache),
+             scratch.data_ptr(), scratch.numel()])
     return y, h_last, cache
 
 
-@_on_device_of(0, "x")
 def selective_scan_backward(x, delta, A, B, C, D, z, delta_bias, delta_softplus, h0, lengths, cache, dy, dh_last=None):
     """Gradients (dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dh0) from those of y (None: zeros) and h_last, and the cache of
     the forward pass of the same arguments; those of arguments that are None are None (dh0 is always given)."""
-    dims_B = B.shape if torch.is_tensor(B) else None
-    x, delta, A, B, C, D, z, delta_bias, S, G, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias)
+    values, kept, S, G, device, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias, delta_softplus)
     T, N, channels = x.shape
     if lengths is not None:
         _check_lengths(lengths, x)
-    kept = _scratch_bytes("haste_hip_selective_scan_kept_bytes", x.device, T, N, channels, S)
-    if not torch.is_tensor(cache) or cache.dtype != torch.uint8 or cache.numel() != kept or cache.device != x.device:
+    size = _scratch_bytes("haste_hip_selective_scan_kept_bytes", x.device, T, N, channels, S)
+    if not torch.is_tensor(cache) or cache.dtype != torch.uint8 or cache.numel() != size or cache.device != x.device:
         raise ValueError("the cache must be that of a forward pass in training over the same arguments")
     dy = _zero_rows(T, N, channels, x) if dy is None else dy
     _activation("dy", dy, x.shape, x)
-    dy = _packed_rows(dy)
     if dh_last is not None:
         dh_last = _float("dh_last", dh_last, (N, channels, S), x)
-    like = dict(device=x.device, dtype=x.dtype)
-    dx, ddelta = torch.empty(T, N, channels, **like), torch.empty(T, N, channels, **like)
-    dz = None if z is None else torch.empty(T, N, channels, **like)
-    dB, dC = torch.empty(dims_B, **like), torch.empty(dims_B, **like)
-    dA, dh0 = torch.empty_like(A), torch.empty(N, channels, S, device=x.device)
-    dD = None if D is None else torch.empty_like(D)
-    dbias = None if delta_bias is None else torch.empty_like(delta_bias)
+    dx, ddelta, dB, dC = x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(B.shape), x.new_empty(B.shape)
+    dz = None if z is None else x.new_empty(x.shape)
+    dA, dD, dbias = (None if t is None else torch.empty_like(t) for t in kept[:3])
+    dh0 = torch.empty((N, channels, S), device=x.device)
     scratch = _scratch("haste_hip_selective_scan_workspace_bytes", x, 1, T, N, channels, S, G)
-    _invoke("haste_hip_selective_scan_backward" + suffix, T, N, channels, S, G, *_strided(x), *_strided(delta), A.data_ptr(),
-            *_strided(B), *_strided(C), _address(D), *_strided(z), _address(delta_bias), bool(delta_softplus),
-            _address(lengths), cache.data_ptr(), *_strided(dy), _address(dh_last), dx.data_ptr(), ddelta.data_ptr(),
-            dA.data_ptr(), dB.data_ptr(), dC.data_ptr(), _address(dD), _address(dz), _address(dbias), dh0.data_ptr(),
-            scratch.data_ptr(), scratch.numel())
+    values = [T, N, channels, S, G, *values, _address(lengths), cache.data_ptr()]
+    _place(values, kept, dy, 2)
+    values += (_address(dh_last), dx.data_ptr(), ddelta.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(), _address(dD),
+               _address(dz), _address(dbias), dh0.data_ptr(), scratch.data_ptr(), scratch.numel())
+    _invoke(device, "haste_hip_selective_scan_backward" + suffix, values)
     return dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0
 
 
-@_on_device_of(0, "x")
 def selective_scan_iterate(x, delta, A, B, C, h, D=None, z=None, delta_bias=None, delta_softplus=False, h_out=None):
     """One step: x, delta, z[N,D], B, C[N,G,S] ([N,S]), h[N,D,S] -> y[N,D], h_out (which may be given, and may be h)."""
-    x, delta, A, B, C, D, z, delta_bias, S, G, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias, steps=False)
+    values, kept, S, G, device, suffix = _scan_arguments(x, delta, A, B, C, D, z, delta_bias, delta_softplus, steps=False)
     N, channels = x.shape
-    h = _float("h", h, (N, channels, S), x)
+    read = _float("h", h, (N, channels, S), x)
     y = x.new_empty((N, channels))
     if h_out is None:
-        h_out = torch.empty_like(h)
+        h_out = torch.empty_like(read)
     else:
         _output("h_out", h_out, (N, channels, S), torch.float32, x)
-    _invoke("haste_hip_selective_scan_iterate" + suffix, N, channels, S, G, x.data_ptr(), x.stride(0), delta.data_ptr(),
-            delta.stride(0), A.data_ptr(), B.data_ptr(), B.stride(0), C.data_ptr(), C.stride(0), _address(D), _address(z),
-            0 if z is None else z.stride(0), _address(delta_bias), bool(delta_softplus), h.data_ptr(), y.data_ptr(),
-            h_out.data_ptr())
+        _apart("h_out", h_out, h, x, delta, A, B, C, D, z, delta_bias)
+    _invoke(device, "haste_hip_selective_scan_iterate" + suffix,
+            [N, channels, S, G, *values, read.data_ptr(), y.data_ptr(), h_out.data_ptr()])
     return y, h_out
 
 
 def _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias):
-    """The arguments checked, activations as [T,N,D]."""
+    """The arguments checked: the inputs as the entry points take them up to before_weight, the weights, the tensors to keep until
+    the call, the device and the suffix."""
     if not isinstance(update, torch.Tensor) or update.dim() not in (2, 3) or not update.numel():
         raise ValueError("update must be [T,N,D] or [N,D], of no size 0, got %s" % _described(update))
     D = update.shape[-1]
@@ -921,57 +924,55 @@ def _norm_arguments(update, residual, gate, scale, after_weight, before_weight, 
             if t is not None:
                 _float(what, t, width, update)
     weights = _contiguous(scale), _contiguous(after_weight), _contiguous(before_weight), _contiguous(before_bias)
-    return (_packed(update), _packed(residual), _packed(gate)), weights, _activation_suffix(update)
+    suffix, values, kept = _activation_suffix(update), [*((1, *full) if len(full) == 2 else full)], [weights]
+    for t in (update, residual, gate):
+        _place_rows(values, kept, t)
+    values += map(_address, weights[:3])
+    return values, weights, kept, device, suffix
 
 
-def _packed(t):
-    return t if t is None else _packed_rows(t)
+def _place_rows(values, kept, t):
+    """_place() of [T,N,D], or of [N,D] as one step."""
+    if t is None or t.dim() == 3:
+        _place(values, kept, t, 2)
+    else:
+        _place(values, kept, t, 1)
+        values.insert(-1, 0)
 
 
-def _norm_rows(t):
-    """As _strided, of [T,N,D] or [N,D]."""
-    if t is None:
-        return None, 0, 0
-    strides = t.stride()
-    return (t.data_ptr(), strides[0], strides[1]) if len(strides) == 3 else (t.data_ptr(), 0, strides[0])
-
-
-@_on_device_of(0, "update")
 def residual_norm_forward(update, residual=None, gate=None, scale=None, after_weight=None, before_weight=None, before_bias=None,
                           centered=False, eps=1e-5):
     """update, residual, gate[T,N,D] (or [N,D]), weights[D] -> out, normed (None without before_weight), stats:
     out = residual + scale norm(update) after_weight gate sigmoid(gate), normed = norm(out) before_weight + before_bias,
     norm(v) = v / sqrt(mean v^2 + eps), centered: of v - mean v.  Parts that are None are left out (update is not normed without
     after_weight); stats is what the backward pass needs."""
-    rows, weights, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
-    T, N, D = update.shape if update.dim() == 3 else (1, *update.shape)
+    values, weights, kept, device, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
     out = update.new_empty(update.shape)
     normed = None if before_weight is None else torch.empty_like(out)
-    stats = torch.empty((T, N, 4), device=update.device)
-    _invoke("haste_hip_residual_norm_forward" + suffix, T, N, D, *_norm_rows(rows[0]), *_norm_rows(rows[1]), *_norm_rows(rows[2]),
-            *map(_address, weights), bool(centered), float(eps), out.data_ptr(), _address(normed), stats.data_ptr())
+    stats = torch.empty((values[0], values[1], 4), device=update.device)
+    values += (_address(weights[3]), bool(centered), float(eps), out.data_ptr(), _address(normed), stats.data_ptr())
+    _invoke(device, "haste_hip_residual_norm_forward" + suffix, values)
     return out, normed, stats
 
 
-@_on_device_of(0, "update")
 def residual_norm_backward(update, residual, gate, scale, after_weight, before_weight, before_bias, stats, dout, dnormed,
                            centered=False):
     """Gradients (dupdate, dresidual, dgate, dscale, dafter_weight, dbefore_weight, dbefore_bias) from those of out and normed
     (either may be None: zeros); those of arguments that are None are None."""
-    rows, weights, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
-    T, N, D = update.shape if update.dim() == 3 else (1, *update.shape)
+    values, weights, kept, device, suffix = _norm_arguments(update, residual, gate, scale, after_weight, before_weight, before_bias)
+    T, N, D = values[:3]
     stats = _float("stats", stats, (T, N, 4), update)
     if dnormed is not None and before_weight is None:
         raise ValueError("dnormed needs before_weight")
     for what, t in (("dout", dout), ("dnormed", dnormed)):
         if t is not None:
             _activation(what, t, update.shape, update)
-    grads = [None if t is None else torch.empty(update.shape, device=update.device, dtype=update.dtype)
-             for t in (update, residual, gate)]
+    grads = [None if t is None else t.new_empty(t.shape) for t in (update, residual, gate)]
     sums = [None if w is None else torch.empty_like(w) for w in weights]
     scratch = _scratch("haste_hip_residual_norm_workspace_bytes", update, T, N, D)
-    dout, dnormed = _packed(dout), _packed(dnormed)
-    _invoke("haste_hip_residual_norm_backward" + suffix, T, N, D, *_norm_rows(rows[0]), *_norm_rows(rows[1]), *_norm_rows(rows[2]),
-            *map(_address, weights[:3]), bool(centered), stats.data_ptr(), *_norm_rows(dout), *_norm_rows(dnormed),
-            *map(_address, grads), *map(_address, sums), scratch.data_ptr(), scratch.numel())
+    values += (bool(centered), stats.data_ptr())
+    _place_rows(values, kept, dout)
+    _place_rows(values, kept, dnormed)
+    values += (*map(_address, grads), *map(_address, sums), scratch.data_ptr(), scratch.numel())
+    _invoke(device, "haste_hip_residual_norm_backward" + suffix, values)
     return (*grads, *sums)

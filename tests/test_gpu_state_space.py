@@ -545,3 +545,36 @@ def test_steps_from_no_state():
         y, h = scan(x, delta, B, C, z)
         y1, h1 = scan.step(x[0], delta[0], B[0], C[0], z[0])
         assert (y[0] - y1).abs().max() <= 1e-5 and (h - h1).abs().max() <= 1e-5
+
+
+def test_outputs_that_overlap_inputs_are_refused():
+    N, D, S, W = 2, 8, 4, 4
+    buffer = torch.randn(W, N, D, device="cuda")
+    kernel = torch.randn(W, D, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):  # the states before and after a step, a row apart
+        ops.causal_conv_iterate(torch.randn(N, D, device="cuda"), buffer[:3], kernel, state_out=buffer[1:])
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.causal_conv_iterate(buffer[3], torch.randn(3, N, D, device="cuda"), kernel, state_out=buffer[1:])
+    states = torch.randn(N + 1, D, S, device="cuda")
+    step = [torch.randn(N, D, device="cuda"), torch.randn(N, D, device="cuda"), -torch.rand(D, S, device="cuda"),
+            torch.randn(N, S, device="cuda"), torch.randn(N, S, device="cuda")]
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.selective_scan_iterate(*step, states[:N], h_out=states[1:])
+    y, h = ops.selective_scan_iterate(*step, states[:N])
+    again = states.clone()
+    y2, h2 = ops.selective_scan_iterate(*step, again[:N], h_out=again[:N])
+    assert torch.equal(y, y2) and torch.equal(h, again[:N]) and torch.equal(states[N], again[N])
+
+
+def test_strided_states_are_copied():
+    q, s = conv_problem(2, torch.float32, 1, 3, 20, 4), scan_problem(2, torch.float32, 1, 3, 20, 4)
+    state = q.g["state"].transpose(0, 1).contiguous().transpose(0, 1)
+    want = ops.causal_conv_iterate(q.g["x"][0], q.g["state"], q.g["kernel"], q.g["bias"], True)
+    got = ops.causal_conv_iterate(q.g["x"][0], state, q.g["kernel"].t().contiguous().t(), q.g["bias"], True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    g = {k: v[0] if k in ("x", "delta", "B", "C", "z") else v for k, v in s.g.items()}
+    h = g["h0"].transpose(1, 2).contiguous().transpose(1, 2)
+    A = g["A"].t().contiguous().t()
+    want = ops.selective_scan_iterate(g["x"], g["delta"], g["A"], g["B"], g["C"], g["h0"])
+    got = ops.selective_scan_iterate(g["x"], g["delta"], A, g["B"], g["C"], h)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
