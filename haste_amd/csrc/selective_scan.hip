@@ -17,8 +17,9 @@
 //
 // The time axis is cut into chunks where there are too few rows and channels to fill the chip: a first
 // pass finds what each chunk adds to a state of zero and sum dt, by which it decays what it is given
-// (exp(A sum dt)), the states at the chunks' starts follow one from the other, and the second pass runs all
-// chunks at once.  The same backwards with G.
+// (exp(A sum dt)); the second pass runs all chunks at once, each from what those before it hand over.
+// The same backwards with G.
+#include <cmath>
 #include <type_traits>
 
 #include "sequence.h"
@@ -235,12 +236,38 @@ struct WalkShared {
   }
 };
 
+// What the chunks before this one hand over: chunk first, first + step, ..., `count` of them, one after the other.  Chunk c
+// decays what it is given (in h) over its sum of dt, sum_dt[c], and adds at[c], what it makes of a state of zero.  Every
+// workgroup does this for itself: a kernel between the two passes costs more, 7 us more of 54 (T=4096 N=1 D=1024 S=16 bf16, 32 chunks)
+// and 19 of 73 (T=8192 N=1 D=256, 64 and 128 chunks).
+__device__ __forceinline__ void join_chunks(float (&h)[K], const float (&A2)[K], const float* at, const float* sum_dt, size_t state,
+                                            size_t states, size_t channel, size_t channels, int first, int step, int count, int s0,
+                                            int S) {
+  constexpr int AHEAD = 4;  // chunks read at once
+  for (int k = 0; k < count; k += AHEAD) {
+    float added[AHEAD][K], dt[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int c = first + step * min(k + j, count - 1);
+      load_states(at + c * states + state, s0, S, added[j]);
+      dt[j] = sum_dt[c * channels + channel];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (k + j >= count) break;
+#pragma unroll
+      for (int r = 0; r < K; ++r)  // (0 times a product of growth beyond float's range is 0, not NaN)
+        h[r] = h[r] == 0.f ? added[j][r] : __builtin_amdgcn_exp2f(A2[r] * dt[j]) * h[r] + added[j][r];
+    }
+  }
+}
+
 // Forward pass over a chunk.  LOCAL: only what the chunk adds to a state of zero, and the sum of dt.
-// starts: the states at the chunks' starts [chunks][N][D][S] (LOCAL: out, what each but the last adds), null when
-// there is one chunk; kept: the states at the tiles' starts [tiles][N][D][S], or null.
+// added: what the chunks but the last add [chunks][N][D][S], and sum_dt [chunks][N][D] (LOCAL: out).  kept: the states at
+// the tiles' starts [tiles][N][D][S], or null.
 template <typename T, int LANES, bool LOCAL>
 __global__ __launch_bounds__(256)
-void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ h0, float* __restrict__ starts,
+void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ h0, float* __restrict__ added,
                                    float* __restrict__ sum_dt, float* __restrict__ kept, T* __restrict__ y,
                                    float* __restrict__ h_last) {
   typedef Place<LANES> P;
@@ -267,8 +294,9 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
 #pragma unroll
     for (int r = 0; r < K; ++r) A2[r] *= kLog2e;
     if (!LOCAL) {
-      if (blockIdx.y > 0) load_states(starts + blockIdx.y * states + state, s0, s.S, h);
-      else if (h0 != nullptr) load_states(h0 + state, s0, s.S, h);
+      if (h0 != nullptr) load_states(h0 + state, s0, s.S, h);
+      if (blockIdx.y > 0)
+        join_chunks(h, A2, added, sum_dt, state, states, (size_t)b.n * s.D + d, (size_t)s.N * s.D, 0, 1, blockIdx.y, s0, s.S);
     }
   }
   float bias[L::WIDTH], skip[L::WIDTH];
@@ -388,7 +416,7 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
 
   if (LOCAL) {
     if (live) {
-      store_states(starts + blockIdx.y * states + state, s0, s.S, h);
+      store_states(added + blockIdx.y * states + state, s0, s.S, h);
       if (s0 == 0) sum_dt[((size_t)blockIdx.y * s.N + b.n) * s.D + d] = dt_sum;
     }
     return;
@@ -407,36 +435,6 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
   }
 }
 
-// The chunks one after the other, in place: at[c] is what chunk c adds to a state of zero, and becomes
-// what it is given.  Forward from `first` at chunk 0, backward (REVERSE) from it at the last chunk.
-template <bool REVERSE>
-__global__ __launch_bounds__(256)
-void scan_chunks_kernel(ScanShape s, const float* __restrict__ A, const float* __restrict__ first,
-                        const float* __restrict__ sum_dt, float* __restrict__ at) {
-  const size_t states = (size_t)s.N * s.D * s.S, i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= states) return;
-  const size_t channel = i / s.S;
-  const float A2 = A[channel % s.D * s.S + i % s.S] * kLog2e;
-  float h = first != nullptr ? first[i] : 0.f;
-  constexpr int AHEAD = 8;  // chunks read at once: only the products follow one from the other
-  for (int k0 = 0; k0 < s.chunks; k0 += AHEAD) {
-    float added[AHEAD], decay[AHEAD];
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int k = k0 + j, c = REVERSE ? s.chunks - 1 - k : k;
-      const bool follows = k + 1 < s.chunks;  // behind the last nothing does, and what it adds was not computed
-      added[j] = follows ? at[c * states + i] : 0.f;
-      decay[j] = follows ? __builtin_amdgcn_exp2f(A2 * sum_dt[(size_t)c * s.N * s.D + channel]) : 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int k = k0 + j, c = REVERSE ? s.chunks - 1 - k : k;
-      if (k < s.chunks) at[c * states + i] = h;
-      h = h == 0.f ? added[j] : decay[j] * h + added[j];  // (0 times a product of growth beyond float's range is 0, not NaN)
-    }
-  }
-}
-
 // What a backward pass writes besides dB and dC.
 template <typename T>
 struct ScanGradients {
@@ -447,12 +445,11 @@ struct ScanGradients {
 };
 
 // Backward pass over a chunk.  LOCAL: only G at the chunk's start for a gradient of zero at its end, and
-// the sum of dt.  ends: [chunks][N][D][S], the gradients at the chunks' ends
-// (LOCAL: out, but for the first chunk), null when there is one chunk.
+// the sum of dt.  added, sum_dt: as forward, of the chunks but the first.
 template <typename T, int LANES, bool LOCAL>
 __global__ __launch_bounds__(256, 2)
 void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ kept, Rows<const T> dy,
-                                    const float* __restrict__ dh_last, float* __restrict__ ends, float* __restrict__ sum_dt,
+                                    const float* __restrict__ dh_last, float* __restrict__ added, float* __restrict__ sum_dt,
                                     ScanGradients<T> out) {
   typedef Place<LANES> P;
   typedef Tile<LANES> L;
@@ -477,17 +474,18 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
 
   float A[K], A2[K], G[K], dA[K], dt_sum = 0.f;
 #pragma unroll
-  for (int r = 0; r < K; ++r) A[r] = G[r] = dA[r] = 0.f;
+  for (int r = 0; r < K; ++r) A[r] = A2[r] = G[r] = dA[r] = 0.f;
   if (live) {
     load_states(in.A + (size_t)d * s.S, s0, s.S, A);
-    if (chunk + 1 == (unsigned)s.chunks) {
-      if (dh_last != nullptr && !LOCAL) load_states(dh_last + state, s0, s.S, G);
-    } else if (!LOCAL) {
-      load_states(ends + chunk * states + state, s0, s.S, G);
+#pragma unroll
+    for (int r = 0; r < K; ++r) A2[r] = A[r] * kLog2e;
+    if (!LOCAL) {
+      if (dh_last != nullptr) load_states(dh_last + state, s0, s.S, G);
+      if (chunk + 1 < (unsigned)s.chunks)
+        join_chunks(G, A2, added, sum_dt, state, states, (size_t)b.n * s.D + d, (size_t)s.N * s.D, s.chunks - 1, -1,
+                    s.chunks - 1 - (int)chunk, s0, s.S);
     }
   }
-#pragma unroll
-  for (int r = 0; r < K; ++r) A2[r] = A[r] * kLog2e;
   const int column = L::column();
   float bias[L::WIDTH], skip[L::WIDTH], dskip[L::WIDTH], dbias[L::WIDTH];
 #pragma unroll
@@ -666,7 +664,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
 
   if (LOCAL) {
     if (live) {
-      store_states(ends + chunk * states + state, s0, s.S, G);
+      store_states(added + chunk * states + state, s0, s.S, G);
       if (s0 == 0) sum_dt[((size_t)chunk * s.N + b.n) * s.D + d] = dt_sum;
     }
     return;
@@ -781,7 +779,9 @@ int with_lanes(int S, F&& f) {
 }
 
 // The time axis is cut where a batch row's channels and the rows make less than a workgroup a CU, into chunks that make about
-// two, of no fewer than 4 tiles.  The first of the two passes costs four fifths of the second, so that at a workgroup a CU or
+// two, of no fewer than 4 tiles and of no more than so many that joining them (a memory round trip for every four) takes the
+// time of the steps saved: 3 sqrt(tiles), T=8192 N=1 D=128 and T=32768 N=1 D=64 forward 46 and 110 us with 64 chunks,
+// 55 and 85 with 128, 54 and 158 with 512.  The first of the two passes costs four fifths of the second, so that at a workgroup a CU or
 // more it is not won back: forward and backward with T=2048, D=4096, S=16 bf16, in two chunks and in one: N=4 (256 workgroups) 826 and
 // 949 us, N=5 1277 and 1253, N=7 1417 and 1237; T=128 N=32 D=512 (256) 81 and 72, T=256 N=12 D=2048 (384) 180 and 166.
 ScanShape shape_of(int T, int N, int D, int S, int G, int softplus) {
@@ -791,7 +791,9 @@ ScanShape shape_of(int T, int N, int D, int S, int G, int softplus) {
   const size_t blocks = (size_t)N * G * s.blocks_group, cus = (size_t)device_cu_count();
   const size_t tiles = ((size_t)T + TS - 1) / TS, most = tiles / 4 > 0 ? tiles / 4 : 1;
   size_t chunks = blocks >= cus ? 1 : 2 * cus / blocks;
+  const size_t join = (size_t)(3.0 * std::sqrt((double)tiles));
   chunks = chunks < most ? chunks : most;
+  chunks = chunks < join ? chunks : join;
   s.chunk = (int)((tiles + chunks - 1) / chunks) * TS;
   s.chunks = (int)(((size_t)T + s.chunk - 1) / s.chunk);
   return s;
@@ -799,7 +801,7 @@ ScanShape shape_of(int T, int N, int D, int S, int G, int softplus) {
 
 // Floats of workspace, in the order they lie there.
 struct ScanWorkspace {
-  size_t at_chunks, sum_dt, partial, sums, dB, dC, total;
+  size_t added, sum_dt, partial, sums, dB, dC, total;
 };
 ScanWorkspace forward_workspace(const ScanShape& s) {
   ScanWorkspace w = {};
@@ -823,24 +825,22 @@ ScanWorkspace backward_workspace(const ScanShape& s) {
 template <typename T>
 int forward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, const float* h0, T* y, float* h_last, float* kept,
             float* workspace, size_t workspace_bytes) {
-  const size_t blocks = (size_t)s.N * s.G * s.blocks_group, states = (size_t)s.N * s.D * s.S;
+  const size_t blocks = (size_t)s.N * s.G * s.blocks_group;
   const ScanWorkspace w = forward_workspace(s);
-  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ || (states + 255) / 256 > kGridLimit)
+  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ)
     return too_large("selective_scan: too many rows of channels");
   if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_forward: the workspace is too small");
   HASTE_HIP_REQUIRE(workspace != nullptr || w.total == 0);
-  float *starts = workspace, *sum_dt = s.chunks > 1 ? workspace + w.sum_dt : nullptr;
+  float *added = workspace, *sum_dt = s.chunks > 1 ? workspace + w.sum_dt : nullptr;
   return with_lanes(s.S, [&](auto lanes) {
     dim3 grid((unsigned)blocks, s.chunks);
     if (s.chunks > 1) {
       ScopedKernelTimer timer("selective_scan_chunks", stream);
-      selective_scan_forward_kernel<T, lanes(), true><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, starts, sum_dt, nullptr, nullptr, nullptr);
-      HASTE_HIP_TRY(hipGetLastError());
-      scan_chunks_kernel<false><<<(unsigned)((states + 255) / 256), 256, 0, stream>>>(s, in.A, h0, sum_dt, starts);
+      selective_scan_forward_kernel<T, lanes(), true><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, added, sum_dt, nullptr, nullptr, nullptr);
       HASTE_HIP_TRY(hipGetLastError());
     }
     ScopedKernelTimer timer("selective_scan_forward", stream);
-    selective_scan_forward_kernel<T, lanes(), false><<<grid, 256, 0, stream>>>(s, in, h0, starts, nullptr, kept, y, h_last);
+    selective_scan_forward_kernel<T, lanes(), false><<<grid, 256, 0, stream>>>(s, in, h0, added, sum_dt, kept, y, h_last);
     HASTE_HIP_TRY(hipGetLastError());
     return HASTE_HIP_OK;
   });
@@ -850,25 +850,23 @@ template <typename T>
 int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, const float* kept, const Rows<const T>& dy,
              const float* dh_last, T* dx, T* ddelta, float* dA, T* dB, T* dC, float* dskip, T* dz, float* dbias, float* dh0,
              float* workspace, size_t workspace_bytes) {
-  const size_t blocks = (size_t)s.N * s.G * s.blocks_group, states = (size_t)s.N * s.D * s.S;
+  const size_t blocks = (size_t)s.N * s.G * s.blocks_group;
   const size_t shared = (size_t)s.T * s.N * s.G * s.S, columns = (size_t)s.D * (s.S + 2);
   const ScanWorkspace w = backward_workspace(s);
-  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ || (states + 255) / 256 > kGridLimit || (shared + 255) / 256 > kGridLimit)
+  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ || (shared + 255) / 256 > kGridLimit)
     return too_large("selective_scan: too many rows of channels");
   if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_backward: the workspace is too small");
-  float *ends = workspace + w.at_chunks, *sum_dt = workspace + w.sum_dt;
+  float *added = workspace + w.added, *sum_dt = workspace + w.sum_dt;
   const ScanGradients<T> out = {dx, ddelta, dz, dh0, workspace + w.partial, workspace + w.dB, workspace + w.dC};
   HASTE_HIP_PROPAGATE(with_lanes(s.S, [&](auto lanes) {
     dim3 grid((unsigned)blocks, s.chunks);
     if (s.chunks > 1) {
       ScopedKernelTimer timer("selective_scan_chunks", stream);
-      selective_scan_backward_kernel<T, lanes(), true><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, dy, dh_last, ends, sum_dt, out);
-      HASTE_HIP_TRY(hipGetLastError());
-      scan_chunks_kernel<true><<<(unsigned)((states + 255) / 256), 256, 0, stream>>>(s, in.A, dh_last, sum_dt, ends);
+      selective_scan_backward_kernel<T, lanes(), true><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, dy, dh_last, added, sum_dt, out);
       HASTE_HIP_TRY(hipGetLastError());
     }
     ScopedKernelTimer timer("selective_scan_backward", stream);
-    selective_scan_backward_kernel<T, lanes(), false><<<grid, 256, 0, stream>>>(s, in, kept, dy, dh_last, ends, sum_dt, out);
+    selective_scan_backward_kernel<T, lanes(), false><<<grid, 256, 0, stream>>>(s, in, kept, dy, dh_last, added, sum_dt, out);
     HASTE_HIP_TRY(hipGetLastError());
     return HASTE_HIP_OK;
   }));

@@ -137,6 +137,7 @@ SCAN_CASES = [
     (50, 2, 36, 64, dict(dh=False)), (31, 2, 40, 5, dict(G=4)), (35, 2, 390, 16, dict(G=3)), (20, 2, 70, 33, dict(G=2)),
     # long enough for the time axis to be cut
     (64, 1, 64, 16, {}), (129, 1, 64, 16, {}), (300, 2, 48, 16, dict(G=2)), (520, 1, 20, 7, {}), (400, 1, 33, 64, {}),
+    (1300, 1, 9, 5, {}), (1300, 2, 20, 16, dict(lengths=[1300, 777])), (1100, 2, 8, 40, dict(lengths=[64, -1], h0=False, dh=False)),
     (20, 6, 30, 16, dict(lengths=[20, 0, 1, 16, 17, -2])), (300, 4, 40, 16, dict(lengths=[300, 0, 70, 128])),
     (200, 3, 17, 12, dict(lengths=[-1, 65, 64], h0=False)), (6, 2, 300, 16, dict(lengths=[0, 0])), (2, 90, 130, 16, {})]
 
