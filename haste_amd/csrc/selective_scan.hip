@@ -778,22 +778,22 @@ int with_lanes(int S, F&& f) {
   }
 }
 
-// The time axis is cut where a batch row's channels and the rows make less than a workgroup a CU, into chunks that make about
-// two, of no fewer than 4 tiles and of no more than so many that joining them (a memory round trip for every four) takes the
-// time of the steps saved: 3 sqrt(tiles), T=8192 N=1 D=128 and T=32768 N=1 D=64 forward 46 and 110 us with 64 chunks,
-// 55 and 85 with 128, 54 and 158 with 512.  The first of the two passes costs four fifths of the second, so that at a workgroup a CU or
-// more it is not won back: forward and backward with T=2048, D=4096, S=16 bf16, in two chunks and in one: N=4 (256 workgroups) 826 and
-// 949 us, N=5 1277 and 1253, N=7 1417 and 1237; T=128 N=32 D=512 (256) 81 and 72, T=256 N=12 D=2048 (384) 180 and 166.
-ScanShape shape_of(int T, int N, int D, int S, int G, int softplus) {
+// The time axis is cut where rows and channels make too few workgroups, into chunks that make about two a CU, of no fewer than 4
+// tiles, and of no more than so many that joining them (a memory round trip for every four) takes the time of the steps saved:
+// 3 sqrt(tiles), T=8192 N=1 D=128 and T=32768 N=1 D=64 forward 46 and 110 us with 64 chunks, 55 and 85 with 128, 54 and 158 with 512.
+// The first of the two passes costs two thirds of the second.  Forward that is not won back by two chunks: one and two with T=2048
+// N=4 D=4096 S=16 bf16 (256 workgroups) 244 and 254 us, T=128 N=32 D=512 18 and 22.  Backward, where it costs two fifths,
+// it is: 680 and 559, 53 and 50.
+ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, bool backward) {
   ScanShape s = {T, N, D, S, G, D / G, 0, 0, 0, softplus};
   const int block = 256 / lanes_for(S);
   s.blocks_group = (s.share + block - 1) / block;
-  const size_t blocks = (size_t)N * G * s.blocks_group, cus = (size_t)device_cu_count();
-  const size_t tiles = ((size_t)T + TS - 1) / TS, most = tiles / 4 > 0 ? tiles / 4 : 1;
-  size_t chunks = blocks >= cus ? 1 : 2 * cus / blocks;
-  const size_t join = (size_t)(3.0 * std::sqrt((double)tiles));
+  const size_t blocks = (size_t)N * G * s.blocks_group, tiles = ((size_t)T + TS - 1) / TS;
+  const size_t least = backward ? 2 : 3, most = tiles / 4, join = (size_t)(3.0 * std::sqrt((double)tiles));
+  size_t chunks = 2 * (size_t)device_cu_count() / blocks;
   chunks = chunks < most ? chunks : most;
   chunks = chunks < join ? chunks : join;
+  if (chunks < least) chunks = 1;
   s.chunk = (int)((tiles + chunks - 1) / chunks) * TS;
   s.chunks = (int)(((size_t)T + s.chunk - 1) / s.chunk);
   return s;
@@ -922,8 +922,8 @@ using namespace haste_hip;
 
 size_t haste_hip_selective_scan_workspace_bytes(int backward, int steps, int batch_size, int channels, int states, int groups) {
   if (check_sizes(steps, batch_size, channels, states, groups) != HASTE_HIP_OK) return 0;
-  const size_t floats = backward ? backward_workspace(shape_of(steps, batch_size, channels, states, groups, 0)).total
-                                 : forward_workspace(shape_of(steps, batch_size, channels, states, groups, 0)).total;
+  const size_t floats = backward ? backward_workspace(shape_of(steps, batch_size, channels, states, groups, 0, true)).total
+                                 : forward_workspace(shape_of(steps, batch_size, channels, states, groups, 0, false)).total;
   return floats * sizeof(float);
 }
 
@@ -944,7 +944,7 @@ size_t haste_hip_selective_scan_kept_bytes(int steps, int batch_size, int channe
                                                 void* stream) {                                                        \
     HASTE_HIP_PROPAGATE(check_sizes(steps, batch_size, channels, states, groups));                                     \
     HASTE_HIP_REQUIRE(x && delta && A && B && C && y);                                                                 \
-    return forward<T>(as_stream(stream), shape_of(steps, batch_size, channels, states, groups, delta_softplus),   \
+    return forward<T>(as_stream(stream), shape_of(steps, batch_size, channels, states, groups, delta_softplus, false), \
                       inputs_of<T>(x, x_step, x_row, delta, delta_step, delta_row, A, B, B_step, B_row, C, C_step,     \
                                    C_row, D, z, z_step, z_row, delta_bias, lengths),                                   \
                       h0, static_cast<T*>(y), h_last, kept, static_cast<float*>(workspace), workspace_bytes);          \
@@ -957,7 +957,7 @@ size_t haste_hip_selective_scan_kept_bytes(int steps, int batch_size, int channe
     HASTE_HIP_PROPAGATE(check_sizes(steps, batch_size, channels, states, groups));                                     \
     HASTE_HIP_REQUIRE(x && delta && A && B && C && kept && dy && dx && ddelta && dA && dB && dC && workspace);         \
     HASTE_HIP_REQUIRE((z == nullptr) == (dz == nullptr));                                                              \
-    return backward<T>(as_stream(stream), shape_of(steps, batch_size, channels, states, groups, delta_softplus), \
+    return backward<T>(as_stream(stream), shape_of(steps, batch_size, channels, states, groups, delta_softplus, true), \
                        inputs_of<T>(x, x_step, x_row, delta, delta_step, delta_row, A, B, B_step, B_row, C, C_step,    \
                                     C_row, D, z, z_step, z_row, delta_bias, lengths),                                  \
                        kept, {static_cast<const T*>(dy), dy_step, dy_row}, dh_last, static_cast<T*>(dx),               \
