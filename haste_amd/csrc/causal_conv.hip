@@ -28,6 +28,14 @@ struct ConvShape {
   int silu;
 };
 
+// The channels of thread `vector` of a row.  The last one's are the row's last V, some of them also its neighbour's: both
+// compute and write the same, and no thread has channels beyond the row.  Not where a thread might read what its neighbour has
+// written: a state in place.
+__device__ __forceinline__ int first_channel(unsigned vector, int D, bool overlap) {
+  const int c = (int)vector * V;
+  return overlap && D >= V ? min(c, D - V) : c;
+}
+
 // X[p] for p >= 0: the state's rows, then the sequence.
 template <typename T>
 __device__ __forceinline__ void load_padded(const Rows<const T>& x, const T* state, int W, int p, int n, int c,
@@ -50,18 +58,7 @@ struct HeldSteps {
   __device__ __forceinline__ void load(const Rows<const T>& rows, int t, int end, int n, int c, int D) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      packed_t w = {};
-      if (t + u < end) {
-        const T* from = rows.at(t + u, n) + c;
-        if (c + V <= D) {
-          w = *reinterpret_cast<const typename Wide<T, V>::type*>(from);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (c + i < D) w[i] = from[i];
-        }
-      }
-      v[u] = w;
+      v[u] = t + u < end ? load_packed<V>(rows.at(t + u, n), c, D) : packed_t{};
     }
   }
   __device__ __forceinline__ void get(int u, float (&f)[V]) const {
@@ -78,7 +75,7 @@ void causal_conv_forward_kernel(ConvShape s, Rows<const T> x, const float* __res
   const unsigned vectors = (D + V - 1) / V;
   const unsigned item = blockIdx.x * 256 + threadIdx.x, n = item / vectors;
   if (n >= (unsigned)N) return;
-  const int c = (int)(item % vectors) * V;
+  const int c = first_channel(item % vectors, D, state_out == nullptr || state_out != state);
   const int t0 = blockIdx.y * s.chunk, t1 = min(T_, t0 + s.chunk);
   const Extent e = extent_of(lengths, n, T_);
   const int end = min(t1, e.steps);
@@ -159,7 +156,7 @@ void causal_conv_backward_kernel(ConvShape s, Rows<const T> x, const float* __re
   const unsigned vectors = (D + V - 1) / V;
   const unsigned item = blockIdx.x * 256 + threadIdx.x, n = item / vectors;
   if (n >= (unsigned)N) return;
-  const int c = (int)(item % vectors) * V;
+  const int c = first_channel(item % vectors, D, true);
   const int t0 = blockIdx.y * s.chunk, t1 = min(T_, t0 + s.chunk);
   const Extent e = extent_of(lengths, n, T_);
   const int own = min(t1, e.steps);                // dpre of steps below it counts towards dkernel here

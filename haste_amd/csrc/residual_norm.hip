@@ -54,16 +54,7 @@ struct Held {
   __device__ __forceinline__ void load(const T* row, int thread, int D) {
 #pragma unroll
     for (int p = 0; p < S::kPieces; ++p) {
-      const int c = S::column(p, thread);
-      packed_t w = {};
-      if (c + S::V <= D) {
-        w = *reinterpret_cast<const typename Wide<T, S::V>::type*>(row + c);
-      } else {
-#pragma unroll
-        for (int i = 0; i < S::V; ++i)
-          if (c + i < D) w[i] = row[c + i];
-      }
-      v[p] = w;
+      v[p] = load_packed<S::V>(row, S::column(p, thread), D);
     }
   }
   __device__ __forceinline__ float get(int i) const { return (float)v[i / S::V][i % S::V]; }
@@ -77,8 +68,7 @@ __device__ __forceinline__ void store_share(U* row, int thread, int D, const flo
     float v[S::V];
 #pragma unroll
     for (int i = 0; i < S::V; ++i) v[i] = f[p * S::V + i];
-    const int c = S::column(p, thread);
-    if (c < D) store_channels<S::V>(row, c, D, v);
+    store_channels<S::V>(row, S::column(p, thread), D, v);
   }
 }
 

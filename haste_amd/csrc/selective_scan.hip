@@ -37,7 +37,8 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 struct ScanShape {
   int T, N, D, S, G;
   int share;         // channels of a group, D / G
-  int blocks_group;  // workgroups of a group
+  int blocks_group;    // workgroups of a group
+  int block_channels;  // channels of a workgroup
   int chunk, chunks; // steps of a chunk (a multiple of TS)
   int softplus;
 };
@@ -119,17 +120,18 @@ __device__ __forceinline__ void store_states(float* p, int s0, int S, const floa
   store_channels<K>(p, s0, S, h);
 }
 
-// Which row and channels a workgroup works on.
+// Which row and channels a workgroup works on: c0 .. c_end-1.  The workgroups of a group share its channels evenly (in fours), so
+// that the last one is not left with one or two.
 template <int LANES>
 struct Block {
-  int n, g, c0, c_end;  // channels c0 .. of a group that ends at c_end
+  int n, g, c0, c_end;
   __device__ __forceinline__ Block(const ScanShape& s, unsigned block) {
     const unsigned per_row = s.G * s.blocks_group;
     n = block / per_row;
     const unsigned rest = block % per_row;
     g = rest / s.blocks_group;
-    c0 = g * s.share + (int)(rest % s.blocks_group) * Place<LANES>::kBlock;
-    c_end = (g + 1) * s.share;
+    c0 = g * s.share + (int)(rest % s.blocks_group) * s.block_channels;
+    c_end = min(c0 + s.block_channels, (g + 1) * s.share);
   }
 };
 
@@ -144,7 +146,15 @@ struct Tile {
   static constexpr int kRowStep = 256 / kPerRow;     // rows between a thread's items
   static constexpr int kShared = (TS * LANES * K + 255) / 256;  // elements of B (of C) a thread loads
   static __device__ __forceinline__ int row(int i) { return i * kRowStep + threadIdx.x / kPerRow; }
-  static __device__ __forceinline__ int column() { return (threadIdx.x % kPerRow) * WIDTH; }
+  // This thread's columns.  Where the workgroup has fewer channels than it could take, the last threads of a row all have its last
+  // ones: they compute and write the same, and no vector ends beyond the channels (`wide`).  The columns behind stay zero in LDS.
+  // Only a workgroup of fewer than WIDTH channels goes by element.  With a last vector that went by element, T=1024 N=8 bf16
+  // took 314 us at D=1001 and 337 at D=1023, forward and backward, now 247 (D=1024: 240).
+  static __device__ __forceinline__ bool wide(const Block<LANES>& b) { return b.c_end - b.c0 >= WIDTH; }
+  static __device__ __forceinline__ int column(const Block<LANES>& b) {
+    const int c = (threadIdx.x % kPerRow) * WIDTH;
+    return wide(b) ? min(c, b.c_end - b.c0 - WIDTH) : c;
+  }
 };
 
 // The elements of one tensor's tile, packed in the tensor's own type until they are worked on.
@@ -163,10 +173,10 @@ struct Walk {
   T* p;         // of the tile's first row here
   size_t step;  // elements between steps
   __device__ __forceinline__ Walk(const Rows<T>& rows, int t0, const Block<LANES>& b)
-      : p(rows.p == nullptr ? nullptr : rows.at(t0, b.n) + (size_t)L::row(0) * rows.step + b.c0 + L::column()), step(rows.step) {}
+      : p(rows.p == nullptr ? nullptr : rows.at(t0, b.n) + (size_t)L::row(0) * rows.step + b.c0 + L::column(b)), step(rows.step) {}
   __device__ __forceinline__ void forth() { p += TS * step; }
   __device__ __forceinline__ void back() { p -= TS * step; }
-  // `rows` of the tile belong to the sequence; whole: all of them do, and all channels to the group
+  // `rows` of the tile belong to the sequence; whole: all of them do, and the workgroup is wide
   template <typename U>
   __device__ __forceinline__ void load(Held<U, LANES>& to, bool whole, int rows, const Block<LANES>& b) const {
     typedef typename Wide<U, L::WIDTH>::type wide_t;
@@ -178,9 +188,13 @@ struct Walk {
       } else {
         typename Held<U, LANES>::packed_t w = {};
         if (L::row(i) < rows) {
+          if (L::wide(b)) {
+            w = *reinterpret_cast<const wide_t*>(from);
+          } else {
 #pragma unroll
-          for (int e = 0; e < L::WIDTH; ++e)
-            if (b.c0 + L::column() + e < b.c_end) w[e] = from[e];
+            for (int e = 0; e < L::WIDTH; ++e)
+              if (b.c0 + L::column(b) + e < b.c_end) w[e] = from[e];
+          }
         }
         to.v[i] = w;
       }
@@ -191,7 +205,7 @@ struct Walk {
 #pragma unroll
     for (int i = 0; i < L::ITEMS; ++i) {
       T* to = p + (size_t)(i * L::kRowStep) * step;
-      if (whole) {
+      if (whole || (L::row(i) < rows && L::wide(b))) {
         wide_t w;
 #pragma unroll
         for (int e = 0; e < L::WIDTH; ++e) w[e] = (T)f[i][e];
@@ -199,7 +213,7 @@ struct Walk {
       } else if (L::row(i) < rows) {
 #pragma unroll
         for (int e = 0; e < L::WIDTH; ++e)
-          if (b.c0 + L::column() + e < b.c_end) to[e] = (T)f[i][e];
+          if (b.c0 + L::column(b) + e < b.c_end) to[e] = (T)f[i][e];
       }
     }
   }
@@ -277,6 +291,11 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
   __shared__ float y_lds[2][LOCAL ? 1 : TS][P::kBlock];
 
   const Block<LANES> b(s, blockIdx.x);
+  const int column = L::column(b);
+  if (b.c_end - b.c0 < P::kBlock) {  // the columns behind the last
+    for (int e = threadIdx.x; e < 2 * TS * P::kBlock; e += 256) (&step_lds[0][0][0])[e] = float2_t{0.f, 0.f};
+    __syncthreads();
+  }
   const int t0 = blockIdx.y * s.chunk, t1 = min(s.T, t0 + s.chunk);
   const Extent extent = extent_of(in.lengths, b.n, s.T);
   const int end = min(t1, extent.steps);
@@ -302,8 +321,8 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
   float bias[L::WIDTH], skip[L::WIDTH];
 #pragma unroll
   for (int e = 0; e < L::WIDTH; ++e) bias[e] = skip[e] = 0.f;
-  if (in.bias != nullptr) load_channels<L::WIDTH>(in.bias, b.c0 + L::column(), b.c_end, bias);
-  if (!LOCAL && in.skip != nullptr) load_channels<L::WIDTH>(in.skip, b.c0 + L::column(), b.c_end, skip);
+  if (in.bias != nullptr) load_channels<L::WIDTH>(in.bias, b.c0 + column, b.c_end, bias);
+  if (!LOCAL && in.skip != nullptr) load_channels<L::WIDTH>(in.skip, b.c0 + column, b.c_end, skip);
 
   // While a tile is scanned, the next one's elements are worked out between its steps, into the other half of LDS, and the one
   // after that is on its way from memory.
@@ -314,11 +333,11 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
   Walk<const T, LANES> x_walk(in.x, t0, b), delta_walk(in.delta, t0, b), z_walk(in.z, t0, b);
   WalkShared<T, LANES> B_walk(in.B, t0, b, s.S), C_walk(in.C, t0, b, s.S);
   Walk<T, LANES> y_walk(packed_rows(y, s.N, s.D), t0, b);
-  const bool all_channels = b.c0 + P::kBlock <= b.c_end, gated = !LOCAL && in.z.p != nullptr;
+  const bool wide = L::wide(b), gated = !LOCAL && in.z.p != nullptr;
   auto fetch = [&](Raw& to, int t) {  // the next tile of every walk, which starts at t
     const int rows = end - t;
     if (rows <= 0) return;
-    const bool whole = all_channels && rows >= TS;
+    const bool whole = wide && rows >= TS;
     x_walk.load(to.x, whole, rows, b);
     delta_walk.load(to.delta, whole, rows, b);
     if (gated) z_walk.load(to.z, whole, rows, b);
@@ -338,7 +357,7 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
     const int i = element / L::WIDTH, e = element % L::WIDTH;
     const float xv = from.x.get(i, e);
     const float dt = step_size(from.delta.get(i, e) + bias[e], s.softplus, t + L::row(i) < end);
-    step_lds[half][L::row(i)][L::column() + e] = float2_t{dt, dt * xv};
+    step_lds[half][L::row(i)][column + e] = float2_t{dt, dt * xv};
     if (LOCAL) return;
     to.skipped[i][e] = skip[e] * xv;
     const float zv = from.z.get(i, e), silu = zv * sigmoid_of(zv);
@@ -350,7 +369,7 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
     for (int i = 0; i < L::ITEMS; ++i)
 #pragma unroll
       for (int e = 0; e < L::WIDTH; ++e)
-        o[i][e] = (y_lds[half][L::row(i)][L::column() + e] + before.skipped[i][e]) * before.gate[i][e];
+        o[i][e] = (y_lds[half][L::row(i)][column + e] + before.skipped[i][e]) * before.gate[i][e];
     y_walk.store(o, whole, rows, b);
   };
 
@@ -367,7 +386,7 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
     fetch(coming, t + 2 * TS);
     __syncthreads();
     if (!LOCAL && t > t0) {  // the tile before
-      put_out(half ^ 1, all_channels, TS);
+      put_out(half ^ 1, wide, TS);
       y_walk.forth();
     }
     before = rest;
@@ -411,7 +430,7 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
   if (!LOCAL && t0 < end) {
     __syncthreads();
     const int rows = (end - t0 - 1) % TS + 1;
-    put_out(half ^ 1, all_channels && rows == TS, rows);
+    put_out(half ^ 1, wide && rows == TS, rows);
   }
 
   if (LOCAL) {
@@ -425,7 +444,7 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
 #pragma unroll
   for (int e = 0; e < L::WIDTH; ++e) fill[e] = extent.fill;
   for (int t = max(t0, end) + (int)threadIdx.x / L::kPerRow; t < t1; t += L::kRowStep)
-    store_channels<L::WIDTH>(y + ((size_t)t * s.N + b.n) * s.D, b.c0 + L::column(), b.c_end, fill);
+    store_channels<L::WIDTH>(y + ((size_t)t * s.N + b.n) * s.D, b.c0 + column, b.c_end, fill);
   if (blockIdx.y + 1 == (unsigned)s.chunks && live && h_last != nullptr) {
     if (extent.fill != 0.f) {  // NaN
 #pragma unroll
@@ -446,7 +465,9 @@ struct ScanGradients {
 
 // Backward pass over a chunk.  LOCAL: only G at the chunk's start for a gradient of zero at its end, and
 // the sum of dt.  added, sum_dt: as forward, of the chunks but the first.
-template <typename T, int LANES, bool LOCAL>
+// EVEN: the channels of a group are a multiple of WIDTH, and a thread's columns aligned to it, which lets LDS move 16 bytes at a
+// time; without, T=2048 N=8 D=4096 S=16 bf16 takes 1060 us, not 1030.
+template <typename T, int LANES, bool LOCAL, bool EVEN>
 __global__ __launch_bounds__(256, 2)
 void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ kept, Rows<const T> dy,
                                     const float* __restrict__ dh_last, float* __restrict__ added, float* __restrict__ sum_dt,
@@ -461,6 +482,11 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   __shared__ float dB_lds[LOCAL ? 1 : 4][TS * LANES * K], dC_lds[LOCAL ? 1 : 4][TS * LANES * K];  // of each wavefront
 
   const Block<LANES> b(s, blockIdx.x);
+  const int column = EVEN ? L::column(b) / L::WIDTH * L::WIDTH : L::column(b);
+  if (b.c_end - b.c0 < P::kBlock) {  // the columns behind the last
+    for (int e = threadIdx.x; e < TS * P::kBlock; e += 256) (&step_lds[0][0])[e] = float4_t{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+  }
   const unsigned chunk = blockIdx.y + (LOCAL ? 1 : 0);  // what goes out of the first chunk is found by the second pass
   const int t0 = chunk * s.chunk, t1 = min(s.T, t0 + s.chunk);
   const Extent extent = extent_of(in.lengths, b.n, s.T);
@@ -486,7 +512,6 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
                     s.chunks - 1 - (int)chunk, s0, s.S);
     }
   }
-  const int column = L::column();
   float bias[L::WIDTH], skip[L::WIDTH], dskip[L::WIDTH], dbias[L::WIDTH];
 #pragma unroll
   for (int e = 0; e < L::WIDTH; ++e) bias[e] = skip[e] = dskip[e] = dbias[e] = 0.f;
@@ -518,11 +543,11 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   WalkShared<T, LANES> B_walk(in.B, from, b, s.S), C_walk(in.C, from, b, s.S);
   Walk<T, LANES> dx_walk(packed_rows(out.dx, s.N, s.D), from, b), ddelta_walk(packed_rows(out.ddelta, s.N, s.D), from, b);
   Walk<T, LANES> dz_walk(packed_rows(out.dz, s.N, s.D), from, b);
-  const bool all_channels = b.c0 + P::kBlock <= b.c_end, gated = in.z.p != nullptr;
+  const bool wide = L::wide(b), gated = in.z.p != nullptr;
   float start[K], start_next[K];
   auto fetch = [&](int t) {  // the tile of every walk, which starts at t
     const int rows = end - t;
-    const bool whole = all_channels && rows >= TS;
+    const bool whole = wide && rows >= TS;
     if (!LOCAL) {
       x_walk.load(x, whole, rows, b);
       x_walk.back();
@@ -644,7 +669,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
         dbias[e] += t + row < end ? ddo[i][e] : 0.f;
       }
     }
-    const bool whole = all_channels && end - t >= TS;
+    const bool whole = wide && end - t >= TS;
     dx_walk.store(dxo, whole, end - t, b);
     ddelta_walk.store(ddo, whole, end - t, b);
     if (gated) dz_walk.store(dzo, whole, end - t, b);
@@ -659,7 +684,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
       out.dB[at] = (dB_lds[0][e] + dB_lds[1][e]) + (dB_lds[2][e] + dB_lds[3][e]);
       out.dC[at] = (dC_lds[0][e] + dC_lds[1][e]) + (dC_lds[2][e] + dC_lds[3][e]);
     }
-    // No barrier: until the next one a thread overwrites only elements that it alone reads here, and B and C, which nobody does.
+    // No barrier: until the next one a wavefront overwrites only elements that it alone reads here, and B and C, which nobody does.
   }
 
   if (LOCAL) {
@@ -785,9 +810,10 @@ int with_lanes(int S, F&& f) {
 // N=4 D=4096 S=16 bf16 (256 workgroups) 244 and 254 us, T=128 N=32 D=512 18 and 22.  Backward, where it costs two fifths,
 // it is: 680 and 559, 53 and 50.
 ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, bool backward) {
-  ScanShape s = {T, N, D, S, G, D / G, 0, 0, 0, softplus};
+  ScanShape s = {T, N, D, S, G, D / G, 0, 0, 0, 0, softplus};
   const int block = 256 / lanes_for(S);
   s.blocks_group = (s.share + block - 1) / block;
+  s.block_channels = ((s.share + s.blocks_group - 1) / s.blocks_group + 3) / 4 * 4;
   const size_t blocks = (size_t)N * G * s.blocks_group, tiles = ((size_t)T + TS - 1) / TS;
   const size_t least = backward ? 2 : 3, most = tiles / 4, join = (size_t)(3.0 * std::sqrt((double)tiles));
   size_t chunks = 2 * (size_t)device_cu_count() / blocks;
@@ -858,17 +884,23 @@ int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, co
   if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_backward: the workspace is too small");
   float *added = workspace + w.added, *sum_dt = workspace + w.sum_dt;
   const ScanGradients<T> out = {dx, ddelta, dz, dh0, workspace + w.partial, workspace + w.dB, workspace + w.dC};
-  HASTE_HIP_PROPAGATE(with_lanes(s.S, [&](auto lanes) {
+  auto launch = [&](auto lanes, auto even) {
     dim3 grid((unsigned)blocks, s.chunks);
     if (s.chunks > 1) {
       ScopedKernelTimer timer("selective_scan_chunks", stream);
-      selective_scan_backward_kernel<T, lanes(), true><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, dy, dh_last, added, sum_dt, out);
+      selective_scan_backward_kernel<T, lanes(), true, even()><<<dim3(grid.x, grid.y - 1), 256, 0, stream>>>(s, in, nullptr, dy, dh_last, added, sum_dt, out);
       HASTE_HIP_TRY(hipGetLastError());
     }
     ScopedKernelTimer timer("selective_scan_backward", stream);
-    selective_scan_backward_kernel<T, lanes(), false><<<grid, 256, 0, stream>>>(s, in, kept, dy, dh_last, added, sum_dt, out);
+    selective_scan_backward_kernel<T, lanes(), false, even()><<<grid, 256, 0, stream>>>(s, in, kept, dy, dh_last, added, sum_dt, out);
     HASTE_HIP_TRY(hipGetLastError());
     return HASTE_HIP_OK;
+  };
+  HASTE_HIP_PROPAGATE(with_lanes(s.S, [&](auto lanes) {
+    if constexpr (Tile<lanes()>::WIDTH > 1) {
+      if (s.share % Tile<lanes()>::WIDTH != 0) return launch(lanes, std::false_type());
+    }
+    return launch(lanes, std::true_type());
   }));
   {
     ScopedKernelTimer timer("selective_scan_shared", stream);
@@ -900,7 +932,7 @@ ScanInputs<T> inputs_of(const void* x, size_t x_step, size_t x_row, const void* 
 template <typename T>
 int step(hipStream_t stream, int N, int D, int S, int G, int softplus, const ScanInputs<T>& in, const float* h, T* y,
          float* h_out) {
-  const ScanShape s = {1, N, D, S, G, D / G, 0, TS, 1, softplus};
+  const ScanShape s = {1, N, D, S, G, D / G, 0, 0, TS, 1, softplus};
   return with_lanes(S, [&](auto lanes) {
     const size_t across = ((size_t)D * lanes() + 255) / 256;  // at most 2^22: D is at most 2^30 / 66
     if (across > kGridLimit) return too_large("selective_scan: too many channels");

@@ -152,6 +152,17 @@ def test_scan(T, N, D, S, options, dtype):
     compare(run_scan(q.g), formulas.scan(q.p), formulas.scan(q.p, True), 12 * T + S + D + T * N + 128)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=short)
+@pytest.mark.parametrize("S", [6, 16, 24, 50])
+def test_scan_of_any_number_of_channels(S, dtype):
+    """Groups that end anywhere within a vector, a workgroup and the last of several workgroups; chunks of the time axis too."""
+    for T in (19, 140):
+        for G, share in ((3, 1), (2, 2), (2, 3), (1, 5), (2, 7), (1, 31), (2, 33), (1, 66), (1, 129), (2, 131), (1, 258)):
+            print("scan channels", T, G, share, S, dtype, flush=True)
+            q = scan_problem(T + share + S, dtype, T, 1, G * share, S, G)
+            compare(run_scan(q.g), formulas.scan(q.p), formulas.scan(q.p, True), 12 * T + S + share + T + 128)
+
+
 def test_scan_of_small_step_sizes():
     """softplus far below zero is exp, to the same relative error: y and h scale with it."""
     for shift in (-5.0, -12.0, -20.0, -60.0):
@@ -244,6 +255,20 @@ def test_norm(shape, options, centered, dtype):
 
 
 # ---- any strides ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES, ids=short)
+def test_rows_that_end_anywhere(dtype):
+    """The last vector of a row, whole or in part; the convolution's in place too."""
+    for D in list(range(1, 18)) + list(range(512, 522)):
+        print("ends", D, dtype, flush=True)
+        norm, conv = norm_problem(D, dtype, (3, 2, D), D % 2 == 1), conv_problem(D, dtype, 7, 2, D, 4, lengths=[7, 3])
+        compare(run_norm(norm.g, D % 2 == 1), formulas.norm(norm.p), formulas.norm(norm.p, True), 8 * (D + 32) + 6)
+        compare(run_conv(conv.g), formulas.conv(conv.p), formulas.conv(conv.p, True), 8 * 4 + 14 + 64)
+        x, state = conv.g["x"][0], conv.g["state"].clone()
+        want = ops.causal_conv_iterate(x, conv.g["state"], conv.g["kernel"], conv.g["bias"], True)
+        y, _ = ops.causal_conv_iterate(x, state, conv.g["kernel"], conv.g["bias"], True, state_out=state)
+        assert torch.equal(y, want[0]) and torch.equal(state, want[1])
+
+
 def relaid(t, how):
     """The values of t in other memory: batch first, as a column block at an odd offset, or with channels apart."""
     if t is None or t.dim() < 3:
