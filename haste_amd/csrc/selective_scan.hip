@@ -75,42 +75,65 @@ __device__ __forceinline__ float step_size(float raw, int softplus, bool inside,
   return inside ? dt : 0.f;
 }
 
-// A lane's place in a wavefront: the states are told apart by the highest of the low four bits of the
-// lane (sums over them rotate rows of 16 lanes), the channels by the rest (sums over them swap halves
-// of the wavefront, which adds two values in one go).
+// A lane's place in a wavefront: the lanes of a channel are neighbours, sums over them stay within a row of 16 lanes.
 template <int LANES>
 struct Place {
   static constexpr int kChannels = 64 / LANES;  // of a wavefront
-  static constexpr int kLow = 16 / LANES;       // of them in a row of 16 lanes
   static constexpr int kBlock = 4 * kChannels;  // of a workgroup
-  static __device__ __forceinline__ int states(int lane) { return (lane & 15) / kLow; }
-  static __device__ __forceinline__ int channel(int lane) { return (lane >> 4) * kLow + (lane & (kLow - 1)); }
+  static __device__ __forceinline__ int states(int lane) { return lane % LANES; }
+  static __device__ __forceinline__ int channel(int lane) { return lane / LANES; }
 };
 
 // Sum over the lanes of a channel, in each of them.
 template <int LANES>
 __device__ __forceinline__ float sum_states(float v) {
-  if (LANES >= 2) v += dpp<kRor8>(v);
-  if (LANES >= 4) v += dpp<kRor4>(v);
-  if (LANES >= 8) v += dpp<kXor2>(v);
-  if (LANES >= 16) v += dpp<kXor1>(v);
+  if (LANES >= 2) v += dpp<kXor1>(v);
+  if (LANES >= 4) v += dpp<kXor2>(v);
+  if (LANES >= 8) v += dpp<kHalfMirror>(v);
+  if (LANES >= 16) v += dpp<kRor8>(v);
   return v;
 }
 
-// Sums of a lane's four values over the channels of the wavefront: row r of 16 lanes gets that of
-// value kSummed(r).
+// Sums of a lane's four values over the channels of the wavefront (parts 1), or of each of its rows of 16 lanes (parts 4).
 template <int LANES>
-__device__ __forceinline__ float sum_channels(const float (&v)[K]) {
-  float s = swap_add_rows(swap_add_halves(v[0], v[1]), swap_add_halves(v[2], v[3]));
-  if (LANES <= 8) s += dpp<kXor1>(s);
-  if (LANES <= 4) s += dpp<kXor2>(s);
-  if (LANES <= 2) s += dpp<kHalfMirror>(s);
-  return s;
-}
-__device__ __forceinline__ int summed_value(int lane) {
-  const int r = lane >> 4;
-  return (r & 1) << 1 | r >> 1;  // 0, 2, 1, 3
-}
+struct ChannelSums {
+  static constexpr int kParts = 1;
+  static __device__ __forceinline__ int part(int) { return 0; }
+  // the value whose sum a lane gets: rows 0, 2, 1, 3
+  static __device__ __forceinline__ int value(int lane) { return (lane >> 4 & 1) << 1 | lane >> 5; }
+  static __device__ __forceinline__ float sum(const float (&v)[K]) {
+    float s = swap_add_rows(swap_add_halves(v[0], v[1]), swap_add_halves(v[2], v[3]));
+    if (LANES <= 8) s += dpp<kRor8>(s);
+    if (LANES <= 4) s += dpp<kRor4>(s);
+    if (LANES <= 2) s += dpp<kXor2>(s);
+    return s;
+  }
+};
+// With four lanes a channel the channels of a row are its four banks, and additions that write some banks only leave each bank with
+// one of the four values: six of them, 24 cycles, for the 44 of swapping rows and halves too, against four times the parts to add
+// up from LDS.  T=2048 N=8 D=4096 S=16 bf16 backward 970 us instead of 1035, T=1024 D=1024 121 instead of 130.
+// (The assembler's form: of the compiler's every addition that leaves banks as they are is a move and an addition.)
+template <>
+struct ChannelSums<4> {
+  static constexpr int kParts = 4;
+  static __device__ __forceinline__ int part(int lane) { return lane >> 4; }
+  static __device__ __forceinline__ int value(int lane) { return (lane >> 2 & 1 ? 0 : 2) | (lane >> 3 & 1); }
+  static __device__ __forceinline__ float sum(const float (&v)[K]) {
+    float low, high, s;
+    // a lane read by another needs two instructions after its write; rotating right, lane i reads i - 8, i - 4, i - 12 (i + 4)
+    asm("s_nop 1\n\t"
+        "v_add_f32_dpp %0, %3, %3 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+        "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+        "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %1, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "s_nop 1\n\t"
+        "v_add_f32_dpp %2, %0, %0 row_ror:4 row_mask:0xf bank_mask:0xa\n\t"
+        "v_add_f32_dpp %2, %1, %1 row_ror:12 row_mask:0xf bank_mask:0x5"
+        : "=&v"(low), "=&v"(high), "=&v"(s)
+        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]));
+    return s;
+  }
+};
 
 // A channel's states [S] of float, this lane's four of them; those beyond S are 0.
 __device__ __forceinline__ void load_states(const float* p, int s0, int S, float (&h)[K]) {
@@ -479,7 +502,9 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   __shared__ float4_t C_lds[TS * LANES], B_lds[LOCAL ? 1 : TS * LANES];
   __shared__ float ypre_lds[LOCAL ? 1 : TS][P::kBlock];
   __shared__ float2_t du_Aw_lds[LOCAL ? 1 : TS][P::kBlock];
-  __shared__ float dB_lds[LOCAL ? 1 : 4][TS * LANES * K], dC_lds[LOCAL ? 1 : 4][TS * LANES * K];  // of each wavefront
+  typedef ChannelSums<LANES> Sums;
+  constexpr int kParts = 4 * Sums::kParts;  // of the workgroup; 16 floats between them keep rows that write at once in banks of their own
+  __shared__ float dB_lds[LOCAL ? 1 : kParts][TS * LANES * K + 16], dC_lds[LOCAL ? 1 : kParts][TS * LANES * K + 16];
 
   const Block<LANES> b(s, blockIdx.x);
   const int column = EVEN ? L::column(b) / L::WIDTH * L::WIDTH : L::column(b);
@@ -493,6 +518,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   const int end = min(t1, extent.steps);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s0 = P::states(lane) * K;
   const int mine = wave * P::kChannels + P::channel(lane);
+  const int part = wave * Sums::kParts + Sums::part(lane), summed = s0 + Sums::value(lane);
   const int d = b.c0 + mine;
   const bool live = d < b.c_end;
   const size_t state = ((size_t)b.n * s.D + d) * s.S, states = (size_t)s.N * s.D * s.S;
@@ -628,7 +654,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
         dCv[r] = now.dt_u_q.z * start[r];
       }
       ypre_lds[j][mine] = sum_states<LANES>(ypre);  // (the lanes of a channel write the same, as do those of a state below)
-      dC_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum_channels<LANES>(dCv);
+      dC_lds[part][j * LANES * K + summed] = Sums::sum(dCv);
       __builtin_amdgcn_sched_barrier(0);
       now = next;
     }
@@ -647,7 +673,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
         dA[r] += w * now.dt_u_q.x;
       }
       du_Aw_lds[j][mine] = float2_t{sum_states<LANES>(du), sum_states<LANES>(Aw)};
-      dB_lds[wave][j * LANES * K + s0 + summed_value(lane)] = sum_channels<LANES>(dBv);
+      dB_lds[part][j * LANES * K + summed] = Sums::sum(dBv);
       __builtin_amdgcn_sched_barrier(0);
       now = next;
     }
@@ -681,8 +707,14 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
       const int j = e / (LANES * K), st = e % (LANES * K);
       if (t + j >= end || st >= s.S) continue;
       const size_t at = ((part + t + j) * s.N + b.n) * shared_row + (size_t)b.g * s.S + st;
-      out.dB[at] = (dB_lds[0][e] + dB_lds[1][e]) + (dB_lds[2][e] + dB_lds[3][e]);
-      out.dC[at] = (dC_lds[0][e] + dC_lds[1][e]) + (dC_lds[2][e] + dC_lds[3][e]);
+      float dBv = 0.f, dCv = 0.f;
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+        dBv += dB_lds[p][e];
+        dCv += dC_lds[p][e];
+      }
+      out.dB[at] = dBv;
+      out.dC[at] = dCv;
     }
     // No barrier: until the next one a wavefront overwrites only elements that it alone reads here, and B and C, which nobody does.
   }
