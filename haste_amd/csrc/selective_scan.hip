@@ -36,10 +36,10 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 
 struct ScanShape {
   int T, N, D, S, G;
-  int share;         // channels of a group, D / G
+  int share;           // channels of a group, D / G
   int blocks_group;    // workgroups of a group
   int block_channels;  // channels of a workgroup
-  int chunk, chunks; // steps of a chunk (a multiple of TS)
+  int chunk, chunks;   // steps of a chunk (a multiple of TS)
   int softplus;
 };
 
@@ -172,7 +172,7 @@ struct Tile {
   // This thread's columns.  Where the workgroup has fewer channels than it could take, the last threads of a row all have its last
   // ones: they compute and write the same, and no vector ends beyond the channels (`wide`).  The columns behind stay zero in LDS.
   // Only a workgroup of fewer than WIDTH channels goes by element.  With a last vector that went by element, T=1024 N=8 bf16
-  // took 314 us at D=1001 and 337 at D=1023, forward and backward, now 247 (D=1024: 240).
+  // took 314 us at D=1001 and 337 at D=1023, forward and backward; so 246 at both (D=1024: 240).
   static __device__ __forceinline__ bool wide(const Block<LANES>& b) { return b.c_end - b.c0 >= WIDTH; }
   static __device__ __forceinline__ int column(const Block<LANES>& b) {
     const int c = (threadIdx.x % kPerRow) * WIDTH;
@@ -489,7 +489,7 @@ struct ScanGradients {
 // Backward pass over a chunk.  LOCAL: only G at the chunk's start for a gradient of zero at its end, and
 // the sum of dt.  added, sum_dt: as forward, of the chunks but the first.
 // EVEN: the channels of a group are a multiple of WIDTH, and a thread's columns aligned to it, which lets LDS move 16 bytes at a
-// time; without, T=2048 N=8 D=4096 S=16 bf16 takes 1060 us, not 1030.
+// time; without, T=2048 N=8 D=4096 S=16 bf16 takes 3 % more.
 template <typename T, int LANES, bool LOCAL, bool EVEN>
 __global__ __launch_bounds__(256, 2)
 void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ kept, Rows<const T> dy,
