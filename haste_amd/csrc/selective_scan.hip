@@ -760,18 +760,19 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   }
 }
 
-// dB, dC = the sums of the blocks' parts, rounded.
+// dB, dC = the sums of the blocks' parts, rounded.  (More elements than a grid has threads go by turns.)
 template <typename T>
 __global__ __launch_bounds__(256)
 void scan_shared_kernel(int parts, size_t count, const float* __restrict__ dB_parts, const float* __restrict__ dC_parts,
                         T* __restrict__ dB, T* __restrict__ dC) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= count) return;
   const float* from = blockIdx.y == 0 ? dB_parts : dC_parts;
-  float sum = 0.f;
+  T* to = blockIdx.y == 0 ? dB : dC;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (size_t)gridDim.x * 256) {
+    float sum = 0.f;
 #pragma unroll 8
-  for (int p = 0; p < parts; ++p) sum += from[p * count + i];
-  (blockIdx.y == 0 ? dB : dC)[i] = (T)sum;
+    for (int p = 0; p < parts; ++p) sum += from[p * count + i];
+    to[i] = (T)sum;
+  }
 }
 
 // A single step: LANES neighbouring lanes a channel, its states in and out as whole lines.  Bound by those lines' bytes, or by
@@ -911,7 +912,7 @@ int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, co
   const size_t blocks = (size_t)s.N * s.G * s.blocks_group;
   const size_t shared = (size_t)s.T * s.N * s.G * s.S, columns = (size_t)s.D * (s.S + 2);
   const ScanWorkspace w = backward_workspace(s);
-  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ || (shared + 255) / 256 > kGridLimit)
+  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ)
     return too_large("selective_scan: too many rows of channels");
   if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_backward: the workspace is too small");
   float *added = workspace + w.added, *sum_dt = workspace + w.sum_dt;
@@ -936,7 +937,8 @@ int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, co
   }));
   {
     ScopedKernelTimer timer("selective_scan_shared", stream);
-    scan_shared_kernel<T><<<dim3((unsigned)((shared + 255) / 256), 2), 256, 0, stream>>>(s.blocks_group, shared, out.dB, out.dC, dB, dC);
+    const size_t groups = (shared + 255) / 256;
+    scan_shared_kernel<T><<<dim3((unsigned)(groups < kGridLimit ? groups : kGridLimit), 2), 256, 0, stream>>>(s.blocks_group, shared, out.dB, out.dC, dB, dC);
     HASTE_HIP_TRY(hipGetLastError());
   }
   const size_t first = (size_t)s.D * s.S;

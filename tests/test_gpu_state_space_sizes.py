@@ -1,0 +1,40 @@
+"""The state space block's operators at sizes beyond those of one grid, one workgroup or one turn."""
+import pytest
+import torch
+
+from haste_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _scan_tensors(seed, T, N, D, S, G, dtype=torch.bfloat16):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, dtype=dtype):
+        return torch.randn(*shape, generator=gen, device="cuda", dtype=dtype)
+
+    return dict(x=normal(T, N, D), delta=normal(T, N, D), A=-torch.rand(D, S, generator=gen, device="cuda"), B=normal(T, N, G, S),
+                C=normal(T, N, G, S), D=normal(D, dtype=torch.float32), z=normal(T, N, D), delta_bias=normal(D, dtype=torch.float32),
+                dy=normal(T, N, D))
+
+
+def _scan(g):
+    ins = [g[k] for k in ("x", "delta", "A", "B", "C", "D", "z", "delta_bias")]
+    y, h, cache = ops.selective_scan_forward(True, *ins, True)
+    grads = ops.selective_scan_backward(*ins, True, None, None, cache, g["dy"])
+    return dict(zip(("dx", "ddelta", "dA", "dB", "dC", "dD", "dz", "ddelta_bias", "dh0"), grads), y=y, h_last=h)
+
+
+def test_scan_with_gradients_of_B_and_C_beyond_a_grid():
+    """2^30 elements of B: more than the threads that a grid has.  The groups' halves by themselves give the same bits."""
+    T, N, S, G = 1024, 8, 64, 2048
+    assert T * N * S * G >= 2 ** 30
+    g = _scan_tensors(1, T, N, G, S, G)
+    got = _scan(g)
+    for half in (slice(0, G // 2), slice(G // 2, G)):
+        part = {k: v[:, :, half].contiguous() if v.dim() > 2 else v[half] for k, v in g.items()}
+        want = _scan(part)
+        for k, v in want.items():
+            mine = got[k][:, half] if k in ("h_last", "dh0") else got[k][:, :, half] if v.dim() > 2 else got[k][half]
+            assert torch.equal(mine, v), k
+        del part, want

@@ -1,0 +1,24 @@
+"""Which sizes the state space operators take, without a GPU: nothing is read, nothing launched."""
+from haste_amd import lib
+
+UNSUPPORTED = 2
+
+
+def _refusal(name, *values):
+    """The code and the reason of a call that is refused."""
+    code = lib.entry(name)(*values, None)
+    return code, lib.load().haste_hip_last_runtime_error().decode()
+
+
+def _scan_backward(T, N, D, S, G, workspace_bytes):
+    ins = [256, N * D, D, 256, N * D, D, 256, 256, N * G * S, G * S, 256, N * G * S, G * S, None, None, 0, 0, None, 1]
+    return _refusal("haste_hip_selective_scan_backward_bf16", T, N, D, S, G, *ins, None, 256, 256, N * D, D, None, 256, 256, 256, 256,
+                    256, None, None, None, None, 256, workspace_bytes)
+
+
+def test_backward_scans_have_no_limit_of_their_own():
+    """T N G S of 2^30 and more, which the forward pass takes: the small workspace is all that is wrong."""
+    for sizes in ((2048, 8, 4096, 16, 4096), (1024, 8, 2048, 64, 2048), (8192, 64, 64, 64, 32)):
+        assert sizes[0] * sizes[1] * sizes[3] * sizes[4] >= 2 ** 30
+        code, reason = _scan_backward(*sizes, 64)
+        assert code == UNSUPPORTED and "workspace is too small" in reason, (sizes, reason)
