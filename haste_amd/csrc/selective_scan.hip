@@ -875,7 +875,7 @@ ScanWorkspace backward_workspace(const ScanShape& s) {
   const size_t parts = (size_t)s.chunks * s.N, columns = (size_t)s.D * (s.S + 2);
   w.partial = w.total;
   w.sums = w.partial + parts * columns;
-  w.dB = w.sums + column_sums_scratch((int)parts, columns);
+  w.dB = w.sums + column_sums_scratch(parts, columns);
   w.dC = w.dB + (size_t)s.blocks_group * s.T * s.N * s.G * s.S;
   w.total = w.dC + (w.dC - w.dB);
   return w;
@@ -943,7 +943,7 @@ int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, co
   }
   const size_t first = (size_t)s.D * s.S;
   const ColumnOutputs to = {{dA, dskip, dbias, nullptr}, {first, first + s.D, columns, columns}};
-  return column_sums(stream, s.chunks * s.N, columns, out.partial, workspace + w.sums, to);
+  return column_sums(stream, (size_t)s.chunks * s.N, columns, out.partial, workspace + w.sums, to);
 }
 
 int check_sizes(int T, int N, int D, int S, int G) {

@@ -165,8 +165,8 @@ struct ColumnOutputs {
   float* out[4];
   size_t end[4];
 };
-size_t column_sums_scratch(int parts, size_t columns);
-int column_sums(hipStream_t stream, int parts, size_t columns, const float* partial, float* scratch,
+size_t column_sums_scratch(size_t parts, size_t columns);
+int column_sums(hipStream_t stream, size_t parts, size_t columns, const float* partial, float* scratch,
                 const ColumnOutputs& to);
 
 constexpr size_t kGridLimit = (size_t(1) << 22) - 1;  // workgroups along x: threads along an axis are counted in 32 bits

@@ -38,3 +38,19 @@ def test_scan_with_gradients_of_B_and_C_beyond_a_grid():
             mine = got[k][:, half] if k in ("h_last", "dh0") else got[k][:, :, half] if v.dim() > 2 else got[k][half]
             assert torch.equal(mine, v), k
         del part, want
+
+
+def test_scan_with_more_sums_than_a_grid():
+    """Gradients of parameters of more than 2^28 columns.  A channel's do not depend on the channels beside it."""
+    D, S = 2 ** 22 + 2 ** 17, 64
+    assert D * (S + 2) > 2 ** 28
+    g = _scan_tensors(2, 1, 1, D, S, 1)
+    got = _scan(g)
+    for half in (slice(0, D // 2), slice(D // 2, D)):
+        want = _scan({k: v if k in ("B", "C") else v[:, :, half].contiguous() if v.dim() > 2 else v[half] for k, v in g.items()})
+        for k, v in want.items():
+            if k in ("dB", "dC"):  # sums over the channels
+                continue
+            mine = got[k][:, half] if k in ("h_last", "dh0") else got[k][:, :, half] if v.dim() > 2 else got[k][half]
+            assert torch.equal(mine, v), k
+        del want
