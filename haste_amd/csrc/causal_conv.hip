@@ -273,13 +273,12 @@ int run_length(int T, size_t items) {
 
 // Floats of workspace a backward pass needs: the runs' partials [parts][columns], and what adding them takes.
 struct ConvPartials {
-  int parts;
-  size_t columns, floats, total;
+  size_t parts, columns, floats, total;
 };
 ConvPartials partials_of(int T, int N, int D, int W) {
   ConvPartials p;
   const size_t chunk = run_length(T, (size_t)N * ((D + V - 1) / V));
-  p.parts = (int)((T + chunk - 1) / chunk * N);
+  p.parts = (T + chunk - 1) / chunk * N;
   p.columns = (size_t)(W + 1) * D;
   p.floats = p.parts * p.columns;
   p.total = p.floats + column_sums_scratch(p.parts, p.columns);

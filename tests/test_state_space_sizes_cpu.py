@@ -1,4 +1,6 @@
 """Which sizes the state space operators take, without a GPU: nothing is read, nothing launched."""
+import ctypes
+
 from haste_amd import lib
 
 UNSUPPORTED = 2
@@ -22,3 +24,15 @@ def test_backward_scans_have_no_limit_of_their_own():
         assert sizes[0] * sizes[1] * sizes[3] * sizes[4] >= 2 ** 30
         code, reason = _scan_backward(*sizes, 64)
         assert code == UNSUPPORTED and "workspace is too small" in reason, (sizes, reason)
+
+
+def _bytes(name, *sizes):
+    fn = lib.load()[name]
+    fn.restype, fn.argtypes = ctypes.c_size_t, [ctypes.c_int] * len(sizes)
+    return fn(*sizes)
+
+
+def test_workspaces_of_more_than_2_31_partials():
+    """Runs of 64 steps or fewer times rows: counted in more than 32 bits."""
+    T, N, D, W = 320, 2 ** 30 - 256, 1, 4
+    assert _bytes("haste_hip_causal_conv_workspace_bytes", T, N, D, W) >= T // 64 * N * (W + 1) * D * 4
