@@ -262,6 +262,9 @@ void causal_conv_backward_kernel(ConvShape s, Rows<const T> x, const float* __re
   store_channels<V>(mine + (size_t)W * D, c, D, db);
 }
 
+// Threads that a run of every row takes.
+size_t items_of(int N, int D) { return (size_t)N * ((D + V - 1) / V); }
+
 // Steps in a run: 64, and down to 8 (the W-1 steps read twice must stay few) where that leaves fewer
 // than two wavefronts a SIMD.
 int run_length(int T, size_t items) {
@@ -277,7 +280,7 @@ struct ConvPartials {
 };
 ConvPartials partials_of(int T, int N, int D, int W) {
   ConvPartials p;
-  const size_t chunk = run_length(T, (size_t)N * ((D + V - 1) / V));
+  const size_t chunk = run_length(T, items_of(N, D));
   p.parts = (T + chunk - 1) / chunk * N;
   p.columns = (size_t)(W + 1) * D;
   p.floats = p.parts * p.columns;
@@ -288,8 +291,7 @@ ConvPartials partials_of(int T, int N, int D, int W) {
 template <typename T, int W>
 int forward(hipStream_t stream, ConvShape s, const Rows<const T>& x, const float* kernel, const float* bias, const T* state,
             const long long* lengths, T* y, T* state_out) {
-  const size_t items = (size_t)s.N * ((s.D + V - 1) / V), blocks = (items + 255) / 256;
-  if (blocks > kGridLimit) return too_large("causal_conv: too many rows of channels");
+  const size_t items = items_of(s.N, s.D), blocks = (items + 255) / 256;
   s.chunk = run_length(s.T, items);
   ScopedKernelTimer timer("causal_conv_forward", stream);
   dim3 grid((unsigned)blocks, (s.T + s.chunk - 1) / s.chunk);
@@ -302,8 +304,7 @@ template <typename T, int W>
 int backward(hipStream_t stream, ConvShape s, const Rows<const T>& x, const float* kernel, const float* bias, const T* state,
              const long long* lengths, const Rows<const T>& dy, const T* dstate_out, T* dx, float* dkernel,
              float* dbias, T* dstate, float* workspace, size_t workspace_bytes) {
-  const size_t items = (size_t)s.N * ((s.D + V - 1) / V), blocks = (items + 255) / 256;
-  if (blocks > kGridLimit) return too_large("causal_conv: too many rows of channels");
+  const size_t items = items_of(s.N, s.D), blocks = (items + 255) / 256;
   s.chunk = run_length(s.T, items);
   const ConvPartials p = partials_of(s.T, s.N, s.D, W);
   if (workspace_bytes < p.total * sizeof(float)) return too_large("causal_conv_backward: the workspace is too small");
@@ -336,7 +337,12 @@ int with_width(int W, F&& f) {
 }
 
 bool sizes_ok(int T, int N, int D, int W) { return T > 0 && N > 0 && D > 0 && W > 0; }
-bool sizes_small(int T, int N, int D) { return T <= kSizeLimit && N <= kSizeLimit && D <= kSizeLimit / kMaxWidth; }
+// For the calls and for the size of their workspace alike.
+int check_limits(int T, int N, int D) {
+  if (T > kSizeLimit || N > kSizeLimit || D > kSizeLimit / kMaxWidth) return too_large("causal_conv: sizes beyond 2^30");
+  if ((items_of(N, D) + 255) / 256 > kGridLimit) return too_large("causal_conv: too many rows of channels");
+  return HASTE_HIP_OK;
+}
 
 template <typename T>
 int forward_entry(int steps, int batch_size, int channels, int width, const void* x, size_t x_step, size_t x_row,
@@ -344,7 +350,7 @@ int forward_entry(int steps, int batch_size, int channels, int width, const void
                   void* state_out, void* stream) {
   HASTE_HIP_REQUIRE(sizes_ok(steps, batch_size, channels, width));
   HASTE_HIP_REQUIRE(x && kernel && y);
-  if (!sizes_small(steps, batch_size, channels)) return too_large("causal_conv: sizes beyond 2^30");
+  HASTE_HIP_PROPAGATE(check_limits(steps, batch_size, channels));
   return with_width(width, [&](auto w) {
     return forward<T, w()>(as_stream(stream), {steps, batch_size, channels, 0, silu}, {static_cast<const T*>(x), x_step, x_row},
                            kernel, bias, static_cast<const T*>(state), static_cast<const long long*>(lengths),
@@ -359,7 +365,7 @@ int backward_entry(int steps, int batch_size, int channels, int width, const voi
                    void* dstate, void* workspace, size_t workspace_bytes, void* stream) {
   HASTE_HIP_REQUIRE(sizes_ok(steps, batch_size, channels, width));
   HASTE_HIP_REQUIRE(x && kernel && dy && dx && dkernel && workspace);
-  if (!sizes_small(steps, batch_size, channels)) return too_large("causal_conv: sizes beyond 2^30");
+  HASTE_HIP_PROPAGATE(check_limits(steps, batch_size, channels));
   return with_width(width, [&](auto w) {
     return backward<T, w()>(as_stream(stream), {steps, batch_size, channels, 0, silu},
                             {static_cast<const T*>(x), x_step, x_row}, kernel, bias, static_cast<const T*>(state),
@@ -377,7 +383,8 @@ extern "C" {
 using namespace haste_hip;
 
 size_t haste_hip_causal_conv_workspace_bytes(int steps, int batch_size, int channels, int width) {
-  if (!sizes_ok(steps, batch_size, channels, width) || !sizes_small(steps, batch_size, channels) || width > kMaxWidth) return 0;
+  if (!sizes_ok(steps, batch_size, channels, width) || width > kMaxWidth) return 0;
+  if (check_limits(steps, batch_size, channels) != HASTE_HIP_OK) return 0;
   return partials_of(steps, batch_size, channels, width).total * sizeof(float);
 }
 

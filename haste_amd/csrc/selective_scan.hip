@@ -836,6 +836,8 @@ int with_lanes(int S, F&& f) {
   }
 }
 
+size_t blocks_of(const ScanShape& s) { return (size_t)s.N * s.G * s.blocks_group; }
+
 // The time axis is cut where rows and channels make too few workgroups, into chunks that make about two a CU, of no fewer than 4
 // tiles, and of no more than so many that joining them (a memory round trip for every four) takes the time of the steps saved:
 // 3 sqrt(tiles), T=8192 N=1 D=128 and T=32768 N=1 D=64 forward 46 and 110 us with 64 chunks, 55 and 85 with 128, 54 and 158 with 512.
@@ -847,7 +849,7 @@ ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, bool backwar
   const int block = 256 / lanes_for(S);
   s.blocks_group = (s.share + block - 1) / block;
   s.block_channels = ((s.share + s.blocks_group - 1) / s.blocks_group + 3) / 4 * 4;
-  const size_t blocks = (size_t)N * G * s.blocks_group, tiles = ((size_t)T + TS - 1) / TS;
+  const size_t blocks = blocks_of(s), tiles = ((size_t)T + TS - 1) / TS;
   const size_t least = backward ? 2 : 3, most = tiles / 4, join = (size_t)(3.0 * std::sqrt((double)tiles));
   size_t chunks = 2 * (size_t)device_cu_count() / blocks;
   chunks = chunks < most ? chunks : most;
@@ -856,6 +858,12 @@ ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, bool backwar
   s.chunk = (int)((tiles + chunks - 1) / chunks) * TS;
   s.chunks = (int)(((size_t)T + s.chunk - 1) / s.chunk);
   return s;
+}
+
+// For the calls and for the size of their workspace alike.
+int check_grid(const ScanShape& s) {
+  if (blocks_of(s) > kGridLimit || (size_t)s.chunks > kGridLimitYZ) return too_large("selective_scan: too many rows of channels");
+  return HASTE_HIP_OK;
 }
 
 // Floats of workspace, in the order they lie there.
@@ -884,10 +892,9 @@ ScanWorkspace backward_workspace(const ScanShape& s) {
 template <typename T>
 int forward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, const float* h0, T* y, float* h_last, float* kept,
             float* workspace, size_t workspace_bytes) {
-  const size_t blocks = (size_t)s.N * s.G * s.blocks_group;
+  const size_t blocks = blocks_of(s);
   const ScanWorkspace w = forward_workspace(s);
-  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ)
-    return too_large("selective_scan: too many rows of channels");
+  HASTE_HIP_PROPAGATE(check_grid(s));
   if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_forward: the workspace is too small");
   HASTE_HIP_REQUIRE(workspace != nullptr || w.total == 0);
   float *added = workspace, *sum_dt = s.chunks > 1 ? workspace + w.sum_dt : nullptr;
@@ -909,11 +916,10 @@ template <typename T>
 int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, const float* kept, const Rows<const T>& dy,
              const float* dh_last, T* dx, T* ddelta, float* dA, T* dB, T* dC, float* dskip, T* dz, float* dbias, float* dh0,
              float* workspace, size_t workspace_bytes) {
-  const size_t blocks = (size_t)s.N * s.G * s.blocks_group;
+  const size_t blocks = blocks_of(s);
   const size_t shared = (size_t)s.T * s.N * s.G * s.S, columns = (size_t)s.D * (s.S + 2);
   const ScanWorkspace w = backward_workspace(s);
-  if (blocks > kGridLimit || (size_t)s.chunks > kGridLimitYZ)
-    return too_large("selective_scan: too many rows of channels");
+  HASTE_HIP_PROPAGATE(check_grid(s));
   if (workspace_bytes < w.total * sizeof(float)) return too_large("selective_scan_backward: the workspace is too small");
   float *added = workspace + w.added, *sum_dt = workspace + w.sum_dt;
   const ScanGradients<T> out = {dx, ddelta, dz, dh0, workspace + w.partial, workspace + w.dB, workspace + w.dC};
@@ -988,9 +994,9 @@ using namespace haste_hip;
 
 size_t haste_hip_selective_scan_workspace_bytes(int backward, int steps, int batch_size, int channels, int states, int groups) {
   if (check_sizes(steps, batch_size, channels, states, groups) != HASTE_HIP_OK) return 0;
-  const size_t floats = backward ? backward_workspace(shape_of(steps, batch_size, channels, states, groups, 0, true)).total
-                                 : forward_workspace(shape_of(steps, batch_size, channels, states, groups, 0, false)).total;
-  return floats * sizeof(float);
+  const ScanShape s = shape_of(steps, batch_size, channels, states, groups, 0, backward != 0);
+  if (check_grid(s) != HASTE_HIP_OK) return 0;
+  return (backward ? backward_workspace(s) : forward_workspace(s)).total * sizeof(float);
 }
 
 size_t haste_hip_selective_scan_kept_bytes(int steps, int batch_size, int channels, int states) {

@@ -36,3 +36,18 @@ def test_workspaces_of_more_than_2_31_partials():
     """Runs of 64 steps or fewer times rows: counted in more than 32 bits."""
     T, N, D, W = 320, 2 ** 30 - 256, 1, 4
     assert _bytes("haste_hip_causal_conv_workspace_bytes", T, N, D, W) >= T // 64 * N * (W + 1) * D * 4
+
+
+def test_workspaces_of_sizes_that_are_refused_are_0():
+    """More workgroups than a grid has."""
+    conv, scan = (64, 2 ** 22, 2 ** 12, 4), (64, 2 ** 20, 64, 16, 8)
+    assert _bytes("haste_hip_causal_conv_workspace_bytes", *conv) == 0
+    code, reason = _refusal("haste_hip_causal_conv_backward_f32", *conv, 256, 0, 0, 256, None, 1, None, None, 256, 0, 0, None, 256, 256,
+                            None, None, 256, 2 ** 62)
+    assert code == UNSUPPORTED and "too many rows" in reason
+    assert _bytes("haste_hip_selective_scan_workspace_bytes", 0, *scan) == _bytes("haste_hip_selective_scan_workspace_bytes", 1, *scan) == 0
+    code, reason = _scan_backward(*scan, 2 ** 62)
+    assert code == UNSUPPORTED and "too many rows" in reason
+    # one row less is taken
+    assert _bytes("haste_hip_selective_scan_workspace_bytes", 1, 64, 2 ** 19 - 1, 64, 16, 8) > 0
+    assert _bytes("haste_hip_causal_conv_workspace_bytes", 64, 2 ** 20 - 1, 2 ** 12, 4) > 0
