@@ -22,6 +22,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "channel_share.h"
 #include "sequence.h"
 
 namespace haste_hip {
@@ -36,9 +37,8 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 
 struct ScanShape {
   int T, N, D, S, G;
-  int share;           // channels of a group, D / G
   int blocks_group;    // workgroups of a group
-  int block_channels;  // channels of a workgroup
+  ChannelShare share;  // of its D / G channels among them
   int chunk, chunks;   // steps of a chunk (a multiple of TS)
   int softplus;
 };
@@ -143,8 +143,9 @@ __device__ __forceinline__ void store_states(float* p, int s0, int S, const floa
   store_channels<K>(p, s0, S, h);
 }
 
-// Which row and channels a workgroup works on: c0 .. c_end-1.  The workgroups of a group share its channels evenly (in fours), so
-// that the last one is not left with one or two.
+// Which row and channels a workgroup works on: c0 .. c_end-1.  The workgroups of a group share its channels evenly: a share of
+// 64 for all but the last one costs that one the whole time axis for the few that are left.  T=1024 N=8 S=16 bf16, forward and
+// backward: D=961 242 us instead of 288, D=1025 315 instead of 385, D=1024 231 either way.
 template <int LANES>
 struct Block {
   int n, g, c0, c_end;
@@ -153,8 +154,9 @@ struct Block {
     n = block / per_row;
     const unsigned rest = block % per_row;
     g = rest / s.blocks_group;
-    c0 = g * s.share + (int)(rest % s.blocks_group) * s.block_channels;
-    c_end = min(c0 + s.block_channels, (g + 1) * s.share);
+    const ChannelRange range = s.share.of((int)(rest % s.blocks_group));
+    c0 = g * s.share.channels + range.first;
+    c_end = g * s.share.channels + range.end;
   }
 };
 
@@ -783,7 +785,7 @@ __global__ __launch_bounds__(256)
 void selective_scan_step_kernel(ScanShape s, ScanInputs<T> in, const float* h, float* h_out, T* __restrict__ y) {
   const unsigned i = blockIdx.x * 256 + threadIdx.x, d = i / LANES, s0 = i % LANES * K;
   if (d >= (unsigned)s.D) return;  // (the lanes of a channel together)
-  const size_t shared = (size_t)(d / s.share) * s.S;
+  const size_t shared = (size_t)(d / s.share.channels) * s.S;
   float A2[K];
   load_states(in.A + (size_t)d * s.S, s0, s.S, A2);
 #pragma unroll
@@ -845,10 +847,8 @@ size_t blocks_of(const ScanShape& s) { return (size_t)s.N * s.G * s.blocks_group
 // N=4 D=4096 S=16 bf16 (256 workgroups) 244 and 254 us, T=128 N=32 D=512 18 and 22.  Backward, where it costs two fifths,
 // it is: 680 and 559, 53 and 50.
 ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, bool backward) {
-  ScanShape s = {T, N, D, S, G, D / G, 0, 0, 0, 0, softplus};
-  const int block = 256 / lanes_for(S);
-  s.blocks_group = (s.share + block - 1) / block;
-  s.block_channels = ((s.share + s.blocks_group - 1) / s.blocks_group + 3) / 4 * 4;
+  const int block = 256 / lanes_for(S), workgroups = (D / G + block - 1) / block;
+  ScanShape s = {T, N, D, S, G, workgroups, {D / G, workgroups}, 0, 0, softplus};
   const size_t blocks = blocks_of(s), tiles = ((size_t)T + TS - 1) / TS;
   const size_t least = backward ? 2 : 3, most = tiles / 4, join = (size_t)(3.0 * std::sqrt((double)tiles));
   size_t chunks = 2 * (size_t)device_cu_count() / blocks;
@@ -937,7 +937,7 @@ int backward(hipStream_t stream, const ScanShape& s, const ScanInputs<T>& in, co
   };
   HASTE_HIP_PROPAGATE(with_lanes(s.S, [&](auto lanes) {
     if constexpr (Tile<lanes()>::WIDTH > 1) {
-      if (s.share % Tile<lanes()>::WIDTH != 0) return launch(lanes, std::false_type());
+      if (s.share.channels % Tile<lanes()>::WIDTH != 0) return launch(lanes, std::false_type());
     }
     return launch(lanes, std::true_type());
   }));
@@ -972,7 +972,7 @@ ScanInputs<T> inputs_of(const void* x, size_t x_step, size_t x_row, const void* 
 template <typename T>
 int step(hipStream_t stream, int N, int D, int S, int G, int softplus, const ScanInputs<T>& in, const float* h, T* y,
          float* h_out) {
-  const ScanShape s = {1, N, D, S, G, D / G, 0, 0, TS, 1, softplus};
+  const ScanShape s = {1, N, D, S, G, 1, {D / G, 1}, TS, 1, softplus};
   return with_lanes(S, [&](auto lanes) {
     const size_t across = ((size_t)D * lanes() + 255) / 256;  // at most 2^22: D is at most 2^30 / 66
     if (across > kGridLimit) return too_large("selective_scan: too many channels");
