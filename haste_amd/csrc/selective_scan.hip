@@ -295,8 +295,12 @@ __device__ __forceinline__ void join_chunks(float (&h)[K], const float (&A2)[K],
     for (int j = 0; j < AHEAD; ++j) {
       if (k + j >= count) break;
 #pragma unroll
-      for (int r = 0; r < K; ++r)  // (0 times a product of growth beyond float's range is 0, not NaN)
-        h[r] = h[r] == 0.f ? added[j][r] : __builtin_amdgcn_exp2f(A2[r] * dt[j]) * h[r] + added[j][r];
+      for (int r = 0; r < K; ++r) {
+        // In two halves: a whole chunk's decay may lie below what a float holds where the state it leaves does not, and growth
+        // above.  (0 times a product of growth beyond float's range is 0, not NaN.)
+        const float half = __builtin_amdgcn_exp2f(0.5f * A2[r] * dt[j]);
+        h[r] = h[r] == 0.f ? added[j][r] : half * (half * h[r]) + added[j][r];
+      }
     }
   }
 }

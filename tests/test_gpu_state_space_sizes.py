@@ -4,6 +4,9 @@ import torch
 
 from haste_amd import ops
 
+import state_space_formulas as formulas
+from test_gpu_state_space import Problem, compare, run_scan
+
 pytestmark = pytest.mark.gpu
 
 
@@ -54,3 +57,26 @@ def test_scan_with_more_sums_than_a_grid():
             mine = got[k][:, half] if k in ("h_last", "dh0") else got[k][:, :, half] if v.dim() > 2 else got[k][half]
             assert torch.equal(mine, v), k
         del want
+
+
+def test_scan_in_chunks_that_decay_and_grow_by_more_than_float_holds():
+    """Over one chunk of the time axis (64 steps here) exp(A sum dt) is 2^-185 and 2^162; the states before and behind it are floats,
+    and stay what they are over the other chunks (steps of 0)."""
+    T, D, S = 1024, 16, 4
+    q = Problem(7, torch.float32)
+    delta = torch.zeros(T, 1, D, dtype=torch.float64)
+    delta[320:384] = 0.25
+    q.put("delta", delta)
+    q.put("A", torch.tensor([-8.0, 7.0, -0.5, 0.0]).expand(D, S))
+    for name in ("x", "dy"):
+        q.put(name, torch.zeros(T, 1, D))
+    for name in ("B", "C"):
+        q.normal(name, T, 1, 1, S)
+    for name in ("h0", "dh_last"):
+        q.put(name, torch.tensor([1e20, 1e-30, 1.0, -3.0]).expand(1, D, S).contiguous())
+    q.absent("D", "z", "delta_bias")
+    q.lengths(None)
+    q.p["softplus"] = q.g["softplus"] = False
+    want = formulas.scan(q.p)
+    assert 1e-36 < want["h_last"][..., 0].min() < 1e-35 and 1e18 < want["dh0"][..., 1].min() < 1e19
+    compare(run_scan(q.g), want, formulas.scan(q.p, True), 12 * T + 512)
