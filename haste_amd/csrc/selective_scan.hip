@@ -19,6 +19,7 @@
 // pass finds what each chunk adds to a state of zero and sum dt, by which it decays what it is given
 // (exp(A sum dt)); the second pass runs all chunks at once, each from what those before it hand over.
 // The same backwards with G.
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -141,6 +142,16 @@ __device__ __forceinline__ void load_states(const float* p, int s0, int S, float
 }
 __device__ __forceinline__ void store_states(float* p, int s0, int S, const float (&h)[K]) {
   store_channels<K>(p, s0, S, h);
+}
+
+// The rates of decay to base 2, all finite: a step of 0, as those behind a row's end in its last tile are, leaves as it is a state that
+// forgets everything at any other.
+__device__ __forceinline__ void base2_rates(const float (&A)[K], float (&A2)[K]) {
+#pragma unroll
+  for (int r = 0; r < K; ++r) {
+    const float rate = A[r] * kLog2e;
+    A2[r] = __builtin_fabsf(rate) == INFINITY ? copysignf(FLT_MAX, rate) : rate;
+  }
 }
 
 // Which row and channels a workgroup works on: c0 .. c_end-1.  The workgroups of a group share its channels evenly: a share of
@@ -338,9 +349,9 @@ void selective_scan_forward_kernel(ScanShape s, ScanInputs<T> in, const float* _
 #pragma unroll
   for (int r = 0; r < K; ++r) A2[r] = h[r] = 0.f;
   if (live) {
-    load_states(in.A + (size_t)d * s.S, s0, s.S, A2);
-#pragma unroll
-    for (int r = 0; r < K; ++r) A2[r] *= kLog2e;
+    float A[K];
+    load_states(in.A + (size_t)d * s.S, s0, s.S, A);
+    base2_rates(A, A2);
     if (!LOCAL) {
       if (h0 != nullptr) load_states(h0 + state, s0, s.S, h);
       if (blockIdx.y > 0)
@@ -535,8 +546,7 @@ void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* 
   for (int r = 0; r < K; ++r) A[r] = A2[r] = G[r] = dA[r] = 0.f;
   if (live) {
     load_states(in.A + (size_t)d * s.S, s0, s.S, A);
-#pragma unroll
-    for (int r = 0; r < K; ++r) A2[r] = A[r] * kLog2e;
+    base2_rates(A, A2);
     if (!LOCAL) {
       if (dh_last != nullptr) load_states(dh_last + state, s0, s.S, G);
       if (chunk + 1 < (unsigned)s.chunks)
@@ -790,10 +800,9 @@ void selective_scan_step_kernel(ScanShape s, ScanInputs<T> in, const float* h, f
   const unsigned i = blockIdx.x * 256 + threadIdx.x, d = i / LANES, s0 = i % LANES * K;
   if (d >= (unsigned)s.D) return;  // (the lanes of a channel together)
   const size_t shared = (size_t)(d / s.share.channels) * s.S;
-  float A2[K];
-  load_states(in.A + (size_t)d * s.S, s0, s.S, A2);
-#pragma unroll
-  for (int r = 0; r < K; ++r) A2[r] *= kLog2e;
+  float A[K], A2[K];
+  load_states(in.A + (size_t)d * s.S, s0, s.S, A);
+  base2_rates(A, A2);
   const float bias = in.bias != nullptr ? in.bias[d] : 0.f, skip = in.skip != nullptr ? in.skip[d] : 0.f;
   const bool gated = in.z.p != nullptr;
 

@@ -5,7 +5,7 @@ import torch
 from haste_amd import ops
 
 import state_space_formulas as formulas
-from test_gpu_state_space import Problem, compare, run_scan
+from test_gpu_state_space import Problem, compare, run_scan, scan_problem
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,24 @@ def test_scan_in_chunks_that_decay_and_grow_by_more_than_float_holds():
     want = formulas.scan(q.p)
     assert 1e-36 < want["h_last"][..., 0].min() < 1e-35 and 1e18 < want["dh0"][..., 1].min() < 1e19
     compare(run_scan(q.g), want, formulas.scan(q.p, True), 12 * T + 512)
+
+
+@pytest.mark.parametrize("T", [16, 20, 203])
+def test_scan_of_states_that_forget_everything(T):
+    """A of -inf: the state is the step's own input, also where the row ends within a tile (and chunks of the time axis are joined)."""
+    q = scan_problem(T, torch.float32, T, 2, 24, 16, softplus=False, lengths=None)
+    q.put("delta", q.p["delta"] + 0.01)
+    A = q.p["A"].clone()
+    A[:, ::3] = -float("inf")
+    q.put("A", A)
+    want, magnitude = formulas.scan(q.p), formulas.scan(q.p, True)
+    got = run_scan(q.g)
+    unknown = ("ddelta", "ddelta_bias")  # 0 times infinity: NaN in the formula too
+    assert want["ddelta"].isnan().all() and want["dx"].isfinite().all()
+    compare({k: v for k, v in got.items() if k not in unknown}, want, magnitude, 12 * T + 200)
+    short = {k: v[:T - 3] if torch.is_tensor(v) and v.dim() > 2 and len(v) == T else v for k, v in q.p.items()}
+    ended = run_scan(dict(q.g, lengths=torch.full((2,), T - 3, device="cuda")))
+    compare({k: ended[k] for k in ("h_last", "dh0", "dA", "dD")}, formulas.scan(short), formulas.scan(short, True), 12 * T + 200)
+    step = {k: v[0] if k in ("x", "delta", "B", "C", "z") else v for k, v in q.g.items()}
+    _, h = ops.selective_scan_iterate(step["x"], torch.zeros_like(step["delta"]), step["A"], step["B"], step["C"], step["h0"])
+    assert torch.equal(h, q.g["h0"])  # a step of 0
