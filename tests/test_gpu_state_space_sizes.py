@@ -4,8 +4,9 @@ import torch
 
 from haste_amd import ops
 
+import state_space_bounds as bounds
 import state_space_formulas as formulas
-from test_gpu_state_space import Problem, compare, run_scan, scan_problem
+from test_gpu_state_space import DTYPES, Problem, compare, norm_problem, run_conv, run_norm, run_scan, scan_problem
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +102,133 @@ def test_scan_of_states_that_forget_everything(T):
     step = {k: v[0] if k in ("x", "delta", "B", "C", "z") else v for k, v in q.g.items()}
     _, h = ops.selective_scan_iterate(step["x"], torch.zeros_like(step["delta"]), step["A"], step["B"], step["C"], step["h0"])
     assert torch.equal(h, q.g["h0"])  # a step of 0
+
+
+# ---- loops that only full grids go through: sizes from the rules by which the kernels are launched --------------
+def _cus():
+    return torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+
+
+def _rows_for_run(T, run, vectors):
+    """Batch rows with which the convolution walks runs of `run` steps: the longest that leave two wavefronts a SIMD."""
+    full = _cus() * 4 * 2 * 64
+    rows = -(-full // (vectors * -(-T // run)))
+    assert run == 64 or rows * vectors * -(-T // (2 * run)) < full, "no number of rows takes such runs"
+    return rows
+
+
+def _parts(entry, sizes, columns):
+    """Partials that a backward pass of these sizes leaves, from the workspace it asks for."""
+    floats = ops._scratch_bytes(entry, torch.device("cuda", torch.cuda.current_device()), *sizes) // 4
+    parts = floats // columns
+    while True:  # what adding them takes lies behind them
+        groups, scratch = -(-parts // 256), 0
+        while groups > 1:
+            scratch, groups = scratch + groups, -(-groups // 256)
+        if (parts + scratch) * columns <= floats:
+            return parts
+        parts -= 1
+
+
+CONV_RUNS = [(64, 63), (64, 64), (64, 65), (64, 127), (64, 128), (64, 129), (64, 200), (32, 33), (32, 64), (32, 65), (32, 96), (32, 97),
+             (16, 17), (16, 32), (16, 33), (16, 49)]
+
+
+@pytest.mark.parametrize("run,T", CONV_RUNS)
+def test_conv_in_long_runs(run, T):
+    """Runs of 16 to 64 steps, whole and in part, with states and with lengths that end anywhere; a few of the channels against the
+    formulas, which know of none beside them."""
+    for dtype, D, W in ((torch.bfloat16, 1021, 4), (torch.float32, 516, 8), (torch.float16, 259, 3)):
+        N = _rows_for_run(T, run, -(-D // 4))
+        print("conv runs", run, T, N, D, W, dtype, flush=True)
+        assert _parts("haste_hip_causal_conv_workspace_bytes", (T, N, D, W), (W + 1) * D) == -(-T // run) * N
+        gen = torch.Generator(device="cuda").manual_seed(T + D)
+        normal = lambda *shape, to=dtype: torch.randn(*shape, generator=gen, device="cuda").to(to)  # noqa: E731, B023
+        g = dict(x=normal(T, N, D), kernel=W ** -0.5 * normal(W, D, to=torch.float32), bias=normal(D, to=torch.float32),
+                 state=normal(W - 1, N, D), dy=normal(T, N, D), dstate_out=normal(W - 1, N, D), silu=True)
+        g["lengths"] = torch.randint(0, T + 1, (N,), generator=gen, device="cuda")
+        g["lengths"][0], g["lengths"][-1] = T, -1
+        behind = ~formulas.inside(g["lengths"].cpu(), T, N)[0].cuda()
+        g["x"][behind] = g["dy"][behind] = float("nan")
+        got = run_conv(g)
+        channels = [0, 1, 5, D // 2, D - 5, D - 4, D - 2, D - 1]
+        p = {k: v[..., channels].double().cpu() if torch.is_tensor(v) and v.is_floating_point() else v for k, v in g.items()}
+        p["lengths"] = g["lengths"].cpu()
+        # a product, sum or slope of W taps within 8 W + 64 roundings; the parameters' sums: a run's steps in turn, then the runs
+        sums = 8 * W + 64 + run + bounds.parts_depth(-(-T // run) * N)
+        bounds.compare({k: v[..., channels] for k, v in got.items()}, formulas.conv(p), formulas.conv(p, True),
+                       {None: 8 * W + 64, "dkernel": sums, "dbias": sums})
+
+
+def _norm_rows(D, waves):
+    """Rows of one turn of all workgroups."""
+    threads = 64
+    while threads * 8 < D:
+        threads *= 2
+    block = max(256, threads)
+    return _cus() * 4 * waves * 64 // block * (block // threads)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=lambda t: str(t).split(".")[1])
+@pytest.mark.parametrize("D", [40, 513, 700, 2048, 4096, 5000, 8192])
+def test_norms_of_more_rows_than_a_turn(D, dtype):
+    """Three turns of the forward pass's workgroups and more of the backward pass's, the last one in part."""
+    forward, backward = _norm_rows(D, 4), _norm_rows(D, 2)
+    rows, centered = 2 * forward + forward // 2 + 3, (D % 1024 == 0) == (dtype == torch.float32)
+    print("norm turns", D, rows, dtype, flush=True)
+    assert _parts("haste_hip_residual_norm_workspace_bytes", (rows, 1, D), 4 * D) == backward
+    q = norm_problem(D, dtype, (rows, 1, D), centered)
+    # every factor, two norms forward and backward, within a row's sum and 32 roundings; sums over rows: turns, then workgroups
+    factors = 8 * (bounds.ROW_SUM + 32)
+    sums = factors + -(-rows // backward) + bounds.parts_depth(backward)
+    bounds.compare(run_norm(q.g, centered), formulas.norm(q.p), formulas.norm(q.p, True),
+                   {None: factors, "dscale": sums, "dafter": sums, "dbefore": sums, "dbias": sums})
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+@pytest.mark.parametrize("D,S,G", [(1024, 16, 1), (500, 64, 4), (2001, 5, 3), (1030, 30, 2)])
+def test_scan_steps_of_more_rows_than_a_turn(D, S, G, dtype):
+    """Workgroups go through three rows, some through two; in place too."""
+    lanes = 2 if S <= 8 else 4 if S <= 16 else 8 if S <= 32 else 16
+    down = _cus() * 8 // -(-D * lanes // 256)
+    N = 2 * down + max(1, down // 3)
+    assert down > 1
+    print("scan step turns", N, D, S, dtype, flush=True)
+    q = scan_problem(D + S, dtype, 1, N, D, S, G)
+    g = {k: v[0] if k in ("x", "delta", "B", "C", "z") else v for k, v in q.g.items()}
+    rest = [g[k] for k in ("D", "z", "delta_bias")]
+    y, h = ops.selective_scan_iterate(g["x"], g["delta"], g["A"], g["B"], g["C"], g["h0"], *rest, True)
+    want, magnitude = formulas.scan(q.p), formulas.scan(q.p, True)
+    for k, v in dict(y=y[None], h_last=h).items():
+        bounds.check(v, want[k], magnitude[k], S + 64, k)
+    state = g["h0"].clone()
+    y2, h2 = ops.selective_scan_iterate(g["x"], g["delta"], g["A"], g["B"], g["C"], state, *rest, True, h_out=state)
+    assert h2 is state and torch.equal(state, h) and torch.equal(y2, y)
+
+
+FORGET = 64  # steps after which a state is exp(-0.2 * 64) = 3e-6 of itself: what is older adds less than a rounding to an output's
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda t: str(t).split(".")[1])
+@pytest.mark.parametrize("T,N,D,S,G", [(100, 520, 10, 16, 1), (60, 260, 18, 33, 1), (1300, 1, 40, 16, 2), (1300, 2, 24, 7, 1),
+                                       (700, 3, 50, 30, 1), (333, 9, 131, 64, 1)])
+def test_scan_within_the_roundings_of_its_memory(T, N, D, S, G, dtype):
+    """Decays of exp(-0.2) and faster: errors of steps long past are forgotten with their states, so that the roundings of a result are
+    those of a memory's steps however long the sequence is.  One piece of the time axis over more workgroups than CUs, and many
+    chunks of it."""
+    print("scan memory", T, N, D, S, G, dtype, flush=True)
+    q = scan_problem(T + D, dtype, T, N, D, S, G, softplus=False)
+    q.put("delta", 0.2 + 0.2 * torch.rand(T, N, D, generator=q.gen, dtype=torch.float64))
+    q.put("A", -1 - 3 * torch.rand(D, S, generator=q.gen, dtype=torch.float64), torch.float32)
+    if T < 1000:
+        q.lengths([T, 0, T - 1] + [1 + (7 * n) % T for n in range(N - 3)])
+        behind = ~formulas.inside(q.p["lengths"], T, N)[0].cuda()
+        for name in ("x", "delta", "z", "B", "C", "dy"):
+            q.g[name][behind] = float("nan")
+    # a step of a state: exponent, exp2, two products, a sum, forward and backward.  Sums over states, over a workgroup's channels and the
+    # workgroups; of parameters: steps in turn (a chunk's, or all of one piece), then chunks and rows
+    each = 12 * FORGET + S + 128
+    shared = each + 64 + -(-D // (16 * G))
+    sums = each + T + bounds.parts_depth(T // 64 * N + N)
+    bounds.compare(run_scan(q.g), formulas.scan(q.p), formulas.scan(q.p, True),
+                   {None: each, "dB": shared, "dC": shared, "dA": sums, "dD": sums, "ddelta_bias": sums}, absent=("ddelta_bias",))
