@@ -865,7 +865,8 @@ def selective_scan_backward(x, delta, A, B, C, D, z, delta_bias, delta_softplus,
     if lengths is not None:
         _check_lengths(lengths, x)
     size = _scratch_bytes("haste_hip_selective_scan_kept_bytes", x.device, T, N, channels, S)
-    if not torch.is_tensor(cache) or cache.dtype != torch.uint8 or cache.numel() != size or cache.device != x.device:
+    if not torch.is_tensor(cache) or cache.dtype != torch.uint8 or cache.numel() != size or cache.device != x.device \
+            or not cache.is_contiguous():
         raise ValueError("the cache must be that of a forward pass in training over the same arguments")
     dy = _zero_rows(T, N, channels, x) if dy is None else dy
     _activation("dy", dy, x.shape, x)

@@ -232,3 +232,14 @@ def test_scan_within_the_roundings_of_its_memory(T, N, D, S, G, dtype):
     sums = each + T + bounds.parts_depth(T // 64 * N + N)
     bounds.compare(run_scan(q.g), formulas.scan(q.p), formulas.scan(q.p, True),
                    {None: each, "dB": shared, "dC": shared, "dA": sums, "dD": sums, "ddelta_bias": sums}, absent=("ddelta_bias",))
+
+
+def test_caches_that_are_not_whole_are_refused():
+    """Views of fewer bytes than they have elements, and of others than the forward pass wrote."""
+    q = scan_problem(3, torch.float32, 20, 2, 24, 16)
+    ins = [q.g[k] for k in ("x", "delta", "A", "B", "C", "D", "z", "delta_bias")]
+    _, _, cache = ops.selective_scan_forward(True, *ins, True, q.g["h0"])
+    spread = torch.stack([cache, cache], -1)[..., 0]
+    for bad in (cache[:1].expand(cache.shape), spread, cache[:-1], cache.float(), cache.cpu(), None):
+        with pytest.raises(ValueError, match="cache"):
+            ops.selective_scan_backward(*ins, True, q.g["h0"], None, bad, q.g["dy"])
