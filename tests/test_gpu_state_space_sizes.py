@@ -243,3 +243,28 @@ def test_caches_that_are_not_whole_are_refused():
     for bad in (cache[:1].expand(cache.shape), spread, cache[:-1], cache.float(), cache.cpu(), None):
         with pytest.raises(ValueError, match="cache"):
             ops.selective_scan_backward(*ins, True, q.g["h0"], None, bad, q.g["dy"])
+
+
+def test_parameters_of_a_long_scan_in_one_piece():
+    """dA adds up T products, here all of one sign, by tiles of 16: their sums' rounding is that of chains of 16, of T / 16 tiles and of 64
+    rows, whose errors add up like steps of a random walk (sqrt(n / 3) of a step where the sum grows evenly).  A single chain of T
+    would be off by sqrt(T / 3) = 52 times a rounding's 0.58 * 2^-24."""
+    T, D, S, N = 8192, 16, 4, _cus() + 4
+    q = Problem(11, torch.float32)
+    positive = lambda *shape: 0.5 + torch.rand(*shape, generator=q.gen, dtype=torch.float64)  # noqa: E731
+    for name in ("x", "dy"):
+        q.put(name, positive(T, 1, D))
+    q.put("delta", 0.1 * positive(T, 1, D))
+    q.put("A", -positive(D, S))
+    for name in ("B", "C"):
+        q.put(name, positive(T, 1, 1, S))
+    q.absent("D", "z", "delta_bias", "h0", "dh_last")
+    q.lengths(None)
+    q.p["softplus"] = q.g["softplus"] = False
+    # the same row for all: enough of them that the time axis is not cut
+    g = {k: v.expand(T, N, *v.shape[2:]) if torch.is_tensor(v) and v.dim() > 2 else v for k, v in q.g.items()}
+    got, want = run_scan(g)["dA"].cpu().double(), N * formulas.scan(q.p)["dA"]
+    assert want.min() > 0
+    error = ((got - want) / want).square().mean().sqrt()
+    # eight roundings for the factors of the products, whose errors have a common part
+    assert error <= 2.0 ** -24 * ((16 / 3 + T / 16 / 3 + 64 / 3) ** 0.5 + 8), error
