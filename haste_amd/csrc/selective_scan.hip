@@ -112,7 +112,8 @@ struct ChannelSums {
 };
 // With four lanes a channel the channels of a row are its four banks, and additions that write some banks only leave each bank with
 // one of the four values: six of them, 24 cycles, for the 44 of swapping rows and halves too, against four times the parts to add
-// up from LDS.  T=2048 N=8 D=4096 S=16 bf16 backward 970 us instead of 1035, T=1024 D=1024 121 instead of 130.
+// up from LDS.  Forward and backward, both builds in turn: T=2048 N=8 D=4096 S=16 bf16 1257 us without, 1211 so (runs differ by 1 %),
+// T=1024 D=1024 239 and 232.
 // (The assembler's form: of the compiler's every addition that leaves banks as they are is a move and an addition.)
 template <>
 struct ChannelSums<4> {
@@ -507,6 +508,10 @@ struct ScanGradients {
 // the sum of dt.  added, sum_dt: as forward, of the chunks but the first.
 // EVEN: the channels of a group are a multiple of WIDTH, and a thread's columns aligned to it, which lets LDS move 16 bytes at a
 // time; without, T=2048 N=8 D=4096 S=16 bf16 takes 3 % more.
+// Two lanes a channel (S up to 8) hold eight elements a thread of each tensor and spill: 36 to 84 bytes a thread in half types, 144 and
+// 152 in float.  T=1024 N=8 D=1024 S=8 78 us in bf16 and 110 in float, where S=16 takes 111 and 113.
+// A workgroup leaves S floats a step of dB and of dC, written here and read to be added up: 4 bytes an element of x at S=16, with 64
+// channels a workgroup, and 64 bytes at S=64, with 16, where adding them up takes 119 us beside 860 (T=2048 N=8 D=1024 bf16).
 template <typename T, int LANES, bool LOCAL, bool EVEN>
 __global__ __launch_bounds__(256, 2)
 void selective_scan_backward_kernel(ScanShape s, ScanInputs<T> in, const float* __restrict__ kept, Rows<const T> dy,
@@ -864,6 +869,9 @@ size_t blocks_of(const ScanShape& s) { return (size_t)s.N * s.G * s.blocks_group
 // The first of the two passes costs two thirds of the second.  Forward that is not won back by two chunks: one and two with T=2048
 // N=4 D=4096 S=16 bf16 (256 workgroups) 244 and 254 us, T=128 N=32 D=512 18 and 22.  Backward, where it costs two fifths,
 // it is: 680 and 559, 53 and 50.
+// From 257 workgroups on there is one chunk.  The backward pass has room for two workgroups a CU (LDS and registers), so that 257
+// to 512 of them take about the time of 512, and a few more those of another round: T=2048 D=4096 S=16 bf16 backward 434 + 131 us at
+// N=4 (two chunks), 844 to 848 at N=5, 6 and 8, 1366 at N=9.
 ScanShape shape_of(int T, int N, int D, int S, int G, int softplus, bool backward) {
   const int block = 256 / lanes_for(S), workgroups = (D / G + block - 1) / block;
   ScanShape s = {T, N, D, S, G, workgroups, {D / G, workgroups}, 0, 0, softplus};
