@@ -100,6 +100,17 @@ class ScratchPrefix {
   size_t saved_;
 };
 
+// While one of these is alive on a host thread, get_workspace() on that thread hands out `memory` (16-byte aligned) as
+// the scratch area and no control block, and never grows it: an entry point whose scratch memory is an argument of its
+// own runs products in it that otherwise use the stream's.
+class CallerScratch {
+ public:
+  CallerScratch(void* memory, size_t bytes);
+  ~CallerScratch();
+  CallerScratch(const CallerScratch&) = delete;
+  CallerScratch& operator=(const CallerScratch&) = delete;
+};
+
 // The scratch part of haste_hip_workspace_bytes(T, N, C, H): what a workspace of that size
 // offers behind its control block.
 size_t workspace_scratch_bound(int T, int N, int C, int H);

@@ -1,0 +1,724 @@
+// A projection with what follows it: y[R,D] = act(x[R,C] W[C,D] + bias) + residual, and its gradients
+//   d = dy act'(pre),  dx = d W^T,  dW = x^T d,  dbias = sum over rows of d.
+// act: none, gelu (v Phi(v), Phi the normal distribution function) or silu (v sigmoid(v)).
+//
+// Half types (f16, bf16).  Bound: the matrix cores (2 R C D flops, dense peak 2.5 PFLOP/s); below some hundred rows the bytes
+// of W.  Products of the matrix cores are exact, sums are float from the first to the last; an output is rounded once.  d is rounded to
+// the activations' type, the matrix cores take no other: what it costs is a rounding of each term of sums that are rounded
+// to that type themselves.  act'(pre) is what the forward pass leaves for the backward pass, in half: it lies between -0.2 and 1.2,
+// where half is eight times as fine as bfloat16, and a float would be as many bytes again as y.
+//
+// One tile kernel makes all three products.  An operand is either stored with the contraction index contiguous (x and d in
+// x W and d W^T, W in d W^T) or with it as the slow index (W in x W, x and d in x^T d).  Tiles go from memory straight into LDS
+// (buffer loads that write LDS: no registers, no wait in between), STAGES of them in a ring: while one is multiplied those behind it are
+// on their way, and a step needs one barrier.  A contiguous operand lies in LDS as rows of BK elements, 16-byte chunk c of row r at
+// position c ^ f(r), so that 16 rows of one chunk cover all banks; an operand of the instruction is one 16-byte read.  A slow
+// one lies as rows of k, 32-byte piece g of row k at g ^ 2 (k % 4), and is read transposed (ds_read_b64_tr_b16: in each 16 lanes,
+// lane i receives element i % 4 of what lanes i / 4 + 4 j address).  Loads beyond an operand's end give zeros.
+// Operands that are not laid out in 16-byte pieces are copied once, rows padded with zeros.
+//
+// Float: the product of gemm.hip (the bf16 matrix cores on floats split in three), with a pass for what follows it.
+#include <type_traits>
+
+#include "sequence.h"
+
+namespace haste_hip {
+namespace {
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef unsigned int uint4_t __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+enum Activation { kNone, kGelu, kSilu };
+
+// Phi(v) and e = exp(-v^2 / 2) for halves: Phi(-x) = t P(t) e with t = 1 / (1 + 0.3 x / sqrt 2) for x >= 0, P the polynomial of
+// degree 8 with the least largest relative error, 4e-8 (fitted to exp(x^2) erfc(x) over 0 <= x <= 14).  For floats the library's
+// function, whose last bits are right too.
+template <typename T>
+__device__ __forceinline__ float normal_below(float v, float& e) {
+  e = __builtin_amdgcn_exp2f(v * v * -0.72134752044f);
+  if constexpr (sizeof(T) == 4) return 0.5f * erfcf(v * -0.70710678119f);
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.21213203436f * fabsf(v));
+  float p = -6.330811700e-02f;
+  p = p * t + 2.359122957e-01f;
+  p = p * t - 2.423442380e-01f;
+  p = p * t + 2.585225439e-01f;
+  p = p * t - 3.702330108e-02f;
+  p = p * t + 1.031920523e-01f;
+  p = p * t + 7.523456362e-02f;
+  p = p * t + 8.521184213e-02f;
+  p = p * t + 8.460237762e-02f;
+  const float below = p * t * e;
+  return v < 0.f ? below : 1.0f - below;
+}
+
+// act(v), and its slope.
+template <typename T>
+__device__ __forceinline__ float activated(int act, float v, float& slope) {
+  if (act == kGelu) {
+    float e;
+    const float below = normal_below<T>(v, e);
+    slope = below + v * e * 0.39894228040f;
+    return v * below;
+  }
+  if (act == kSilu) {
+    const float s = sigmoid_of(v);
+    slope = silu_slope(v, s);
+    return v * s;
+  }
+  slope = 1.0f;
+  return v;
+}
+
+// What becomes of a product's elements.
+template <typename T>
+struct Finish {
+  T* out;
+  size_t ld;
+  int act;
+  const T* bias;                                                              // may be null, like the rest
+  const T* residual;
+  size_t residual_ld;
+  typename std::conditional<sizeof(T) == 4, float, _Float16>::type* slope;    // [rows][columns]
+};
+
+// Eight neighbouring elements of a row, with the bias of their columns.
+template <typename T>
+__device__ __forceinline__ void finish(const Finish<T>& to, float (&v)[8], const float (&bias)[8], size_t row, int col, int columns) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += bias[i];
+  if (to.act != kNone) {
+    float slope[8];
+    if (to.act == kGelu) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = activated<T>(kGelu, v[i], slope[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = activated<T>(kSilu, v[i], slope[i]);
+    }
+    if (to.slope != nullptr) store_channels<8>(to.slope + row * columns, col, columns, slope);
+  }
+  if (to.residual != nullptr) {
+    float r[8];
+    load_channels<8>(to.residual + row * to.residual_ld, col, columns, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += r[i];
+  }
+  store_channels<8>(to.out + row * to.ld, col, columns, v);
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias(const Finish<T>& to, int col, int columns, float (&bias)[8]) {
+  if (to.bias != nullptr) {
+    load_channels<8>(to.bias, col, columns, bias);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bias[i] = 0.f;
+  }
+}
+
+// ---- the tile kernel ---------------------------------------------------------------------
+__device__ __forceinline__ float16_t mfma(_Float16, uint4_t a, uint4_t b, float16_t c) {
+  typedef _Float16 v __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float16_t mfma(__bf16, uint4_t a, uint4_t b, float16_t c) {
+  typedef __bf16 v __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+}
+
+constexpr unsigned int kNowhere = 0x7ffffff0u;  // an offset beyond any resource: the load gives zeros
+
+__device__ __forceinline__ uint4_t resource(const void* base, long long bytes) {
+  const unsigned long long a = reinterpret_cast<unsigned long long>(base);
+  const long long most = 0x7fffffe0ll;
+  return uint4_t{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, (unsigned)(bytes < 0 ? 0 : bytes < most ? bytes : most), 0x00020000u};
+}
+
+// 16 bytes a lane from the resource into LDS at `lds` and the 1008 bytes behind it, lane by lane.  The load has no register
+// to write; it is waited for by count, in tile_ready().
+__device__ __forceinline__ void load_to_lds(unsigned lds, unsigned offset, uint4_t from, unsigned shift) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(from),
+               "s"(shift)
+               : "memory");
+}
+
+// Waits until at most LEFT of this wavefront's loads are on their way and all its reads of LDS have returned, then for the others.
+template <int LEFT>
+__device__ __forceinline__ void tile_ready() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// One operand's part of a stage: WIDTH rows (columns) of the product, BK of the contraction, loaded by WAVES wavefronts.
+template <bool SLOW, int WIDTH, int BK, int WAVES>
+struct Panel {
+  static constexpr int kBytes = WIDTH * BK * 2;
+  static constexpr int kLoads = kBytes / 1024 / WAVES;  // of a wavefront
+  static_assert(kLoads * 1024 * WAVES == kBytes, "a stage is loaded in whole kilobytes");
+  static_assert(BK == 32, "rows of 64 bytes: 16 of a load, which is what turn() repeats after");
+  static constexpr int kChunks = BK / 8;                // 16-byte chunks of a contiguous row
+  static __device__ __forceinline__ int turn(int row) { return (row >> 2) & 3; }
+
+  uint4_t from;
+  const char* base;
+  long long ld_bytes;
+  unsigned offset[kLoads];
+  int columns;     // SLOW: those from the tile's first on, in whole chunks (a load that ends beyond a resource loses its last elements)
+  unsigned chunk;  // contiguous: the lane's first k of a stage
+
+  // first: of the tile's rows (columns), of `count` in all.
+  __device__ __forceinline__ void start(const void* p, long long ld, int first, int count, int k_end, int wave, int lane) {
+    ld_bytes = ld * 2;
+    const int left = count - first;
+    if constexpr (SLOW) {
+      base = static_cast<const char*>(p) + (size_t)first * 2;
+      columns = (left + 7) & ~7;
+      constexpr int LANES = WIDTH / 8, ROWS = 64 / LANES;  // lanes of a row of k, rows of a load
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int k = (i * WAVES + wave) * ROWS + lane / LANES, unit = lane % LANES;
+        const int column = ((unit >> 1) ^ (2 * (k & 3))) * 16 + (unit & 1) * 8;
+        offset[i] = column < left ? (unsigned)(k * ld_bytes + column * 2) : kNowhere;
+      }
+    } else {
+      base = static_cast<const char*>(p) + (size_t)first * ld_bytes;
+      const int rows = left < WIDTH ? left : WIDTH;
+      from = resource(base, (rows - 1) * ld_bytes + (long long)((k_end + 7) & ~7) * 2);
+      constexpr int ROWS = 64 / kChunks;
+      const int in_row = lane / kChunks;
+      chunk = ((lane % kChunks) ^ turn(in_row)) * 8;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = (i * WAVES + wave) * ROWS + in_row;
+        offset[i] = row < rows ? (unsigned)(row * ld_bytes + chunk * 2) : kNowhere;
+      }
+    }
+  }
+  __device__ __forceinline__ void request(unsigned lds, int k0, int k_end, int wave) {
+    if constexpr (SLOW) {
+      const uint4_t at = resource(base + k0 * ld_bytes, (long long)(k_end - k0 - 1) * ld_bytes + (long long)columns * 2);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load_to_lds(lds + (i * WAVES + wave) * 1024, offset[i], at, 0);
+    } else {
+      const bool gone = k0 + (int)chunk >= k_end;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        load_to_lds(lds + (i * WAVES + wave) * 1024, gone ? kNowhere : offset[i], from, (unsigned)k0 * 2);
+    }
+  }
+  // Eight k of step ks of row (column) `first` + lane % 32: k = 16 ks + 8 (lane / 32) on.
+  static __device__ __forceinline__ uint4_t operand(const char* stage, int first, int ks, int lane) {
+    if constexpr (SLOW) {
+      uint4_t v;
+      const int q = lane >> 4, i = lane & 15;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = 16 * ks + 8 * (q >> 1) + 4 * h + (i >> 2);
+        const int piece = ((first >> 4) + (q & 1)) ^ (2 * (k & 3));
+        typedef __attribute__((address_space(3))) short4_t* lds_t;
+        const short4_t part = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(stage + k * (WIDTH * 2) + piece * 32 + (i & 3) * 8));
+        __builtin_memcpy(reinterpret_cast<char*>(&v) + 8 * h, &part, 8);
+      }
+      return v;
+    } else {
+      const int row = first + (lane & 31), c = 2 * ks + (lane >> 5);
+      return *reinterpret_cast<const uint4_t*>(stage + row * (BK * 2) + (c ^ turn(row)) * 16);
+    }
+  }
+};
+
+template <bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_, int BK_, int STAGES_>
+struct Tile {
+  static constexpr bool A_SLOW = A_SLOW_, B_SLOW = B_SLOW_;
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, WAVES = WAVES_M * WAVES_N, BK = BK_, STAGES = STAGES_;
+  static constexpr int MI = BM / WAVES_M / 32, NJ = BN / WAVES_N / 32;
+  typedef Panel<A_SLOW, BM, BK, WAVES> PA;
+  typedef Panel<B_SLOW, BN, BK, WAVES> PB;
+  static constexpr int kStage = PA::kBytes + PB::kBytes;
+  static constexpr int kSlabLd = NJ * 32 + 4;           // floats of a row of a wavefront's results in LDS
+  static constexpr int kSlabs = WAVES * 32 * kSlabLd * 4;
+  static constexpr int kLds = kStage * STAGES > kSlabs ? kStage * STAGES : kSlabs;
+};
+
+struct Product {
+  int M, N, K;
+  const void *A, *B;
+  long long lda, ldb;
+  int tiles_m, tiles_n, k_per_piece;  // tiles whole, or cut along K
+  float* partial;                     // [piece][M][N], null: whole
+};
+
+constexpr int kTallest = 8;  // rows of tiles that are gone through side by side
+
+template <typename T, class G>
+__global__ __launch_bounds__(64 * G::WAVES, 2)
+void linear_tile_kernel(Product p, Finish<T> to) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups go to the XCDs in turn; each XCD is given a range of the work, in blocks of tiles that share rows of A and
+  // columns of B.
+  const unsigned each = gridDim.x >> 3, rest = gridDim.x & 7, xcd = blockIdx.x & 7;
+  const unsigned work = xcd * each + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+  const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
+  const int piece = work / tiles, tile = work % tiles;
+  const int band = tile / (kTallest * p.tiles_n), in_band = tile % (kTallest * p.tiles_n);
+  const int tall = p.tiles_m - band * kTallest < kTallest ? p.tiles_m - band * kTallest : kTallest;
+  const int m0 = (band * kTallest + in_band % tall) * G::BM, n0 = in_band / tall * G::BN;
+  const int k_begin = piece * p.k_per_piece;
+  const int k_end = k_begin + p.k_per_piece < p.K ? k_begin + p.k_per_piece : p.K;
+  const int wm = wave / G::WAVES_N * (G::MI * 32), wn = wave % G::WAVES_N * (G::NJ * 32);
+
+  typename G::PA pa;
+  typename G::PB pb;
+  pa.start(p.A, p.lda, m0, p.M, k_end, wave, lane);
+  pb.start(p.B, p.ldb, n0, p.N, k_end, wave, lane);
+  const unsigned lds_at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
+
+  float16_t acc[G::MI][G::NJ];
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  const int steps = (k_end - k_begin + G::BK - 1) / G::BK;
+  auto request = [&](int step) {
+    const unsigned at = lds_at + step % G::STAGES * G::kStage;
+    pa.request(at, k_begin + step * G::BK, k_end, wave);
+    pb.request(at + G::PA::kBytes, k_begin + step * G::BK, k_end, wave);
+  };
+  constexpr int kAhead = G::STAGES - 1, kLoads = G::PA::kLoads + G::PB::kLoads;
+  for (int s = 0; s < kAhead && s < steps; ++s) request(s);
+  for (int s = 0; s < steps; ++s) {
+    if (s + kAhead <= steps) tile_ready<(kAhead - 1) * kLoads>();
+    else tile_ready<0>();
+    if (s + kAhead < steps) request(s + kAhead);  // over the stage of step s - 1, which all have read
+    const char* stage = lds + s % G::STAGES * G::kStage;
+#pragma unroll
+    for (int ks = 0; ks < G::BK / 16; ++ks) {
+      uint4_t a[G::MI], b[G::NJ];
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i) a[i] = G::PA::operand(stage, wm + 32 * i, ks, lane);
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) b[j] = G::PB::operand(stage + G::PA::kBytes, wn + 32 * j, ks, lane);
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = mfma(T(), a[i], b[j], acc[i][j]);
+    }
+  }
+  tile_ready<0>();
+
+  // 32 rows of a wavefront's results at a time go through LDS, so that a lane has eight neighbouring elements of a row.
+  float* slab = reinterpret_cast<float*>(lds) + wave * 32 * G::kSlabLd;
+  constexpr int LANES = G::NJ * 4, ROWS = 64 / LANES;  // lanes of a row, rows at a time
+  const int col = n0 + wn + lane % LANES * 8;
+  float bias[8];
+  if (p.partial == nullptr) load_bias(to, col, p.N, bias);
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) {
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        slab[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * G::kSlabLd + 32 * j + (lane & 31)] = acc[i][j][e];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+    for (int r = 0; r < 32; r += ROWS) {
+      const int in_slab = r + lane / LANES, row = m0 + wm + 32 * i + in_slab;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = slab[in_slab * G::kSlabLd + lane % LANES * 8 + e];
+      if (row < p.M) {
+        if (p.partial != nullptr) store_channels<8>(p.partial + ((size_t)piece * p.M + row) * p.N, col, p.N, v);
+        else finish(to, v, bias, row, col, p.N);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The pieces of a product, added in order, and what follows.  PIECES null: the elements lie in `to.out` already (float).
+template <typename T>
+__global__ __launch_bounds__(256)
+void linear_finish_kernel(int M, int N, int pieces, const float* __restrict__ partial, Finish<T> to) {
+  const unsigned groups = (N + 7) / 8;
+  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < (size_t)M * groups; i += (size_t)gridDim.x * 256) {
+    const size_t row = i / groups;
+    const int col = (int)(i % groups) * 8;
+    float v[8], bias[8];
+    load_bias(to, col, N, bias);
+    if (partial == nullptr) {
+      load_channels<8>(to.out + row * to.ld, col, N, v);
+    } else {
+      load_channels<8>(partial + row * N, col, N, v);
+      for (int z = 1; z < pieces; ++z) {
+        float w[8];
+        load_channels<8>(partial + ((size_t)z * M + row) * N, col, N, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += w[e];
+      }
+    }
+    finish(to, v, bias, row, col, N);
+  }
+}
+
+// rows x columns, rows padded with zeros to a multiple of eight elements.
+template <typename T>
+__global__ __launch_bounds__(256)
+void linear_pack_kernel(int rows, int columns, const T* __restrict__ in, size_t ld, T* __restrict__ out) {
+  const unsigned groups = (columns + 7) / 8;
+  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < (size_t)rows * groups; i += (size_t)gridDim.x * 256) {
+    const size_t row = i / groups;
+    const int col = (int)(i % groups) * 8;
+    *reinterpret_cast<typename Packed<T, 8>::type*>(out + i * 8) = load_packed<8>(in + row * ld, col, columns);
+  }
+}
+
+// d = dy slope, rows padded as above, and its sums over the rows of a workgroup.  Bound: HBM.  A workgroup takes 512 columns,
+// eight a lane; its four wavefronts take the rows of its share in turn.
+constexpr int kSumColumns = 512;
+template <typename T>
+__global__ __launch_bounds__(256)
+void linear_slope_kernel(int M, int N, int rows_each, const T* __restrict__ dy, size_t dy_ld,
+                         const typename std::conditional<sizeof(T) == 4, float, _Float16>::type* __restrict__ slope,
+                         T* __restrict__ d, size_t d_ld, float* __restrict__ partial) {
+  __shared__ float red[4][kSumColumns];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = blockIdx.x * kSumColumns + lane * 8;
+  const int first = blockIdx.y * rows_each, last = M - first < rows_each ? M : first + rows_each;
+  float sum[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+#pragma unroll 4
+  for (int row = first + wave; row < last; row += 4) {
+    float v[8];
+    load_channels<8>(dy + row * dy_ld, col, N, v);
+    if (slope != nullptr) {
+      float s[8];
+      load_channels<8>(slope + (size_t)row * N, col, N, s);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= s[i];
+    }
+    if (d != nullptr && col < (int)d_ld) store_channels<8>(d + row * d_ld, col, (int)d_ld, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += v[i];
+  }
+  if (partial == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[wave][lane * 8 + i] = sum[i];
+  __syncthreads();
+  for (int c = threadIdx.x; c < kSumColumns; c += 256)
+    if (blockIdx.x * kSumColumns + c < (unsigned)N)
+      partial[(size_t)blockIdx.y * N + blockIdx.x * kSumColumns + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256)
+void linear_round_kernel(int n, const float* __restrict__ in, T* __restrict__ out) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) out[i] = (T)in[i];
+}
+
+// ---- plans -------------------------------------------------------------------------------
+int cus() { return device_cu_count() > 0 ? device_cu_count() : 256; }
+
+struct Plan {
+  bool large;  // tiles of 256 x 256, otherwise of 128 x 128
+  int tiles_m, tiles_n, pieces, k_per_piece;
+  size_t floats;
+};
+
+Plan plan_product(int M, int N, int K) {
+  Plan best = {};
+  double least = 1e300;
+  for (int large = 0; large < 2; ++large) {
+    const int side = large ? 256 : 128;
+    const long long tm = (M + side - 1) / side, tn = (N + side - 1) / side, tiles = tm * tn;
+    const int slots = large ? cus() : 2 * cus();
+    for (int s = 1; s <= 32; ++s) {
+      int per = (K + s - 1) / s;
+      per = (per + 63) / 64 * 64;
+      const int pieces = (K + per - 1) / per;
+      if (pieces != s || (s > 1 && (per < 128 || tiles * s > 4ll * slots))) continue;
+      const double rounds = (double)((tiles * s + slots - 1) / slots);
+      double cost = rounds * (per + 256) * (large ? 4.0 : 2.4);
+      if (s > 1) cost += 2000 + (double)s * M * N * 8 / 2.2e6;
+      if (cost < least) {
+        least = cost;
+        best = {large != 0, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, class G>
+int launch_tiles(hipStream_t stream, const Product& p, int pieces, const Finish<T>& to) {
+  linear_tile_kernel<T, G><<<dim3((unsigned)(p.tiles_m * p.tiles_n * pieces)), dim3(64 * G::WAVES), 0, stream>>>(p, to);
+  HASTE_HIP_TRY(hipGetLastError());
+  return HASTE_HIP_OK;
+}
+
+int blocks_for(size_t threads) {
+  const size_t b = (threads + 255) / 256, most = (size_t)cus() * 32;
+  return (int)(b < most ? b : most);
+}
+
+// to = A B, as the operands are stored; `scratch`: what plan_product() says.
+template <typename T, bool A_SLOW, bool B_SLOW>
+int product(hipStream_t stream, int M, int N, int K, const void* A, long long lda, const void* B, long long ldb, const Finish<T>& to,
+            float* scratch) {
+  const Plan plan = plan_product(M, N, K);
+  Product p = {M, N, K, A, B, lda, ldb, plan.tiles_m, plan.tiles_n, plan.k_per_piece, plan.pieces > 1 ? scratch : nullptr};
+  {
+    ScopedKernelTimer timer("linear_product", stream);
+    if (plan.large) HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 256, 256, 2, 4, 32, 4>>(stream, p, plan.pieces, to)));
+    else HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 128, 128, 2, 2, 32, 4>>(stream, p, plan.pieces, to)));
+  }
+  if (plan.pieces > 1) {
+    ScopedKernelTimer timer("linear_finish", stream);
+    linear_finish_kernel<T><<<blocks_for((size_t)M * ((N + 7) / 8)), 256, 0, stream>>>(M, N, plan.pieces, scratch, to);
+    HASTE_HIP_TRY(hipGetLastError());
+  }
+  return HASTE_HIP_OK;
+}
+
+size_t whole(size_t bytes) { return (bytes + 255) / 256 * 256; }
+long long eights(long long n) { return (n + 7) / 8 * 8; }
+
+struct SumPlan {
+  int blocks, rows_each;
+  size_t floats, scratch;
+};
+SumPlan plan_sums(int rows, int columns) {
+  const int across = (columns + kSumColumns - 1) / kSumColumns;
+  long long blocks = (4ll * cus() + across - 1) / across;
+  const long long most = (rows + 15) / 16;
+  blocks = blocks < most ? blocks : most;
+  SumPlan s;
+  s.rows_each = (int)((rows + blocks - 1) / blocks);
+  s.blocks = (rows + s.rows_each - 1) / s.rows_each;
+  s.floats = (size_t)s.blocks * columns;
+  s.scratch = column_sums_scratch(s.blocks, columns);
+  return s;
+}
+
+// Where what a call keeps in its workspace lies; sizes in bytes.
+struct Layout {
+  size_t x, kernel, d, sums, product, total;
+};
+
+size_t float_product_bytes(int M, int N, int K) {
+  // a contraction that exceeds the float product's panels is cut into runs, whose pieces are bounded by four tiles a CU
+  const size_t bytes = gemm_f32_scratch_bytes(M, N, K);
+  if ((long long)K * (M > N ? M : N) < (1ll << 28)) return bytes;
+  const size_t bound = (size_t)4 * cus() * 128 * 128 * sizeof(float);
+  return bytes > bound ? bytes : bound;
+}
+
+Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) {
+  Layout l = {};
+  const bool pack_x = element == 2 && (!aligned || C % 8 != 0), pack_kernel = element == 2 && (!aligned || D % 8 != 0);
+  size_t at = 0;
+  auto place = [&](size_t bytes) {
+    const size_t here = at;
+    at += whole(bytes);
+    return here;
+  };
+  l.x = place(pack_x ? (size_t)R * eights(C) * 2 : 0);
+  l.kernel = place(pack_kernel ? (size_t)C * eights(D) * 2 : 0);
+  if (backward) {
+    l.d = place(element == 2 ? (size_t)R * eights(D) * 2 : (size_t)R * D * 4);
+    if (element == 4) l.kernel = place((size_t)C * D * 4);  // transposed
+    const SumPlan s = plan_sums(R, D);
+    l.sums = place((s.floats + s.scratch + D) * sizeof(float));
+  }
+  l.product = at;
+  size_t need;
+  if (element == 2) {
+    const size_t a = backward ? plan_product(R, C, D).floats : plan_product(R, D, C).floats;
+    const size_t b = backward ? plan_product(C, D, R).floats : 0;
+    need = (a > b ? a : b) * sizeof(float);
+  } else {
+    const size_t a = backward ? float_product_bytes(R, C, D) : float_product_bytes(R, D, C);
+    const size_t b = backward ? float_product_bytes(C, D, R) : 0;
+    need = a > b ? a : b;
+  }
+  l.total = at + whole(need);
+  return l;
+}
+
+int check_sizes(int R, int C, int D, int element) {
+  HASTE_HIP_REQUIRE(R > 0 && C > 0 && D > 0);
+  if (R > kSizeLimit || C > (1 << 20) || D > (1 << 20)) return too_large("linear: more than 2^30 rows or 2^20 columns");
+  const auto tiles = [](long long m, long long n) { return ((m + 127) / 128) * ((n + 127) / 128); };
+  const long long most = element == 2 ? (1ll << 22) : (1ll << 24);
+  if (tiles(R, D) >= most || tiles(R, C) >= most || tiles(C, D) >= most) return too_large("linear: more tiles than a grid takes");
+  return HASTE_HIP_OK;
+}
+
+bool in_pieces(const void* p, size_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
+
+template <typename T>
+int pack(hipStream_t stream, int rows, int columns, const T* in, size_t ld, T* out) {
+  linear_pack_kernel<T><<<blocks_for((size_t)rows * ((columns + 7) / 8)), 256, 0, stream>>>(rows, columns, in, ld, out);
+  HASTE_HIP_TRY(hipGetLastError());
+  return HASTE_HIP_OK;
+}
+
+// An operand in 16-byte pieces: itself, or its copy.  The rows of a contiguous operand have to end with zeros.
+template <typename T>
+int placed(hipStream_t stream, int rows, int columns, const T*& p, size_t& ld, T* copy, bool aligned) {
+  if (columns % 8 == 0 && in_pieces(p, ld)) return HASTE_HIP_OK;
+  if (aligned && columns % 8 == 0) return HASTE_HIP_ERROR_INVALID_ARGUMENT;  // the workspace has no room for it
+  HASTE_HIP_PROPAGATE(pack(stream, rows, columns, p, ld, copy));
+  p = copy;
+  ld = (size_t)eights(columns);
+  return HASTE_HIP_OK;
+}
+
+bool workspace_ok(const void* workspace, size_t bytes, size_t need) {
+  return need == 0 || (workspace != nullptr && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0);
+}
+
+template <typename T>
+int forward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kernel, const T* bias, int act, const T* residual,
+                  size_t residual_row, T* y, void* cache, void* workspace, size_t workspace_bytes, void* stream_) {
+  HASTE_HIP_PROPAGATE(check_sizes(R, C, D, sizeof(T)));
+  HASTE_HIP_REQUIRE(x != nullptr && kernel != nullptr && y != nullptr && act >= kNone && act <= kSilu);
+  HASTE_HIP_REQUIRE(R == 1 || x_row >= (size_t)C);
+  if (R == 1) x_row = C;
+  if (x_row > (size_t)(1 << 22)) return too_large("linear: rows of x more than 2^22 elements apart");
+  hipStream_t stream = as_stream(stream_);
+  const bool aligned = in_pieces(x, x_row) && in_pieces(kernel, 8);
+  const Layout l = layout_of(false, sizeof(T), R, C, D, aligned);
+  HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
+  char* ws = static_cast<char*>(workspace);
+  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type slope_t;
+  Finish<T> to = {y, (size_t)D, act, bias, residual, residual_row, act == kNone ? nullptr : static_cast<slope_t*>(cache)};
+  if constexpr (sizeof(T) == 4) {
+    {
+      CallerScratch scratch(ws + l.product, l.total - l.product);
+      HASTE_HIP_PROPAGATE(gemm_f32(stream, false, R, D, C, x, (int)x_row, kernel, D, y, D, false));
+    }
+    if (act == kNone && bias == nullptr && residual == nullptr) return HASTE_HIP_OK;
+    ScopedKernelTimer timer("linear_finish", stream);
+    linear_finish_kernel<T><<<blocks_for((size_t)R * ((D + 7) / 8)), 256, 0, stream>>>(R, D, 0, nullptr, to);
+    HASTE_HIP_TRY(hipGetLastError());
+    return HASTE_HIP_OK;
+  } else {
+    size_t kernel_row = D;
+    HASTE_HIP_PROPAGATE(placed(stream, R, C, x, x_row, reinterpret_cast<T*>(ws + l.x), aligned));
+    HASTE_HIP_PROPAGATE(placed(stream, C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel), aligned));
+    return product<T, false, true>(stream, R, D, C, x, x_row, kernel, kernel_row, to, reinterpret_cast<float*>(ws + l.product));
+  }
+}
+
+template <typename T>
+int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kernel, int act, const void* cache, const T* dy, size_t dy_row,
+                   T* dx, T* dkernel, T* dbias, void* workspace, size_t workspace_bytes, void* stream_) {
+  HASTE_HIP_PROPAGATE(check_sizes(R, C, D, sizeof(T)));
+  HASTE_HIP_REQUIRE(x != nullptr && kernel != nullptr && dy != nullptr && act >= kNone && act <= kSilu);
+  HASTE_HIP_REQUIRE(act == kNone || cache != nullptr);
+  HASTE_HIP_REQUIRE(R == 1 || (x_row >= (size_t)C && dy_row >= (size_t)D));
+  if (R == 1) x_row = C, dy_row = D;
+  if (x_row > (size_t)(1 << 22) || dy_row > (size_t)(1 << 22)) return too_large("linear: rows more than 2^22 elements apart");
+  hipStream_t stream = as_stream(stream_);
+  const bool aligned = in_pieces(x, x_row) && in_pieces(kernel, 8);
+  const Layout l = layout_of(true, sizeof(T), R, C, D, aligned);
+  HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
+  char* ws = static_cast<char*>(workspace);
+  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type slope_t;
+
+  // d and its sums
+  const T* d = dy;
+  size_t d_row = dy_row;
+  const bool own = act != kNone || (sizeof(T) == 2 && (D % 8 != 0 || !in_pieces(dy, dy_row)));
+  if (own) {
+    d = reinterpret_cast<T*>(ws + l.d);
+    d_row = sizeof(T) == 2 ? (size_t)eights(D) : (size_t)D;
+  }
+  if (own || dbias != nullptr) {
+    const SumPlan s = plan_sums(R, D);
+    float* sums = reinterpret_cast<float*>(ws + l.sums);
+    {
+      ScopedKernelTimer timer("linear_slope", stream);
+      linear_slope_kernel<T><<<dim3((unsigned)((D + kSumColumns - 1) / kSumColumns), (unsigned)s.blocks), 256, 0, stream>>>(
+          R, D, s.rows_each, dy, dy_row, act == kNone ? nullptr : static_cast<const slope_t*>(cache),
+          own ? reinterpret_cast<T*>(ws + l.d) : nullptr, d_row, dbias != nullptr ? sums : nullptr);
+      HASTE_HIP_TRY(hipGetLastError());
+    }
+    if (dbias != nullptr) {
+      const size_t n = D;
+      float* total = sizeof(T) == 4 ? reinterpret_cast<float*>(dbias) : sums + s.floats + s.scratch;
+      HASTE_HIP_PROPAGATE(column_sums(stream, s.blocks, n, sums, sums + s.floats, {{total}, {n, n, n, n}}));
+      if (sizeof(T) == 2) {
+        linear_round_kernel<T><<<(D + 255) / 256, 256, 0, stream>>>(D, total, dbias);
+        HASTE_HIP_TRY(hipGetLastError());
+      }
+    }
+  }
+  if constexpr (sizeof(T) == 4) {
+    CallerScratch scratch(ws + l.product, l.total - l.product);
+    if (dx != nullptr) {
+      float* turned = reinterpret_cast<float*>(ws + l.kernel);
+      HASTE_HIP_PROPAGATE(haste_hip_transpose_f32(C, D, kernel, turned, stream_));
+      HASTE_HIP_PROPAGATE(gemm_f32(stream, false, R, C, D, d, (int)d_row, turned, C, dx, C, false));
+    }
+    if (dkernel != nullptr) HASTE_HIP_PROPAGATE(gemm_f32(stream, true, C, D, R, x, (int)x_row, d, (int)d_row, dkernel, D, false));
+    return HASTE_HIP_OK;
+  } else {
+    float* scratch = reinterpret_cast<float*>(ws + l.product);
+    if (dx != nullptr) {
+      size_t kernel_row = D;
+      HASTE_HIP_PROPAGATE(placed(stream, C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel), aligned));
+      const Finish<T> to = {dx, (size_t)C, kNone, nullptr, nullptr, 0, nullptr};
+      HASTE_HIP_PROPAGATE((product<T, false, false>(stream, R, C, D, d, d_row, kernel, kernel_row, to, scratch)));
+    }
+    if (dkernel != nullptr) {
+      HASTE_HIP_PROPAGATE(placed(stream, R, C, x, x_row, reinterpret_cast<T*>(ws + l.x), aligned));
+      const Finish<T> to = {dkernel, (size_t)D, kNone, nullptr, nullptr, 0, nullptr};
+      HASTE_HIP_PROPAGATE((product<T, true, true>(stream, C, D, R, x, x_row, d, d_row, to, scratch)));
+    }
+    return HASTE_HIP_OK;
+  }
+}
+
+}  // namespace
+}  // namespace haste_hip
+
+extern "C" {
+
+using namespace haste_hip;
+
+size_t haste_hip_linear_workspace_bytes(int backward, int element_bytes, int rows, int inputs, int outputs, int aligned) {
+  if ((element_bytes != 2 && element_bytes != 4) || check_sizes(rows, inputs, outputs, element_bytes) != HASTE_HIP_OK) return 0;
+  return layout_of(backward != 0, element_bytes, rows, inputs, outputs, aligned != 0).total;
+}
+
+#define HASTE_HIP_LINEAR(SUFFIX, T)                                                                                        \
+  int haste_hip_linear_forward_##SUFFIX(int rows, int inputs, int outputs, const void* x, size_t x_row, const void* kernel, \
+                                        const void* bias, int activation, const void* residual, size_t residual_row,       \
+                                        void* y, void* cache, void* workspace, size_t workspace_bytes, void* stream) {     \
+    return forward_entry<T>(rows, inputs, outputs, static_cast<const T*>(x), x_row, static_cast<const T*>(kernel),         \
+                            static_cast<const T*>(bias), activation, static_cast<const T*>(residual), residual_row,        \
+                            static_cast<T*>(y), cache, workspace, workspace_bytes, stream);                                \
+  }                                                                                                                        \
+  int haste_hip_linear_backward_##SUFFIX(int rows, int inputs, int outputs, const void* x, size_t x_row,                   \
+                                         const void* kernel, int activation, const void* cache, const void* dy,            \
+                                         size_t dy_row, void* dx, void* dkernel, void* dbias, void* workspace,             \
+                                         size_t workspace_bytes, void* stream) {                                           \
+    return backward_entry<T>(rows, inputs, outputs, static_cast<const T*>(x), x_row, static_cast<const T*>(kernel),        \
+                             activation, cache, static_cast<const T*>(dy), dy_row, static_cast<T*>(dx),                    \
+                             static_cast<T*>(dkernel), static_cast<T*>(dbias), workspace, workspace_bytes, stream);        \
+  }
+
+HASTE_HIP_LINEAR(f32, float)
+HASTE_HIP_LINEAR(f16, _Float16)
+HASTE_HIP_LINEAR(bf16, __bf16)
+
+}  // extern "C"

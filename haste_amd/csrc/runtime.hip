@@ -232,6 +232,8 @@ namespace {
 thread_local int t_assumed_cus = 0, t_assumed_xcds = 0;
 thread_local PlannedPass* t_planned = nullptr;
 thread_local size_t t_scratch_prefix = 0;
+thread_local float* t_caller_scratch = nullptr;
+thread_local size_t t_caller_scratch_bytes = 0;
 }  // namespace
 
 PlannedPass* planned_pass() { return t_planned; }
@@ -399,7 +401,24 @@ int recover_from_abort_locked(int dev, hipStream_t stream, Workspace& ws, unsign
 ScratchPrefix::ScratchPrefix(size_t bytes) : saved_(t_scratch_prefix) { t_scratch_prefix = saved_ + bytes; }
 ScratchPrefix::~ScratchPrefix() { t_scratch_prefix = saved_; }
 
+CallerScratch::CallerScratch(void* memory, size_t bytes) {
+  t_caller_scratch = static_cast<float*>(memory);
+  t_caller_scratch_bytes = bytes;
+}
+CallerScratch::~CallerScratch() { t_caller_scratch = nullptr; }
+
 int get_workspace(hipStream_t stream, size_t scratch_bytes, Workspace* out) {
+  if (t_caller_scratch != nullptr) {
+    if (scratch_bytes > t_caller_scratch_bytes) {
+      set_error_text("the call's workspace is too small");
+      return HASTE_HIP_ERROR_UNSUPPORTED_SIZE;
+    }
+    *out = Workspace();
+    out->scratch = t_caller_scratch;
+    out->scratch_bytes = t_caller_scratch_bytes;
+    out->caller_owned = true;
+    return HASTE_HIP_OK;
+  }
   if (PlannedPass* pass = planned_pass()) {
     if (pass->lent > 0 && scratch_bytes > pass->lent) return HASTE_HIP_ERROR_UNSUPPORTED_SIZE;
     pass->asked = pass->asked > scratch_bytes ? pass->asked : scratch_bytes;

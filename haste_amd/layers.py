@@ -1038,3 +1038,180 @@ class ResidualNorm(_BlockLayer):
         if self._fused(update) or update.is_cuda and not list(self.parameters()):
             return _ResidualNormFunction.apply(update, residual, gate, *map(_as_float, weights), self.centered, self.eps)
         return _eager_residual_norm(update, residual, gate, *weights, self.centered, self.eps)
+
+
+# ---- the layers of a gated linear recurrent block, and the clipping of gradients ----------------------
+class _LinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, training, x, kernel, bias, activation, residual):
+        y, cache = ops.linear_forward(training and any(ctx.needs_input_grad), x, kernel, bias, activation, residual)
+        ctx.save_for_backward(x, kernel, bias, cache)
+        ctx.activation, ctx.has_residual = activation, residual is not None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, kernel, bias, cache = ctx.saved_tensors
+        wanted = ctx.needs_input_grad
+        dx = dkernel = dbias = None
+        if any(wanted[1:4]):
+            dx, dkernel, dbias = ops.linear_backward(x, kernel, bias, ctx.activation, cache, dy, wanted[1], wanted[2])
+        return None, dx, dkernel, dbias, None, dy if ctx.has_residual else None
+
+
+class _GatedRecurrenceFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, training, x, forget, admit, z, decay, forget_bias, admit_bias, h0, lengths):
+        y, h_last, cache = ops.gated_recurrence_forward(training and any(ctx.needs_input_grad), x, forget, admit, z, decay, forget_bias,
+                                                        admit_bias, h0, lengths)
+        ctx.save_for_backward(x, forget, admit, z, decay, forget_bias, admit_bias, h0, lengths, cache)
+        ctx.set_materialize_grads(False)
+        return y, h_last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh_last):
+        return (None, *ops.gated_recurrence_backward(*ctx.saved_tensors, dy, dh_last), None)
+
+
+def _eager_linear(x, kernel, bias, activation, residual):
+    dtype = x.dtype
+    x, kernel, bias, residual = _wide(x, kernel, bias, residual)
+    y = x @ kernel if bias is None else x @ kernel + bias
+    y = {"none": lambda v: v, "gelu": F.gelu, "silu": F.silu}[activation](y)
+    return (y if residual is None else y + residual).to(dtype)
+
+
+def _eager_gated_recurrence(x, forget, admit, z, decay, forget_bias, admit_bias, h0, lengths):
+    dtype, (T, N, D) = x.dtype, x.shape
+    x, forget, admit, z, decay, forget_bias, admit_bias, h = _wide(x, forget, admit, z, decay, forget_bias, admit_bias, h0)
+    inside = _inside(lengths, T, N, x)[..., None]
+    x, forget, admit, z = (t if t is None else torch.where(inside, t, 0.0) for t in (x, forget, admit, z))
+    raw = forget if forget_bias is None else forget + forget_bias
+    r = torch.sigmoid(raw)
+    i = None if admit is None else torch.sigmoid(admit if admit_bias is None else admit + admit_bias)
+    fed = x if i is None else x * i
+    if decay is None:
+        a, u = r, fed if i is not None else torch.sigmoid(-raw) * x
+    else:
+        a, u = torch.exp(-decay * r), torch.sqrt(-torch.expm1(-2 * decay * r)) * fed
+    h = x.new_zeros(N, D) if h is None else h
+    ys = []
+    for t in range(T):
+        h = torch.where(inside[t], a[t] * h + u[t], h)
+        ys.append(h)
+    y = torch.stack(ys)
+    y = y if z is None else y * F.silu(z)
+    return torch.where(inside, y, 0.0).to(dtype), h
+
+
+class Linear(_BlockLayer):
+    """A projection with what follows it: act(input kernel + bias) + residual.  activation: "none", "gelu" (v times the normal
+    distribution function) or "silu" (v sigmoid(v)).  Parameters: kernel [inputs, outputs] (uniform in +-sqrt(6 / (inputs + outputs))),
+    bias [outputs] (zeros); they are handed over in the input's type, and their gradients come back in the type they have."""
+    _name = "Linear"
+
+    def __init__(self, inputs, outputs, bias=True, activation="none"):
+        super().__init__()
+        if activation not in ("none", "gelu", "silu"):
+            raise ValueError("%s: activation must be none, gelu or silu, got %r" % (self._name, activation))
+        self.inputs, self.outputs, self.activation = inputs, outputs, activation
+        self.kernel = nn.Parameter(torch.empty(inputs, outputs))
+        self.bias = nn.Parameter(torch.empty(outputs)) if bias else None
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            nn.init.xavier_uniform_(self.kernel)
+            if self.bias is not None:
+                self.bias.zero_()
+
+    def forward(self, input, residual=None):
+        """input [T,N,inputs] (in whatever order, or [N,inputs]), residual [T,N,outputs] -> [T,N,outputs]."""
+        kernel, bias = self.kernel, self.bias
+        if self._fused(input):
+            return _LinearFunction.apply(torch.is_grad_enabled(), input, kernel.to(input.dtype),
+                                         None if bias is None else bias.to(input.dtype), self.activation, residual)
+        return _eager_linear(input, kernel, bias, self.activation, residual)
+
+
+class GatedRecurrence(_BlockLayer):
+    """Gated linear recurrence, one state a channel: with r = sigmoid(forget + forget_bias), i = sigmoid(admit + admit_bias)
+    h[t] = a h[t-1] + sqrt(1 - a^2) i x with a = exp(-exp(log_decay) r), or (decay=False) h[t] = r h[t-1] + i x;  output h silu(z).
+    admit=False: no gate on inputs, i = 1 (without a decay i = 1 - r).  Parameters, each [channels]: log_decay (decays of
+    0.81 to 0.998 under an open gate), forget_bias (zeros; without a decay from 0.5 to 6), admit_bias (zeros)."""
+    _name = "GatedRecurrence"
+
+    def __init__(self, channels, decay=True, admit=True, batch_first=False):
+        super().__init__()
+        self.channels, self.batch_first = channels, batch_first
+        self.log_decay = nn.Parameter(torch.empty(channels)) if decay else None
+        self.forget_bias = nn.Parameter(torch.empty(channels))
+        self.admit_bias = nn.Parameter(torch.empty(channels)) if admit else None
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            if self.log_decay is not None:
+                self.log_decay.copy_(torch.log(-2 * torch.log(torch.empty_like(self.log_decay, dtype=torch.float32).uniform_(0.9, 0.999))))
+                self.forget_bias.zero_()
+            else:
+                self.forget_bias.uniform_(0.5, 6.0)
+            if self.admit_bias is not None:
+                self.admit_bias.zero_()
+
+    def _arguments(self, x, forget, admit, z):
+        if (admit is None) != (self.admit_bias is None):
+            raise ValueError("%s: admit must be %s" % (self._name, "left out" if self.admit_bias is None else "given"))
+        fused = self._fused(x)
+        of = _as_float if fused else lambda p: p
+        decay = None if self.log_decay is None else torch.exp(of(self.log_decay))
+        return fused, (x, forget, admit, z, decay, of(self.forget_bias), of(self.admit_bias))
+
+    def forward(self, x, forget, admit=None, z=None, state=None, lengths=None):
+        """x, forget, admit, z [T,N,channels] ([N,T,channels] if batch_first) -> (output, state): state [N,channels], float32,
+        before the first step (None: zeros) and after the last (of the row's length).  Outputs behind a row's length are 0."""
+        x, forget, admit, z = (self._rows(t) for t in (x, forget, admit, z))
+        lengths = self._lengths(lengths, x)
+        fused, arguments = self._arguments(x, forget, admit, z)
+        if fused:
+            y, state = _GatedRecurrenceFunction.apply(torch.is_grad_enabled(), *arguments, state, lengths)
+        else:
+            y, state = _eager_gated_recurrence(*arguments, state, lengths)
+        return self._rows(y), state
+
+    def step(self, x, forget, admit=None, z=None, state=None):
+        """One step without gradients: x, forget, admit, z [N,channels] -> (output, state)."""
+        with torch.no_grad():
+            if state is None:
+                state = torch.zeros(x.shape, device=x.device, dtype=x.dtype if x.dtype == torch.float64 else torch.float32)
+            fused, arguments = self._arguments(x, forget, admit, z)
+            if fused:
+                return ops.gated_recurrence_iterate(*arguments[:2], state, *arguments[2:])
+            steps = (t if t is None else t.unsqueeze(0) for t in arguments[:4])
+            y, state = _eager_gated_recurrence(*steps, *arguments[4:], state, None)
+            return y[0], state
+
+
+def clip_gradients_(parameters, max_norm):
+    """Scales the gradients of `parameters` (a tensor or several; those without one are left out) in place so that their norm
+    together is at most max_norm: each times min(1, max_norm / (norm + 1e-6)).  Returns the norm before, a tensor of no axes; on the GPU
+    nothing is waited for.  Gradients of float32, float64, float16 and bfloat16 may be mixed, on one device."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    with torch.no_grad():
+        if grads[0].is_cuda:
+            return ops.clip_gradients(grads, max_norm, out=grads)[1]
+        if any(g.is_cuda for g in grads):
+            raise ValueError("gradients must be on one device")
+        if not float(max_norm) >= 0:
+            raise ValueError("max_norm must not be below 0, got %r" % max_norm)
+        wide = torch.float64 if any(g.dtype == torch.float64 for g in grads) else torch.float32
+        norm = torch.sqrt(sum(g.double().square().sum() for g in grads)).to(wide)
+        factor = (float(max_norm) / (norm.double() + 1e-6)).clamp(max=1.0)
+        for g in grads:
+            g.copy_(g.double() * factor if g.dtype == torch.float64 else g.float() * factor.float())
+        return norm

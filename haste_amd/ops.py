@@ -977,3 +977,261 @@ def residual_norm_backward(update, residual, gate, scale, after_weight, before_w
     values += (*map(_address, grads), *map(_address, sums), scratch.data_ptr(), scratch.numel())
     _invoke(device, "haste_hip_residual_norm_backward" + suffix, values)
     return (*grads, *sums)
+
+
+# ---- The operators of a gated linear recurrent block -----------------------------------
+# Projections with what follows them, the gated linear recurrence, and the clipping of gradients.  They have no counterpart in the
+# reference.  Types, strides, lengths and scratch memory are as for the state space operators above; a projection's parameters have
+# the activations' type.
+_LINEAR_ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2}
+
+
+def _linear_rows(t):
+    """[T,N,D] or [N,D] as rows of contiguous columns that are equally far apart: the tensor (or a copy) and their distance."""
+    strides, shape = t.stride(), t.shape
+    if strides[-1] == 1 or shape[-1] == 1:
+        row = strides[-2] if shape[-2] != 1 else strides[0] if len(shape) == 3 and shape[0] != 1 else shape[-1]
+        if row >= shape[-1] and (len(shape) == 2 or shape[0] == 1 or shape[1] == 1 or strides[0] == strides[1] * shape[1]):
+            return t, row
+    t = t.contiguous()
+    return t, shape[-1]
+
+
+def _linear_arguments(x, kernel, bias, activation):
+    """The arguments checked: the sizes, x as rows, the kernel, its bias, the activation's number, the device and the suffix."""
+    if not isinstance(x, torch.Tensor) or x.dim() not in (2, 3) or not x.numel():
+        raise ValueError("x must be [T,N,C] or [N,C], of no size 0, got %s" % _described(x))
+    if not isinstance(kernel, torch.Tensor) or kernel.dim() != 2 or not kernel.numel():
+        raise ValueError("kernel must be [C,D], of no size 0, got %s" % _described(kernel))
+    number = _LINEAR_ACTIVATIONS.get(activation)
+    if number is None:
+        raise ValueError("activation must be one of %s, got %r" % (sorted(_LINEAR_ACTIVATIONS), activation))
+    C, D, device = x.shape[-1], kernel.shape[1], x.get_device()
+    if not (_alike(x.dtype, device, kernel, bias) and kernel.shape[0] == C and (bias is None or bias.shape == (D,))):
+        _activation("kernel", kernel, (C, D), x)  # one of these says what is wrong
+        _activation("bias", bias, (D,), x)
+    suffix = _activation_suffix(x)
+    rows, step = _linear_rows(x)
+    return (x.numel() // C, C, D), rows, step, _contiguous(kernel), _contiguous(bias), number, device, suffix
+
+
+def _linear_scratch(backward, x, sizes, rows, step, kernel):
+    aligned = not (rows.data_ptr() | kernel.data_ptr()) & 15 and not step & 7
+    size = _scratch_bytes("haste_hip_linear_workspace_bytes", x.device, backward, x.element_size(), *sizes, int(aligned))
+    return torch.empty(max(1, size), device=x.device, dtype=torch.uint8)
+
+
+def linear_forward(training, x, kernel, bias=None, activation="none", residual=None):
+    """x[T,N,C] (or [N,C]), kernel[C,D], bias[D], residual[T,N,D], all of one type -> y[T,N,D], cache (what the backward pass needs
+    of the activation; None unless training, and without one): y = act(x kernel + bias) + residual.  activation: "none",
+    "gelu" (v times the normal distribution function) or "silu" (v sigmoid(v))."""
+    sizes, rows, step, kernel, bias, number, device, suffix = _linear_arguments(x, kernel, bias, activation)
+    shape, residual_step = (*x.shape[:-1], sizes[2]), 0
+    if residual is not None:
+        _activation("residual", residual, shape, x)
+        residual, residual_step = _linear_rows(residual)
+    y, cache = x.new_empty(shape), None
+    if training and number:
+        cache = torch.empty(shape, device=x.device, dtype=torch.float32 if x.dtype is torch.float32 else torch.float16)
+    scratch = _linear_scratch(0, x, sizes, rows, step, kernel)
+    _invoke(device, "haste_hip_linear_forward" + suffix,
+            [*sizes, rows.data_ptr(), step, kernel.data_ptr(), _address(bias), number, _address(residual), residual_step, y.data_ptr(),
+             _address(cache), scratch.data_ptr(), scratch.numel()])
+    return y, cache
+
+
+def linear_backward(x, kernel, bias, activation, cache, dy, with_dx=True, with_dkernel=True):
+    """Gradients (dx, dkernel, dbias) from that of y, which is the residual's as well, and the cache of the forward pass in training of
+    the same arguments; dbias is None where there is no bias, the others where they are not wanted."""
+    sizes, rows, step, kernel, bias, number, device, suffix = _linear_arguments(x, kernel, bias, activation)
+    shape = (*x.shape[:-1], sizes[2])
+    _activation("dy", dy, shape, x)
+    if number:
+        kept = torch.float32 if x.dtype is torch.float32 else torch.float16
+        if not _is(cache, shape, kept, device) or not cache.is_contiguous():
+            raise ValueError("the cache must be that of a forward pass in training over the same arguments")
+    else:
+        cache = None
+    dy, dy_step = _linear_rows(dy)
+    dx = x.new_empty(x.shape) if with_dx else None
+    dkernel = torch.empty_like(kernel) if with_dkernel else None
+    dbias = None if bias is None else torch.empty_like(bias)
+    scratch = _linear_scratch(1, x, sizes, rows, step, kernel)
+    _invoke(device, "haste_hip_linear_backward" + suffix,
+            [*sizes, rows.data_ptr(), step, kernel.data_ptr(), number, _address(cache), dy.data_ptr(), dy_step, _address(dx),
+             _address(dkernel), _address(dbias), scratch.data_ptr(), scratch.numel()])
+    return dx, dkernel, dbias
+
+
+def _gated_arguments(x, forget, admit, z, decay, forget_bias, admit_bias, steps=True):
+    """The arguments checked: the inputs as the entry points take them, the tensors (decay, forget_bias, admit_bias, ...) to keep
+    until the call, the device and the suffix."""
+    dims = 3 if steps else 2
+    if not isinstance(x, torch.Tensor) or x.dim() != dims or not x.numel():
+        raise ValueError("x must be [%s], of no size 0, got %s" % ("T,N,D" if steps else "N,D", _described(x)))
+    if admit is None and admit_bias is not None:
+        raise ValueError("admit_bias needs admit")
+    full, device, width = x.shape, x.get_device(), (x.shape[-1],)
+    if not (_alike(x.dtype, device, forget, admit, z) and _alike(torch.float32, device, decay, forget_bias, admit_bias)
+            and forget is not None and forget.shape == full and (admit is None or admit.shape == full)
+            and (z is None or z.shape == full) and (decay is None or decay.shape == width)
+            and (forget_bias is None or forget_bias.shape == width) and (admit_bias is None or admit_bias.shape == width)):
+        _activation("forget", forget, full, x)  # one of these says what is wrong
+        for what, t in (("admit", admit), ("z", z)):
+            if t is not None:
+                _activation(what, t, full, x)
+        for what, t in (("decay", decay), ("forget_bias", forget_bias), ("admit_bias", admit_bias)):
+            if t is not None:
+                _float(what, t, width, x)
+    suffix, axes, values = _activation_suffix(x), dims - 1, []
+    kept = [_contiguous(decay), _contiguous(forget_bias), _contiguous(admit_bias)]
+    _place(values, kept, x, axes)
+    _place(values, kept, forget, axes)
+    _place(values, kept, admit, axes)
+    _place(values, kept, z, axes)
+    values += map(_address, kept[:3])
+    return values, kept, device, suffix
+
+
+def gated_recurrence_forward(training, x, forget, admit=None, z=None, decay=None, forget_bias=None, admit_bias=None, h0=None,
+                             lengths=None):
+    """x, forget, admit, z[T,N,D], decay, forget_bias, admit_bias[D], h0[N,D] -> y[T,N,D], h_last[N,D], cache (what the backward pass
+    needs; None unless training).  With r = sigmoid(forget + forget_bias), i = sigmoid(admit + admit_bias):
+    decay given (not below 0): a = exp(-decay r), u = sqrt(1 - a^2) i x (i = 1 without admit); otherwise a = r, u = i x, or
+    (1 - r) x without admit; h[t] = a h[t-1] + u, y = h z sigmoid(z).  Parts that are None are left out."""
+    values, kept, device, suffix = _gated_arguments(x, forget, admit, z, decay, forget_bias, admit_bias)
+    T, N, D = x.shape
+    if h0 is not None:
+        h0 = _float("h0", h0, (N, D), x)
+    if lengths is not None:
+        _check_lengths(lengths, x)
+    y, h_last = x.new_empty(x.shape), torch.empty((N, D), device=x.device)
+    cache = _scratch("haste_hip_gated_recurrence_kept_bytes", x, T, N, D) if training else None
+    scratch = _scratch("haste_hip_gated_recurrence_workspace_bytes", x, 0, T, N, D)
+    _invoke(device, "haste_hip_gated_recurrence_forward" + suffix,
+            [T, N, D, *values, _address(h0), _address(lengths), y.data_ptr(), h_last.data_ptr(), _address(cache), scratch.data_ptr(),
+             scratch.numel()])
+    return y, h_last, cache
+
+
+def gated_recurrence_backward(x, forget, admit, z, decay, forget_bias, admit_bias, h0, lengths, cache, dy, dh_last=None):
+    """Gradients (dx, dforget, dadmit, dz, ddecay, dforget_bias, dadmit_bias, dh0) from those of y (None: zeros) and h_last, and the
+    cache of the forward pass of the same arguments; those of arguments that are None are None."""
+    values, kept, device, suffix = _gated_arguments(x, forget, admit, z, decay, forget_bias, admit_bias)
+    T, N, D = x.shape
+    if h0 is not None:
+        _float("h0", h0, (N, D), x)
+    if lengths is not None:
+        _check_lengths(lengths, x)
+    size = _scratch_bytes("haste_hip_gated_recurrence_kept_bytes", x.device, T, N, D)
+    if not torch.is_tensor(cache) or cache.dtype != torch.uint8 or cache.numel() != size or cache.device != x.device \
+            or not cache.is_contiguous():
+        raise ValueError("the cache must be that of a forward pass in training over the same arguments")
+    dy = _zero_rows(T, N, D, x) if dy is None else dy
+    _activation("dy", dy, x.shape, x)
+    if dh_last is not None:
+        dh_last = _float("dh_last", dh_last, (N, D), x)
+    grads = [None if t is None else x.new_empty(x.shape) for t in (x, forget, admit, z)]
+    sums = [None if t is None else torch.empty_like(t) for t in kept[:3]]
+    dh0 = None if h0 is None else torch.empty((N, D), device=x.device)
+    scratch = _scratch("haste_hip_gated_recurrence_workspace_bytes", x, 1, T, N, D)
+    values = [T, N, D, *values, _address(lengths), cache.data_ptr()]
+    _place(values, kept, dy, 2)
+    values += (_address(dh_last), *map(_address, grads), *map(_address, sums), _address(dh0), scratch.data_ptr(), scratch.numel())
+    _invoke(device, "haste_hip_gated_recurrence_backward" + suffix, values)
+    return (*grads, *sums, dh0)
+
+
+def gated_recurrence_iterate(x, forget, h, admit=None, z=None, decay=None, forget_bias=None, admit_bias=None, h_out=None):
+    """One step: x, forget, admit, z[N,D], h[N,D] -> y[N,D], h_out (which may be given, and may be h)."""
+    values, kept, device, suffix = _gated_arguments(x, forget, admit, z, decay, forget_bias, admit_bias, steps=False)
+    N, D = x.shape
+    read = _float("h", h, (N, D), x)
+    y = x.new_empty((N, D))
+    if h_out is None:
+        h_out = torch.empty_like(read)
+    else:
+        _output("h_out", h_out, (N, D), torch.float32, x)
+        _apart("h_out", h_out, h, x, forget, admit, z, decay, forget_bias, admit_bias)
+    _invoke(device, "haste_hip_gated_recurrence_iterate" + suffix, [N, D, *values, read.data_ptr(), y.data_ptr(), h_out.data_ptr()])
+    return y, h_out
+
+
+_GRADIENTS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float64: 3}
+
+
+def _dense(t):
+    """Whether the elements fill their memory from the first to the last, in whatever order."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for step, size in sorted((step, size) for step, size in zip(t.stride(), t.shape) if size != 1):
+        if step != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _gradient_arguments(grads):
+    """The gradients as arrays (addresses, elements, types), the device of all, and the type of their norm."""
+    if isinstance(grads, torch.Tensor) or not grads:
+        raise ValueError("grads must be a list of tensors, at least one, got %s" % _described(grads))
+    addresses, elements, types, device, wide = [], [], [], None, torch.float32
+    for t in grads:
+        kind = _GRADIENTS.get(t.dtype) if isinstance(t, torch.Tensor) else None
+        if kind is None or t.layout is not torch.strided:
+            raise ValueError("gradients must be tensors of float32, float64, float16 or bfloat16, got %s" % _described(t))
+        here = t.get_device()
+        if device is None:
+            device = here
+        if here != device or here < 0:
+            raise ValueError("gradients must be GPU tensors on one device, got %s and %s" % (grads[0].device, t.device))
+        if not _dense(t):
+            raise ValueError("gradients must fill their memory, got strides %s of %s" % (t.stride(), list(t.shape)))
+        if kind == 3:
+            wide = torch.float64
+        addresses.append(t.data_ptr())
+        elements.append(t.numel())
+        types.append(kind)
+    count = len(addresses)
+    return (ctypes.c_void_p * count)(*addresses), (ctypes.c_size_t * count)(*elements), (ctypes.c_int * count)(*types), device, wide
+
+
+def gradient_norm(grads):
+    """The norm of all elements of all tensors together, sqrt(sum g^2), without waiting for it: a tensor of no axes, float32
+    (float64 if a gradient is).  grads: a list of float32, float64, float16 or bfloat16 tensors on one device."""
+    addresses, elements, types, device, wide = _gradient_arguments(grads)
+    norm = torch.empty((), device=grads[0].device, dtype=wide)
+    scratch = _scratch("haste_hip_gradient_norm_workspace_bytes", norm, len(grads))
+    _invoke(device, "haste_hip_gradient_norm", [len(grads), addresses, elements, types, norm.data_ptr(), wide is torch.float64,
+                                                scratch.data_ptr(), scratch.numel()])
+    return norm
+
+
+def clip_gradients(grads, max_norm, norm=None, out=None):
+    """grads, a list as of gradient_norm() -> clipped, norm: each gradient times min(1, max_norm / (norm + 1e-6)).  norm: that of
+    gradient_norm(), or of more than these gradients (of the ranks that share a model); None: that of these.  out: the list of
+    tensors to write, alike in type and strides; its tensors may be the gradients, and may overlap nothing else."""
+    addresses, elements, types, device, wide = _gradient_arguments(grads)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError("max_norm must not be below 0, got %r" % max_norm)
+    if out is None:
+        out = [torch.empty_like(t, memory_format=torch.preserve_format) for t in grads]
+    elif len(out) != len(grads):
+        raise ValueError("out must be a list of %d tensors, got %d" % (len(grads), len(out)))
+    for t, to in zip(grads, out):
+        if to is not t and not (_is(to, t.shape, t.dtype, device) and to.stride() == t.stride()):
+            raise ValueError("out must be like the gradients: %s, strides %s, got %s" % (_described(t), t.stride(), _described(to)))
+    given = norm is not None
+    if not given:
+        norm = torch.empty((), device=grads[0].device, dtype=wide)
+    elif not isinstance(norm, torch.Tensor) or norm.numel() != 1 or norm.get_device() != device \
+            or norm.dtype not in (torch.float32, torch.float64):
+        raise ValueError("norm must be float32 or float64 of one element on %s, got %s" % (grads[0].device, _described(norm)))
+    count = len(grads)
+    scratch = None if given else _scratch("haste_hip_gradient_norm_workspace_bytes", norm, count)
+    _invoke(device, "haste_hip_clip_gradients",
+            [count, addresses, (ctypes.c_void_p * count)(*[t.data_ptr() for t in out]), elements, types, max_norm, given,
+             norm.data_ptr(), norm.dtype is torch.float64, _address(scratch), 0 if given else scratch.numel()])
+    return out, norm

@@ -800,6 +800,114 @@ int haste_hip_residual_norm_backward_bf16(int steps, int batch_size, int channel
     void* dupdate, void* dresidual, void* dgate, float* dscale, float* dafter_weight, float* dbefore_weight,
     float* dbefore_bias, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- The operators of a gated linear recurrent block -----------------------------------------
+ * Projections with what follows them, a gated linear recurrence, and the clipping of gradients; no counterpart in the
+ * reference.  Types, scratch memory and assignment of outputs as for the operators of a state space block.
+ *
+ * Projection: y = act(x W + bias) + residual; x[R,C] (rows `x_row` elements apart, at least C), W[C,D], bias[D],
+ * residual, y[R,D] all of one type; activation 0: none, 1: gelu (v times the normal distribution function), 2: silu
+ * (v sigmoid(v)); bias, residual may be NULL.  cache: what the backward pass needs of an activation, [R,D] in float (_f32)
+ * or half (_f16, _bf16), or NULL; without an activation there is none.  Backward: dx[R,C], dW[C,D], dbias[D] from
+ * dy[R,D], which is the residual's gradient too; each may be NULL (not wanted).  Workspace: aligned to 16 bytes; `aligned`
+ * says that x and W start at, and rows of x are, multiples of 16 bytes. */
+size_t haste_hip_linear_workspace_bytes(int backward, int element_bytes, int rows, int inputs, int outputs,
+                                        int aligned);
+int haste_hip_linear_forward_f32(int rows, int inputs, int outputs, const void* x, size_t x_row,
+    const void* kernel, const void* bias, int activation, const void* residual, size_t residual_row, void* y,
+    void* cache, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_linear_backward_f32(int rows, int inputs, int outputs, const void* x, size_t x_row,
+    const void* kernel, int activation, const void* cache, const void* dy, size_t dy_row, void* dx, void* dkernel,
+    void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_linear_forward_f16(int rows, int inputs, int outputs, const void* x, size_t x_row,
+    const void* kernel, const void* bias, int activation, const void* residual, size_t residual_row, void* y,
+    void* cache, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_linear_backward_f16(int rows, int inputs, int outputs, const void* x, size_t x_row,
+    const void* kernel, int activation, const void* cache, const void* dy, size_t dy_row, void* dx, void* dkernel,
+    void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_linear_forward_bf16(int rows, int inputs, int outputs, const void* x, size_t x_row,
+    const void* kernel, const void* bias, int activation, const void* residual, size_t residual_row, void* y,
+    void* cache, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_linear_backward_bf16(int rows, int inputs, int outputs, const void* x, size_t x_row,
+    const void* kernel, int activation, const void* cache, const void* dy, size_t dy_row, void* dx, void* dkernel,
+    void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gated linear recurrence, one state a channel: r = sigmoid(forget + forget_bias), i = sigmoid(admit + admit_bias),
+ *   with decay (not below 0):  a = exp(-decay r),  u = sqrt(1 - a^2) i x   (admit NULL: i = 1)
+ *   decay NULL:                a = r,              u = i x                 (admit NULL: u = (1 - r) x)
+ *   h[t] = a h[t-1] + u,  y = h silu(z)   (z NULL: y = h)
+ * x,forget,admit,z,y[T,N,D] decay,biases[D] h0,h_last[N,D]; h0, h_last, biases may be NULL.  kept: NULL, or
+ * haste_hip_gated_recurrence_kept_bytes of memory for what the backward pass needs of the states.  Backward: dh_last, the
+ * gradient of h_last, or NULL; dadmit, dz NULL without admit, z; ddecay, dforget_bias, dadmit_bias, dh0 may be
+ * NULL.  Where 1 - a^2 is 0 the square root's slope is taken as 0.  iterate: one step, tensors without the step axis, h_out
+ * may be h. */
+size_t haste_hip_gated_recurrence_workspace_bytes(int backward, int steps, int batch_size, int channels);
+size_t haste_hip_gated_recurrence_kept_bytes(int steps, int batch_size, int channels);
+int haste_hip_gated_recurrence_forward_f32(int steps, int batch_size, int channels,
+    const void* x, size_t x_step, size_t x_row, const void* forget, size_t forget_step, size_t forget_row,
+    const void* admit, size_t admit_step, size_t admit_row, const void* z, size_t z_step, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias,
+    const float* h0, const void* lengths, void* y, float* h_last, float* kept, void* workspace,
+    size_t workspace_bytes, void* stream);
+int haste_hip_gated_recurrence_backward_f32(int steps, int batch_size, int channels,
+    const void* x, size_t x_step, size_t x_row, const void* forget, size_t forget_step, size_t forget_row,
+    const void* admit, size_t admit_step, size_t admit_row, const void* z, size_t z_step, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias,
+    const void* lengths, const float* kept, const void* dy, size_t dy_step, size_t dy_row, const float* dh_last,
+    void* dx, void* dforget, void* dadmit, void* dz, float* ddecay, float* dforget_bias, float* dadmit_bias,
+    float* dh0, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_gated_recurrence_iterate_f32(int batch_size, int channels, const void* x, size_t x_row,
+    const void* forget, size_t forget_row, const void* admit, size_t admit_row, const void* z, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias, const float* h, void* y, float* h_out,
+    void* stream);
+int haste_hip_gated_recurrence_forward_f16(int steps, int batch_size, int channels,
+    const void* x, size_t x_step, size_t x_row, const void* forget, size_t forget_step, size_t forget_row,
+    const void* admit, size_t admit_step, size_t admit_row, const void* z, size_t z_step, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias,
+    const float* h0, const void* lengths, void* y, float* h_last, float* kept, void* workspace,
+    size_t workspace_bytes, void* stream);
+int haste_hip_gated_recurrence_backward_f16(int steps, int batch_size, int channels,
+    const void* x, size_t x_step, size_t x_row, const void* forget, size_t forget_step, size_t forget_row,
+    const void* admit, size_t admit_step, size_t admit_row, const void* z, size_t z_step, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias,
+    const void* lengths, const float* kept, const void* dy, size_t dy_step, size_t dy_row, const float* dh_last,
+    void* dx, void* dforget, void* dadmit, void* dz, float* ddecay, float* dforget_bias, float* dadmit_bias,
+    float* dh0, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_gated_recurrence_iterate_f16(int batch_size, int channels, const void* x, size_t x_row,
+    const void* forget, size_t forget_row, const void* admit, size_t admit_row, const void* z, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias, const float* h, void* y, float* h_out,
+    void* stream);
+int haste_hip_gated_recurrence_forward_bf16(int steps, int batch_size, int channels,
+    const void* x, size_t x_step, size_t x_row, const void* forget, size_t forget_step, size_t forget_row,
+    const void* admit, size_t admit_step, size_t admit_row, const void* z, size_t z_step, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias,
+    const float* h0, const void* lengths, void* y, float* h_last, float* kept, void* workspace,
+    size_t workspace_bytes, void* stream);
+int haste_hip_gated_recurrence_backward_bf16(int steps, int batch_size, int channels,
+    const void* x, size_t x_step, size_t x_row, const void* forget, size_t forget_step, size_t forget_row,
+    const void* admit, size_t admit_step, size_t admit_row, const void* z, size_t z_step, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias,
+    const void* lengths, const float* kept, const void* dy, size_t dy_step, size_t dy_row, const float* dh_last,
+    void* dx, void* dforget, void* dadmit, void* dz, float* ddecay, float* dforget_bias, float* dadmit_bias,
+    float* dh0, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_gated_recurrence_iterate_bf16(int batch_size, int channels, const void* x, size_t x_row,
+    const void* forget, size_t forget_row, const void* admit, size_t admit_row, const void* z, size_t z_row,
+    const float* decay, const float* forget_bias, const float* admit_bias, const float* h, void* y, float* h_out,
+    void* stream);
+
+/* The global norm of `count` gradients, sqrt of the sum of all their squares, and their clipping by it:
+ * clipped = gradient min(1, max_norm / (norm + 1e-6)).  gradients, clipped, elements, types: arrays of `count` on the host, read
+ * during the call: device addresses, elements (each tensor contiguous; 0: left out), and types (0 float, 1 half, 2 bfloat16, 3
+ * double).  norm: a float (norm_in_double: a double) on the device; norm_given: it is read (the gradients are a part
+ * of what was normed), otherwise written.  A clipped tensor may be its gradient, and may overlap nothing else.  Squares are
+ * added in double.  A norm that is no number makes all gradients none; an infinite one makes them 0, infinite ones NaN.
+ * Workspace (not used where the norm is given): aligned to 8 bytes. */
+size_t haste_hip_gradient_norm_workspace_bytes(int count);
+int haste_hip_gradient_norm(int count, const void* const* gradients, const size_t* elements, const int* types,
+    void* norm, int norm_in_double, void* workspace, size_t workspace_bytes, void* stream);
+int haste_hip_clip_gradients(int count, const void* const* gradients, void* const* clipped,
+    const size_t* elements, const int* types, double max_norm, int norm_given, void* norm, int norm_in_double,
+    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
