@@ -25,7 +25,7 @@
 namespace haste_hip {
 namespace {
 
-typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef unsigned int uint4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
@@ -118,15 +118,16 @@ __device__ __forceinline__ void load_bias(const Finish<T>& to, int col, int colu
 }
 
 // ---- the tile kernel ---------------------------------------------------------------------
-__device__ __forceinline__ float16_t mfma(_Float16, uint4_t a, uint4_t b, float16_t c) {
+__device__ __forceinline__ float4_t mfma(_Float16, uint4_t a, uint4_t b, float4_t c) {
   typedef _Float16 v __attribute__((ext_vector_type(8)));
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ float16_t mfma(__bf16, uint4_t a, uint4_t b, float16_t c) {
+__device__ __forceinline__ float4_t mfma(__bf16, uint4_t a, uint4_t b, float4_t c) {
   typedef __bf16 v __attribute__((ext_vector_type(8)));
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
 }
 
+constexpr int BK = 64;                          // of the contraction in a stage: 128 bytes, whole cache lines
 constexpr unsigned int kNowhere = 0x7ffffff0u;  // an offset beyond any resource: the load gives zeros
 
 __device__ __forceinline__ uint4_t resource(const void* base, long long bytes) {
@@ -149,26 +150,35 @@ __device__ __forceinline__ void tile_ready() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
+// Waits for this wavefront's reads of LDS, then for the others'.
+__device__ __forceinline__ void all_have_read() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// What is written before stays before.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // One operand's part of a stage: WIDTH rows (columns) of the product, BK of the contraction, loaded by WAVES wavefronts.
-template <bool SLOW, int WIDTH, int BK, int WAVES>
+template <bool SLOW, int WIDTH, int WAVES>
 struct Panel {
   static constexpr int kBytes = WIDTH * BK * 2;
   static constexpr int kLoads = kBytes / 1024 / WAVES;  // of a wavefront
-  static_assert(kLoads * 1024 * WAVES == kBytes, "a stage is loaded in whole kilobytes");
-  static_assert(BK == 32, "rows of 64 bytes: 16 of a load, which is what turn() repeats after");
-  static constexpr int kChunks = BK / 8;                // 16-byte chunks of a contiguous row
-  static __device__ __forceinline__ int turn(int row) { return (row >> 2) & 3; }
+  static_assert(kLoads * 1024 * WAVES == kBytes && WAVES % 2 == 0, "a stage is loaded in whole kilobytes");
+  static __device__ __forceinline__ int turn(int row) { return (row >> 1) & 7; }
+  static __device__ __forceinline__ int turn_slow(int k) { return 2 * (k & 3) + ((k >> 3) & 1); }
 
-  uint4_t from;
   const char* base;
   long long ld_bytes;
   unsigned offset[kLoads];
   int columns;     // SLOW: those from the tile's first on, in whole chunks (a load that ends beyond a resource loses its last elements)
   unsigned chunk;  // contiguous: the lane's first k of a stage
+  uint4_t from;    // what the stage in hand is loaded from
+  unsigned shift;
+  bool gone;
 
   // first: of the tile's rows (columns), of `count` in all.
   __device__ __forceinline__ void start(const void* p, long long ld, int first, int count, int k_end, int wave, int lane) {
     ld_bytes = ld * 2;
+    shift = 0;
+    gone = false;
     const int left = count - first;
     if constexpr (SLOW) {
       base = static_cast<const char*>(p) + (size_t)first * 2;
@@ -177,67 +187,66 @@ struct Panel {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int k = (i * WAVES + wave) * ROWS + lane / LANES, unit = lane % LANES;
-        const int column = ((unit >> 1) ^ (2 * (k & 3))) * 16 + (unit & 1) * 8;
+        const int column = ((unit >> 1) ^ turn_slow(k)) * 16 + (unit & 1) * 8;
         offset[i] = column < left ? (unsigned)(k * ld_bytes + column * 2) : kNowhere;
       }
     } else {
       base = static_cast<const char*>(p) + (size_t)first * ld_bytes;
       const int rows = left < WIDTH ? left : WIDTH;
       from = resource(base, (rows - 1) * ld_bytes + (long long)((k_end + 7) & ~7) * 2);
-      constexpr int ROWS = 64 / kChunks;
-      const int in_row = lane / kChunks;
-      chunk = ((lane % kChunks) ^ turn(in_row)) * 8;
+      const int in_load = lane / 8;  // a load's eight rows start at a multiple of 8 that has the wavefront's parity
+      chunk = ((lane % 8) ^ turn(in_load + 8 * (wave & 1))) * 8;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int row = (i * WAVES + wave) * ROWS + in_row;
+        const int row = (i * WAVES + wave) * 8 + in_load;
         offset[i] = row < rows ? (unsigned)(row * ld_bytes + chunk * 2) : kNowhere;
       }
     }
   }
-  __device__ __forceinline__ void request(unsigned lds, int k0, int k_end, int wave) {
+  // The stage that starts at k0, and load i of it into LDS at `lds`.
+  __device__ __forceinline__ void stage(int k0, int k_end) {
     if constexpr (SLOW) {
-      const uint4_t at = resource(base + k0 * ld_bytes, (long long)(k_end - k0 - 1) * ld_bytes + (long long)columns * 2);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) load_to_lds(lds + (i * WAVES + wave) * 1024, offset[i], at, 0);
+      from = resource(base + k0 * ld_bytes, (long long)(k_end - k0 - 1) * ld_bytes + (long long)columns * 2);
     } else {
-      const bool gone = k0 + (int)chunk >= k_end;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        load_to_lds(lds + (i * WAVES + wave) * 1024, gone ? kNowhere : offset[i], from, (unsigned)k0 * 2);
+      shift = (unsigned)k0 * 2;
+      gone = k0 + (int)chunk >= k_end;
     }
   }
-  // Eight k of step ks of row (column) `first` + lane % 32: k = 16 ks + 8 (lane / 32) on.
-  static __device__ __forceinline__ uint4_t operand(const char* stage, int first, int ks, int lane) {
+  __device__ __forceinline__ void load(int i, unsigned lds, int wave) const {
+    load_to_lds(lds + (i * WAVES + wave) * 1024, !SLOW && gone ? kNowhere : offset[i], from, shift);
+  }
+  // Eight k of row (column) `first` + lane % 16: those from 32 half + 8 (lane / 16) on.
+  static __device__ __forceinline__ uint4_t operand(const char* stage, int first, int half, int lane) {
     if constexpr (SLOW) {
       uint4_t v;
       const int q = lane >> 4, i = lane & 15;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = 16 * ks + 8 * (q >> 1) + 4 * h + (i >> 2);
-        const int piece = ((first >> 4) + (q & 1)) ^ (2 * (k & 3));
+        const int k = 32 * half + 8 * q + 4 * h + (i >> 2);
+        const int piece = (first >> 4) ^ turn_slow(k);
         typedef __attribute__((address_space(3))) short4_t* lds_t;
         const short4_t part = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(stage + k * (WIDTH * 2) + piece * 32 + (i & 3) * 8));
         __builtin_memcpy(reinterpret_cast<char*>(&v) + 8 * h, &part, 8);
       }
       return v;
     } else {
-      const int row = first + (lane & 31), c = 2 * ks + (lane >> 5);
+      const int row = first + (lane & 15), c = 4 * half + (lane >> 4);
       return *reinterpret_cast<const uint4_t*>(stage + row * (BK * 2) + (c ^ turn(row)) * 16);
     }
   }
 };
 
-template <bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_, int BK_, int STAGES_>
+template <bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_>
 struct Tile {
   static constexpr bool A_SLOW = A_SLOW_, B_SLOW = B_SLOW_;
-  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, WAVES = WAVES_M * WAVES_N, BK = BK_, STAGES = STAGES_;
-  static constexpr int MI = BM / WAVES_M / 32, NJ = BN / WAVES_N / 32;
-  typedef Panel<A_SLOW, BM, BK, WAVES> PA;
-  typedef Panel<B_SLOW, BN, BK, WAVES> PB;
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, WAVES = WAVES_M * WAVES_N;
+  static constexpr int MI = BM / WAVES_M / 16, NJ = BN / WAVES_N / 16;  // of 16 x 16 elements
+  typedef Panel<A_SLOW, BM, WAVES> PA;
+  typedef Panel<B_SLOW, BN, WAVES> PB;
   static constexpr int kStage = PA::kBytes + PB::kBytes;
-  static constexpr int kSlabLd = NJ * 32 + 4;           // floats of a row of a wavefront's results in LDS
+  static constexpr int kSlabLd = NJ * 16 + 4;           // floats of a row of a wavefront's results in LDS
   static constexpr int kSlabs = WAVES * 32 * kSlabLd * 4;
-  static constexpr int kLds = kStage * STAGES > kSlabs ? kStage * STAGES : kSlabs;
+  static constexpr int kLds = 2 * kStage > kSlabs ? 2 * kStage : kSlabs;
 };
 
 struct Product {
@@ -266,7 +275,7 @@ void linear_tile_kernel(Product p, Finish<T> to) {
   const int m0 = (band * kTallest + in_band % tall) * G::BM, n0 = in_band / tall * G::BN;
   const int k_begin = piece * p.k_per_piece;
   const int k_end = k_begin + p.k_per_piece < p.K ? k_begin + p.k_per_piece : p.K;
-  const int wm = wave / G::WAVES_N * (G::MI * 32), wn = wave % G::WAVES_N * (G::NJ * 32);
+  const int wm = wave / G::WAVES_N * (G::MI * 16), wn = wave % G::WAVES_N * (G::NJ * 16);
 
   typename G::PA pa;
   typename G::PB pb;
@@ -274,55 +283,116 @@ void linear_tile_kernel(Product p, Finish<T> to) {
   pb.start(p.B, p.ldb, n0, p.N, k_end, wave, lane);
   const unsigned lds_at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
 
-  float16_t acc[G::MI][G::NJ];
+  float4_t acc[G::MI][G::NJ];
 #pragma unroll
   for (int i = 0; i < G::MI; ++i)
 #pragma unroll
     for (int j = 0; j < G::NJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
 
-  const int steps = (k_end - k_begin + G::BK - 1) / G::BK;
-  auto request = [&](int step) {
-    const unsigned at = lds_at + step % G::STAGES * G::kStage;
-    pa.request(at, k_begin + step * G::BK, k_end, wave);
-    pb.request(at + G::PA::kBytes, k_begin + step * G::BK, k_end, wave);
+  const int steps = (k_end - k_begin + BK - 1) / BK;
+  // A stage is multiplied in four quarters: each half of its k with each half of the wavefront's rows.
+  constexpr int kLoads = G::PA::kLoads + G::PB::kLoads, RI = G::MI / 2, kProducts = RI * G::NJ;
+  uint4_t a[2][RI], b[2][G::NJ];  // the operands of a quarter and of the next, of a half and of the next
+  auto stage = [&](int step) {
+    pa.stage(k_begin + step * BK, k_end);
+    pb.stage(k_begin + step * BK, k_end);
   };
-  constexpr int kAhead = G::STAGES - 1, kLoads = G::PA::kLoads + G::PB::kLoads;
-  for (int s = 0; s < kAhead && s < steps; ++s) request(s);
-  for (int s = 0; s < steps; ++s) {
-    if (s + kAhead <= steps) tile_ready<(kAhead - 1) * kLoads>();
-    else tile_ready<0>();
-    if (s + kAhead < steps) request(s + kAhead);  // over the stage of step s - 1, which all have read
-    const char* stage = lds + s % G::STAGES * G::kStage;
+  // A wavefront's loads of a stage, in the order in which what they replace has been read: those of A that quarters 0 and 1 (SLOW), or
+  // 0 and 2, read, those of B, the rest of A.
+  constexpr int kEarly = G::PA::kLoads / 2 + G::PB::kLoads;
+  auto load = [&](int i, int step) {
+    const unsigned at = lds_at + (step & 1) * G::kStage;
+    const int late = i >= kEarly, of_a = late ? i - kEarly : i;
+    if (!late && i >= G::PA::kLoads / 2) pb.load(i - G::PA::kLoads / 2, at + G::PA::kBytes, wave);
+    else pa.load(G::A_SLOW ? of_a + late * (G::PA::kLoads / 2) : 2 * of_a + late, at, wave);
+  };
+  auto read_a = [&](int i, int step, int quarter) {
+    const char* from = lds + (step & 1) * G::kStage;
+    a[quarter & 1][i] = G::PA::operand(from, wm + 16 * ((quarter & 1) * RI + i), quarter >> 1, lane);
+  };
+  auto read_b = [&](int j, int step, int half) {
+    b[half][j] = G::PB::operand(lds + (step & 1) * G::kStage + G::PA::kBytes, wn + 16 * j, half, lane);
+  };
+  // The products of a quarter; beside each of them goes what `beside` has for its place, in that order: reads of LDS in a row
+  // would fill its queue, and the products wait for their turn behind them.
+  auto multiply = [&](int quarter, auto beside) {
 #pragma unroll
-    for (int ks = 0; ks < G::BK / 16; ++ks) {
-      uint4_t a[G::MI], b[G::NJ];
+    for (int i = 0; i < RI; ++i)
 #pragma unroll
-      for (int i = 0; i < G::MI; ++i) a[i] = G::PA::operand(stage, wm + 32 * i, ks, lane);
+      for (int j = 0; j < G::NJ; ++j) {
+        float4_t& to = acc[(quarter & 1) * RI + i][j];
+        to = mfma(T(), a[quarter & 1][i], b[quarter >> 1][j], to);
+        in_order();
+        beside(i * G::NJ + j);
+        in_order();
+      }
+  };
+  // things [0, count) spread over the places of a quarter
+  auto spread = [&](int place, int count, auto thing) {
 #pragma unroll
-      for (int j = 0; j < G::NJ; ++j) b[j] = G::PB::operand(stage + G::PA::kBytes, wn + 32 * j, ks, lane);
-#pragma unroll
-      for (int i = 0; i < G::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < G::NJ; ++j) acc[i][j] = mfma(T(), a[i], b[j], acc[i][j]);
+    for (int r = place * count / kProducts; r < (place + 1) * count / kProducts; ++r) thing(r);
+  };
+  // A step: its operands are read a quarter ahead.  Behind the barrier in its middle all have read B and half of A, behind the one
+  // before the last quarter the rest: into their places the step after the next is loaded (LOAD), which has a step and a quarter to arrive.
+  // Behind the second the next step's has (NEXT).  No branch within: where two ways meet, the compiler waits for the reads of both.
+  auto step = [&](auto load_c, auto next_c, int s) {
+    constexpr bool LOAD = decltype(load_c)::value, NEXT = decltype(next_c)::value;
+    multiply(0, [&](int place) {
+      spread(place, RI + G::NJ / 2, [&](int r) { r < RI ? read_a(r, s, 1) : read_b(r - RI, s, 1); });
+    });
+    multiply(1, [&](int place) {
+      spread(place, RI + G::NJ / 2, [&](int r) { r < RI ? read_a(r, s, 2) : read_b(r - RI + G::NJ / 2, s, 1); });
+    });
+    if constexpr (LOAD) {
+      all_have_read();
+      stage(s + 2);
+      in_order();
     }
+    multiply(2, [&](int place) {
+      spread(place, RI, [&](int r) { read_a(r, s, 3); });
+      if constexpr (LOAD) spread(place, kEarly, [&](int r) { load(r, s + 2); });
+    });
+    if constexpr (NEXT) tile_ready<LOAD ? kEarly : 0>();
+    in_order();
+    multiply(3, [&](int place) {
+      if constexpr (NEXT) spread(place, RI + G::NJ, [&](int r) { r < G::NJ ? read_b(r, s + 1, 0) : read_a(r - G::NJ, s + 1, 0); });
+      if constexpr (LOAD) spread(place, kLoads - kEarly, [&](int r) { load(kEarly + r, s + 2); });
+    });
+  };
+  for (int s = 0; s < 2 && s < steps; ++s) {
+    stage(s);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load(i, s);
   }
+  if (steps > 1) tile_ready<kLoads>();
+  else tile_ready<0>();
+#pragma unroll
+  for (int i = 0; i < RI; ++i) read_a(i, 0, 0);
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) read_b(j, 0, 0);
+  int s = 0;
+  for (; s + 2 < steps; ++s) step(std::true_type(), std::true_type(), s);
+  if (s + 1 < steps) step(std::false_type(), std::true_type(), s++);
+  step(std::false_type(), std::false_type(), s);
   tile_ready<0>();
 
   // 32 rows of a wavefront's results at a time go through LDS, so that a lane has eight neighbouring elements of a row.
   float* slab = reinterpret_cast<float*>(lds) + wave * 32 * G::kSlabLd;
-  constexpr int LANES = G::NJ * 4, ROWS = 64 / LANES;  // lanes of a row, rows at a time
+  constexpr int LANES = G::NJ * 2, ROWS = 64 / LANES;  // lanes of a row, rows at a time
   const int col = n0 + wn + lane % LANES * 8;
   float bias[8];
   if (p.partial == nullptr) load_bias(to, col, p.N, bias);
 #pragma unroll
-  for (int i = 0; i < G::MI; ++i) {
+  for (int i = 0; i < G::MI / 2; ++i) {
 #pragma unroll
-    for (int j = 0; j < G::NJ; ++j)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        slab[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * G::kSlabLd + 32 * j + (lane & 31)] = acc[i][j][e];
+      for (int j = 0; j < G::NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          slab[(16 * h + 4 * (lane >> 4) + e) * G::kSlabLd + 16 * j + (lane & 15)] = acc[2 * i + h][j][e];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll 2
@@ -355,11 +425,16 @@ void linear_finish_kernel(int M, int N, int pieces, const float* __restrict__ pa
       load_channels<8>(to.out + row * to.ld, col, N, v);
     } else {
       load_channels<8>(partial + row * N, col, N, v);
-      for (int z = 1; z < pieces; ++z) {
-        float w[8];
-        load_channels<8>(partial + ((size_t)z * M + row) * N, col, N, w);
+      constexpr int AT_ONCE = 4;
+      for (int z = 1; z < pieces; z += AT_ONCE) {
+        float w[AT_ONCE][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += w[e];
+        for (int k = 0; k < AT_ONCE; ++k)  // beyond the last piece it once more, not added
+          load_channels<8>(partial + ((size_t)(z + k < pieces ? z + k : pieces - 1) * M + row) * N, col, N, w[k]);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += z + k < pieces ? w[k][e] : 0.f;
       }
     }
     finish(to, v, bias, row, col, N);
@@ -432,21 +507,26 @@ struct Plan {
   size_t floats;
 };
 
+// The cheapest of both tiles and of 1 to 32 pieces by what they were measured to cost, in ns: k of a tile of 256 x 256 21, of 128 x 128 9, or
+// 13.9 for two on a CU; 5000 and 3500 for a round of workgroups, 2500 for adding the pieces up, whose elements are written and read at
+// 4 TB/s.  us, estimate / measured: 128 x 4096 x 4096 (M, N, K) in 4 / 8 pieces of small tiles 19.4 / 18.3, 19.0 / 18.8, in 8 of large ones
+// 26 / 24; 1024 x 2048 x 8192 in 4 of small 51 / 48, in 8 of large 63 / 51; 512 x 512 x 16384 in 16 of small 24 / 26; 8192 x 1024 x 2048
+// whole, small / large tiles 32, 48 / 34, 48.
 Plan plan_product(int M, int N, int K) {
   Plan best = {};
   double least = 1e300;
   for (int large = 0; large < 2; ++large) {
     const int side = large ? 256 : 128;
-    const long long tm = (M + side - 1) / side, tn = (N + side - 1) / side, tiles = tm * tn;
-    const int slots = large ? cus() : 2 * cus();
+    const long long tm = ((long long)M + side - 1) / side, tn = ((long long)N + side - 1) / side, tiles = tm * tn;
+    const long long slots = large ? cus() : 2 * cus();
     for (int s = 1; s <= 32; ++s) {
       int per = (K + s - 1) / s;
-      per = (per + 63) / 64 * 64;
-      const int pieces = (K + per - 1) / per;
-      if (pieces != s || (s > 1 && (per < 128 || tiles * s > 4ll * slots))) continue;
-      const double rounds = (double)((tiles * s + slots - 1) / slots);
-      double cost = rounds * (per + 256) * (large ? 4.0 : 2.4);
-      if (s > 1) cost += 2000 + (double)s * M * N * 8 / 2.2e6;
+      per = (per + BK - 1) / BK * BK;
+      if ((K + per - 1) / per != s || (s > 1 && (per < 2 * BK || tiles * s > 2 * slots))) continue;
+      const long long rounds = tiles * s / slots, rest = tiles * s % slots;
+      double cost = (double)rounds * (large ? 21.0 * per + 5000 : 13.9 * per + 3500);
+      if (rest > 0) cost += large ? 21.0 * per + 5000 : (rest <= cus() ? 9.0 : 13.9) * per + 3500;
+      if (s > 1) cost += 2500 + (double)s * M * N * 8 / 4000;
       if (cost < least) {
         least = cost;
         best = {large != 0, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0};
@@ -476,8 +556,8 @@ int product(hipStream_t stream, int M, int N, int K, const void* A, long long ld
   Product p = {M, N, K, A, B, lda, ldb, plan.tiles_m, plan.tiles_n, plan.k_per_piece, plan.pieces > 1 ? scratch : nullptr};
   {
     ScopedKernelTimer timer("linear_product", stream);
-    if (plan.large) HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 256, 256, 2, 4, 32, 4>>(stream, p, plan.pieces, to)));
-    else HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 128, 128, 2, 2, 32, 4>>(stream, p, plan.pieces, to)));
+    if (plan.large) HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 256, 256, 2, 4>>(stream, p, plan.pieces, to)));
+    else HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 128, 128, 2, 2>>(stream, p, plan.pieces, to)));
   }
   if (plan.pieces > 1) {
     ScopedKernelTimer timer("linear_finish", stream);
