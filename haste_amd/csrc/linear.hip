@@ -257,6 +257,12 @@ struct Product {
   float* partial;                     // [piece][M][N], null: whole
 };
 
+// Workgroups go to the XCDs in turn; each XCD is given a range of the work.
+__device__ __forceinline__ unsigned work_of_xcd() {
+  const unsigned each = gridDim.x >> 3, rest = gridDim.x & 7, xcd = blockIdx.x & 7;
+  return xcd * each + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+}
+
 constexpr int kTallest = 8;  // rows of tiles that are gone through side by side
 
 template <typename T, class G>
@@ -264,10 +270,7 @@ __global__ __launch_bounds__(64 * G::WAVES, 2)
 void linear_tile_kernel(Product p, Finish<T> to) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroups go to the XCDs in turn; each XCD is given a range of the work, in blocks of tiles that share rows of A and
-  // columns of B.
-  const unsigned each = gridDim.x >> 3, rest = gridDim.x & 7, xcd = blockIdx.x & 7;
-  const unsigned work = xcd * each + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+  const unsigned work = work_of_xcd();  // in blocks of tiles that share rows of A and columns of B
   const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
   const int piece = work / tiles, tile = work % tiles;
   const int band = tile / (kTallest * p.tiles_n), in_band = tile % (kTallest * p.tiles_n);
@@ -411,6 +414,129 @@ void linear_tile_kernel(Product p, Finish<T> to) {
   }
 }
 
+// ---- few rows ----------------------------------------------------------------------------
+// Up to 16 MT rows, the whole product in one launch.  Bound: how fast a CU takes in pieces of rows of W and x, some 2 ns each whether they
+// have 32 or 64 bytes; the fewer columns a workgroup has, the more CUs take part.  Each of its wavefronts takes the 32 k of every eighth unit,
+// two units on their way while two are multiplied: W goes through registers (rows may start anywhere, what is beyond them is 0) into the
+// wavefront's own part of LDS and comes back transposed, x comes as the instruction wants it.  The wavefronts' sums meet in LDS.
+// C x D = 1024 x 4096 and 4096 x 4096, 1 / 16 / 32 rows: 4.5 / 5.1 / 6.0 and 10.4 / 12.6 / 15.9 us (the tile kernel and the sums of its
+// pieces 8.6 / 10.1 / 10.4 and 13.9 / 14.0 / 14.0); with four units 4.8 / 5.1 / 5.8 and 11.4 / 13.1 / 16.6.
+constexpr int kRowWaves = 8, kUnits = 2;
+template <typename T, int MT, int COLUMNS>
+__global__ __launch_bounds__(64 * kRowWaves, 2)
+void linear_rows_kernel(int R, int D, int K, const T* __restrict__ x, size_t x_ld, const T* __restrict__ W, Finish<T> to) {
+  typedef typename Packed<T, 8>::type vec_t;
+  constexpr int kUnitBytes = 32 * COLUMNS * 2, kPitch = COLUMNS + 4, NJ = COLUMNS / 16;
+  constexpr int LANES = COLUMNS / 8, ROWS = 64 / LANES, kLoads = 32 / ROWS;  // lanes of a row of W, rows of a load, loads of a unit
+  constexpr int kTurned = kRowWaves * kUnits * kUnitBytes, kSums = kRowWaves * MT * 16 * kPitch * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kTurned > kSums ? kTurned : kSums];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = work_of_xcd() * COLUMNS;  // (a cache line has the columns of several workgroups)
+  char* own = lds + wave * kUnits * kUnitBytes;
+  const int units = (K + 31) / 32;
+  const int col = n0 + lane % LANES * 8;
+  // Where 32 bytes of row k of a unit lie: what half a wavefront reads at once, rows 0 .. 3 and 8 .. 11, on different banks.
+  auto place = [](int k, int piece) {
+    const int turn = k >> 3 & 1;
+    return COLUMNS == 16 ? (k ^ 4 * turn) * 32 : k * 64 + (piece ^ turn) * 32;
+  };
+
+  vec_t w[2][kUnits][kLoads], a[2][kUnits][MT];
+  const T* rows[MT];  // those beyond the last are not wanted: it once more
+#pragma unroll
+  for (int m = 0; m < MT; ++m) rows[m] = x + (size_t)(16 * m + (lane & 15) < R ? 16 * m + (lane & 15) : R - 1) * x_ld;
+  auto fetch = [&](auto set, int first) {  // the units first + wave, first + wave + kRowWaves ..
+    if ((first + kUnits * kRowWaves) * 32 <= K && n0 + COLUMNS <= D) {  // nothing to leave out
+#pragma unroll
+      for (int g = 0; g < kUnits; ++g) {
+        const int k0 = (first + g * kRowWaves + wave) * 32;
+#pragma unroll
+        for (int h = 0; h < kLoads; ++h)
+          w[set][g][h] = *reinterpret_cast<const typename Wide<T, 8>::type*>(W + (size_t)(k0 + ROWS * h + lane / LANES) * D + col);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) a[set][g][m] = *reinterpret_cast<const typename Wide<T, 8>::type*>(rows[m] + k0 + lane / 16 * 8);
+      }
+      return;
+    }
+#pragma unroll
+    for (int g = 0; g < kUnits; ++g) {
+      const int k0 = (first + g * kRowWaves + wave) * 32;
+#pragma unroll
+      for (int h = 0; h < kLoads; ++h) {
+        const int k = k0 + ROWS * h + lane / LANES;
+        w[set][g][h] = vec_t{};
+        if (k < K) w[set][g][h] = load_packed<8>(W + (size_t)k * D, col, D);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) a[set][g][m] = load_packed<8>(rows[m], k0 + lane / 16 * 8, K);
+    }
+  };
+  float4_t acc[MT][NJ];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[m][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](auto set) {
+#pragma unroll
+    for (int g = 0; g < kUnits; ++g)
+#pragma unroll
+      for (int h = 0; h < kLoads; ++h)
+        *reinterpret_cast<vec_t*>(own + g * kUnitBytes + place(ROWS * h + lane / LANES, lane % LANES >> 1) + (lane & 1) * 16) = w[set][g][h];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int g = 0; g < kUnits; ++g)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        uint4_t b;
+        const int q = lane >> 4, i = lane & 15;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          typedef __attribute__((address_space(3))) short4_t* lds_t;
+          const short4_t part =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(own + g * kUnitBytes + place(8 * q + 4 * h + (i >> 2), j) + (i & 3) * 8));
+          __builtin_memcpy(reinterpret_cast<char*>(&b) + 8 * h, &part, 8);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m][j] = mfma(T(), __builtin_bit_cast(uint4_t, a[set][g][m]), b, acc[m][j]);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  constexpr std::integral_constant<int, 0> even;
+  constexpr std::integral_constant<int, 1> odd;
+  constexpr int kGroup = kUnits * kRowWaves;
+  fetch(even, 0);
+  for (int u = 0; u < units; u += 2 * kGroup) {
+    if (u + kGroup < units) fetch(odd, u + kGroup);
+    multiply(even);
+    if (u + kGroup < units) {
+      if (u + 2 * kGroup < units) fetch(even, u + 2 * kGroup);
+      multiply(odd);
+    }
+  }
+  __syncthreads();
+  float(*sums)[MT * 16][kPitch] = reinterpret_cast<float(*)[MT * 16][kPitch]>(lds);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[wave][16 * m + 4 * (lane >> 4) + e][16 * j + (lane & 15)] = acc[m][j][e];
+  __syncthreads();
+  const int row = threadIdx.x / LANES, c = threadIdx.x % LANES * 8;
+  if (row >= MT * 16 || row >= R) return;
+  float v[8], bias[8];
+  load_bias(to, n0 + c, D, bias);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = sums[0][row][c + e];
+#pragma unroll
+  for (int z = 1; z < kRowWaves; ++z)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += sums[z][row][c + e];
+  finish(to, v, bias, row, n0 + c, D);
+}
+
 // The pieces of a product, added in order, and what follows.  PIECES null: the elements lie in `to.out` already (float).
 template <typename T>
 __global__ __launch_bounds__(256)
@@ -522,7 +648,8 @@ Plan plan_product(int M, int N, int K) {
     for (int s = 1; s <= 32; ++s) {
       int per = (K + s - 1) / s;
       per = (per + BK - 1) / BK * BK;
-      if ((K + per - 1) / per != s || (s > 1 && (per < 2 * BK || tiles * s > 2 * slots))) continue;
+      if (s > 1 && (per < 2 * BK || tiles * s > 2 * slots)) break;
+      if ((K + per - 1) / per != s) continue;
       const long long rounds = tiles * s / slots, rest = tiles * s % slots;
       double cost = (double)rounds * (large ? 21.0 * per + 5000 : 13.9 * per + 3500);
       if (rest > 0) cost += large ? 21.0 * per + 5000 : (rest <= cus() ? 9.0 : 13.9) * per + 3500;
@@ -534,6 +661,25 @@ Plan plan_product(int M, int N, int K) {
     }
   }
   return best;
+}
+
+// Whether linear_rows_kernel has the forward product: with more than 16 rows of a long contraction tiles are faster.
+bool few_rows(int element, int R, int K) { return element == 2 && R <= (K <= 2048 ? 32 : 16); }
+
+template <typename T>
+int product_of_few_rows(hipStream_t stream, int R, int D, int K, const T* x, size_t x_ld, const T* W, const Finish<T>& to) {
+  ScopedKernelTimer timer("linear_rows", stream);
+  const bool narrow = D <= 32 * cus();
+  const dim3 grid((unsigned)((D + (narrow ? 15 : 31)) / (narrow ? 16 : 32)));
+#define HASTE_LAUNCH_ROWS(MT_, COLUMNS_) \
+  linear_rows_kernel<T, MT_, COLUMNS_><<<grid, 64 * kRowWaves, 0, stream>>>(R, D, K, x, x_ld, W, to)
+  if (R <= 16 && narrow) HASTE_LAUNCH_ROWS(1, 16);
+  else if (R <= 16) HASTE_LAUNCH_ROWS(1, 32);
+  else if (narrow) HASTE_LAUNCH_ROWS(2, 16);
+  else HASTE_LAUNCH_ROWS(2, 32);
+#undef HASTE_LAUNCH_ROWS
+  HASTE_HIP_TRY(hipGetLastError());
+  return HASTE_HIP_OK;
 }
 
 template <typename T, class G>
@@ -548,11 +694,10 @@ int blocks_for(size_t threads) {
   return (int)(b < most ? b : most);
 }
 
-// to = A B, as the operands are stored; `scratch`: what plan_product() says.
+// to = A B, as the operands are stored and plan_product() says, with as much scratch.
 template <typename T, bool A_SLOW, bool B_SLOW>
-int product(hipStream_t stream, int M, int N, int K, const void* A, long long lda, const void* B, long long ldb, const Finish<T>& to,
-            float* scratch) {
-  const Plan plan = plan_product(M, N, K);
+int product(hipStream_t stream, const Plan& plan, int M, int N, int K, const void* A, long long lda, const void* B, long long ldb,
+            const Finish<T>& to, float* scratch) {
   Product p = {M, N, K, A, B, lda, ldb, plan.tiles_m, plan.tiles_n, plan.k_per_piece, plan.pieces > 1 ? scratch : nullptr};
   {
     ScopedKernelTimer timer("linear_product", stream);
@@ -590,6 +735,7 @@ SumPlan plan_sums(int rows, int columns) {
 // Where what a call keeps in its workspace lies; sizes in bytes.
 struct Layout {
   size_t x, kernel, d, sums, product, total;
+  Plan plan, plan_kernel;  // of the product forward, or of dx and dkernel; half types
 };
 
 size_t float_product_bytes(int M, int N, int K) {
@@ -602,6 +748,7 @@ size_t float_product_bytes(int M, int N, int K) {
 
 Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) {
   Layout l = {};
+  if (!backward && few_rows(element, R, C)) return l;
   const bool pack_x = element == 2 && (!aligned || C % 8 != 0), pack_kernel = element == 2 && (!aligned || D % 8 != 0);
   size_t at = 0;
   auto place = [&](size_t bytes) {
@@ -620,9 +767,9 @@ Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) 
   l.product = at;
   size_t need;
   if (element == 2) {
-    const size_t a = backward ? plan_product(R, C, D).floats : plan_product(R, D, C).floats;
-    const size_t b = backward ? plan_product(C, D, R).floats : 0;
-    need = (a > b ? a : b) * sizeof(float);
+    l.plan = backward ? plan_product(R, C, D) : plan_product(R, D, C);
+    if (backward) l.plan_kernel = plan_product(C, D, R);
+    need = (l.plan.floats > l.plan_kernel.floats ? l.plan.floats : l.plan_kernel.floats) * sizeof(float);
   } else {
     const size_t a = backward ? float_product_bytes(R, C, D) : float_product_bytes(R, D, C);
     const size_t b = backward ? float_product_bytes(C, D, R) : 0;
@@ -691,10 +838,11 @@ int forward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kernel
     HASTE_HIP_TRY(hipGetLastError());
     return HASTE_HIP_OK;
   } else {
+    if (few_rows(sizeof(T), R, C)) return product_of_few_rows(stream, R, D, C, x, x_row, kernel, to);
     size_t kernel_row = D;
     HASTE_HIP_PROPAGATE(placed(stream, R, C, x, x_row, reinterpret_cast<T*>(ws + l.x), aligned));
     HASTE_HIP_PROPAGATE(placed(stream, C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel), aligned));
-    return product<T, false, true>(stream, R, D, C, x, x_row, kernel, kernel_row, to, reinterpret_cast<float*>(ws + l.product));
+    return product<T, false, true>(stream, l.plan, R, D, C, x, x_row, kernel, kernel_row, to, reinterpret_cast<float*>(ws + l.product));
   }
 }
 
@@ -757,12 +905,12 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
       size_t kernel_row = D;
       HASTE_HIP_PROPAGATE(placed(stream, C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel), aligned));
       const Finish<T> to = {dx, (size_t)C, kNone, nullptr, nullptr, 0, nullptr};
-      HASTE_HIP_PROPAGATE((product<T, false, false>(stream, R, C, D, d, d_row, kernel, kernel_row, to, scratch)));
+      HASTE_HIP_PROPAGATE((product<T, false, false>(stream, l.plan, R, C, D, d, d_row, kernel, kernel_row, to, scratch)));
     }
     if (dkernel != nullptr) {
       HASTE_HIP_PROPAGATE(placed(stream, R, C, x, x_row, reinterpret_cast<T*>(ws + l.x), aligned));
       const Finish<T> to = {dkernel, (size_t)D, kNone, nullptr, nullptr, 0, nullptr};
-      HASTE_HIP_PROPAGATE((product<T, true, true>(stream, C, D, R, x, x_row, d, d_row, to, scratch)));
+      HASTE_HIP_PROPAGATE((product<T, true, true>(stream, l.plan_kernel, C, D, R, x, x_row, d, d_row, to, scratch)));
     }
     return HASTE_HIP_OK;
   }
