@@ -617,11 +617,34 @@ void linear_slope_kernel(int M, int N, int rows_each, const T* __restrict__ dy, 
       partial[(size_t)blockIdx.y * N + blockIdx.x * kSumColumns + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
 }
 
+// What the workgroups left, added up: 64 columns a workgroup, its sixteen wavefronts a part of the rows each, eight of them on their way.
+constexpr int kBiasWaves = 16;
 template <typename T>
-__global__ __launch_bounds__(256)
-void linear_round_kernel(int n, const float* __restrict__ in, T* __restrict__ out) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < n) out[i] = (T)in[i];
+__global__ __launch_bounds__(64 * kBiasWaves)
+void linear_bias_kernel(int parts, int N, const float* __restrict__ partial, T* __restrict__ dbias) {
+  __shared__ float red[kBiasWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+  float sum = 0.f;
+  if (col < N) {
+    constexpr int AT_ONCE = 8;
+    for (int p = wave; p < parts; p += AT_ONCE * kBiasWaves) {
+      float v[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int at = p + i * kBiasWaves;
+        v[i] = partial[(size_t)(at < parts ? at : p) * N + col];
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) sum += p + i * kBiasWaves < parts ? v[i] : 0.f;
+    }
+  }
+  red[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || col >= N) return;
+  sum = red[0][lane];
+#pragma unroll
+  for (int w = 1; w < kBiasWaves; ++w) sum += red[w][lane];
+  dbias[col] = (T)sum;
 }
 
 // ---- plans -------------------------------------------------------------------------------
@@ -717,7 +740,7 @@ long long eights(long long n) { return (n + 7) / 8 * 8; }
 
 struct SumPlan {
   int blocks, rows_each;
-  size_t floats, scratch;
+  size_t floats;
 };
 SumPlan plan_sums(int rows, int columns) {
   const int across = (columns + kSumColumns - 1) / kSumColumns;
@@ -728,7 +751,6 @@ SumPlan plan_sums(int rows, int columns) {
   s.rows_each = (int)((rows + blocks - 1) / blocks);
   s.blocks = (rows + s.rows_each - 1) / s.rows_each;
   s.floats = (size_t)s.blocks * columns;
-  s.scratch = column_sums_scratch(s.blocks, columns);
   return s;
 }
 
@@ -762,7 +784,7 @@ Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) 
     l.d = place(element == 2 ? (size_t)R * eights(D) * 2 : (size_t)R * D * 4);
     if (element == 4) l.kernel = place((size_t)C * D * 4);  // transposed
     const SumPlan s = plan_sums(R, D);
-    l.sums = place((s.floats + s.scratch + D) * sizeof(float));
+    l.sums = place(s.floats * sizeof(float));
   }
   l.product = at;
   size_t need;
@@ -881,13 +903,9 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
       HASTE_HIP_TRY(hipGetLastError());
     }
     if (dbias != nullptr) {
-      const size_t n = D;
-      float* total = sizeof(T) == 4 ? reinterpret_cast<float*>(dbias) : sums + s.floats + s.scratch;
-      HASTE_HIP_PROPAGATE(column_sums(stream, s.blocks, n, sums, sums + s.floats, {{total}, {n, n, n, n}}));
-      if (sizeof(T) == 2) {
-        linear_round_kernel<T><<<(D + 255) / 256, 256, 0, stream>>>(D, total, dbias);
-        HASTE_HIP_TRY(hipGetLastError());
-      }
+      ScopedKernelTimer timer("linear_bias", stream);
+      linear_bias_kernel<T><<<(D + 63) / 64, 64 * kBiasWaves, 0, stream>>>(s.blocks, D, sums, dbias);
+      HASTE_HIP_TRY(hipGetLastError());
     }
   }
   if constexpr (sizeof(T) == 4) {
