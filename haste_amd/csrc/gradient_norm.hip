@@ -9,8 +9,8 @@
 // are parked per workgroup and added in order.
 //
 // The gradients are scaled from the last chunk to the first, and neither they nor the results are kept in the caches any more: what the norm
-// read last is then still in the last-level cache.  us, forwards / backwards / and so: 537 million gradients (1.07 GB) 611 / 608 / 560, 134
-// million in bf16 84 / 84 / 69.
+// read last is then still in the last-level cache.  us, forwards / backwards / and so: 537 million gradients (1.07 GB) 611 / 608 / 560, 67
+// million in bf16 (134 MB) 84 / 84 / 69.
 //
 // Where nothing is to be clipped the factor is 1, and what lies in place is left alone.
 #include <algorithm>

@@ -73,13 +73,14 @@ __device__ __forceinline__ float activated(int act, float v, float& slope) {
 // What becomes of a product's elements.
 template <typename T>
 struct Finish {
+  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type slope_t;
   T* out;
   size_t ld;
   int act;
   const T* bias;                                                              // may be null, like the rest
   const T* residual;
   size_t residual_ld;
-  typename std::conditional<sizeof(T) == 4, float, _Float16>::type* slope;    // [rows][columns]
+  slope_t* slope;                                                             // [rows][columns]
 };
 
 // Eight neighbouring elements of a row, with the bias of their columns.
@@ -257,21 +258,18 @@ struct Product {
   float* partial;                     // [piece][M][N], null: whole
 };
 
-// Workgroups go to the XCDs in turn; each XCD is given a range of the work.
-__device__ __forceinline__ unsigned work_of_xcd() {
-  const unsigned each = gridDim.x >> 3, rest = gridDim.x & 7, xcd = blockIdx.x & 7;
-  return xcd * each + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+// Workgroups go to the XCDs in turn; each XCD is given a range of a product's work.
+__device__ __forceinline__ unsigned work_of_xcd(unsigned block, unsigned blocks) {
+  const unsigned each = blocks >> 3, rest = blocks & 7, xcd = block & 7;
+  return xcd * each + (xcd < rest ? xcd : rest) + (block >> 3);
 }
 
 constexpr int kTallest = 8;  // rows of tiles that are gone through side by side
 
 template <typename T, class G>
-__global__ __launch_bounds__(64 * G::WAVES, 2)
-void linear_tile_kernel(Product p, Finish<T> to) {
-  __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
+__device__ __forceinline__ void multiply_tile(char* lds, const Product& p, const Finish<T>& to, unsigned work) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned work = work_of_xcd();  // in blocks of tiles that share rows of A and columns of B
-  const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
+  const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;  // the work goes through blocks of them that share rows of A and columns of B
   const int piece = work / tiles, tile = work % tiles;
   const int band = tile / (kTallest * p.tiles_n), in_band = tile % (kTallest * p.tiles_n);
   const int tall = p.tiles_m - band * kTallest < kTallest ? p.tiles_m - band * kTallest : kTallest;
@@ -414,6 +412,23 @@ void linear_tile_kernel(Product p, Finish<T> to) {
   }
 }
 
+template <typename T, class G>
+__global__ __launch_bounds__(64 * G::WAVES, 2)
+void linear_tile_kernel(Product p, Finish<T> to) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
+  multiply_tile<T, G>(lds, p, to, work_of_xcd(blockIdx.x, gridDim.x));
+}
+
+// Two products that do not wait for one another: the first has the first `blocks` workgroups.
+template <typename T, class G, class H>
+__global__ __launch_bounds__(64 * G::WAVES, 2)
+void linear_two_tiles_kernel(Product p, Finish<T> to, unsigned blocks, Product q, Finish<T> q_to) {
+  static_assert(G::WAVES == H::WAVES, "one shape of workgroups");
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds > H::kLds ? G::kLds : H::kLds];
+  if (blockIdx.x < blocks) multiply_tile<T, G>(lds, p, to, work_of_xcd(blockIdx.x, blocks));
+  else multiply_tile<T, H>(lds, q, q_to, work_of_xcd(blockIdx.x - blocks, gridDim.x - blocks));
+}
+
 // ---- few rows ----------------------------------------------------------------------------
 // Up to 16 MT rows, the whole product in one launch.  Bound: how fast a CU takes in pieces of rows of W and x, some 2 ns each whether they
 // have 32 or 64 bytes; the fewer columns a workgroup has, the more CUs take part.  Each of its wavefronts takes the 32 k of every eighth unit,
@@ -431,7 +446,7 @@ void linear_rows_kernel(int R, int D, int K, const T* __restrict__ x, size_t x_l
   constexpr int kTurned = kRowWaves * kUnits * kUnitBytes, kSums = kRowWaves * MT * 16 * kPitch * 4;
   __shared__ __attribute__((aligned(16))) char lds[kTurned > kSums ? kTurned : kSums];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = work_of_xcd() * COLUMNS;  // (a cache line has the columns of several workgroups)
+  const int n0 = work_of_xcd(blockIdx.x, gridDim.x) * COLUMNS;  // (a cache line has the columns of several workgroups)
   char* own = lds + wave * kUnits * kUnitBytes;
   const int units = (K + 31) / 32;
   const int col = n0 + lane % LANES * 8;
@@ -537,45 +552,23 @@ void linear_rows_kernel(int R, int D, int K, const T* __restrict__ x, size_t x_l
   finish(to, v, bias, row, n0 + c, D);
 }
 
-// The pieces of a product, added in order, and what follows.  PIECES null: the elements lie in `to.out` already (float).
+// ---- what is done before and behind the products: each in one launch, whose workgroups are dealt out to its parts -----------
+// rows x columns of an operand in 16-byte pieces: rows padded with zeros to a multiple of eight elements.
 template <typename T>
-__global__ __launch_bounds__(256)
-void linear_finish_kernel(int M, int N, int pieces, const float* __restrict__ partial, Finish<T> to) {
-  const unsigned groups = (N + 7) / 8;
-  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < (size_t)M * groups; i += (size_t)gridDim.x * 256) {
+struct Copy {
+  int rows, columns;
+  const T* in;
+  size_t ld;
+  T* out;
+  unsigned blocks;  // 0: none
+};
+template <typename T>
+__device__ __forceinline__ void make_copy(const Copy<T>& c, unsigned block) {
+  const unsigned groups = (c.columns + 7) / 8;
+  for (size_t i = block * (size_t)256 + threadIdx.x; i < (size_t)c.rows * groups; i += (size_t)c.blocks * 256) {
     const size_t row = i / groups;
     const int col = (int)(i % groups) * 8;
-    float v[8], bias[8];
-    load_bias(to, col, N, bias);
-    if (partial == nullptr) {
-      load_channels<8>(to.out + row * to.ld, col, N, v);
-    } else {
-      load_channels<8>(partial + row * N, col, N, v);
-      constexpr int AT_ONCE = 4;
-      for (int z = 1; z < pieces; z += AT_ONCE) {
-        float w[AT_ONCE][8];
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k)  // beyond the last piece it once more, not added
-          load_channels<8>(partial + ((size_t)(z + k < pieces ? z + k : pieces - 1) * M + row) * N, col, N, w[k]);
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += z + k < pieces ? w[k][e] : 0.f;
-      }
-    }
-    finish(to, v, bias, row, col, N);
-  }
-}
-
-// rows x columns, rows padded with zeros to a multiple of eight elements.
-template <typename T>
-__global__ __launch_bounds__(256)
-void linear_pack_kernel(int rows, int columns, const T* __restrict__ in, size_t ld, T* __restrict__ out) {
-  const unsigned groups = (columns + 7) / 8;
-  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < (size_t)rows * groups; i += (size_t)gridDim.x * 256) {
-    const size_t row = i / groups;
-    const int col = (int)(i % groups) * 8;
-    *reinterpret_cast<typename Packed<T, 8>::type*>(out + i * 8) = load_packed<8>(in + row * ld, col, columns);
+    *reinterpret_cast<typename Packed<T, 8>::type*>(c.out + i * 8) = load_packed<8>(c.in + row * c.ld, col, c.columns);
   }
 }
 
@@ -583,68 +576,131 @@ void linear_pack_kernel(int rows, int columns, const T* __restrict__ in, size_t 
 // eight a lane; its four wavefronts take the rows of its share in turn.
 constexpr int kSumColumns = 512;
 template <typename T>
-__global__ __launch_bounds__(256)
-void linear_slope_kernel(int M, int N, int rows_each, const T* __restrict__ dy, size_t dy_ld,
-                         const typename std::conditional<sizeof(T) == 4, float, _Float16>::type* __restrict__ slope,
-                         T* __restrict__ d, size_t d_ld, float* __restrict__ partial) {
+struct Slopes {
+  int M, N, rows_each;
+  const T* dy;
+  size_t dy_ld;
+  const typename Finish<T>::slope_t* slope;  // null: 1
+  T* d;                                      // null: not wanted
+  size_t d_ld;
+  float* partial;                            // null: not wanted
+  unsigned across, blocks;                   // 0: none
+};
+template <typename T>
+__device__ __forceinline__ void apply_slopes(const Slopes<T>& s, unsigned block) {
   __shared__ float red[4][kSumColumns];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = blockIdx.x * kSumColumns + lane * 8;
-  const int first = blockIdx.y * rows_each, last = M - first < rows_each ? M : first + rows_each;
+  const unsigned part = block / s.across, first_col = block % s.across * kSumColumns;
+  const int col = first_col + lane * 8;
+  const int first = part * s.rows_each, last = s.M - first < s.rows_each ? s.M : first + s.rows_each;
   float sum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[i] = 0.f;
 #pragma unroll 4
   for (int row = first + wave; row < last; row += 4) {
     float v[8];
-    load_channels<8>(dy + row * dy_ld, col, N, v);
-    if (slope != nullptr) {
-      float s[8];
-      load_channels<8>(slope + (size_t)row * N, col, N, s);
+    load_channels<8>(s.dy + row * s.dy_ld, col, s.N, v);
+    if (s.slope != nullptr) {
+      float by[8];
+      load_channels<8>(s.slope + (size_t)row * s.N, col, s.N, by);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= s[i];
+      for (int i = 0; i < 8; ++i) v[i] *= by[i];
     }
-    if (d != nullptr && col < (int)d_ld) store_channels<8>(d + row * d_ld, col, (int)d_ld, v);
+    if (s.d != nullptr && col < (int)s.d_ld) store_channels<8>(s.d + row * s.d_ld, col, (int)s.d_ld, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] += v[i];
   }
-  if (partial == nullptr) return;
+  if (s.partial == nullptr) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) red[wave][lane * 8 + i] = sum[i];
   __syncthreads();
   for (int c = threadIdx.x; c < kSumColumns; c += 256)
-    if (blockIdx.x * kSumColumns + c < (unsigned)N)
-      partial[(size_t)blockIdx.y * N + blockIdx.x * kSumColumns + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+    if (first_col + c < (unsigned)s.N) s.partial[(size_t)part * s.N + first_col + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
 }
 
-// What the workgroups left, added up: 64 columns a workgroup, its sixteen wavefronts a part of the rows each, eight of them on their way.
-constexpr int kBiasWaves = 16;
 template <typename T>
-__global__ __launch_bounds__(64 * kBiasWaves)
-void linear_bias_kernel(int parts, int N, const float* __restrict__ partial, T* __restrict__ dbias) {
-  __shared__ float red[kBiasWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+__global__ __launch_bounds__(256)
+void linear_prepare_kernel(Slopes<T> slopes, Copy<T> first, Copy<T> second) {
+  unsigned block = blockIdx.x;
+  if (block < slopes.blocks) return apply_slopes(slopes, block);
+  block -= slopes.blocks;
+  if (block < first.blocks) return make_copy(first, block);
+  make_copy(second, block - first.blocks);
+}
+
+// The pieces of a product, added in order, and what follows.  No pieces: the elements lie in `to.out` already (float).
+template <typename T>
+struct Join {
+  int M, N, pieces;
+  const float* partial;
+  Finish<T> to;
+  unsigned blocks;  // 0: none
+};
+template <typename T>
+__device__ __forceinline__ void join_pieces(const Join<T>& j, unsigned block) {
+  const unsigned groups = (j.N + 7) / 8;
+  for (size_t i = block * (size_t)256 + threadIdx.x; i < (size_t)j.M * groups; i += (size_t)j.blocks * 256) {
+    const size_t row = i / groups;
+    const int col = (int)(i % groups) * 8;
+    float v[8], bias[8];
+    load_bias(j.to, col, j.N, bias);
+    if (j.partial == nullptr) {
+      load_channels<8>(j.to.out + row * j.to.ld, col, j.N, v);
+    } else {
+      load_channels<8>(j.partial + row * j.N, col, j.N, v);
+      constexpr int AT_ONCE = 4;
+      for (int z = 1; z < j.pieces; z += AT_ONCE) {
+        float w[AT_ONCE][8];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)  // beyond the last piece it once more, not added
+          load_channels<8>(j.partial + ((size_t)(z + k < j.pieces ? z + k : j.pieces - 1) * j.M + row) * j.N, col, j.N, w[k]);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += z + k < j.pieces ? w[k][e] : 0.f;
+      }
+    }
+    finish(j.to, v, bias, row, col, j.N);
+  }
+}
+
+// The gradient of the bias from what the workgroups of d left: 64 columns a workgroup, its four wavefronts a part of the rows each, sixteen
+// of them on their way.
+template <typename T>
+struct Bias {
+  int parts, N;
+  const float* partial;
+  T* out;
+  unsigned blocks;  // 0: none
+};
+template <typename T>
+__device__ __forceinline__ void add_bias(const Bias<T>& b, unsigned block) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = block * 64 + lane;
   float sum = 0.f;
-  if (col < N) {
-    constexpr int AT_ONCE = 8;
-    for (int p = wave; p < parts; p += AT_ONCE * kBiasWaves) {
+  if (col < b.N) {
+    constexpr int AT_ONCE = 16;
+    for (int p = wave; p < b.parts; p += AT_ONCE * 4) {
       float v[AT_ONCE];
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const int at = p + i * kBiasWaves;
-        v[i] = partial[(size_t)(at < parts ? at : p) * N + col];
-      }
+      for (int i = 0; i < AT_ONCE; ++i) v[i] = b.partial[(size_t)(p + 4 * i < b.parts ? p + 4 * i : p) * b.N + col];
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) sum += p + i * kBiasWaves < parts ? v[i] : 0.f;
+      for (int i = 0; i < AT_ONCE; ++i) sum += p + 4 * i < b.parts ? v[i] : 0.f;
     }
   }
   red[wave][lane] = sum;
   __syncthreads();
-  if (wave != 0 || col >= N) return;
-  sum = red[0][lane];
-#pragma unroll
-  for (int w = 1; w < kBiasWaves; ++w) sum += red[w][lane];
-  dbias[col] = (T)sum;
+  if (wave == 0 && col < b.N) b.out[col] = (T)((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256)
+void linear_finish_kernel(Bias<T> bias, Join<T> first, Join<T> second) {
+  unsigned block = blockIdx.x;
+  if (block < bias.blocks) return add_bias(bias, block);
+  block -= bias.blocks;
+  if (block < first.blocks) return join_pieces(first, block);
+  join_pieces(second, block - first.blocks);
 }
 
 // ---- plans -------------------------------------------------------------------------------
@@ -705,33 +761,57 @@ int product_of_few_rows(hipStream_t stream, int R, int D, int K, const T* x, siz
   return HASTE_HIP_OK;
 }
 
-template <typename T, class G>
-int launch_tiles(hipStream_t stream, const Product& p, int pieces, const Finish<T>& to) {
-  linear_tile_kernel<T, G><<<dim3((unsigned)(p.tiles_m * p.tiles_n * pieces)), dim3(64 * G::WAVES), 0, stream>>>(p, to);
-  HASTE_HIP_TRY(hipGetLastError());
-  return HASTE_HIP_OK;
-}
-
 int blocks_for(size_t threads) {
   const size_t b = (threads + 255) / 256, most = (size_t)cus() * 32;
   return (int)(b < most ? b : most);
 }
 
-// to = A B, as the operands are stored and plan_product() says, with as much scratch.
-template <typename T, bool A_SLOW, bool B_SLOW>
-int product(hipStream_t stream, const Plan& plan, int M, int N, int K, const void* A, long long lda, const void* B, long long ldb,
-            const Finish<T>& to, float* scratch) {
-  Product p = {M, N, K, A, B, lda, ldb, plan.tiles_m, plan.tiles_n, plan.k_per_piece, plan.pieces > 1 ? scratch : nullptr};
-  {
-    ScopedKernelTimer timer("linear_product", stream);
-    if (plan.large) HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 256, 256, 2, 4>>(stream, p, plan.pieces, to)));
-    else HASTE_HIP_PROPAGATE((launch_tiles<T, Tile<A_SLOW, B_SLOW, 128, 128, 2, 2>>(stream, p, plan.pieces, to)));
-  }
-  if (plan.pieces > 1) {
-    ScopedKernelTimer timer("linear_finish", stream);
-    linear_finish_kernel<T><<<blocks_for((size_t)M * ((N + 7) / 8)), 256, 0, stream>>>(M, N, plan.pieces, scratch, to);
-    HASTE_HIP_TRY(hipGetLastError());
-  }
+// A product as plan_product() says, and as much scratch for its pieces.
+Product product_of(const Plan& plan, int M, int N, int K, const void* A, size_t lda, const void* B, size_t ldb, char* scratch) {
+  return {M, N, K, A, B, (long long)lda, (long long)ldb, plan.tiles_m, plan.tiles_n, plan.k_per_piece,
+          plan.pieces > 1 ? reinterpret_cast<float*>(scratch) : nullptr};
+}
+unsigned workgroups(const Plan& plan) { return (unsigned)(plan.tiles_m * plan.tiles_n * plan.pieces); }
+
+// What is left to be done behind it.
+template <typename T>
+Join<T> joined(const Plan& plan, const Product& p, const Finish<T>& to) {
+  if (plan.pieces <= 1) return {};
+  return {p.M, p.N, plan.pieces, p.partial, to, (unsigned)blocks_for((size_t)p.M * ((p.N + 7) / 8))};
+}
+
+template <bool A_SLOW, bool B_SLOW>
+struct Tiles {
+  typedef Tile<A_SLOW, B_SLOW, 256, 256, 2, 4> large;
+  typedef Tile<A_SLOW, B_SLOW, 128, 128, 2, 2> small;
+};
+
+template <typename T, class TILES>
+int multiply(hipStream_t stream, const Plan& plan, const Product& p, const Finish<T>& to) {
+  ScopedKernelTimer timer("linear_product", stream);
+  if (plan.large) linear_tile_kernel<T, typename TILES::large><<<workgroups(plan), 64 * TILES::large::WAVES, 0, stream>>>(p, to);
+  else linear_tile_kernel<T, typename TILES::small><<<workgroups(plan), 64 * TILES::small::WAVES, 0, stream>>>(p, to);
+  HASTE_HIP_TRY(hipGetLastError());
+  return HASTE_HIP_OK;
+}
+
+template <typename T>
+int prepare(hipStream_t stream, const Slopes<T>& slopes, const Copy<T>& first, const Copy<T>& second) {
+  const unsigned blocks = slopes.blocks + first.blocks + second.blocks;
+  if (blocks == 0) return HASTE_HIP_OK;
+  ScopedKernelTimer timer("linear_prepare", stream);
+  linear_prepare_kernel<T><<<blocks, 256, 0, stream>>>(slopes, first, second);
+  HASTE_HIP_TRY(hipGetLastError());
+  return HASTE_HIP_OK;
+}
+
+template <typename T>
+int finish_all(hipStream_t stream, const Bias<T>& bias, const Join<T>& first, const Join<T>& second) {
+  const unsigned blocks = bias.blocks + first.blocks + second.blocks;
+  if (blocks == 0) return HASTE_HIP_OK;
+  ScopedKernelTimer timer("linear_finish", stream);
+  linear_finish_kernel<T><<<blocks, 256, 0, stream>>>(bias, first, second);
+  HASTE_HIP_TRY(hipGetLastError());
   return HASTE_HIP_OK;
 }
 
@@ -756,7 +836,7 @@ SumPlan plan_sums(int rows, int columns) {
 
 // Where what a call keeps in its workspace lies; sizes in bytes.
 struct Layout {
-  size_t x, kernel, d, sums, product, total;
+  size_t x, kernel, d, sums, product, product_kernel, total;
   Plan plan, plan_kernel;  // of the product forward, or of dx and dkernel; half types
 };
 
@@ -791,7 +871,8 @@ Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) 
   if (element == 2) {
     l.plan = backward ? plan_product(R, C, D) : plan_product(R, D, C);
     if (backward) l.plan_kernel = plan_product(C, D, R);
-    need = (l.plan.floats > l.plan_kernel.floats ? l.plan.floats : l.plan_kernel.floats) * sizeof(float);
+    l.product_kernel = l.product + whole(l.plan.floats * sizeof(float));
+    need = l.product_kernel - l.product + l.plan_kernel.floats * sizeof(float);
   } else {
     const size_t a = backward ? float_product_bytes(R, C, D) : float_product_bytes(R, D, C);
     const size_t b = backward ? float_product_bytes(C, D, R) : 0;
@@ -812,22 +893,14 @@ int check_sizes(int R, int C, int D, int element) {
 
 bool in_pieces(const void* p, size_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
 
+// An operand in 16-byte pieces: itself, or a copy that is to be made.  The rows of a contiguous operand have to end with zeros.
 template <typename T>
-int pack(hipStream_t stream, int rows, int columns, const T* in, size_t ld, T* out) {
-  linear_pack_kernel<T><<<blocks_for((size_t)rows * ((columns + 7) / 8)), 256, 0, stream>>>(rows, columns, in, ld, out);
-  HASTE_HIP_TRY(hipGetLastError());
-  return HASTE_HIP_OK;
-}
-
-// An operand in 16-byte pieces: itself, or its copy.  The rows of a contiguous operand have to end with zeros.
-template <typename T>
-int placed(hipStream_t stream, int rows, int columns, const T*& p, size_t& ld, T* copy, bool aligned) {
-  if (columns % 8 == 0 && in_pieces(p, ld)) return HASTE_HIP_OK;
-  if (aligned && columns % 8 == 0) return HASTE_HIP_ERROR_INVALID_ARGUMENT;  // the workspace has no room for it
-  HASTE_HIP_PROPAGATE(pack(stream, rows, columns, p, ld, copy));
+Copy<T> placed(int rows, int columns, const T*& p, size_t& ld, T* copy) {
+  if (columns % 8 == 0 && in_pieces(p, ld)) return {};
+  const Copy<T> c = {rows, columns, p, ld, copy, (unsigned)blocks_for((size_t)rows * ((columns + 7) / 8))};
   p = copy;
   ld = (size_t)eights(columns);
-  return HASTE_HIP_OK;
+  return c;
 }
 
 bool workspace_ok(const void* workspace, size_t bytes, size_t need) {
@@ -847,24 +920,24 @@ int forward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kernel
   const Layout l = layout_of(false, sizeof(T), R, C, D, aligned);
   HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
   char* ws = static_cast<char*>(workspace);
-  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type slope_t;
-  Finish<T> to = {y, (size_t)D, act, bias, residual, residual_row, act == kNone ? nullptr : static_cast<slope_t*>(cache)};
+  typedef typename Finish<T>::slope_t slope_t;
+  const Finish<T> to = {y, (size_t)D, act, bias, residual, residual_row, act == kNone ? nullptr : static_cast<slope_t*>(cache)};
   if constexpr (sizeof(T) == 4) {
     {
       CallerScratch scratch(ws + l.product, l.total - l.product);
       HASTE_HIP_PROPAGATE(gemm_f32(stream, false, R, D, C, x, (int)x_row, kernel, D, y, D, false));
     }
     if (act == kNone && bias == nullptr && residual == nullptr) return HASTE_HIP_OK;
-    ScopedKernelTimer timer("linear_finish", stream);
-    linear_finish_kernel<T><<<blocks_for((size_t)R * ((D + 7) / 8)), 256, 0, stream>>>(R, D, 0, nullptr, to);
-    HASTE_HIP_TRY(hipGetLastError());
-    return HASTE_HIP_OK;
+    return finish_all<T>(stream, {}, {R, D, 0, nullptr, to, (unsigned)blocks_for((size_t)R * ((D + 7) / 8))}, {});
   } else {
     if (few_rows(sizeof(T), R, C)) return product_of_few_rows(stream, R, D, C, x, x_row, kernel, to);
     size_t kernel_row = D;
-    HASTE_HIP_PROPAGATE(placed(stream, R, C, x, x_row, reinterpret_cast<T*>(ws + l.x), aligned));
-    HASTE_HIP_PROPAGATE(placed(stream, C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel), aligned));
-    return product<T, false, true>(stream, l.plan, R, D, C, x, x_row, kernel, kernel_row, to, reinterpret_cast<float*>(ws + l.product));
+    const Copy<T> of_x = placed(R, C, x, x_row, reinterpret_cast<T*>(ws + l.x));
+    const Copy<T> of_kernel = placed(C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel));
+    HASTE_HIP_PROPAGATE(prepare<T>(stream, {}, of_x, of_kernel));
+    const Product p = product_of(l.plan, R, D, C, x, x_row, kernel, kernel_row, ws + l.product);
+    HASTE_HIP_PROPAGATE((multiply<T, Tiles<false, true>>(stream, l.plan, p, to)));
+    return finish_all<T>(stream, {}, joined(l.plan, p, to), {});
   }
 }
 
@@ -882,8 +955,6 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
   const Layout l = layout_of(true, sizeof(T), R, C, D, aligned);
   HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
   char* ws = static_cast<char*>(workspace);
-  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type slope_t;
-
   // d and its sums
   const T* d = dy;
   size_t d_row = dy_row;
@@ -892,23 +963,19 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
     d = reinterpret_cast<T*>(ws + l.d);
     d_row = sizeof(T) == 2 ? (size_t)eights(D) : (size_t)D;
   }
+  Slopes<T> slopes = {};
+  Bias<T> of_bias = {};
   if (own || dbias != nullptr) {
     const SumPlan s = plan_sums(R, D);
-    float* sums = reinterpret_cast<float*>(ws + l.sums);
-    {
-      ScopedKernelTimer timer("linear_slope", stream);
-      linear_slope_kernel<T><<<dim3((unsigned)((D + kSumColumns - 1) / kSumColumns), (unsigned)s.blocks), 256, 0, stream>>>(
-          R, D, s.rows_each, dy, dy_row, act == kNone ? nullptr : static_cast<const slope_t*>(cache),
-          own ? reinterpret_cast<T*>(ws + l.d) : nullptr, d_row, dbias != nullptr ? sums : nullptr);
-      HASTE_HIP_TRY(hipGetLastError());
-    }
-    if (dbias != nullptr) {
-      ScopedKernelTimer timer("linear_bias", stream);
-      linear_bias_kernel<T><<<(D + 63) / 64, 64 * kBiasWaves, 0, stream>>>(s.blocks, D, sums, dbias);
-      HASTE_HIP_TRY(hipGetLastError());
-    }
+    const unsigned across = (unsigned)((D + kSumColumns - 1) / kSumColumns);
+    float* sums = dbias != nullptr ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
+    slopes = {R, D, s.rows_each, dy, dy_row, act == kNone ? nullptr : static_cast<const typename Finish<T>::slope_t*>(cache),
+              own ? reinterpret_cast<T*>(ws + l.d) : nullptr, d_row, sums, across, across * s.blocks};
+    if (dbias != nullptr) of_bias = {s.blocks, D, sums, dbias, (unsigned)((D + 63) / 64)};
   }
   if constexpr (sizeof(T) == 4) {
+    HASTE_HIP_PROPAGATE(prepare<T>(stream, slopes, {}, {}));
+    HASTE_HIP_PROPAGATE(finish_all<T>(stream, of_bias, {}, {}));
     CallerScratch scratch(ws + l.product, l.total - l.product);
     if (dx != nullptr) {
       float* turned = reinterpret_cast<float*>(ws + l.kernel);
@@ -918,19 +985,29 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
     if (dkernel != nullptr) HASTE_HIP_PROPAGATE(gemm_f32(stream, true, C, D, R, x, (int)x_row, d, (int)d_row, dkernel, D, false));
     return HASTE_HIP_OK;
   } else {
-    float* scratch = reinterpret_cast<float*>(ws + l.product);
-    if (dx != nullptr) {
-      size_t kernel_row = D;
-      HASTE_HIP_PROPAGATE(placed(stream, C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel), aligned));
-      const Finish<T> to = {dx, (size_t)C, kNone, nullptr, nullptr, 0, nullptr};
-      HASTE_HIP_PROPAGATE((product<T, false, false>(stream, l.plan, R, C, D, d, d_row, kernel, kernel_row, to, scratch)));
+    size_t kernel_row = D;
+    Copy<T> of_kernel = {}, of_x = {};
+    if (dx != nullptr) of_kernel = placed(C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel));
+    if (dkernel != nullptr) of_x = placed(R, C, x, x_row, reinterpret_cast<T*>(ws + l.x));
+    HASTE_HIP_PROPAGATE(prepare<T>(stream, slopes, of_kernel, of_x));
+    const Finish<T> to_dx = {dx, (size_t)C, kNone, nullptr, nullptr, 0, nullptr};
+    const Finish<T> to_dkernel = {dkernel, (size_t)D, kNone, nullptr, nullptr, 0, nullptr};
+    const Product of_dx = product_of(l.plan, R, C, D, d, d_row, kernel, kernel_row, ws + l.product);
+    const Product of_dkernel = product_of(l.plan_kernel, C, D, R, x, x_row, d, d_row, ws + l.product_kernel);
+    typedef Tiles<false, false> tiles_dx;
+    typedef Tiles<true, true> tiles_dkernel;
+    if (dx != nullptr && dkernel != nullptr && !l.plan.large && !l.plan_kernel.large) {
+      ScopedKernelTimer timer("linear_product", stream);
+      const unsigned first = workgroups(l.plan), second = workgroups(l.plan_kernel);
+      linear_two_tiles_kernel<T, tiles_dx::small, tiles_dkernel::small><<<first + second, 64 * tiles_dx::small::WAVES, 0, stream>>>(
+          of_dx, to_dx, first, of_dkernel, to_dkernel);
+      HASTE_HIP_TRY(hipGetLastError());
+    } else {
+      if (dx != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dx>(stream, l.plan, of_dx, to_dx)));
+      if (dkernel != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dkernel>(stream, l.plan_kernel, of_dkernel, to_dkernel)));
     }
-    if (dkernel != nullptr) {
-      HASTE_HIP_PROPAGATE(placed(stream, R, C, x, x_row, reinterpret_cast<T*>(ws + l.x), aligned));
-      const Finish<T> to = {dkernel, (size_t)D, kNone, nullptr, nullptr, 0, nullptr};
-      HASTE_HIP_PROPAGATE((product<T, true, true>(stream, l.plan_kernel, C, D, R, x, x_row, d, d_row, to, scratch)));
-    }
-    return HASTE_HIP_OK;
+    return finish_all(stream, of_bias, dx != nullptr ? joined(l.plan, of_dx, to_dx) : Join<T>(),
+                      dkernel != nullptr ? joined(l.plan_kernel, of_dkernel, to_dkernel) : Join<T>());
   }
 }
 
