@@ -556,7 +556,7 @@ void gated_backward_kernel(Shape s, Inputs<T> in, const float* __restrict__ kept
         dx = grad * scale[l][v];
         if constexpr (DECAY) {
           const float dlog = grad * (was * a[l][v] - u[l][v] * slope[l][v]);
-          tile_decay[v] -= inside ? dlog * r[l][v] : 0.f;
+          tile_decay[v] -= inside ? dlog * r[l][v] : extent.fill;
           df = dlog * dr[l][v];
         } else {
           df = grad * (ADMIT ? was : was - r[l][v]) * dr[l][v];
@@ -724,7 +724,7 @@ int forward_entry(int steps, int N, int D, const Inputs<T>& in, const float* h0,
   return with_kind(in, vector_of(N, D), [&](auto vector, auto decay, auto admit) {
     constexpr int V = decltype(vector)::value;
     constexpr bool DECAY = decltype(decay)::value, ADMIT = decltype(admit)::value;
-    if (s.segments > 1) {
+    if constexpr (V == 1) if (s.segments > 1) {  // (where lanes take two channels there are too many workgroups for a cut)
       ScopedKernelTimer timer("gated_compose", as_stream(stream));
       gated_compose_kernel<T, V, DECAY, ADMIT, false><<<grid_of(s, s.segments - 1), 64 * kWaves, 0, as_stream(stream)>>>(s, in, {}, sums);
       HASTE_HIP_TRY(hipGetLastError());
@@ -751,7 +751,7 @@ int backward_entry(int steps, int N, int D, const Inputs<T>& in, const float* ke
   HASTE_HIP_PROPAGATE(with_kind(in, vector_of(N, D), [&](auto vector, auto decay, auto admit) {
     constexpr int V = decltype(vector)::value;
     constexpr bool DECAY = decltype(decay)::value, ADMIT = decltype(admit)::value;
-    if (s.segments > 1) {
+    if constexpr (V == 1) if (s.segments > 1) {
       ScopedKernelTimer timer("gated_compose", as_stream(stream));
       gated_compose_kernel<T, V, DECAY, ADMIT, true><<<grid_of(s, s.segments - 1), 64 * kWaves, 0, as_stream(stream)>>>(s, in, dy, sums);
       HASTE_HIP_TRY(hipGetLastError());

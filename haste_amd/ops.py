@@ -984,14 +984,15 @@ def residual_norm_backward(update, residual, gate, scale, after_weight, before_w
 # reference.  Types, strides, lengths and scratch memory are as for the state space operators above; a projection's parameters have
 # the activations' type.
 _LINEAR_ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2}
+_FARTHEST_ROWS = 2 ** 22  # elements between rows that the entry points take
 
 
 def _linear_rows(t):
-    """[T,N,D] or [N,D] as rows of contiguous columns that are equally far apart: the tensor (or a copy) and their distance."""
+    """[T,N,D] or [N,D] as rows of contiguous columns that are equally far apart, not too far: the tensor (or a copy) and their distance."""
     strides, shape = t.stride(), t.shape
     if strides[-1] == 1 or shape[-1] == 1:
         row = strides[-2] if shape[-2] != 1 else strides[0] if len(shape) == 3 and shape[0] != 1 else shape[-1]
-        if row >= shape[-1] and (len(shape) == 2 or shape[0] == 1 or shape[1] == 1 or strides[0] == strides[1] * shape[1]):
+        if shape[-1] <= row <= _FARTHEST_ROWS and (len(shape) == 2 or shape[0] == 1 or shape[1] == 1 or strides[0] == strides[1] * shape[1]):
             return t, row
     t = t.contiguous()
     return t, shape[-1]

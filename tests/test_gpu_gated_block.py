@@ -171,6 +171,63 @@ def test_linear_gradients_may_be_left_out():
     assert none is None and torch.equal(y, want["y"])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=short)
+def test_linear_of_few_rows_and_more(dtype):
+    """Around the numbers of rows and the lengths of the contraction at which another kernel takes over, with few and many columns."""
+    for C in (2040, 2048, 2056):
+        for R in (15, 16, 17, 31, 32, 33):
+            print("few", R, C, dtype, flush=True)
+            q = linear_problem(R + C, dtype, (R,), C, 200, "silu")
+            compare_linear(run_linear(q.g), exact_linear(q))
+    for R, D in ((1, 8192), (1, 8193), (16, 8200), (17, 8191), (32, 8210), (5, 20001)):
+        print("wide", R, D, dtype, flush=True)
+        q = linear_problem(R + D, dtype, (R,), 72, D, "gelu")
+        compare_linear(run_linear(q.g), exact_linear(q))
+
+
+@pytest.mark.parametrize("R,C,D", [
+    (20000, 64, 72),      # small tiles, whole and in many pieces
+    (300, 6000, 4200),    # dx in pieces, dkernel whole
+    (9000, 520, 1030),    # odd rows, both gradients in small tiles
+    (4096, 4096, 1024), (1100, 4104, 4104)])
+def test_linear_of_every_plan(R, C, D):
+    for activation in ("none", "silu"):
+        print("plan", R, C, D, activation, flush=True)
+        q = linear_problem(R, torch.bfloat16, (R,), C, D, activation)
+        compare_linear(run_linear(q.g), exact_linear(q))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=short)
+def test_linear_beyond_32_bits(dtype):
+    """More than 2^31 outputs: the last rows and the last columns."""
+    R, C, D, rows, columns = 66000, 24, 32768 + 8, 40, 16
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    normal = lambda *shape: torch.randn(*shape, generator=gen, device="cuda", dtype=dtype)  # noqa: E731
+    g = dict(x=normal(R, C), kernel=normal(C, D) * C ** -0.5, bias=normal(D), residual=None, dy=normal(R, D), activation="silu")
+    got = run_linear(g)
+    part = lambda **cut: {"dtype": dtype, "activation": "silu", "residual": None,  # noqa: E731
+                          **{k: g[k].double() if i is None else g[k][i].double() for k, i in cut.items()}}
+    want = formulas.linear(part(x=slice(-rows, None), kernel=None, bias=None, dy=slice(-rows, None)))
+    for k in ("y", "dx"):
+        formulas.check_error(got[k][-rows:], *want[k], k)
+    last = (slice(None), slice(-columns, None))
+    want = formulas.linear(part(x=None, kernel=last, bias=slice(-columns, None), dy=last))
+    formulas.check_error(got["y"][last], *want["y"], "y")
+    formulas.check_error(got["dkernel"][last], *want["dkernel"], "dkernel")
+    formulas.check_error(got["dbias"][-columns:], *want["dbias"], "dbias")
+
+
+def test_linear_of_rows_far_apart():
+    """The last steps of sequences that lie one behind the other, as the head of a model takes them."""
+    whole = torch.empty(5, 70000, 64, device="cuda", dtype=torch.bfloat16)
+    q = linear_problem(11, torch.bfloat16, (5,), 64, 64, "silu")
+    want = run_linear(q.g)
+    for name in ("x", "residual", "dy"):
+        whole[:, -1] = q.g[name]
+        got = run_linear(dict(q.g, **{name: whole[:, -1]}))
+        assert all(torch.equal(want[k], got[k]) for k in want), name
+
+
 def test_linear_rows_behind_the_last_are_left_alone():
     q = linear_problem(10, torch.bfloat16, (70,), 40, 33, "none", True, False)
     x, kernel, bias = q.g["x"], q.g["kernel"], q.g["bias"]
@@ -282,6 +339,30 @@ def test_gated_strides_beyond_32_bits():
     assert all(torch.equal(want[k], got[k]) for k in want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=short)
+def test_gated_of_one_and_two_channels_a_lane(dtype):
+    """On both sides of where a lane takes two channels, and of where the time axis is cut; initial states and lengths of both."""
+    for N, D in ((47, 512), (48, 512), (48, 450), (191, 65), (192, 65), (5, 2048), (40, 200), (41, 200)):
+        print("lanes", N, D, dtype, flush=True)
+        q = gated_problem(N, dtype, 131, N, D, lengths=[131 - 5 * n % 140 if n % 3 else 131 for n in range(N)])
+        q.poison("x", "forget", "admit", "z", "dy")
+        compare_gated(run_gated(q.g), q)
+
+
+def test_gated_beyond_32_bits():
+    """More than 2^31 elements: the last channels of the last row."""
+    T, N, D, last = 264, 255, 32768, 40
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    g = {k: torch.randn(T, N, D, generator=gen, device="cuda", dtype=torch.bfloat16) for k in ("x", "forget", "dy")}
+    g.update({k: None for k in PARTS + ("h0", "dh_last", "lengths")}, decay=torch.rand(D, generator=gen, device="cuda"))
+    got = run_gated(g)
+    q = Problem(4, torch.bfloat16)
+    q.p = {k: v if v is None else v[-last:].double().cpu() if k == "decay" else v[:, -1:, -last:].double().cpu() for k, v in g.items()}
+    want, most = formulas.gated(q.p), formulas.gated(q.p, True)
+    got = {k: got[k][:, -1:, -last:] if k != "h_last" else got[k][-1:, -last:] for k in ("y", "dx", "dforget", "h_last")}
+    bounds.compare(got, {k: want[k] for k in got}, most, 24 * T + 64)
+
+
 def test_gated_expanded_inputs():
     q = gated_problem(4, torch.bfloat16, 40, 3, 30)
     g = dict(q.g)
@@ -299,6 +380,8 @@ def test_gated_lengths_out_of_range_give_nans_for_their_rows():
             assert got[k][:, 1:].isnan().all() and torch.equal(got[k][:, 0], good[k][:, 0]), k
         for k in ("h_last", "dh0"):
             assert got[k][1:].isnan().all() and torch.equal(got[k][0], good[k][0]), k
+        for k in ("ddecay", "dforget_bias", "dadmit_bias"):
+            assert got[k].isnan().all(), k
 
 
 def test_gated_extreme_gates():
@@ -482,6 +565,21 @@ def test_clip_of_orders_and_overlaps():
     for out in ([torch.empty(5, device="cuda")], [torch.empty(10, device="cuda", dtype=torch.float16)], [], [torch.empty(20, device="cuda")[::2]]):
         with pytest.raises(ValueError):
             ops.clip_gradients([flat[:10]], 1.0, out=out)
+
+
+def test_clip_many_large_tensors():
+    """More parts of the norm than a workgroup adds up for itself, in two lists, and a tensor of more than 2^31 elements."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for sizes in ([300001] * 130, [2 ** 31 + 16411, 77]):
+        grads = [torch.randn(n, generator=gen, device="cuda", dtype=torch.bfloat16) for n in sizes]
+        norm = math.sqrt(math.fsum(float(p.double().square().sum()) for g in grads for p in g.split(1 << 28)))
+        got = ops.gradient_norm(grads)
+        assert abs(float(got) - norm) <= norm * 2.0 ** -24
+        kept = [(g[:5000].clone(), g[-5000:].clone()) for g in grads]
+        same, n = ops.clip_gradients(grads, 2.0, out=grads)
+        assert same is grads and torch.equal(n, got)
+        for g, (head, tail) in zip(grads, kept):
+            check_clipped([g[:5000], g[-5000:]], [head, tail], norm, 2.0)
 
 
 # ---- order, streams, graphs, a run of all ------------------------------------------------
