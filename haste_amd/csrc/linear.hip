@@ -419,16 +419,6 @@ void linear_tile_kernel(Product p, Finish<T> to) {
   multiply_tile<T, G>(lds, p, to, work_of_xcd(blockIdx.x, gridDim.x));
 }
 
-// Two products that do not wait for one another: the first has the first `blocks` workgroups.
-template <typename T, class G, class H>
-__global__ __launch_bounds__(64 * G::WAVES, 2)
-void linear_two_tiles_kernel(Product p, Finish<T> to, unsigned blocks, Product q, Finish<T> q_to) {
-  static_assert(G::WAVES == H::WAVES, "one shape of workgroups");
-  __shared__ __attribute__((aligned(1024))) char lds[G::kLds > H::kLds ? G::kLds : H::kLds];
-  if (blockIdx.x < blocks) multiply_tile<T, G>(lds, p, to, work_of_xcd(blockIdx.x, blocks));
-  else multiply_tile<T, H>(lds, q, q_to, work_of_xcd(blockIdx.x - blocks, gridDim.x - blocks));
-}
-
 // ---- few rows ----------------------------------------------------------------------------
 // Up to 16 MT rows, the whole product in one launch.  Bound: how fast a CU takes in pieces of rows of W and x, some 2 ns each whether they
 // have 32 or 64 bytes; the fewer columns a workgroup has, the more CUs take part.  Each of its wavefronts takes the 32 k of every eighth unit,
@@ -701,6 +691,18 @@ void linear_finish_kernel(Bias<T> bias, Join<T> first, Join<T> second) {
   block -= bias.blocks;
   if (block < first.blocks) return join_pieces(first, block);
   join_pieces(second, block - first.blocks);
+}
+
+// Two products that do not wait for one another, and the gradient of the bias ahead of them.
+template <typename T, class G, class H>
+__global__ __launch_bounds__(64 * G::WAVES, 2)
+void linear_gradients_kernel(Bias<T> bias, Product p, Finish<T> to, unsigned blocks, Product q, Finish<T> q_to) {
+  static_assert(G::WAVES == H::WAVES && 64 * G::WAVES == 256, "one shape of workgroups");
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds > H::kLds ? G::kLds : H::kLds];
+  if (blockIdx.x < bias.blocks) return add_bias(bias, blockIdx.x);
+  const unsigned block = blockIdx.x - bias.blocks, all = gridDim.x - bias.blocks;
+  if (block < blocks) multiply_tile<T, G>(lds, p, to, work_of_xcd(block, blocks));
+  else multiply_tile<T, H>(lds, q, q_to, work_of_xcd(block - blocks, all - blocks));
 }
 
 // ---- plans -------------------------------------------------------------------------------
@@ -999,9 +1001,10 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
     if (dx != nullptr && dkernel != nullptr && !l.plan.large && !l.plan_kernel.large) {
       ScopedKernelTimer timer("linear_product", stream);
       const unsigned first = workgroups(l.plan), second = workgroups(l.plan_kernel);
-      linear_two_tiles_kernel<T, tiles_dx::small, tiles_dkernel::small><<<first + second, 64 * tiles_dx::small::WAVES, 0, stream>>>(
-          of_dx, to_dx, first, of_dkernel, to_dkernel);
+      linear_gradients_kernel<T, typename tiles_dx::small, typename tiles_dkernel::small><<<of_bias.blocks + first + second, 256, 0, stream>>>(
+          of_bias, of_dx, to_dx, first, of_dkernel, to_dkernel);
       HASTE_HIP_TRY(hipGetLastError());
+      of_bias.blocks = 0;
     } else {
       if (dx != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dx>(stream, l.plan, of_dx, to_dx)));
       if (dkernel != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dkernel>(stream, l.plan_kernel, of_dkernel, to_dkernel)));
