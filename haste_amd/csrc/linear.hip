@@ -10,12 +10,20 @@
 //
 // One tile kernel makes all three products.  An operand is either stored with the contraction index contiguous (x and d in
 // x W and d W^T, W in d W^T) or with it as the slow index (W in x W, x and d in x^T d).  Tiles go from memory straight into LDS
-// (buffer loads that write LDS: no registers, no wait in between), STAGES of them in a ring: while one is multiplied those behind it are
-// on their way, and a step needs one barrier.  A contiguous operand lies in LDS as rows of BK elements, 16-byte chunk c of row r at
-// position c ^ f(r), so that 16 rows of one chunk cover all banks; an operand of the instruction is one 16-byte read.  A slow
-// one lies as rows of k, 32-byte piece g of row k at g ^ 2 (k % 4), and is read transposed (ds_read_b64_tr_b16: in each 16 lanes,
-// lane i receives element i % 4 of what lanes i / 4 + 4 j address).  Loads beyond an operand's end give zeros.
-// Operands that are not laid out in 16-byte pieces are copied once, rows padded with zeros.
+// (buffer loads that write LDS: no registers, no wait in between), two stages of BK of the contraction: while one is multiplied the next
+// is on its way, and what has been read of the first is replaced piece by piece.  A contiguous operand lies in LDS as rows of BK elements,
+// 16-byte chunk c of row r at position c ^ turn(r), so that 16 rows of one chunk cover all banks; an operand of the instruction is one
+// 16-byte read.  A slow one lies as rows of k, 32-byte piece g of row k at g ^ turn_slow(k), and is read transposed (ds_read_b64_tr_b16: in
+// each 16 lanes, lane i receives element i % 4 of what lanes i / 4 + 4 j address).  Loads beyond an operand's end give zeros.
+// Tiles of 256 x 256 halve what the L2s have to deliver (at 128 x 128 it is their rate that bounds); bands of kTallest of them, gone through
+// column by column, keep what an XCD works on in its L2.  bf16, x W / d W^T / x^T d of R x C x D, us (TFLOP/s):
+//   16384 x 4096 x 4096   406 (1353) / 390 (1410) / 411 (1339)   tiles of 128 x 128   498 / 462 / 527   kTallest 1   429 / 421 / 431
+//    4096 x 4096 x 4096   103 (1336) / 100 (1374) / 104 (1319)                        124 / 116 / 136                105 / 101 / 105
+//    8192 x 1024 x 2048    32 (1061) /  33 (1053) /  48 (719)                          37 /  33 /  48                 32 /  33 /  47
+// (kTallest 32: 431 / 417 / 404 of the first).  The matrix cores are busy for 71 to 80 % of the cycles, at the 1.75 to 1.9 GHz that are left of
+// the clock under this load.
+// Operands that are not laid out in 16-byte pieces are copied once, rows padded with zeros: unaligned 16-byte loads are two to four
+// times as slow (8191 x 2047 x 1023 through registers 96 us, with copies 50).
 //
 // Float: the product of gemm.hip (the bf16 matrix cores on floats split in three), with a pass for what follows it.
 #include <type_traits>
@@ -563,7 +571,7 @@ __device__ __forceinline__ void make_copy(const Copy<T>& c, unsigned block) {
 }
 
 // d = dy slope, rows padded as above, and its sums over the rows of a workgroup.  Bound: HBM.  A workgroup takes 512 columns,
-// eight a lane; its four wavefronts take the rows of its share in turn.
+// eight a lane; its four wavefronts take the rows of its share in turn.  16384 x 4096 in bf16 (403 MB in and out) 75 us, 5.3 TB/s.
 constexpr int kSumColumns = 512;
 template <typename T>
 struct Slopes {
@@ -618,7 +626,7 @@ void linear_prepare_kernel(Slopes<T> slopes, Copy<T> first, Copy<T> second) {
   make_copy(second, block - first.blocks);
 }
 
-// The pieces of a product, added in order, and what follows.  No pieces: the elements lie in `to.out` already (float).
+// The pieces of a product, added in order, and what follows.  Bound: HBM; 8 pieces of 128 x 4096 4.7 us.  No pieces: the elements lie in `to.out` already (float).
 template <typename T>
 struct Join {
   int M, N, pieces;
