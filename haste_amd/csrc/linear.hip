@@ -172,7 +172,9 @@ struct Panel {
   static constexpr int kLoads = kBytes / 1024 / WAVES;  // of a wavefront
   static_assert(kLoads * 1024 * WAVES == kBytes && WAVES % 2 == 0, "a stage is loaded in whole kilobytes");
   static __device__ __forceinline__ int turn(int row) { return (row >> 1) & 7; }
-  static __device__ __forceinline__ int turn_slow(int k) { return 2 * (k & 3) + ((k >> 3) & 1); }
+  static __device__ __forceinline__ int turn_slow(int k) {
+    return WIDTH == 64 ? (k & 2) + ((k >> 3) & 1) : 2 * (k & 3) + ((k >> 3) & 1);  // (rows of 128 bytes: two lie side by side)
+  }
 
   const char* base;
   long long ld_bytes;
@@ -245,8 +247,9 @@ struct Panel {
   }
 };
 
-template <bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_>
+template <bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_, int STAGES_ = 2>
 struct Tile {
+  static constexpr int STAGES = STAGES_;
   static constexpr bool A_SLOW = A_SLOW_, B_SLOW = B_SLOW_;
   static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, WAVES = WAVES_M * WAVES_N;
   static constexpr int MI = BM / WAVES_M / 16, NJ = BN / WAVES_N / 16;  // of 16 x 16 elements
@@ -255,7 +258,7 @@ struct Tile {
   static constexpr int kStage = PA::kBytes + PB::kBytes;
   static constexpr int kSlabLd = NJ * 16 + 4;           // floats of a row of a wavefront's results in LDS
   static constexpr int kSlabs = WAVES * 32 * kSlabLd * 4;
-  static constexpr int kLds = 2 * kStage > kSlabs ? 2 * kStage : kSlabs;
+  static constexpr int kLds = STAGES * kStage > kSlabs ? STAGES * kStage : kSlabs;
 };
 
 struct Product {
@@ -275,21 +278,69 @@ __device__ __forceinline__ unsigned work_of_xcd(unsigned block, unsigned blocks)
 constexpr int kTallest = 8;  // rows of tiles that are gone through side by side
 
 template <typename T, class G>
-__device__ __forceinline__ void multiply_tile(char* lds, const Product& p, const Finish<T>& to, unsigned work) {
+__device__ __forceinline__ void store_tile(char* lds, const Product& p, const Finish<T>& to, const float4_t (&acc)[G::MI][G::NJ], int piece, int m0,
+                                           int n0) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;  // the work goes through blocks of them that share rows of A and columns of B
-  const int piece = work / tiles, tile = work % tiles;
+  const int wm = wave / G::WAVES_N * (G::MI * 16), wn = wave % G::WAVES_N * (G::NJ * 16);
+  // 32 rows of a wavefront's results at a time go through LDS, so that a lane has eight neighbouring elements of a row.
+  float* slab = reinterpret_cast<float*>(lds) + wave * 32 * G::kSlabLd;
+  constexpr int LANES = G::NJ * 2, ROWS = 64 / LANES;  // lanes of a row, rows at a time
+  const int col = n0 + wn + lane % LANES * 8;
+  float bias[8];
+  if (p.partial == nullptr) load_bias(to, col, p.N, bias);
+#pragma unroll
+  for (int i = 0; i < G::MI / 2; ++i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          slab[(16 * h + 4 * (lane >> 4) + e) * G::kSlabLd + 16 * j + (lane & 15)] = acc[2 * i + h][j][e];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+    for (int r = 0; r < 32; r += ROWS) {
+      const int in_slab = r + lane / LANES, row = m0 + wm + 32 * i + in_slab;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = slab[in_slab * G::kSlabLd + lane % LANES * 8 + e];
+      if (row < p.M) {
+        if (p.partial != nullptr) store_channels<8>(p.partial + ((size_t)piece * p.M + row) * p.N, col, p.N, v);
+        else finish(to, v, bias, row, col, p.N);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// What a workgroup has to do.
+struct Work {
+  int piece, m0, n0, k_begin, k_end;
+};
+template <class G>
+__device__ __forceinline__ Work work_of(const Product& p, unsigned turn) {
+  const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;  // it goes through blocks of them that share rows of A and columns of B
+  const int piece = turn / tiles, tile = turn % tiles;
   const int band = tile / (kTallest * p.tiles_n), in_band = tile % (kTallest * p.tiles_n);
   const int tall = p.tiles_m - band * kTallest < kTallest ? p.tiles_m - band * kTallest : kTallest;
-  const int m0 = (band * kTallest + in_band % tall) * G::BM, n0 = in_band / tall * G::BN;
   const int k_begin = piece * p.k_per_piece;
-  const int k_end = k_begin + p.k_per_piece < p.K ? k_begin + p.k_per_piece : p.K;
+  return {piece, (band * kTallest + in_band % tall) * G::BM, in_band / tall * G::BN, k_begin,
+          k_begin + p.k_per_piece < p.K ? k_begin + p.k_per_piece : p.K};
+}
+
+template <typename T, class G>
+__device__ __forceinline__ void multiply_tile(char* lds, const Product& p, const Finish<T>& to, unsigned turn) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Work work = work_of<G>(p, turn);
+  const int k_begin = work.k_begin, k_end = work.k_end;
   const int wm = wave / G::WAVES_N * (G::MI * 16), wn = wave % G::WAVES_N * (G::NJ * 16);
 
   typename G::PA pa;
   typename G::PB pb;
-  pa.start(p.A, p.lda, m0, p.M, k_end, wave, lane);
-  pb.start(p.B, p.ldb, n0, p.N, k_end, wave, lane);
+  pa.start(p.A, p.lda, work.m0, p.M, k_end, wave, lane);
+  pb.start(p.B, p.ldb, work.n0, p.N, k_end, wave, lane);
   const unsigned lds_at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
 
   float4_t acc[G::MI][G::NJ];
@@ -387,44 +438,76 @@ __device__ __forceinline__ void multiply_tile(char* lds, const Product& p, const
   step(std::false_type(), std::false_type(), s);
   tile_ready<0>();
 
-  // 32 rows of a wavefront's results at a time go through LDS, so that a lane has eight neighbouring elements of a row.
-  float* slab = reinterpret_cast<float*>(lds) + wave * 32 * G::kSlabLd;
-  constexpr int LANES = G::NJ * 2, ROWS = 64 / LANES;  // lanes of a row, rows at a time
-  const int col = n0 + wn + lane % LANES * 8;
-  float bias[8];
-  if (p.partial == nullptr) load_bias(to, col, p.N, bias);
+  store_tile<T, G>(lds, p, to, acc, work.piece, work.m0, work.n0);
+}
+
+// Few tiles, of which each has its steps' latency to bear: STAGES of them in a ring, all but one on their way.
+template <typename T, class G>
+__device__ __forceinline__ void multiply_narrow_tile(char* lds, const Product& p, const Finish<T>& to, unsigned turn) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Work work = work_of<G>(p, turn);
+  const int wm = wave / G::WAVES_N * (G::MI * 16), wn = wave % G::WAVES_N * (G::NJ * 16);
+  typename G::PA pa;
+  typename G::PB pb;
+  pa.start(p.A, p.lda, work.m0, p.M, work.k_end, wave, lane);
+  pb.start(p.B, p.ldb, work.n0, p.N, work.k_end, wave, lane);
+  const unsigned lds_at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
+  constexpr int kLoads = G::PA::kLoads + G::PB::kLoads;
+  auto load = [&](int step, int place) {  // beyond the last step: zeros, so that as many are on their way
+    const int k0 = work.k_begin + step * BK;
+    pa.stage(k0, work.k_end);
+    pb.stage(k0, work.k_end);
+    const unsigned at = lds_at + place * G::kStage;
 #pragma unroll
-  for (int i = 0; i < G::MI / 2; ++i) {
+    for (int i = 0; i < G::PA::kLoads; ++i) pa.load(i, at, wave);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < G::PB::kLoads; ++i) pb.load(i, at + G::PA::kBytes, wave);
+  };
+  float4_t acc[G::MI][G::NJ];
 #pragma unroll
-      for (int j = 0; j < G::NJ; ++j)
+  for (int i = 0; i < G::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          slab[(16 * h + 4 * (lane >> 4) + e) * G::kSlabLd + 16 * j + (lane & 15)] = acc[2 * i + h][j][e];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-    for (int r = 0; r < 32; r += ROWS) {
-      const int in_slab = r + lane / LANES, row = m0 + wm + 32 * i + in_slab;
-      float v[8];
+    for (int j = 0; j < G::NJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = slab[in_slab * G::kSlabLd + lane % LANES * 8 + e];
-      if (row < p.M) {
-        if (p.partial != nullptr) store_channels<8>(p.partial + ((size_t)piece * p.M + row) * p.N, col, p.N, v);
-        else finish(to, v, bias, row, col, p.N);
-      }
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+  const int steps = (work.k_end - work.k_begin + BK - 1) / BK;
+#pragma unroll
+  for (int s = 0; s < G::STAGES - 1; ++s) load(s, s);
+  int place = 0, free = G::STAGES - 1;
+  for (int s = 0; s < steps; ++s) {
+    tile_ready<kLoads * (G::STAGES - 2)>();  // and all have read what the next goes into
+    load(s + G::STAGES - 1, free);
+    free = place;
+    const char* stage = lds + place * G::kStage;
+    place = place + 1 < G::STAGES ? place + 1 : 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint4_t a[G::MI], b[G::NJ];
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i) a[i] = G::PA::operand(stage, wm + 16 * i, half, lane);
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) b[j] = G::PB::operand(stage + G::PA::kBytes, wn + 16 * j, half, lane);
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = mfma(T(), a[i], b[j], acc[i][j]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
+  tile_ready<0>();
+  store_tile<T, G>(lds, p, to, acc, work.piece, work.m0, work.n0);
 }
 
 template <typename T, class G>
-__global__ __launch_bounds__(64 * G::WAVES, 2)
+__device__ __forceinline__ void multiply(char* lds, const Product& p, const Finish<T>& to, unsigned block, unsigned blocks) {
+  if constexpr (G::STAGES == 2) multiply_tile<T, G>(lds, p, to, work_of_xcd(block, blocks));
+  else multiply_narrow_tile<T, G>(lds, p, to, work_of_xcd(block, blocks));
+}
+
+template <typename T, class G>
+__global__ __launch_bounds__(64 * G::WAVES, G::STAGES)
 void linear_tile_kernel(Product p, Finish<T> to) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
-  multiply_tile<T, G>(lds, p, to, work_of_xcd(blockIdx.x, gridDim.x));
+  multiply<T, G>(lds, p, to, blockIdx.x, gridDim.x);
 }
 
 // ---- few rows ----------------------------------------------------------------------------
@@ -432,8 +515,8 @@ void linear_tile_kernel(Product p, Finish<T> to) {
 // have 32 or 64 bytes; the fewer columns a workgroup has, the more CUs take part.  Each of its wavefronts takes the 32 k of every eighth unit,
 // two units on their way while two are multiplied: W goes through registers (rows may start anywhere, what is beyond them is 0) into the
 // wavefront's own part of LDS and comes back transposed, x comes as the instruction wants it.  The wavefronts' sums meet in LDS.
-// C x D = 1024 x 4096 and 4096 x 4096, 1 / 16 / 32 rows: 4.5 / 5.1 / 6.0 and 10.4 / 12.6 / 15.9 us (the tile kernel and the sums of its
-// pieces 8.6 / 10.1 / 10.4 and 13.9 / 14.0 / 14.0); with four units 4.8 / 5.1 / 5.8 and 11.4 / 13.1 / 16.6.
+// C x D = 1024 x 4096 and 4096 x 4096, 1 / 16 / 32 rows: 4.2 / 4.7 / 5.5 and 10.5 / 12.4 / 15.9 us (tiles, and the sums of their
+// pieces, 7.8 / 7.3 / 7.8 and 13.1 / 13.7 / 14.5); with four units 4.8 / 5.1 / 5.8 and 11.4 / 13.1 / 16.6.
 constexpr int kRowWaves = 8, kUnits = 2;
 template <typename T, int MT, int COLUMNS>
 __global__ __launch_bounds__(64 * kRowWaves, 2)
@@ -703,49 +786,56 @@ void linear_finish_kernel(Bias<T> bias, Join<T> first, Join<T> second) {
 
 // Two products that do not wait for one another, and the gradient of the bias ahead of them.
 template <typename T, class G, class H>
-__global__ __launch_bounds__(64 * G::WAVES, 2)
+__global__ __launch_bounds__(64 * G::WAVES, G::STAGES < H::STAGES ? G::STAGES : H::STAGES)
 void linear_gradients_kernel(Bias<T> bias, Product p, Finish<T> to, unsigned blocks, Product q, Finish<T> q_to) {
   static_assert(G::WAVES == H::WAVES && 64 * G::WAVES == 256, "one shape of workgroups");
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds > H::kLds ? G::kLds : H::kLds];
   if (blockIdx.x < bias.blocks) return add_bias(bias, blockIdx.x);
   const unsigned block = blockIdx.x - bias.blocks, all = gridDim.x - bias.blocks;
-  if (block < blocks) multiply_tile<T, G>(lds, p, to, work_of_xcd(block, blocks));
-  else multiply_tile<T, H>(lds, q, q_to, work_of_xcd(block - blocks, all - blocks));
+  if (block < blocks) multiply<T, G>(lds, p, to, block, blocks);
+  else multiply<T, H>(lds, q, q_to, block - blocks, all - blocks);
 }
 
 // ---- plans -------------------------------------------------------------------------------
 int cus() { return device_cu_count() > 0 ? device_cu_count() : 256; }
 
+enum { kLarge, kSmall, kNarrow, kTiles };
 struct Plan {
-  bool large;  // tiles of 256 x 256, otherwise of 128 x 128
+  int kind;  // tiles of 256 x 256, 128 x 128 or 64 x 64
   int tiles_m, tiles_n, pieces, k_per_piece;
   size_t floats;
 };
 
-// The cheapest of both tiles and of 1 to 32 pieces by what they were measured to cost, in ns: k of a tile of 256 x 256 21, of 128 x 128 9, or
-// 13.9 for two on a CU; 5000 and 3500 for a round of workgroups, 2500 for adding the pieces up, whose elements are written and read at
-// 4 TB/s.  us, estimate / measured: 128 x 4096 x 4096 (M, N, K) in 4 / 8 pieces of small tiles 19.4 / 18.3, 19.0 / 18.8, in 8 of large ones
-// 26 / 24; 1024 x 2048 x 8192 in 4 of small 51 / 48, in 8 of large 63 / 51; 512 x 512 x 16384 in 16 of small 24 / 26; 8192 x 1024 x 2048
-// whole, small / large tiles 32, 48 / 34, 48.
+// What a k of a tile was measured to cost, in ns, by how many of its kind a CU has: one to three.
+constexpr int kSide[kTiles] = {256, 128, 64}, kPerCu[kTiles] = {1, 2, 3};
+constexpr double kStep[kTiles][3] = {{21.0}, {9.0, 13.9}, {4.2, 6.3, 8.4}}, kRound[kTiles] = {5000, 3500, 3500};
+
+// The cheapest of the tiles and of 1 to 32 pieces by what they were measured to cost: steps and rounds of workgroups as above, 2500 ns for
+// adding pieces up, whose elements are written and read at 4 TB/s.  us, estimate / measured: 128 x 4096 x 4096 (M, K, N) in 4 / 8
+// pieces of 128 x 128 19.4 / 18.3, 19.0 / 18.8, in 8 of 256 x 256 26 / 24, in 2 / 4 of 64 x 64 16.7 / 16.8, 16.6 / 17.0; 1024 x 8192 x 2048 in 4 of
+// 128 x 128 51 / 48, in 8 of 256 x 256 63 / 51; 512 x 16384 x 512 in 16 of 128 x 128 24 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
+// 34, 48; 512 x 2048 x 2048 whole of 64 x 64 12 / 13 (before there were those: 20.7), 1024 x 1024 x 1024 7.8 / 8.6 (14.0), 512 x 512 x 512 5.7 / 5.7
+// (9.1), 2048 x 2048 x 2048 whole of 128 x 128 / 64 x 64 32 / 24, 29 / 29.
 Plan plan_product(int M, int N, int K) {
   Plan best = {};
   double least = 1e300;
-  for (int large = 0; large < 2; ++large) {
-    const int side = large ? 256 : 128;
+  for (int kind = 0; kind < kTiles; ++kind) {
+    const int side = kSide[kind];
     const long long tm = ((long long)M + side - 1) / side, tn = ((long long)N + side - 1) / side, tiles = tm * tn;
-    const long long slots = large ? cus() : 2 * cus();
+    if (kind == kNarrow && tiles > (long long)kGridLimit) break;
+    const long long slots = (long long)kPerCu[kind] * cus();
     for (int s = 1; s <= 32; ++s) {
       int per = (K + s - 1) / s;
       per = (per + BK - 1) / BK * BK;
       if (s > 1 && (per < 2 * BK || tiles * s > 2 * slots)) break;
       if ((K + per - 1) / per != s) continue;
       const long long rounds = tiles * s / slots, rest = tiles * s % slots;
-      double cost = (double)rounds * (large ? 21.0 * per + 5000 : 13.9 * per + 3500);
-      if (rest > 0) cost += large ? 21.0 * per + 5000 : (rest <= cus() ? 9.0 : 13.9) * per + 3500;
+      double cost = (double)rounds * (kStep[kind][kPerCu[kind] - 1] * per + kRound[kind]);
+      if (rest > 0) cost += kStep[kind][(rest - 1) / cus()] * per + kRound[kind];
       if (s > 1) cost += 2500 + (double)s * M * N * 8 / 4000;
       if (cost < least) {
         least = cost;
-        best = {large != 0, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0};
+        best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0};
       }
     }
   }
@@ -794,13 +884,26 @@ template <bool A_SLOW, bool B_SLOW>
 struct Tiles {
   typedef Tile<A_SLOW, B_SLOW, 256, 256, 2, 4> large;
   typedef Tile<A_SLOW, B_SLOW, 128, 128, 2, 2> small;
+  typedef Tile<A_SLOW, B_SLOW, 64, 64, 2, 2, 3> narrow;
 };
 
 template <typename T, class TILES>
 int multiply(hipStream_t stream, const Plan& plan, const Product& p, const Finish<T>& to) {
   ScopedKernelTimer timer("linear_product", stream);
-  if (plan.large) linear_tile_kernel<T, typename TILES::large><<<workgroups(plan), 64 * TILES::large::WAVES, 0, stream>>>(p, to);
-  else linear_tile_kernel<T, typename TILES::small><<<workgroups(plan), 64 * TILES::small::WAVES, 0, stream>>>(p, to);
+  const unsigned blocks = workgroups(plan);
+  if (plan.kind == kLarge) linear_tile_kernel<T, typename TILES::large><<<blocks, 64 * TILES::large::WAVES, 0, stream>>>(p, to);
+  else if (plan.kind == kSmall) linear_tile_kernel<T, typename TILES::small><<<blocks, 256, 0, stream>>>(p, to);
+  else linear_tile_kernel<T, typename TILES::narrow><<<blocks, 256, 0, stream>>>(p, to);
+  HASTE_HIP_TRY(hipGetLastError());
+  return HASTE_HIP_OK;
+}
+
+template <typename T, class G, class H>
+int both_gradients(hipStream_t stream, const Bias<T>& bias, const Plan& plan, const Product& p, const Finish<T>& to, const Plan& q_plan,
+                   const Product& q, const Finish<T>& q_to) {
+  ScopedKernelTimer timer("linear_product", stream);
+  const unsigned first = workgroups(plan);
+  linear_gradients_kernel<T, G, H><<<bias.blocks + first + workgroups(q_plan), 256, 0, stream>>>(bias, p, to, first, q, q_to);
   HASTE_HIP_TRY(hipGetLastError());
   return HASTE_HIP_OK;
 }
@@ -1006,12 +1109,16 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
     const Product of_dkernel = product_of(l.plan_kernel, C, D, R, x, x_row, d, d_row, ws + l.product_kernel);
     typedef Tiles<false, false> tiles_dx;
     typedef Tiles<true, true> tiles_dkernel;
-    if (dx != nullptr && dkernel != nullptr && !l.plan.large && !l.plan_kernel.large) {
-      ScopedKernelTimer timer("linear_product", stream);
-      const unsigned first = workgroups(l.plan), second = workgroups(l.plan_kernel);
-      linear_gradients_kernel<T, typename tiles_dx::small, typename tiles_dkernel::small><<<of_bias.blocks + first + second, 256, 0, stream>>>(
-          of_bias, of_dx, to_dx, first, of_dkernel, to_dkernel);
-      HASTE_HIP_TRY(hipGetLastError());
+    if (dx != nullptr && dkernel != nullptr && l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) {
+      const auto run = [&](auto of_first, auto of_second) {
+        return both_gradients<T, decltype(of_first), decltype(of_second)>(stream, of_bias, l.plan, of_dx, to_dx, l.plan_kernel, of_dkernel, to_dkernel);
+      };
+      const typename tiles_dx::small small_dx;
+      const typename tiles_dx::narrow narrow_dx;
+      const typename tiles_dkernel::small small_dkernel;
+      const typename tiles_dkernel::narrow narrow_dkernel;
+      if (l.plan.kind == kSmall) HASTE_HIP_PROPAGATE(l.plan_kernel.kind == kSmall ? run(small_dx, small_dkernel) : run(small_dx, narrow_dkernel));
+      else HASTE_HIP_PROPAGATE(l.plan_kernel.kind == kSmall ? run(narrow_dx, small_dkernel) : run(narrow_dx, narrow_dkernel));
       of_bias.blocks = 0;
     } else {
       if (dx != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dx>(stream, l.plan, of_dx, to_dx)));
