@@ -26,6 +26,7 @@
 // times as slow (8191 x 2047 x 1023 through registers 96 us, with copies 50).
 //
 // Float: the product of gemm.hip (the bf16 matrix cores on floats split in three), with a pass for what follows it.
+#include <cmath>
 #include <type_traits>
 
 #include "sequence.h"
@@ -784,16 +785,17 @@ void linear_finish_kernel(Bias<T> bias, Join<T> first, Join<T> second) {
   join_pieces(second, block - first.blocks);
 }
 
-// Two products that do not wait for one another, and the gradient of the bias ahead of them.
+// Two products that do not wait for one another, and the gradient of the bias ahead of them.  The workgroups [first, first + blocks)
+// behind those are the first product's.
 template <typename T, class G, class H>
 __global__ __launch_bounds__(64 * G::WAVES, G::STAGES < H::STAGES ? G::STAGES : H::STAGES)
-void linear_gradients_kernel(Bias<T> bias, Product p, Finish<T> to, unsigned blocks, Product q, Finish<T> q_to) {
+void linear_gradients_kernel(Bias<T> bias, Product p, Finish<T> to, unsigned first, unsigned blocks, Product q, Finish<T> q_to) {
   static_assert(G::WAVES == H::WAVES && 64 * G::WAVES == 256, "one shape of workgroups");
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds > H::kLds ? G::kLds : H::kLds];
   if (blockIdx.x < bias.blocks) return add_bias(bias, blockIdx.x);
-  const unsigned block = blockIdx.x - bias.blocks, all = gridDim.x - bias.blocks;
-  if (block < blocks) multiply<T, G>(lds, p, to, block, blocks);
-  else multiply<T, H>(lds, q, q_to, block - blocks, all - blocks);
+  const unsigned block = blockIdx.x - bias.blocks, others = gridDim.x - bias.blocks - blocks;
+  if (block - first < blocks) multiply<T, G>(lds, p, to, block - first, blocks);
+  else multiply<T, H>(lds, q, q_to, block < first ? block : block - blocks, others);
 }
 
 // ---- plans -------------------------------------------------------------------------------
@@ -810,36 +812,59 @@ struct Plan {
 constexpr int kSide[kTiles] = {256, 128, 64}, kPerCu[kTiles] = {1, 2, 3};
 constexpr double kStep[kTiles][3] = {{21.0}, {9.0, 13.9}, {4.2, 6.3, 8.4}}, kRound[kTiles] = {5000, 3500, 3500};
 
-// The cheapest of the tiles and of 1 to 32 pieces by what they were measured to cost: steps and rounds of workgroups as above, 2500 ns for
-// adding pieces up, whose elements are written and read at 4 TB/s.  us, estimate / measured: 128 x 4096 x 4096 (M, K, N) in 4 / 8
-// pieces of 128 x 128 19.4 / 18.3, 19.0 / 18.8, in 8 of 256 x 256 26 / 24, in 2 / 4 of 64 x 64 16.7 / 16.8, 16.6 / 17.0; 1024 x 8192 x 2048 in 4 of
-// 128 x 128 51 / 48, in 8 of 256 x 256 63 / 51; 512 x 16384 x 512 in 16 of 128 x 128 24 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
-// 34, 48; 512 x 2048 x 2048 whole of 64 x 64 12 / 13 (before there were those: 20.7), 1024 x 1024 x 1024 7.8 / 8.6 (14.0), 512 x 512 x 512 5.7 / 5.7
-// (9.1), 2048 x 2048 x 2048 whole of 128 x 128 / 64 x 64 32 / 24, 29 / 29.
-Plan plan_product(int M, int N, int K) {
+// The cheapest of the tiles from `first` on and of 1 to 32 pieces by cost(kind, workgroups, k of a workgroup), beside which adding
+// pieces up takes 2500 ns, and writing and reading their elements at 4 TB/s.
+template <class Cost>
+Plan cheapest(int first, int M, int N, int K, Cost cost) {
   Plan best = {};
   double least = 1e300;
-  for (int kind = 0; kind < kTiles; ++kind) {
+  for (int kind = first; kind < kTiles; ++kind) {
     const int side = kSide[kind];
     const long long tm = ((long long)M + side - 1) / side, tn = ((long long)N + side - 1) / side, tiles = tm * tn;
     if (kind == kNarrow && tiles > (long long)kGridLimit) break;
-    const long long slots = (long long)kPerCu[kind] * cus();
     for (int s = 1; s <= 32; ++s) {
       int per = (K + s - 1) / s;
       per = (per + BK - 1) / BK * BK;
-      if (s > 1 && (per < 2 * BK || tiles * s > 2 * slots)) break;
+      if (s > 1 && (per < 2 * BK || tiles * s > 2ll * kPerCu[kind] * cus())) break;
       if ((K + per - 1) / per != s) continue;
-      const long long rounds = tiles * s / slots, rest = tiles * s % slots;
-      double cost = (double)rounds * (kStep[kind][kPerCu[kind] - 1] * per + kRound[kind]);
-      if (rest > 0) cost += kStep[kind][(rest - 1) / cus()] * per + kRound[kind];
-      if (s > 1) cost += 2500 + (double)s * M * N * 8 / 4000;
-      if (cost < least) {
-        least = cost;
+      const double here = cost(kind, tiles * s, per) + (s > 1 ? 2500 + (double)s * M * N * 8 / 4000 : 0.0);
+      if (here < least) {
+        least = here;
         best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0};
       }
     }
   }
   return best;
+}
+
+// A product by itself: its steps in rounds of workgroups.  us, estimate / measured: 128 x 4096 x 4096 (M, K, N) in 4 / 8
+// pieces of 128 x 128 19.4 / 18.3, 19.0 / 18.8, in 8 of 256 x 256 26 / 24, in 2 / 4 of 64 x 64 16.7 / 16.8, 16.6 / 17.0; 1024 x 8192 x 2048 in 4 of
+// 128 x 128 51 / 48, in 8 of 256 x 256 63 / 51; 512 x 16384 x 512 in 16 of 128 x 128 24 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
+// 34, 48; 512 x 2048 x 2048 whole of 64 x 64 12 / 13 (before there were those: 20.7), 1024 x 1024 x 1024 7.8 / 8.6 (14.0), 512 x 512 x 512 5.7 / 5.7
+// (9.1), 2048 x 2048 x 2048 whole of 128 x 128 / 64 x 64 32 / 24, 29 / 29.
+Plan plan_product(int M, int N, int K) {
+  return cheapest(kLarge, M, N, K, [](int kind, long long workgroups, int per) {
+    const long long slots = (long long)kPerCu[kind] * cus(), rounds = workgroups / slots, rest = workgroups % slots;
+    return (double)rounds * (kStep[kind][kPerCu[kind] - 1] * per + kRound[kind]) +
+           (rest > 0 ? kStep[kind][(rest - 1) / cus()] * per + kRound[kind] : 0.0);
+  });
+}
+
+// One that is launched with `other`: all workgroups' shares of a full CU, which has as many as fit of the larger tiles, or the
+// longest's time where that is more.  us, estimate / measured: both gradients of
+// 8192 x 1024 x 2048 with that of the kernel in 2 / 3 / 4 pieces 73 / 76, 78 / 80, 83 / 81 (by itself 4 would be best), of 4096 x 2048 x 1024 in 2 / 4
+// 45 / 45, 52 / 49.
+Plan plan_product_beside(const Plan& other, int M, int N, int K) {
+  const double others = (double)other.tiles_m * other.tiles_n * other.pieces;
+  return cheapest(kSmall, M, N, K, [&](int kind, long long workgroups, int per) {
+    const int fit = kPerCu[kind] < kPerCu[other.kind] ? kPerCu[kind] : kPerCu[other.kind];
+    const double on_a_cu = (workgroups + others) / cus();
+    const int here = on_a_cu < fit ? (int)std::ceil(on_a_cu) : fit;
+    const double longest = kStep[kind][here - 1] * per + kRound[kind];
+    const double shares = (workgroups * (kStep[kind][fit - 1] * per + kRound[kind]) +
+                           others * (kStep[other.kind][fit - 1] * other.k_per_piece + kRound[other.kind])) / ((double)fit * cus());
+    return shares > longest ? shares : longest;
+  });
 }
 
 // Whether linear_rows_kernel has the forward product: with more than 16 rows of a long contraction tiles are faster.
@@ -902,8 +927,9 @@ template <typename T, class G, class H>
 int both_gradients(hipStream_t stream, const Bias<T>& bias, const Plan& plan, const Product& p, const Finish<T>& to, const Plan& q_plan,
                    const Product& q, const Finish<T>& q_to) {
   ScopedKernelTimer timer("linear_product", stream);
-  const unsigned first = workgroups(plan);
-  linear_gradients_kernel<T, G, H><<<bias.blocks + first + workgroups(q_plan), 256, 0, stream>>>(bias, p, to, first, q, q_to);
+  const unsigned blocks = workgroups(plan), others = workgroups(q_plan);
+  const unsigned first = q_plan.k_per_piece > plan.k_per_piece ? others : 0;  // those that take longer start first
+  linear_gradients_kernel<T, G, H><<<bias.blocks + blocks + others, 256, 0, stream>>>(bias, p, to, first, blocks, q, q_to);
   HASTE_HIP_TRY(hipGetLastError());
   return HASTE_HIP_OK;
 }
@@ -984,6 +1010,7 @@ Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) 
   if (element == 2) {
     l.plan = backward ? plan_product(R, C, D) : plan_product(R, D, C);
     if (backward) l.plan_kernel = plan_product(C, D, R);
+    if (backward && l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) l.plan_kernel = plan_product_beside(l.plan, C, D, R);
     l.product_kernel = l.product + whole(l.plan.floats * sizeof(float));
     need = l.product_kernel - l.product + l.plan_kernel.floats * sizeof(float);
   } else {
