@@ -25,7 +25,8 @@
 // Operands that are not laid out in 16-byte pieces are copied once, rows padded with zeros: unaligned 16-byte loads are two to four
 // times as slow (8191 x 2047 x 1023 through registers 96 us, with copies 50).
 //
-// Float: the product of gemm.hip (the bf16 matrix cores on floats split in three), with a pass for what follows it.
+// Float: large products by gemm.hip (the bf16 matrix cores on floats split in three: 190 TFLOP/s), with a pass for what follows them;
+// small ones by the tile kernel, with the float instruction.
 #include <cmath>
 #include <type_traits>
 
@@ -137,7 +138,8 @@ __device__ __forceinline__ float4_t mfma(__bf16, uint4_t a, uint4_t b, float4_t 
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
 }
 
-constexpr int BK = 64;                          // of the contraction in a stage: 128 bytes, whole cache lines
+constexpr int kStageBytes = 128;                // of the contraction in a stage: whole cache lines
+constexpr int BK = 64;                          // of halves; pieces of a product are cut at multiples of it
 constexpr unsigned int kNowhere = 0x7ffffff0u;  // an offset beyond any resource: the load gives zeros
 
 __device__ __forceinline__ uint4_t resource(const void* base, long long bytes) {
@@ -166,14 +168,17 @@ __device__ __forceinline__ void all_have_read() { asm volatile("s_waitcnt lgkmcn
 // What is written before stays before.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// One operand's part of a stage: WIDTH rows (columns) of the product, BK of the contraction, loaded by WAVES wavefronts.
-template <bool SLOW, int WIDTH, int WAVES>
+// One operand's part of a stage: WIDTH rows (columns) of the product, kStageBytes of the contraction in elements of E bytes, loaded by
+// WAVES wavefronts.
+template <int E, bool SLOW, int WIDTH, int WAVES>
 struct Panel {
-  static constexpr int kBytes = WIDTH * BK * 2;
+  static constexpr int kBytes = WIDTH * kStageBytes, kChunk = 16 / E;  // elements of 16 bytes
   static constexpr int kLoads = kBytes / 1024 / WAVES;  // of a wavefront
   static_assert(kLoads * 1024 * WAVES == kBytes && WAVES % 2 == 0, "a stage is loaded in whole kilobytes");
   static __device__ __forceinline__ int turn(int row) { return (row >> 1) & 7; }
+  static constexpr int kPiece = E == 2 ? 32 : 64;  // bytes of 16 neighbours, which are read together
   static __device__ __forceinline__ int turn_slow(int k) {
+    if (E == 4) return (k >> 2) & 3;                                               // four rows of k at once, four apart
     return WIDTH == 64 ? (k & 2) + ((k >> 3) & 1) : 2 * (k & 3) + ((k >> 3) & 1);  // (rows of 128 bytes: two lie side by side)
   }
 
@@ -188,48 +193,56 @@ struct Panel {
 
   // first: of the tile's rows (columns), of `count` in all.
   __device__ __forceinline__ void start(const void* p, long long ld, int first, int count, int k_end, int wave, int lane) {
-    ld_bytes = ld * 2;
+    ld_bytes = ld * E;
     shift = 0;
     gone = false;
     const int left = count - first;
     if constexpr (SLOW) {
-      base = static_cast<const char*>(p) + (size_t)first * 2;
-      columns = (left + 7) & ~7;
-      constexpr int LANES = WIDTH / 8, ROWS = 64 / LANES;  // lanes of a row of k, rows of a load
+      base = static_cast<const char*>(p) + (size_t)first * E;
+      columns = (left + kChunk - 1) & ~(kChunk - 1);
+      constexpr int LANES = WIDTH / kChunk, ROWS = 64 / LANES, CHUNKS = kPiece / 16;  // lanes of a row of k, rows of a load, loads of a piece
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int k = (i * WAVES + wave) * ROWS + lane / LANES, unit = lane % LANES;
-        const int column = ((unit >> 1) ^ turn_slow(k)) * 16 + (unit & 1) * 8;
-        offset[i] = column < left ? (unsigned)(k * ld_bytes + column * 2) : kNowhere;
+        const int column = ((unit / CHUNKS) ^ turn_slow(k)) * 16 + unit % CHUNKS * kChunk;
+        offset[i] = column < left ? (unsigned)(k * ld_bytes + column * E) : kNowhere;
       }
     } else {
       base = static_cast<const char*>(p) + (size_t)first * ld_bytes;
       const int rows = left < WIDTH ? left : WIDTH;
-      from = resource(base, (rows - 1) * ld_bytes + (long long)((k_end + 7) & ~7) * 2);
+      from = resource(base, (rows - 1) * ld_bytes + (long long)((k_end + kChunk - 1) & ~(kChunk - 1)) * E);
       const int in_load = lane / 8;  // a load's eight rows start at a multiple of 8 that has the wavefront's parity
-      chunk = ((lane % 8) ^ turn(in_load + 8 * (wave & 1))) * 8;
+      chunk = ((lane % 8) ^ turn(in_load + 8 * (wave & 1))) * kChunk;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = (i * WAVES + wave) * 8 + in_load;
-        offset[i] = row < rows ? (unsigned)(row * ld_bytes + chunk * 2) : kNowhere;
+        offset[i] = row < rows ? (unsigned)(row * ld_bytes + chunk * E) : kNowhere;
       }
     }
   }
   // The stage that starts at k0, and load i of it into LDS at `lds`.
   __device__ __forceinline__ void stage(int k0, int k_end) {
     if constexpr (SLOW) {
-      from = resource(base + k0 * ld_bytes, (long long)(k_end - k0 - 1) * ld_bytes + (long long)columns * 2);
+      from = resource(base + k0 * ld_bytes, (long long)(k_end - k0 - 1) * ld_bytes + (long long)columns * E);
     } else {
-      shift = (unsigned)k0 * 2;
+      shift = (unsigned)k0 * E;
       gone = k0 + (int)chunk >= k_end;
     }
   }
   __device__ __forceinline__ void load(int i, unsigned lds, int wave) const {
     load_to_lds(lds + (i * WAVES + wave) * 1024, !SLOW && gone ? kNowhere : offset[i], from, shift);
   }
-  // Eight k of row (column) `first` + lane % 16: those from 32 half + 8 (lane / 16) on.
+  // 16 bytes of k of row (column) `first` + lane % 16: those from kChunk (4 half + lane / 16) on.
   static __device__ __forceinline__ uint4_t operand(const char* stage, int first, int half, int lane) {
-    if constexpr (SLOW) {
+    if constexpr (SLOW && E == 4) {
+      uint4_t v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = 16 * half + 4 * (lane >> 4) + e;
+        v[e] = *reinterpret_cast<const unsigned*>(stage + k * (WIDTH * 4) + ((first >> 4) ^ turn_slow(k)) * kPiece + (lane & 15) * 4);
+      }
+      return v;
+    } else if constexpr (SLOW) {
       uint4_t v;
       const int q = lane >> 4, i = lane & 15;
 #pragma unroll
@@ -243,19 +256,19 @@ struct Panel {
       return v;
     } else {
       const int row = first + (lane & 15), c = 4 * half + (lane >> 4);
-      return *reinterpret_cast<const uint4_t*>(stage + row * (BK * 2) + (c ^ turn(row)) * 16);
+      return *reinterpret_cast<const uint4_t*>(stage + row * kStageBytes + (c ^ turn(row)) * 16);
     }
   }
 };
 
-template <bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_, int STAGES_ = 2>
+template <int E, bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_, int STAGES_ = 2>
 struct Tile {
   static constexpr int STAGES = STAGES_;
   static constexpr bool A_SLOW = A_SLOW_, B_SLOW = B_SLOW_;
   static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, WAVES = WAVES_M * WAVES_N;
   static constexpr int MI = BM / WAVES_M / 16, NJ = BN / WAVES_N / 16;  // of 16 x 16 elements
-  typedef Panel<A_SLOW, BM, WAVES> PA;
-  typedef Panel<B_SLOW, BN, WAVES> PB;
+  typedef Panel<E, A_SLOW, BM, WAVES> PA;
+  typedef Panel<E, B_SLOW, BN, WAVES> PB;
   static constexpr int kStage = PA::kBytes + PB::kBytes;
   static constexpr int kSlabLd = NJ * 16 + 4;           // floats of a row of a wavefront's results in LDS
   static constexpr int kSlabs = WAVES * 32 * kSlabLd * 4;
@@ -443,6 +456,8 @@ __device__ __forceinline__ void multiply_tile(char* lds, const Product& p, const
 }
 
 // Few tiles, of which each has its steps' latency to bear: STAGES of them in a ring, all but one on their way.
+// Floats go through the float instruction, four k at a time, of which lane group q has 4 q + e at turn e; a stage's sum is added to what there
+// is as a whole, so that a sum of K is rounded K / 32 + 32 times.
 template <typename T, class G>
 __device__ __forceinline__ void multiply_narrow_tile(char* lds, const Product& p, const Finish<T>& to, unsigned turn) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -453,9 +468,9 @@ __device__ __forceinline__ void multiply_narrow_tile(char* lds, const Product& p
   pa.start(p.A, p.lda, work.m0, p.M, work.k_end, wave, lane);
   pb.start(p.B, p.ldb, work.n0, p.N, work.k_end, wave, lane);
   const unsigned lds_at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
-  constexpr int kLoads = G::PA::kLoads + G::PB::kLoads;
+  constexpr int kLoads = G::PA::kLoads + G::PB::kLoads, kStep = kStageBytes / (int)sizeof(T);
   auto load = [&](int step, int place) {  // beyond the last step: zeros, so that as many are on their way
-    const int k0 = work.k_begin + step * BK;
+    const int k0 = work.k_begin + step * kStep;
     pa.stage(k0, work.k_end);
     pb.stage(k0, work.k_end);
     const unsigned at = lds_at + place * G::kStage;
@@ -471,7 +486,7 @@ __device__ __forceinline__ void multiply_narrow_tile(char* lds, const Product& p
     for (int j = 0; j < G::NJ; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-  const int steps = (work.k_end - work.k_begin + BK - 1) / BK;
+  const int steps = (work.k_end - work.k_begin + kStep - 1) / kStep;
 #pragma unroll
   for (int s = 0; s < G::STAGES - 1; ++s) load(s, s);
   int place = 0, free = G::STAGES - 1;
@@ -481,6 +496,7 @@ __device__ __forceinline__ void multiply_narrow_tile(char* lds, const Product& p
     free = place;
     const char* stage = lds + place * G::kStage;
     place = place + 1 < G::STAGES ? place + 1 : 0;
+    float4_t sum[sizeof(T) == 4 ? G::MI : 1][G::NJ] = {};
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint4_t a[G::MI], b[G::NJ];
@@ -488,10 +504,26 @@ __device__ __forceinline__ void multiply_narrow_tile(char* lds, const Product& p
       for (int i = 0; i < G::MI; ++i) a[i] = G::PA::operand(stage, wm + 16 * i, half, lane);
 #pragma unroll
       for (int j = 0; j < G::NJ; ++j) b[j] = G::PB::operand(stage + G::PA::kBytes, wn + 16 * j, half, lane);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < G::NJ; ++j)
+              sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i][e]), __uint_as_float(b[j][e]), sum[i][j], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+          for (int j = 0; j < G::NJ; ++j) acc[i][j] = mfma(T(), a[i], b[j], acc[i][j]);
+      }
+    }
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < G::MI; ++i)
 #pragma unroll
-        for (int j = 0; j < G::NJ; ++j) acc[i][j] = mfma(T(), a[i], b[j], acc[i][j]);
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] += sum[i][j];
     }
   }
   tile_ready<0>();
@@ -806,18 +838,21 @@ struct Plan {
   int kind;  // tiles of 256 x 256, 128 x 128 or 64 x 64
   int tiles_m, tiles_n, pieces, k_per_piece;
   size_t floats;
+  double cost;  // ns
 };
 
 // What a k of a tile was measured to cost, in ns, by how many of its kind a CU has: one to three.
 constexpr int kSide[kTiles] = {256, 128, 64}, kPerCu[kTiles] = {1, 2, 3};
 constexpr double kStep[kTiles][3] = {{21.0}, {9.0, 13.9}, {4.2, 6.3, 8.4}}, kRound[kTiles] = {5000, 3500, 3500};
+constexpr double kFloatStep[3] = {23.0, 38.0, 56.0};  // floats, 64 x 64
+double step_cost(int element, int kind, int on_a_cu) { return element == 4 ? kFloatStep[on_a_cu - 1] : kStep[kind][on_a_cu - 1]; }
 
 // The cheapest of the tiles from `first` on and of 1 to 32 pieces by cost(kind, workgroups, k of a workgroup), beside which adding
 // pieces up takes 2500 ns, and writing and reading their elements at 4 TB/s.
 template <class Cost>
 Plan cheapest(int first, int M, int N, int K, Cost cost) {
   Plan best = {};
-  double least = 1e300;
+  best.cost = 1e300;
   for (int kind = first; kind < kTiles; ++kind) {
     const int side = kSide[kind];
     const long long tm = ((long long)M + side - 1) / side, tn = ((long long)N + side - 1) / side, tiles = tm * tn;
@@ -828,10 +863,7 @@ Plan cheapest(int first, int M, int N, int K, Cost cost) {
       if (s > 1 && (per < 2 * BK || tiles * s > 2ll * kPerCu[kind] * cus())) break;
       if ((K + per - 1) / per != s) continue;
       const double here = cost(kind, tiles * s, per) + (s > 1 ? 2500 + (double)s * M * N * 8 / 4000 : 0.0);
-      if (here < least) {
-        least = here;
-        best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0};
-      }
+      if (here < best.cost) best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0, here};
     }
   }
   return best;
@@ -842,11 +874,11 @@ Plan cheapest(int first, int M, int N, int K, Cost cost) {
 // 128 x 128 51 / 48, in 8 of 256 x 256 63 / 51; 512 x 16384 x 512 in 16 of 128 x 128 24 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
 // 34, 48; 512 x 2048 x 2048 whole of 64 x 64 12 / 13 (before there were those: 20.7), 1024 x 1024 x 1024 7.8 / 8.6 (14.0), 512 x 512 x 512 5.7 / 5.7
 // (9.1), 2048 x 2048 x 2048 whole of 128 x 128 / 64 x 64 32 / 24, 29 / 29.
-Plan plan_product(int M, int N, int K) {
-  return cheapest(kLarge, M, N, K, [](int kind, long long workgroups, int per) {
+Plan plan_product(int element, int M, int N, int K) {
+  return cheapest(element == 4 ? kNarrow : kLarge, M, N, K, [=](int kind, long long workgroups, int per) {
     const long long slots = (long long)kPerCu[kind] * cus(), rounds = workgroups / slots, rest = workgroups % slots;
-    return (double)rounds * (kStep[kind][kPerCu[kind] - 1] * per + kRound[kind]) +
-           (rest > 0 ? kStep[kind][(rest - 1) / cus()] * per + kRound[kind] : 0.0);
+    return (double)rounds * (step_cost(element, kind, kPerCu[kind]) * per + kRound[kind]) +
+           (rest > 0 ? step_cost(element, kind, (int)((rest - 1) / cus()) + 1) * per + kRound[kind] : 0.0);
   });
 }
 
@@ -854,15 +886,15 @@ Plan plan_product(int M, int N, int K) {
 // longest's time where that is more.  us, estimate / measured: both gradients of
 // 8192 x 1024 x 2048 with that of the kernel in 2 / 3 / 4 pieces 73 / 76, 78 / 80, 83 / 81 (by itself 4 would be best), of 4096 x 2048 x 1024 in 2 / 4
 // 45 / 45, 52 / 49.
-Plan plan_product_beside(const Plan& other, int M, int N, int K) {
+Plan plan_product_beside(int element, const Plan& other, int M, int N, int K) {
   const double others = (double)other.tiles_m * other.tiles_n * other.pieces;
-  return cheapest(kSmall, M, N, K, [&](int kind, long long workgroups, int per) {
+  return cheapest(element == 4 ? kNarrow : kSmall, M, N, K, [&](int kind, long long workgroups, int per) {
     const int fit = kPerCu[kind] < kPerCu[other.kind] ? kPerCu[kind] : kPerCu[other.kind];
     const double on_a_cu = (workgroups + others) / cus();
     const int here = on_a_cu < fit ? (int)std::ceil(on_a_cu) : fit;
-    const double longest = kStep[kind][here - 1] * per + kRound[kind];
-    const double shares = (workgroups * (kStep[kind][fit - 1] * per + kRound[kind]) +
-                           others * (kStep[other.kind][fit - 1] * other.k_per_piece + kRound[other.kind])) / ((double)fit * cus());
+    const double longest = step_cost(element, kind, here) * per + kRound[kind];
+    const double shares = (workgroups * (step_cost(element, kind, fit) * per + kRound[kind]) +
+                           others * (step_cost(element, other.kind, fit) * other.k_per_piece + kRound[other.kind])) / ((double)fit * cus());
     return shares > longest ? shares : longest;
   });
 }
@@ -905,20 +937,22 @@ Join<T> joined(const Plan& plan, const Product& p, const Finish<T>& to) {
   return {p.M, p.N, plan.pieces, p.partial, to, (unsigned)blocks_for((size_t)p.M * ((p.N + 7) / 8))};
 }
 
-template <bool A_SLOW, bool B_SLOW>
+template <int E, bool A_SLOW, bool B_SLOW>
 struct Tiles {
-  typedef Tile<A_SLOW, B_SLOW, 256, 256, 2, 4> large;
-  typedef Tile<A_SLOW, B_SLOW, 128, 128, 2, 2> small;
-  typedef Tile<A_SLOW, B_SLOW, 64, 64, 2, 2, 3> narrow;
+  typedef Tile<E, A_SLOW, B_SLOW, 256, 256, 2, 4> large;
+  typedef Tile<E, A_SLOW, B_SLOW, 128, 128, 2, 2> small;
+  typedef Tile<E, A_SLOW, B_SLOW, 64, 64, 2, 2, 3> narrow;
 };
 
 template <typename T, class TILES>
 int multiply(hipStream_t stream, const Plan& plan, const Product& p, const Finish<T>& to) {
   ScopedKernelTimer timer("linear_product", stream);
   const unsigned blocks = workgroups(plan);
-  if (plan.kind == kLarge) linear_tile_kernel<T, typename TILES::large><<<blocks, 64 * TILES::large::WAVES, 0, stream>>>(p, to);
-  else if (plan.kind == kSmall) linear_tile_kernel<T, typename TILES::small><<<blocks, 256, 0, stream>>>(p, to);
-  else linear_tile_kernel<T, typename TILES::narrow><<<blocks, 256, 0, stream>>>(p, to);
+  if constexpr (sizeof(T) == 2) {
+    if (plan.kind == kLarge) linear_tile_kernel<T, typename TILES::large><<<blocks, 64 * TILES::large::WAVES, 0, stream>>>(p, to);
+    else if (plan.kind == kSmall) linear_tile_kernel<T, typename TILES::small><<<blocks, 256, 0, stream>>>(p, to);
+  }
+  if (plan.kind == kNarrow) linear_tile_kernel<T, typename TILES::narrow><<<blocks, 256, 0, stream>>>(p, to);
   HASTE_HIP_TRY(hipGetLastError());
   return HASTE_HIP_OK;
 }
@@ -976,7 +1010,8 @@ SumPlan plan_sums(int rows, int columns) {
 // Where what a call keeps in its workspace lies; sizes in bytes.
 struct Layout {
   size_t x, kernel, d, sums, product, product_kernel, total;
-  Plan plan, plan_kernel;  // of the product forward, or of dx and dkernel; half types
+  bool tiles;              // otherwise the products are those of gemm.hip
+  Plan plan, plan_kernel;  // of the product forward, or of dx and dkernel
 };
 
 size_t float_product_bytes(int M, int N, int K) {
@@ -987,30 +1022,43 @@ size_t float_product_bytes(int M, int N, int K) {
   return bytes > bound ? bytes : bound;
 }
 
+// What gemm.hip's product of M rows takes, ns: 190 TFLOP/s, and beside them less for few rows.  Products of floats go by tiles of the float
+// instruction where those cost less, which have no pass behind them.  us, tiles / gemm.hip: 512 x 512 x 512 (R, C, D) 10.9 / 15.7, both
+// gradients 16.2 / 33.8; 1024 x 1024 x 1024 27.7 / 31.7, 43 / 65; 1296 x 224 x 630 12.4 / 18.9; 3071 x 300 x 1001 28.5 / 28.8, 59 / 68;
+// 64 x 1024 x 4096 14.4 / 17.6, but 64 x 4096 x 4096 31.1 / 27.6; 2048 x 1024 x 1024 41.6 / 38.5, 99 / 77; 2048 x 2048 x 2048 150 / 99.
+double product_of_floats(int M, int R, int C, int D) { return (M < 80 ? 9500 + 80.0 * M : 16000) + 2.0 * R * C * D / 190e3; }
+
 Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) {
   Layout l = {};
   if (!backward && few_rows(element, R, C)) return l;
-  const bool pack_x = element == 2 && (!aligned || C % 8 != 0), pack_kernel = element == 2 && (!aligned || D % 8 != 0);
+  l.plan = backward ? plan_product(element, R, C, D) : plan_product(element, R, D, C);
+  double cost = l.plan.cost;
+  if (backward) {
+    l.plan_kernel = plan_product(element, C, D, R);
+    cost += l.plan_kernel.cost;
+    if (l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) {
+      l.plan_kernel = plan_product_beside(element, l.plan, C, D, R);
+      cost = l.plan_kernel.cost;
+    }
+  }
+  l.tiles = element == 2 || cost < product_of_floats(R, R, C, D) + (backward ? product_of_floats(C, R, C, D) : 0.0);
+  const int piece = 16 / element;
   size_t at = 0;
   auto place = [&](size_t bytes) {
     const size_t here = at;
     at += whole(bytes);
     return here;
   };
-  l.x = place(pack_x ? (size_t)R * eights(C) * 2 : 0);
-  l.kernel = place(pack_kernel ? (size_t)C * eights(D) * 2 : 0);
+  l.x = place(l.tiles && (!aligned || C % piece != 0) ? (size_t)R * eights(C) * element : 0);
+  l.kernel = place(!l.tiles ? (backward ? (size_t)C * D * 4 : 0) : !aligned || D % piece != 0 ? (size_t)C * eights(D) * element : 0);
   if (backward) {
-    l.d = place(element == 2 ? (size_t)R * eights(D) * 2 : (size_t)R * D * 4);
-    if (element == 4) l.kernel = place((size_t)C * D * 4);  // transposed
+    l.d = place((size_t)R * (l.tiles ? eights(D) : D) * element);
     const SumPlan s = plan_sums(R, D);
     l.sums = place(s.floats * sizeof(float));
   }
   l.product = at;
   size_t need;
-  if (element == 2) {
-    l.plan = backward ? plan_product(R, C, D) : plan_product(R, D, C);
-    if (backward) l.plan_kernel = plan_product(C, D, R);
-    if (backward && l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) l.plan_kernel = plan_product_beside(l.plan, C, D, R);
+  if (l.tiles) {
     l.product_kernel = l.product + whole(l.plan.floats * sizeof(float));
     need = l.product_kernel - l.product + l.plan_kernel.floats * sizeof(float);
   } else {
@@ -1031,12 +1079,12 @@ int check_sizes(int R, int C, int D, int element) {
   return HASTE_HIP_OK;
 }
 
-bool in_pieces(const void* p, size_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
+bool in_pieces(const void* p, size_t ld, int element) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld * element % 16 == 0; }
 
 // An operand in 16-byte pieces: itself, or a copy that is to be made.  The rows of a contiguous operand have to end with zeros.
 template <typename T>
 Copy<T> placed(int rows, int columns, const T*& p, size_t& ld, T* copy) {
-  if (columns % 8 == 0 && in_pieces(p, ld)) return {};
+  if (columns * sizeof(T) % 16 == 0 && in_pieces(p, ld, sizeof(T))) return {};
   const Copy<T> c = {rows, columns, p, ld, copy, (unsigned)blocks_for((size_t)rows * ((columns + 7) / 8))};
   p = copy;
   ld = (size_t)eights(columns);
@@ -1056,29 +1104,31 @@ int forward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kernel
   if (R == 1) x_row = C;
   if (x_row > (size_t)(1 << 22)) return too_large("linear: rows of x more than 2^22 elements apart");
   hipStream_t stream = as_stream(stream_);
-  const bool aligned = in_pieces(x, x_row) && in_pieces(kernel, 8);
+  const bool aligned = in_pieces(x, x_row, sizeof(T)) && in_pieces(kernel, 8, sizeof(T));
   const Layout l = layout_of(false, sizeof(T), R, C, D, aligned);
   HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
   char* ws = static_cast<char*>(workspace);
   typedef typename Finish<T>::slope_t slope_t;
   const Finish<T> to = {y, (size_t)D, act, bias, residual, residual_row, act == kNone ? nullptr : static_cast<slope_t*>(cache)};
   if constexpr (sizeof(T) == 4) {
-    {
-      CallerScratch scratch(ws + l.product, l.total - l.product);
-      HASTE_HIP_PROPAGATE(gemm_f32(stream, false, R, D, C, x, (int)x_row, kernel, D, y, D, false));
+    if (!l.tiles) {
+      {
+        CallerScratch scratch(ws + l.product, l.total - l.product);
+        HASTE_HIP_PROPAGATE(gemm_f32(stream, false, R, D, C, x, (int)x_row, kernel, D, y, D, false));
+      }
+      if (act == kNone && bias == nullptr && residual == nullptr) return HASTE_HIP_OK;
+      return finish_all<T>(stream, {}, {R, D, 0, nullptr, to, (unsigned)blocks_for((size_t)R * ((D + 7) / 8))}, {});
     }
-    if (act == kNone && bias == nullptr && residual == nullptr) return HASTE_HIP_OK;
-    return finish_all<T>(stream, {}, {R, D, 0, nullptr, to, (unsigned)blocks_for((size_t)R * ((D + 7) / 8))}, {});
-  } else {
-    if (few_rows(sizeof(T), R, C)) return product_of_few_rows(stream, R, D, C, x, x_row, kernel, to);
-    size_t kernel_row = D;
-    const Copy<T> of_x = placed(R, C, x, x_row, reinterpret_cast<T*>(ws + l.x));
-    const Copy<T> of_kernel = placed(C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel));
-    HASTE_HIP_PROPAGATE(prepare<T>(stream, {}, of_x, of_kernel));
-    const Product p = product_of(l.plan, R, D, C, x, x_row, kernel, kernel_row, ws + l.product);
-    HASTE_HIP_PROPAGATE((multiply<T, Tiles<false, true>>(stream, l.plan, p, to)));
-    return finish_all<T>(stream, {}, joined(l.plan, p, to), {});
+  } else if (few_rows(sizeof(T), R, C)) {
+    return product_of_few_rows(stream, R, D, C, x, x_row, kernel, to);
   }
+  size_t kernel_row = D;
+  const Copy<T> of_x = placed(R, C, x, x_row, reinterpret_cast<T*>(ws + l.x));
+  const Copy<T> of_kernel = placed(C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel));
+  HASTE_HIP_PROPAGATE(prepare<T>(stream, {}, of_x, of_kernel));
+  const Product p = product_of(l.plan, R, D, C, x, x_row, kernel, kernel_row, ws + l.product);
+  HASTE_HIP_PROPAGATE((multiply<T, Tiles<sizeof(T), false, true>>(stream, l.plan, p, to)));
+  return finish_all<T>(stream, {}, joined(l.plan, p, to), {});
 }
 
 template <typename T>
@@ -1091,17 +1141,17 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
   if (R == 1) x_row = C, dy_row = D;
   if (x_row > (size_t)(1 << 22) || dy_row > (size_t)(1 << 22)) return too_large("linear: rows more than 2^22 elements apart");
   hipStream_t stream = as_stream(stream_);
-  const bool aligned = in_pieces(x, x_row) && in_pieces(kernel, 8);
+  const bool aligned = in_pieces(x, x_row, sizeof(T)) && in_pieces(kernel, 8, sizeof(T));
   const Layout l = layout_of(true, sizeof(T), R, C, D, aligned);
   HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
   char* ws = static_cast<char*>(workspace);
   // d and its sums
   const T* d = dy;
   size_t d_row = dy_row;
-  const bool own = act != kNone || (sizeof(T) == 2 && (D % 8 != 0 || !in_pieces(dy, dy_row)));
+  const bool own = act != kNone || (l.tiles && (D * sizeof(T) % 16 != 0 || !in_pieces(dy, dy_row, sizeof(T))));
   if (own) {
     d = reinterpret_cast<T*>(ws + l.d);
-    d_row = sizeof(T) == 2 ? (size_t)eights(D) : (size_t)D;
+    d_row = l.tiles ? (size_t)eights(D) : (size_t)D;
   }
   Slopes<T> slopes = {};
   Bias<T> of_bias = {};
@@ -1114,46 +1164,51 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
     if (dbias != nullptr) of_bias = {s.blocks, D, sums, dbias, (unsigned)((D + 63) / 64)};
   }
   if constexpr (sizeof(T) == 4) {
-    HASTE_HIP_PROPAGATE(prepare<T>(stream, slopes, {}, {}));
-    HASTE_HIP_PROPAGATE(finish_all<T>(stream, of_bias, {}, {}));
-    CallerScratch scratch(ws + l.product, l.total - l.product);
-    if (dx != nullptr) {
-      float* turned = reinterpret_cast<float*>(ws + l.kernel);
-      HASTE_HIP_PROPAGATE(haste_hip_transpose_f32(C, D, kernel, turned, stream_));
-      HASTE_HIP_PROPAGATE(gemm_f32(stream, false, R, C, D, d, (int)d_row, turned, C, dx, C, false));
+    if (!l.tiles) {
+      HASTE_HIP_PROPAGATE(prepare<T>(stream, slopes, {}, {}));
+      HASTE_HIP_PROPAGATE(finish_all<T>(stream, of_bias, {}, {}));
+      CallerScratch scratch(ws + l.product, l.total - l.product);
+      if (dx != nullptr) {
+        float* turned = reinterpret_cast<float*>(ws + l.kernel);
+        HASTE_HIP_PROPAGATE(haste_hip_transpose_f32(C, D, kernel, turned, stream_));
+        HASTE_HIP_PROPAGATE(gemm_f32(stream, false, R, C, D, d, (int)d_row, turned, C, dx, C, false));
+      }
+      if (dkernel != nullptr) HASTE_HIP_PROPAGATE(gemm_f32(stream, true, C, D, R, x, (int)x_row, d, (int)d_row, dkernel, D, false));
+      return HASTE_HIP_OK;
     }
-    if (dkernel != nullptr) HASTE_HIP_PROPAGATE(gemm_f32(stream, true, C, D, R, x, (int)x_row, d, (int)d_row, dkernel, D, false));
-    return HASTE_HIP_OK;
-  } else {
-    size_t kernel_row = D;
-    Copy<T> of_kernel = {}, of_x = {};
-    if (dx != nullptr) of_kernel = placed(C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel));
-    if (dkernel != nullptr) of_x = placed(R, C, x, x_row, reinterpret_cast<T*>(ws + l.x));
-    HASTE_HIP_PROPAGATE(prepare<T>(stream, slopes, of_kernel, of_x));
-    const Finish<T> to_dx = {dx, (size_t)C, kNone, nullptr, nullptr, 0, nullptr};
-    const Finish<T> to_dkernel = {dkernel, (size_t)D, kNone, nullptr, nullptr, 0, nullptr};
-    const Product of_dx = product_of(l.plan, R, C, D, d, d_row, kernel, kernel_row, ws + l.product);
-    const Product of_dkernel = product_of(l.plan_kernel, C, D, R, x, x_row, d, d_row, ws + l.product_kernel);
-    typedef Tiles<false, false> tiles_dx;
-    typedef Tiles<true, true> tiles_dkernel;
-    if (dx != nullptr && dkernel != nullptr && l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) {
-      const auto run = [&](auto of_first, auto of_second) {
-        return both_gradients<T, decltype(of_first), decltype(of_second)>(stream, of_bias, l.plan, of_dx, to_dx, l.plan_kernel, of_dkernel, to_dkernel);
-      };
+  }
+  size_t kernel_row = D;
+  Copy<T> of_kernel = {}, of_x = {};
+  if (dx != nullptr) of_kernel = placed(C, D, kernel, kernel_row, reinterpret_cast<T*>(ws + l.kernel));
+  if (dkernel != nullptr) of_x = placed(R, C, x, x_row, reinterpret_cast<T*>(ws + l.x));
+  HASTE_HIP_PROPAGATE(prepare<T>(stream, slopes, of_kernel, of_x));
+  const Finish<T> to_dx = {dx, (size_t)C, kNone, nullptr, nullptr, 0, nullptr};
+  const Finish<T> to_dkernel = {dkernel, (size_t)D, kNone, nullptr, nullptr, 0, nullptr};
+  const Product of_dx = product_of(l.plan, R, C, D, d, d_row, kernel, kernel_row, ws + l.product);
+  const Product of_dkernel = product_of(l.plan_kernel, C, D, R, x, x_row, d, d_row, ws + l.product_kernel);
+  typedef Tiles<sizeof(T), false, false> tiles_dx;
+  typedef Tiles<sizeof(T), true, true> tiles_dkernel;
+  if (dx != nullptr && dkernel != nullptr && l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) {
+    const auto run = [&](auto of_first, auto of_second) {
+      return both_gradients<T, decltype(of_first), decltype(of_second)>(stream, of_bias, l.plan, of_dx, to_dx, l.plan_kernel, of_dkernel, to_dkernel);
+    };
+    const typename tiles_dx::narrow narrow_dx;
+    const typename tiles_dkernel::narrow narrow_dkernel;
+    if constexpr (sizeof(T) == 2) {
       const typename tiles_dx::small small_dx;
-      const typename tiles_dx::narrow narrow_dx;
       const typename tiles_dkernel::small small_dkernel;
-      const typename tiles_dkernel::narrow narrow_dkernel;
       if (l.plan.kind == kSmall) HASTE_HIP_PROPAGATE(l.plan_kernel.kind == kSmall ? run(small_dx, small_dkernel) : run(small_dx, narrow_dkernel));
       else HASTE_HIP_PROPAGATE(l.plan_kernel.kind == kSmall ? run(narrow_dx, small_dkernel) : run(narrow_dx, narrow_dkernel));
-      of_bias.blocks = 0;
     } else {
-      if (dx != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dx>(stream, l.plan, of_dx, to_dx)));
-      if (dkernel != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dkernel>(stream, l.plan_kernel, of_dkernel, to_dkernel)));
+      HASTE_HIP_PROPAGATE(run(narrow_dx, narrow_dkernel));
     }
-    return finish_all(stream, of_bias, dx != nullptr ? joined(l.plan, of_dx, to_dx) : Join<T>(),
-                      dkernel != nullptr ? joined(l.plan_kernel, of_dkernel, to_dkernel) : Join<T>());
+    of_bias.blocks = 0;
+  } else {
+    if (dx != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dx>(stream, l.plan, of_dx, to_dx)));
+    if (dkernel != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dkernel>(stream, l.plan_kernel, of_dkernel, to_dkernel)));
   }
+  return finish_all(stream, of_bias, dx != nullptr ? joined(l.plan, of_dx, to_dx) : Join<T>(),
+                    dkernel != nullptr ? joined(l.plan_kernel, of_dkernel, to_dkernel) : Join<T>());
 }
 
 }  // namespace

@@ -23,7 +23,8 @@ def linear(p):
 
     Sums: of K terms, at most K / 16 + 16 roundings one after another (the matrix instruction adds 16 terms at a time to
     what it is given, pieces of K are added up behind) of the sum of the terms' absolute values; floats are split in three
-    parts whose six products go through two such sums, and what is left out is below two more roundings.
+    parts whose six products go through two such sums, and what is left out is below two more roundings.  Few tiles of floats
+    go through the float instruction instead, whose four terms take at most four roundings, 32 terms at a time: within K / 32 + 32.
     act(pre): its slope is at most 1.13, and its own evaluation is off by at most 16 roundings of |pre| + |act(pre)| (exponentials of
     arguments of a few units, whose relative error is as many roundings).
     d = dy act'(pre): act'' is at most 0.8, so that it is off by 0.8 times the error of pre and 16 roundings; kept in half

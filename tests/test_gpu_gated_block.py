@@ -197,6 +197,16 @@ def test_linear_of_every_plan(R, C, D):
         compare_linear(run_linear(q.g), exact_linear(q))
 
 
+@pytest.mark.parametrize("R,C,D", [
+    (3001, 300, 1001), (64, 1024, 4100), (200, 1500, 1500),  # tiles of the float instruction, in pieces and whole, of odd rows
+    (70, 4096, 4096), (2048, 1030, 1024)])                  # on the other side
+def test_linear_of_every_plan_of_floats(R, C, D):
+    for activation in ("none", "gelu"):
+        print("floats", R, C, D, activation, flush=True)
+        q = linear_problem(R, torch.float32, (R,), C, D, activation)
+        compare_linear(run_linear(q.g), exact_linear(q))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=short)
 def test_linear_beyond_32_bits(dtype):
     """More than 2^31 outputs: the last rows and the last columns."""
