@@ -850,7 +850,7 @@ double step_cost(int element, int kind, int on_a_cu) { return element == 4 ? kFl
 // The cheapest of the tiles from `first` on and of 1 to 32 pieces by cost(kind, workgroups, k of a workgroup), beside which adding
 // pieces up takes 2500 ns, and writing and reading their elements at 4 TB/s.
 template <class Cost>
-Plan cheapest(int first, int M, int N, int K, Cost cost) {
+Plan cheapest(int cus, int first, int M, int N, int K, Cost cost) {
   Plan best = {};
   best.cost = 1e300;
   for (int kind = first; kind < kTiles; ++kind) {
@@ -860,7 +860,7 @@ Plan cheapest(int first, int M, int N, int K, Cost cost) {
     for (int s = 1; s <= 32; ++s) {
       int per = (K + s - 1) / s;
       per = (per + BK - 1) / BK * BK;
-      if (s > 1 && (per < 2 * BK || tiles * s > 2ll * kPerCu[kind] * cus())) break;
+      if (s > 1 && (per < 2 * BK || tiles * s > 2ll * kPerCu[kind] * cus)) break;
       if ((K + per - 1) / per != s) continue;
       const double here = cost(kind, tiles * s, per) + (s > 1 ? 2500 + (double)s * M * N * 8 / 4000 : 0.0);
       if (here < best.cost) best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0, here};
@@ -874,11 +874,11 @@ Plan cheapest(int first, int M, int N, int K, Cost cost) {
 // 128 x 128 51 / 48, in 8 of 256 x 256 63 / 51; 512 x 16384 x 512 in 16 of 128 x 128 24 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
 // 34, 48; 512 x 2048 x 2048 whole of 64 x 64 12 / 13 (before there were those: 20.7), 1024 x 1024 x 1024 7.8 / 8.6 (14.0), 512 x 512 x 512 5.7 / 5.7
 // (9.1), 2048 x 2048 x 2048 whole of 128 x 128 / 64 x 64 32 / 24, 29 / 29.
-Plan plan_product(int element, int M, int N, int K) {
-  return cheapest(element == 4 ? kNarrow : kLarge, M, N, K, [=](int kind, long long workgroups, int per) {
-    const long long slots = (long long)kPerCu[kind] * cus(), rounds = workgroups / slots, rest = workgroups % slots;
+Plan plan_product(int cus, int element, int M, int N, int K) {
+  return cheapest(cus, element == 4 ? kNarrow : kLarge, M, N, K, [=](int kind, long long workgroups, int per) {
+    const unsigned slots = (unsigned)(kPerCu[kind] * cus), all = (unsigned)workgroups, rounds = all / slots, rest = all % slots;
     return (double)rounds * (step_cost(element, kind, kPerCu[kind]) * per + kRound[kind]) +
-           (rest > 0 ? step_cost(element, kind, (int)((rest - 1) / cus()) + 1) * per + kRound[kind] : 0.0);
+           (rest > 0 ? step_cost(element, kind, (int)((rest - 1) / (unsigned)cus) + 1) * per + kRound[kind] : 0.0);
   });
 }
 
@@ -886,15 +886,15 @@ Plan plan_product(int element, int M, int N, int K) {
 // longest's time where that is more.  us, estimate / measured: both gradients of
 // 8192 x 1024 x 2048 with that of the kernel in 2 / 3 / 4 pieces 73 / 76, 78 / 80, 83 / 81 (by itself 4 would be best), of 4096 x 2048 x 1024 in 2 / 4
 // 45 / 45, 52 / 49.
-Plan plan_product_beside(int element, const Plan& other, int M, int N, int K) {
+Plan plan_product_beside(int cus, int element, const Plan& other, int M, int N, int K) {
   const double others = (double)other.tiles_m * other.tiles_n * other.pieces;
-  return cheapest(element == 4 ? kNarrow : kSmall, M, N, K, [&](int kind, long long workgroups, int per) {
+  return cheapest(cus, element == 4 ? kNarrow : kSmall, M, N, K, [&](int kind, long long workgroups, int per) {
     const int fit = kPerCu[kind] < kPerCu[other.kind] ? kPerCu[kind] : kPerCu[other.kind];
-    const double on_a_cu = (workgroups + others) / cus();
+    const double on_a_cu = (workgroups + others) / cus;
     const int here = on_a_cu < fit ? (int)std::ceil(on_a_cu) : fit;
     const double longest = step_cost(element, kind, here) * per + kRound[kind];
     const double shares = (workgroups * (step_cost(element, kind, fit) * per + kRound[kind]) +
-                           others * (step_cost(element, other.kind, fit) * other.k_per_piece + kRound[other.kind])) / ((double)fit * cus());
+                           others * (step_cost(element, other.kind, fit) * other.k_per_piece + kRound[other.kind])) / ((double)fit * cus);
     return shares > longest ? shares : longest;
   });
 }
@@ -1031,13 +1031,14 @@ double product_of_floats(int M, int R, int C, int D) { return (M < 80 ? 9500 + 8
 Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) {
   Layout l = {};
   if (!backward && few_rows(element, R, C)) return l;
-  l.plan = backward ? plan_product(element, R, C, D) : plan_product(element, R, D, C);
+  const int cus = haste_hip::cus();
+  l.plan = backward ? plan_product(cus, element, R, C, D) : plan_product(cus, element, R, D, C);
   double cost = l.plan.cost;
   if (backward) {
-    l.plan_kernel = plan_product(element, C, D, R);
+    l.plan_kernel = plan_product(cus, element, C, D, R);
     cost += l.plan_kernel.cost;
     if (l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) {
-      l.plan_kernel = plan_product_beside(element, l.plan, C, D, R);
+      l.plan_kernel = plan_product_beside(cus, element, l.plan, C, D, R);
       cost = l.plan_kernel.cost;
     }
   }
