@@ -778,8 +778,9 @@ __device__ __forceinline__ void join_pieces(const Join<T>& j, unsigned block) {
   }
 }
 
-// The gradient of the bias from what the workgroups of d left: 64 columns a workgroup, its four wavefronts a part of the rows each, sixteen
-// of them on their way.
+// The gradient of the bias from what the workgroups of d left: 16 columns a workgroup, whose 16 groups of lanes take the parts in turn, 16 of
+// them on their way.
+constexpr int kBiasColumns = 16;
 template <typename T>
 struct Bias {
   int parts, N;
@@ -789,22 +790,24 @@ struct Bias {
 };
 template <typename T>
 __device__ __forceinline__ void add_bias(const Bias<T>& b, unsigned block) {
-  __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = block * 64 + lane;
+  constexpr int GROUPS = 256 / kBiasColumns, AT_ONCE = 16;
+  __shared__ float red[GROUPS][kBiasColumns];
+  const int lane = threadIdx.x % kBiasColumns, group = threadIdx.x / kBiasColumns, col = block * kBiasColumns + lane;
   float sum = 0.f;
   if (col < b.N) {
-    constexpr int AT_ONCE = 16;
-    for (int p = wave; p < b.parts; p += AT_ONCE * 4) {
+    for (int p = group; p < b.parts; p += AT_ONCE * GROUPS) {
       float v[AT_ONCE];
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) v[i] = b.partial[(size_t)(p + 4 * i < b.parts ? p + 4 * i : p) * b.N + col];
+      for (int i = 0; i < AT_ONCE; ++i) v[i] = b.partial[(size_t)(p + GROUPS * i < b.parts ? p + GROUPS * i : p) * b.N + col];
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) sum += p + 4 * i < b.parts ? v[i] : 0.f;
+      for (int i = 0; i < AT_ONCE; ++i) sum += p + GROUPS * i < b.parts ? v[i] : 0.f;
     }
   }
-  red[wave][lane] = sum;
+  red[group][lane] = sum;
   __syncthreads();
-  if (wave == 0 && col < b.N) b.out[col] = (T)((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+  if (group != 0 || col >= b.N) return;
+  for (int g = 1; g < GROUPS; ++g) sum += red[g][lane];
+  b.out[col] = (T)sum;
 }
 
 template <typename T>
@@ -1162,7 +1165,7 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
     float* sums = dbias != nullptr ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
     slopes = {R, D, s.rows_each, dy, dy_row, act == kNone ? nullptr : static_cast<const typename Finish<T>::slope_t*>(cache),
               own ? reinterpret_cast<T*>(ws + l.d) : nullptr, d_row, sums, across, across * s.blocks};
-    if (dbias != nullptr) of_bias = {s.blocks, D, sums, dbias, (unsigned)((D + 63) / 64)};
+    if (dbias != nullptr) of_bias = {s.blocks, D, sums, dbias, (unsigned)((D + kBiasColumns - 1) / kBiasColumns)};
   }
   if constexpr (sizeof(T) == 4) {
     if (!l.tiles) {
