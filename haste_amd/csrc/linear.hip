@@ -263,7 +263,7 @@ struct Panel {
 
 template <int E, bool A_SLOW_, bool B_SLOW_, int BM_, int BN_, int WAVES_M_, int WAVES_N_, int STAGES_ = 2>
 struct Tile {
-  static constexpr int STAGES = STAGES_;
+  static constexpr int STAGES = STAGES_, ON_A_SIMD = STAGES == 2 ? 2 : 3;  // wavefronts that registers and LDS leave room for
   static constexpr bool A_SLOW = A_SLOW_, B_SLOW = B_SLOW_;
   static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, WAVES = WAVES_M * WAVES_N;
   static constexpr int MI = BM / WAVES_M / 16, NJ = BN / WAVES_N / 16;  // of 16 x 16 elements
@@ -455,7 +455,9 @@ __device__ __forceinline__ void multiply_tile(char* lds, const Product& p, const
   store_tile<T, G>(lds, p, to, acc, work.piece, work.m0, work.n0);
 }
 
-// Few tiles, of which each has its steps' latency to bear: STAGES of them in a ring, all but one on their way.
+// Few tiles, of which each has its steps' latency to bear: STAGES of them in a ring, all but one on their way, and three workgroups a CU. A
+// k of one takes 4.2 ns, of two on a CU 6.3, of three 8.4 (128 x 128: 9.0, of two 13.9).  Eight stages, which leave one a CU, 512 x 2048 x 2048 16.1
+// us instead of 13.1; operands read half a stage ahead 13.4.
 // Floats go through the float instruction, four k at a time, of which lane group q has 4 q + e at turn e; a stage's sum is added to what there
 // is as a whole, so that a sum of K is rounded K / 32 + 32 times.
 template <typename T, class G>
@@ -537,7 +539,7 @@ __device__ __forceinline__ void multiply(char* lds, const Product& p, const Fini
 }
 
 template <typename T, class G>
-__global__ __launch_bounds__(64 * G::WAVES, G::STAGES)
+__global__ __launch_bounds__(64 * G::WAVES, G::ON_A_SIMD)
 void linear_tile_kernel(Product p, Finish<T> to) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   multiply<T, G>(lds, p, to, blockIdx.x, gridDim.x);
@@ -820,14 +822,15 @@ void linear_finish_kernel(Bias<T> bias, Join<T> first, Join<T> second) {
   join_pieces(second, block - first.blocks);
 }
 
-// Two products that do not wait for one another, and the gradient of the bias ahead of them.  The workgroups [first, first + blocks)
+// Two products that do not wait for one another, and (of 256 threads) the gradient of the bias ahead of them.  The workgroups [first, first + blocks)
 // behind those are the first product's.
 template <typename T, class G, class H>
-__global__ __launch_bounds__(64 * G::WAVES, G::STAGES < H::STAGES ? G::STAGES : H::STAGES)
+__global__ __launch_bounds__(64 * G::WAVES, G::ON_A_SIMD < H::ON_A_SIMD ? G::ON_A_SIMD : H::ON_A_SIMD)
 void linear_gradients_kernel(Bias<T> bias, Product p, Finish<T> to, unsigned first, unsigned blocks, Product q, Finish<T> q_to) {
-  static_assert(G::WAVES == H::WAVES && 64 * G::WAVES == 256, "one shape of workgroups");
+  static_assert(G::WAVES == H::WAVES, "one shape of workgroups");
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds > H::kLds ? G::kLds : H::kLds];
-  if (blockIdx.x < bias.blocks) return add_bias(bias, blockIdx.x);
+  if constexpr (64 * G::WAVES == 256)
+    if (blockIdx.x < bias.blocks) return add_bias(bias, blockIdx.x);
   const unsigned block = blockIdx.x - bias.blocks, others = gridDim.x - bias.blocks - blocks;
   if (block - first < blocks) multiply<T, G>(lds, p, to, block - first, blocks);
   else multiply<T, H>(lds, q, q_to, block < first ? block : block - blocks, others);
@@ -850,13 +853,15 @@ constexpr double kStep[kTiles][3] = {{21.0}, {9.0, 13.9}, {4.2, 6.3, 8.4}}, kRou
 constexpr double kFloatStep[3] = {23.0, 38.0, 56.0};  // floats, 64 x 64
 double step_cost(int element, int kind, int on_a_cu) { return element == 4 ? kFloatStep[on_a_cu - 1] : kStep[kind][on_a_cu - 1]; }
 
-// The cheapest of the tiles from `first` on and of 1 to 32 pieces by cost(kind, workgroups, k of a workgroup), beside which adding
-// pieces up takes 2500 ns, and writing and reading their elements at 4 TB/s.
+// Adding pieces up, and writing and reading their elements at 4 TB/s.
+double join_cost(int pieces, int M, int N) { return pieces > 1 ? 2500 + (double)pieces * M * N * 8 / 4000 : 0.0; }
+
+// The cheapest of the tiles from `first` to `last` and of 1 to 32 pieces by cost(kind, workgroups, k of a workgroup), and its joins.
 template <class Cost>
-Plan cheapest(int cus, int first, int M, int N, int K, Cost cost) {
+Plan cheapest(int cus, int first, int last, int M, int N, int K, Cost cost) {
   Plan best = {};
   best.cost = 1e300;
-  for (int kind = first; kind < kTiles; ++kind) {
+  for (int kind = first; kind <= last; ++kind) {
     const int side = kSide[kind];
     const long long tm = ((long long)M + side - 1) / side, tn = ((long long)N + side - 1) / side, tiles = tm * tn;
     if (kind == kNarrow && tiles > (long long)kGridLimit) break;
@@ -865,7 +870,7 @@ Plan cheapest(int cus, int first, int M, int N, int K, Cost cost) {
       per = (per + BK - 1) / BK * BK;
       if (s > 1 && (per < 2 * BK || tiles * s > 2ll * kPerCu[kind] * cus)) break;
       if ((K + per - 1) / per != s) continue;
-      const double here = cost(kind, tiles * s, per) + (s > 1 ? 2500 + (double)s * M * N * 8 / 4000 : 0.0);
+      const double here = cost(kind, tiles * s, per) + join_cost(s, M, N);
       if (here < best.cost) best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0, here};
     }
   }
@@ -877,8 +882,8 @@ Plan cheapest(int cus, int first, int M, int N, int K, Cost cost) {
 // 128 x 128 51 / 48, in 8 of 256 x 256 63 / 51; 512 x 16384 x 512 in 16 of 128 x 128 24 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
 // 34, 48; 512 x 2048 x 2048 whole of 64 x 64 12 / 13 (before there were those: 20.7), 1024 x 1024 x 1024 7.8 / 8.6 (14.0), 512 x 512 x 512 5.7 / 5.7
 // (9.1), 2048 x 2048 x 2048 whole of 128 x 128 / 64 x 64 32 / 24, 29 / 29.
-Plan plan_product(int cus, int element, int M, int N, int K) {
-  return cheapest(cus, element == 4 ? kNarrow : kLarge, M, N, K, [=](int kind, long long workgroups, int per) {
+Plan plan_product(int cus, int element, int first, int last, int M, int N, int K) {
+  return cheapest(cus, first, last, M, N, K, [=](int kind, long long workgroups, int per) {
     const unsigned slots = (unsigned)(kPerCu[kind] * cus), all = (unsigned)workgroups, rounds = all / slots, rest = all % slots;
     return (double)rounds * (step_cost(element, kind, kPerCu[kind]) * per + kRound[kind]) +
            (rest > 0 ? step_cost(element, kind, (int)((rest - 1) / (unsigned)cus) + 1) * per + kRound[kind] : 0.0);
@@ -891,7 +896,7 @@ Plan plan_product(int cus, int element, int M, int N, int K) {
 // 45 / 45, 52 / 49.
 Plan plan_product_beside(int cus, int element, const Plan& other, int M, int N, int K) {
   const double others = (double)other.tiles_m * other.tiles_n * other.pieces;
-  return cheapest(cus, element == 4 ? kNarrow : kSmall, M, N, K, [&](int kind, long long workgroups, int per) {
+  return cheapest(cus, element == 4 ? kNarrow : kSmall, kNarrow, M, N, K, [&](int kind, long long workgroups, int per) {
     const int fit = kPerCu[kind] < kPerCu[other.kind] ? kPerCu[kind] : kPerCu[other.kind];
     const double on_a_cu = (workgroups + others) / cus;
     const int here = on_a_cu < fit ? (int)std::ceil(on_a_cu) : fit;
@@ -899,6 +904,27 @@ Plan plan_product_beside(int cus, int element, const Plan& other, int M, int N, 
     const double shares = (workgroups * (step_cost(element, kind, fit) * per + kRound[kind]) +
                            others * (step_cost(element, other.kind, fit) * other.k_per_piece + kRound[other.kind])) / ((double)fit * cus);
     return shares > longest ? shares : longest;
+  });
+}
+
+// The same with one of 256 x 256, of which a CU has one at a time: those that take longer come first, the others where there is room. us, both
+// gradients apart or of smaller tiles / so: 8192 x 2048 x 2048 149 / 128, 8192 x 1024 x 2048 78 / 72, 65536 x 512 x 512 105 / 95, 16384 x 4096 x 4096 817 / 802.
+Plan plan_large_beside(int cus, const Plan& other, int M, int N, int K) {
+  const long long others = (long long)other.tiles_m * other.tiles_n * other.pieces;
+  return cheapest(cus, kLarge, kLarge, M, N, K, [&](int, long long workgroups, int per) {
+    const bool longer = per > other.k_per_piece;
+    const double slow = kStep[kLarge][0] * (longer ? per : other.k_per_piece) + kRound[kLarge];
+    const double quick = kStep[kLarge][0] * (longer ? other.k_per_piece : per) + kRound[kLarge];
+    const long long first = longer ? workgroups : others, second = longer ? others : workgroups;
+    const long long rounds = first / cus, late = first % cus;  // CUs that have one more of the first
+    const auto room = [&](double until) {
+      const double early = std::floor((until - rounds * slow) / quick + 1e-6), there = std::floor((until - (rounds + 1) * slow) / quick + 1e-6);
+      return (early > 0 ? early : 0) * (double)(cus - late) + (there > 0 ? there : 0) * (double)late;
+    };
+    double low = (rounds + (late > 0)) * slow, high = low + ((double)second / cus + 1) * quick;
+    if (room(low) >= (double)second) return low;
+    for (int i = 0; i < 24; ++i) (room(0.5 * (low + high)) >= (double)second ? high : low) = 0.5 * (low + high);
+    return high;
   });
 }
 
@@ -966,7 +992,7 @@ int both_gradients(hipStream_t stream, const Bias<T>& bias, const Plan& plan, co
   ScopedKernelTimer timer("linear_product", stream);
   const unsigned blocks = workgroups(plan), others = workgroups(q_plan);
   const unsigned first = q_plan.k_per_piece > plan.k_per_piece ? others : 0;  // those that take longer start first
-  linear_gradients_kernel<T, G, H><<<bias.blocks + blocks + others, 256, 0, stream>>>(bias, p, to, first, blocks, q, q_to);
+  linear_gradients_kernel<T, G, H><<<bias.blocks + blocks + others, 64 * G::WAVES, 0, stream>>>(bias, p, to, first, blocks, q, q_to);
   HASTE_HIP_TRY(hipGetLastError());
   return HASTE_HIP_OK;
 }
@@ -1014,6 +1040,7 @@ SumPlan plan_sums(int rows, int columns) {
 struct Layout {
   size_t x, kernel, d, sums, product, product_kernel, total;
   bool tiles;              // otherwise the products are those of gemm.hip
+  bool together;           // both gradients in one launch
   Plan plan, plan_kernel;  // of the product forward, or of dx and dkernel
 };
 
@@ -1034,15 +1061,25 @@ double product_of_floats(int M, int R, int C, int D) { return (M < 80 ? 9500 + 8
 Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) {
   Layout l = {};
   if (!backward && few_rows(element, R, C)) return l;
-  const int cus = haste_hip::cus();
-  l.plan = backward ? plan_product(cus, element, R, C, D) : plan_product(cus, element, R, D, C);
-  double cost = l.plan.cost;
-  if (backward) {
-    l.plan_kernel = plan_product(cus, element, C, D, R);
-    cost += l.plan_kernel.cost;
-    if (l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) {
-      l.plan_kernel = plan_product_beside(cus, element, l.plan, C, D, R);
-      cost = l.plan_kernel.cost;
+  const int cus = haste_hip::cus(), first = element == 4 ? kNarrow : kLarge;
+  double cost;
+  if (!backward) {
+    l.plan = plan_product(cus, element, first, kNarrow, R, D, C);
+    cost = l.plan.cost;
+  } else {
+    l.plan = plan_product(cus, element, first, kNarrow, R, C, D);
+    l.plan_kernel = plan_product(cus, element, first, kNarrow, C, D, R);
+    cost = l.plan.cost + l.plan_kernel.cost;
+    const auto consider = [&](const Plan& plan, const Plan& plan_kernel) {  // in one launch
+      const double here = plan_kernel.cost + join_cost(plan.pieces, R, C);
+      if (here < cost) l.plan = plan, l.plan_kernel = plan_kernel, cost = here, l.together = true;
+    };
+    const Plan small = l.plan.kind >= kSmall ? l.plan : plan_product(cus, element, kSmall, kNarrow, R, C, D);
+    if (small.cost < 1e300) consider(small, plan_product_beside(cus, element, small, C, D, R));
+    if (element == 2) {
+      Plan whole = plan_product(cus, element, kLarge, kLarge, R, C, D);
+      whole.pieces = 1, whole.k_per_piece = (D + BK - 1) / BK * BK, whole.floats = 0;
+      consider(whole, plan_large_beside(cus, whole, C, D, R));
     }
   }
   l.tiles = element == 2 || cost < product_of_floats(R, R, C, D) + (backward ? product_of_floats(C, R, C, D) : 0.0);
@@ -1192,21 +1229,26 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
   const Product of_dkernel = product_of(l.plan_kernel, C, D, R, x, x_row, d, d_row, ws + l.product_kernel);
   typedef Tiles<sizeof(T), false, false> tiles_dx;
   typedef Tiles<sizeof(T), true, true> tiles_dkernel;
-  if (dx != nullptr && dkernel != nullptr && l.plan.kind != kLarge && l.plan_kernel.kind != kLarge) {
+  if (dx != nullptr && dkernel != nullptr && l.together) {
     const auto run = [&](auto of_first, auto of_second) {
-      return both_gradients<T, decltype(of_first), decltype(of_second)>(stream, of_bias, l.plan, of_dx, to_dx, l.plan_kernel, of_dkernel, to_dkernel);
+      typedef decltype(of_first) first_t;
+      const bool with_bias = 64 * first_t::WAVES == 256;
+      HASTE_HIP_PROPAGATE((both_gradients<T, first_t, decltype(of_second)>(stream, with_bias ? of_bias : Bias<T>(), l.plan, of_dx, to_dx, l.plan_kernel,
+                                                                          of_dkernel, to_dkernel)));
+      if (with_bias) of_bias.blocks = 0;
+      return HASTE_HIP_OK;
     };
     const typename tiles_dx::narrow narrow_dx;
     const typename tiles_dkernel::narrow narrow_dkernel;
     if constexpr (sizeof(T) == 2) {
       const typename tiles_dx::small small_dx;
       const typename tiles_dkernel::small small_dkernel;
-      if (l.plan.kind == kSmall) HASTE_HIP_PROPAGATE(l.plan_kernel.kind == kSmall ? run(small_dx, small_dkernel) : run(small_dx, narrow_dkernel));
+      if (l.plan.kind == kLarge) HASTE_HIP_PROPAGATE(run(typename tiles_dx::large(), typename tiles_dkernel::large()));
+      else if (l.plan.kind == kSmall) HASTE_HIP_PROPAGATE(l.plan_kernel.kind == kSmall ? run(small_dx, small_dkernel) : run(small_dx, narrow_dkernel));
       else HASTE_HIP_PROPAGATE(l.plan_kernel.kind == kSmall ? run(narrow_dx, small_dkernel) : run(narrow_dx, narrow_dkernel));
     } else {
       HASTE_HIP_PROPAGATE(run(narrow_dx, narrow_dkernel));
     }
-    of_bias.blocks = 0;
   } else {
     if (dx != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dx>(stream, l.plan, of_dx, to_dx)));
     if (dkernel != nullptr) HASTE_HIP_PROPAGATE((multiply<T, tiles_dkernel>(stream, l.plan_kernel, of_dkernel, to_dkernel)));
