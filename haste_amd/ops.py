@@ -1016,10 +1016,17 @@ def _linear_arguments(x, kernel, bias, activation):
     return (x.numel() // C, C, D), rows, step, _contiguous(kernel), _contiguous(bias), number, device, suffix
 
 
+def _scratch_of(size, like):
+    """(memory, its address, size); many calls need none (1 us of a short one's 10)."""
+    if not size:
+        return None, None, 0
+    scratch = torch.empty(size, device=like.device, dtype=torch.uint8)
+    return scratch, scratch.data_ptr(), size
+
+
 def _linear_scratch(backward, x, sizes, rows, step, kernel):
     aligned = not (rows.data_ptr() | kernel.data_ptr()) & 15 and not step & 7
-    size = _scratch_bytes("haste_hip_linear_workspace_bytes", x.device, backward, x.element_size(), *sizes, int(aligned))
-    return torch.empty(max(1, size), device=x.device, dtype=torch.uint8)
+    return _scratch_of(_scratch_bytes("haste_hip_linear_workspace_bytes", x.device, backward, x.element_size(), *sizes, int(aligned)), x)
 
 
 def linear_forward(training, x, kernel, bias=None, activation="none", residual=None):
@@ -1034,10 +1041,10 @@ def linear_forward(training, x, kernel, bias=None, activation="none", residual=N
     y, cache = x.new_empty(shape), None
     if training and number:
         cache = torch.empty(shape, device=x.device, dtype=torch.float32 if x.dtype is torch.float32 else torch.float16)
-    scratch = _linear_scratch(0, x, sizes, rows, step, kernel)
+    scratch, address, size = _linear_scratch(0, x, sizes, rows, step, kernel)
     _invoke(device, "haste_hip_linear_forward" + suffix,
             [*sizes, rows.data_ptr(), step, kernel.data_ptr(), _address(bias), number, _address(residual), residual_step, y.data_ptr(),
-             _address(cache), scratch.data_ptr(), scratch.numel()])
+             _address(cache), address, size])
     return y, cache
 
 
@@ -1057,10 +1064,10 @@ def linear_backward(x, kernel, bias, activation, cache, dy, with_dx=True, with_d
     dx = x.new_empty(x.shape) if with_dx else None
     dkernel = torch.empty_like(kernel) if with_dkernel else None
     dbias = None if bias is None else torch.empty_like(bias)
-    scratch = _linear_scratch(1, x, sizes, rows, step, kernel)
+    scratch, address, size = _linear_scratch(1, x, sizes, rows, step, kernel)
     _invoke(device, "haste_hip_linear_backward" + suffix,
             [*sizes, rows.data_ptr(), step, kernel.data_ptr(), number, _address(cache), dy.data_ptr(), dy_step, _address(dx),
-             _address(dkernel), _address(dbias), scratch.data_ptr(), scratch.numel()])
+             _address(dkernel), _address(dbias), address, size])
     return dx, dkernel, dbias
 
 
@@ -1108,10 +1115,9 @@ def gated_recurrence_forward(training, x, forget, admit=None, z=None, decay=None
         _check_lengths(lengths, x)
     y, h_last = x.new_empty(x.shape), torch.empty((N, D), device=x.device)
     cache = _scratch("haste_hip_gated_recurrence_kept_bytes", x, T, N, D) if training else None
-    scratch = _scratch("haste_hip_gated_recurrence_workspace_bytes", x, 0, T, N, D)
+    scratch, address, size = _scratch_of(_scratch_bytes("haste_hip_gated_recurrence_workspace_bytes", x.device, 0, T, N, D), x)
     _invoke(device, "haste_hip_gated_recurrence_forward" + suffix,
-            [T, N, D, *values, _address(h0), _address(lengths), y.data_ptr(), h_last.data_ptr(), _address(cache), scratch.data_ptr(),
-             scratch.numel()])
+            [T, N, D, *values, _address(h0), _address(lengths), y.data_ptr(), h_last.data_ptr(), _address(cache), address, size])
     return y, h_last, cache
 
 
