@@ -419,6 +419,20 @@ def test_gated_extreme_gates():
     assert got["y"].isfinite().all() and got["dx"].isfinite().all() and got["h_last"].isfinite().all()
 
 
+def test_gated_roundings_even_out():
+    """Gates a little below 1 that multiply a state for hundreds of steps.  Each is rounded once and the product once, by a relative 2^-24 at
+    most either way: a spread of sqrt(2 / 3) 2^-24 a step, of which sqrt(T) add up and sqrt(n) even out in the mean of n channels; what
+    is not even-handed, two instructions' last bits, is in 1 - gate alone."""
+    T, N, D = 470, 4, 1024
+    q = Problem(13, torch.float32)
+    q.put("forget", torch.empty(T, N, D, dtype=torch.float64).uniform_(5, 9, generator=q.gen))
+    _, h, _ = ops.gated_recurrence_forward(False, torch.zeros(T, N, D, device="cuda"), q.g["forget"], h0=torch.ones(N, D, device="cuda"))
+    exact = torch.sigmoid(q.p["forget"]).prod(0)
+    mean = float((h.cpu().double() / exact - 1).mean())
+    bound = 6 * (T * 2 / 3) ** 0.5 * 2.0 ** -24 / (N * D) ** 0.5 + T * float(torch.sigmoid(-q.p["forget"]).mean()) * 2.0 ** -22
+    assert abs(mean) <= bound, (mean, bound)
+
+
 def test_gated_keeps_bad_values_to_their_channels():
     for T in (150, 900):
         q = gated_problem(3, torch.float32, T, 3, 40)
