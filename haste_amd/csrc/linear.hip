@@ -5,8 +5,9 @@
 // Half types (f16, bf16).  Bound: the matrix cores (2 R C D flops, dense peak 2.5 PFLOP/s); below some hundred rows the bytes
 // of W.  Products of the matrix cores are exact, sums are float from the first to the last; an output is rounded once.  d is rounded to
 // the activations' type, the matrix cores take no other: what it costs is a rounding of each term of sums that are rounded
-// to that type themselves.  act'(pre) is what the forward pass leaves for the backward pass, in half: it lies between -0.2 and 1.2,
-// where half is eight times as fine as bfloat16, and a float would be as many bytes again as y.
+// to that type themselves.  act'(pre) is what the forward pass leaves for the backward pass, beside bf16 in half: it lies between -0.2 and
+// 1.2, where half is eight times as fine as bfloat16, and a float would be as many bytes again as y.  Beside f16 it is a float: rounded to
+// half it would cost as much precision as d (dx and dW 2.9e-4 off by the 2-norm instead of 3.7e-4, where 2.1e-4 is the results' own rounding).
 //
 // One tile kernel makes all three products.  An operand is either stored with the contraction index contiguous (x and d in
 // x W and d W^T, W in d W^T) or with it as the slow index (W in x W, x and d in x^T d).  Tiles go from memory straight into LDS
@@ -83,7 +84,7 @@ __device__ __forceinline__ float activated(int act, float v, float& slope) {
 // What becomes of a product's elements.
 template <typename T>
 struct Finish {
-  typedef typename std::conditional<sizeof(T) == 4, float, _Float16>::type slope_t;
+  typedef typename std::conditional<std::is_same<T, __bf16>::value, _Float16, float>::type slope_t;
   T* out;
   size_t ld;
   int act;

@@ -1040,7 +1040,7 @@ def linear_forward(training, x, kernel, bias=None, activation="none", residual=N
         residual, residual_step = _linear_rows(residual)
     y, cache = x.new_empty(shape), None
     if training and number:
-        cache = torch.empty(shape, device=x.device, dtype=torch.float32 if x.dtype is torch.float32 else torch.float16)
+        cache = torch.empty(shape, device=x.device, dtype=torch.float16 if x.dtype is torch.bfloat16 else torch.float32)
     scratch, address, size = _linear_scratch(0, x, sizes, rows, step, kernel)
     _invoke(device, "haste_hip_linear_forward" + suffix,
             [*sizes, rows.data_ptr(), step, kernel.data_ptr(), _address(bias), number, _address(residual), residual_step, y.data_ptr(),
@@ -1055,7 +1055,7 @@ def linear_backward(x, kernel, bias, activation, cache, dy, with_dx=True, with_d
     shape = (*x.shape[:-1], sizes[2])
     _activation("dy", dy, shape, x)
     if number:
-        kept = torch.float32 if x.dtype is torch.float32 else torch.float16
+        kept = torch.float16 if x.dtype is torch.bfloat16 else torch.float32
         if not _is(cache, shape, kept, device) or not cache.is_contiguous():
             raise ValueError("the cache must be that of a forward pass in training over the same arguments")
     else:

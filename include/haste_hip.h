@@ -806,8 +806,8 @@ int haste_hip_residual_norm_backward_bf16(int steps, int batch_size, int channel
  *
  * Projection: y = act(x W + bias) + residual; x[R,C] (rows `x_row` elements apart, at least C), W[C,D], bias[D],
  * residual, y[R,D] all of one type; activation 0: none, 1: gelu (v times the normal distribution function), 2: silu
- * (v sigmoid(v)); bias, residual may be NULL.  cache: what the backward pass needs of an activation, [R,D] in float (_f32)
- * or half (_f16, _bf16), or NULL; without an activation there is none.  Backward: dx[R,C], dW[C,D], dbias[D] from
+ * (v sigmoid(v)); bias, residual may be NULL.  cache: what the backward pass needs of an activation, [R,D] in float (_f32,
+ * _f16) or half (_bf16), or NULL; without an activation there is none.  Backward: dx[R,C], dW[C,D], dbias[D] from
  * dy[R,D], which is the residual's gradient too; each may be NULL (not wanted).  Workspace: aligned to 16 bytes; `aligned`
  * says that x and W start at, and rows of x are, multiples of 16 bytes. */
 size_t haste_hip_linear_workspace_bytes(int backward, int element_bytes, int rows, int inputs, int outputs,

@@ -28,7 +28,7 @@ def linear(p):
     act(pre): its slope is at most 1.13, and its own evaluation is off by at most 16 roundings of |pre| + |act(pre)| (exponentials of
     arguments of a few units, whose relative error is as many roundings).
     d = dy act'(pre): act'' is at most 0.8, so that it is off by 0.8 times the error of pre and 16 roundings; kept in half
-    and d itself in the type of x (no half, no rounding, for float and without an activation)."""
+    (beside bfloat16; a float otherwise) and d itself in the type of x (no half, no rounding, for float and without an activation)."""
     x, W, bias, residual, dy, kind = (p[k] for k in ("x", "kernel", "bias", "residual", "dy", "activation"))
     dtype = p["dtype"]
     x, dy, shape = x.flatten(0, -2), dy.flatten(0, -2), (*x.shape[:-1], W.shape[1])
