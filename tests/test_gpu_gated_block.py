@@ -189,6 +189,7 @@ def test_linear_of_few_rows_and_more(dtype):
     (20000, 64, 72),      # small tiles, whole and in many pieces
     (300, 6000, 4200),    # dx in pieces, dkernel whole
     (9000, 520, 1030),    # odd rows, both gradients in small tiles
+    (8192, 1024, 2048), (8200, 2051, 2050),  # both in large tiles in one launch
     (4096, 4096, 1024), (1100, 4104, 4104)])
 def test_linear_of_every_plan(R, C, D):
     for activation in ("none", "silu"):
