@@ -281,8 +281,9 @@ struct Product {
   const void *A, *B;
   long long lda, ldb;
   int tiles_m, tiles_n, k_per_piece;  // tiles whole, or cut along K
-  float* partial;                     // [piece][M][N], null: whole
+  float* partial;                     // [piece][M][N to whole eights], null: whole
 };
+__host__ __device__ constexpr long long eights(long long n) { return (n + 7) / 8 * 8; }
 
 // Workgroups go to the XCDs in turn; each XCD is given a range of a product's work.
 __device__ __forceinline__ unsigned work_of_xcd(unsigned block, unsigned blocks) {
@@ -321,7 +322,7 @@ __device__ __forceinline__ void store_tile(char* lds, const Product& p, const Fi
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = slab[in_slab * G::kSlabLd + lane % LANES * 8 + e];
       if (row < p.M) {
-        if (p.partial != nullptr) store_channels<8>(p.partial + ((size_t)piece * p.M + row) * p.N, col, p.N, v);
+        if (p.partial != nullptr) store_channels<8>(p.partial + ((size_t)piece * p.M + row) * eights(p.N), col, (int)eights(p.N), v);
         else finish(to, v, bias, row, col, p.N);
       }
     }
@@ -753,6 +754,10 @@ struct Join {
   Finish<T> to;
   unsigned blocks;  // 0: none
 };
+__device__ __forceinline__ void load_floats(const float* from, float (&v)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) *reinterpret_cast<float4_t*>(v + 4 * h) = *reinterpret_cast<const float4_t*>(from + 4 * h);
+}
 template <typename T>
 __device__ __forceinline__ void join_pieces(const Join<T>& j, unsigned block) {
   const unsigned groups = (j.N + 7) / 8;
@@ -764,13 +769,15 @@ __device__ __forceinline__ void join_pieces(const Join<T>& j, unsigned block) {
     if (j.partial == nullptr) {
       load_channels<8>(j.to.out + row * j.to.ld, col, j.N, v);
     } else {
-      load_channels<8>(j.partial + row * j.N, col, j.N, v);
-      constexpr int AT_ONCE = 4;
+      const size_t piece = (size_t)j.M * groups * 8;
+      const float* from = j.partial + i * 8;
+      load_floats(from, v);
+      constexpr int AT_ONCE = 8;
       for (int z = 1; z < j.pieces; z += AT_ONCE) {
         float w[AT_ONCE][8];
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k)  // beyond the last piece it once more, not added
-          load_channels<8>(j.partial + ((size_t)(z + k < j.pieces ? z + k : j.pieces - 1) * j.M + row) * j.N, col, j.N, w[k]);
+          load_floats(from + (z + k < j.pieces ? z + k : j.pieces - 1) * piece, w[k]);
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k)
 #pragma unroll
@@ -872,7 +879,7 @@ Plan cheapest(int cus, int first, int last, int M, int N, int K, Cost cost) {
       if (s > 1 && (per < 2 * BK || tiles * s > 2ll * kPerCu[kind] * cus)) break;
       if ((K + per - 1) / per != s) continue;
       const double here = cost(kind, tiles * s, per) + join_cost(s, M, N);
-      if (here < best.cost) best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * N : 0, here};
+      if (here < best.cost) best = {kind, (int)tm, (int)tn, s, per, s > 1 ? (size_t)s * M * eights(N) : 0, here};
     }
   }
   return best;
@@ -1019,8 +1026,6 @@ int finish_all(hipStream_t stream, const Bias<T>& bias, const Join<T>& first, co
 }
 
 size_t whole(size_t bytes) { return (bytes + 255) / 256 * 256; }
-long long eights(long long n) { return (n + 7) / 8 * 8; }
-
 struct SumPlan {
   int blocks, rows_each;
   size_t floats;
