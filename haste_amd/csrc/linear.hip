@@ -746,7 +746,7 @@ void linear_prepare_kernel(Slopes<T> slopes, Copy<T> first, Copy<T> second) {
   make_copy(second, block - first.blocks);
 }
 
-// The pieces of a product, added in order, and what follows.  Bound: HBM; 8 pieces of 128 x 4096 4.7 us.  No pieces: the elements lie in `to.out` already (float).
+// The pieces of a product, added in order, and what follows.  Bound: HBM; 2 pieces of 128 x 4096 4.2 us.  No pieces: the elements lie in `to.out` already (float).
 template <typename T>
 struct Join {
   int M, N, pieces;
@@ -861,8 +861,9 @@ constexpr double kStep[kTiles][3] = {{21.0}, {9.0, 13.9}, {4.2, 6.3, 8.4}}, kRou
 constexpr double kFloatStep[3] = {23.0, 38.0, 56.0};  // floats, 64 x 64
 double step_cost(int element, int kind, int on_a_cu) { return element == 4 ? kFloatStep[on_a_cu - 1] : kStep[kind][on_a_cu - 1]; }
 
-// Adding pieces up, and writing and reading their elements at 4 TB/s.
-double join_cost(int pieces, int M, int N) { return pieces > 1 ? 2500 + (double)pieces * M * N * 8 / 4000 : 0.0; }
+// Adding pieces up, 2500 ns and 1000 for a launch more, which the host bears; and writing and reading their elements at 4 TB/s. (The estimates
+// below are without the 1000.)
+double join_cost(int pieces, int M, int N) { return pieces > 1 ? 3500 + (double)pieces * M * N * 8 / 4000 : 0.0; }
 
 // The cheapest of the tiles from `first` to `last` and of 1 to 32 pieces by cost(kind, workgroups, k of a workgroup), and its joins.
 template <class Cost>
