@@ -722,7 +722,9 @@ int gemm_f32_once(hipStream_t stream, bool trans_a, int M, int N, int K,
 // B, all of K) with 32-bit byte offsets, so a panel must stay under 2 GiB.  A longer
 // contraction -- the dW and dR products of a backward pass contract over T*N with rows of 4H
 // floats, 2 GiB from T*N*H = 2^27 on -- is cut into runs of K that fit, each accumulating into
-// C; where the cuts fall depends on the shape only.
+// C; where the cuts fall depends on the shape and the leading dimensions only.  Runs are multiples
+// of 1024, or of a stage where rows are so long (2^19 floats and more) that 1024 do not fit: those up to
+// 2^22 floats apart run, 127 of them to a panel.
 int gemm_f32(hipStream_t stream, bool trans_a, int M, int N, int K,
              const float* A, int lda, const float* B, int ldb,
              float* C, int ldc, bool accumulate, size_t scratch_offset) {
@@ -734,14 +736,14 @@ int gemm_f32(hipStream_t stream, bool trans_a, int M, int N, int K,
   if (trans_a) {
     const long long a_run = (limit - 128) / lda;
     run = a_run < run ? a_run : run;
-  } else if (128ll * lda + K >= limit) {
-    run = 0;  // 128 rows of A alone exceed the limit
+  } else if (127ll * lda + K >= limit) {
+    run = 0;  // a tile's 128 rows of A alone exceed the limit
   }
   if (run >= K) return gemm_f32_once(stream, trans_a, M, N, K, A, lda, B, ldb, C, ldc, accumulate, scratch_offset);
-  run = run / 1024 * 1024;
+  run = run >= 1024 ? run / 1024 * 1024 : run / SK * SK;
   if (run <= 0) {
     set_error_text("gemm: a row of an operand is too long for the kernel's 32-bit panel offsets "
-                   "(leading dimension of 2^19 floats or more per 1024 rows)");
+                   "(leading dimension of more than 2^22 floats)");
     return HASTE_HIP_ERROR_UNSUPPORTED_SIZE;
   }
   for (long long k0 = 0; k0 < K; k0 += run) {
@@ -778,7 +780,7 @@ int gemm_f32_once(hipStream_t stream, bool trans_a, int M, int N, int K,
   }
   // A workgroup addresses its operand panels (its rows of A, its columns of B, all of K)
   // with 32-bit byte offsets.
-  HASTE_HIP_REQUIRE(((long long)(trans_a ? K : bm) * lda + (trans_a ? bm : K)) * 4 < (1ll << 31));
+  HASTE_HIP_REQUIRE(((long long)(trans_a ? K : bm - 1) * lda + (trans_a ? bm : K)) * 4 < (1ll << 31));
   HASTE_HIP_REQUIRE(((long long)K * ldb + BN) * 4 < (1ll << 31));
   if (planned_pass() != nullptr) return HASTE_HIP_OK;
   dim3 grid((unsigned)(whole_tiles + pieces)), block(256);

@@ -1,0 +1,53 @@
+"""Which sizes and rows the operators of a gated linear recurrent block take, without a GPU: a call that is taken gets as far as its
+first launch, which finds no device."""
+import ctypes
+
+import pytest
+import torch
+
+from haste_amd import lib
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="calls with addresses of nothing, for machines on which nothing is launched")
+INVALID, UNSUPPORTED, RUNTIME = 1, 2, 3
+
+
+def _bytes(name, *sizes):
+    fn = lib.load()[name]
+    fn.restype, fn.argtypes = ctypes.c_size_t, [ctypes.c_int] * len(sizes)
+    return fn(*sizes)
+
+
+def _forward(sfx, R, C, D, x_row=None, x=2 ** 12, kernel=2 ** 13, workspace=2 ** 14, size=None):
+    """The code of a projection whose caller has as much scratch memory as is said to be needed (or `size` bytes)."""
+    size = _bytes("haste_hip_linear_workspace_bytes", 0, 4 if sfx == "_f32" else 2, R, C, D, 1) if size is None else size
+    return lib.entry("haste_hip_linear_forward" + sfx)(R, C, D, x, x_row or C, kernel, None, 0, None, 0, 2 ** 15, None, workspace, size, None)
+
+
+def _backward(sfx, R, C, D, x_row=None, dy_row=None, dx=2 ** 15, dkernel=2 ** 16, size=None):
+    size = _bytes("haste_hip_linear_workspace_bytes", 1, 4 if sfx == "_f32" else 2, R, C, D, 1) if size is None else size
+    return lib.entry("haste_hip_linear_backward" + sfx)(R, C, D, 2 ** 12, x_row or C, 2 ** 13, 0, None, 2 ** 17, dy_row or D, dx, dkernel, None,
+                                                        2 ** 14, size, None)
+
+
+# ---- rows far apart, and long ones ----------------------------------------------------
+@pytest.mark.parametrize("sfx", ["_f32", "_bf16"])
+def test_long_rows_are_taken(sfx):
+    """2^20 columns and rows 2^22 elements apart, whichever kernel a product goes by."""
+    for sizes in (dict(R=2048, C=1024, D=600000), dict(R=2048, C=1024, D=4096, x_row=2 ** 22), dict(R=200, C=4096, D=4096, x_row=2 ** 22),
+                  dict(R=2048, C=4096, D=2 ** 20), dict(R=2048, C=2 ** 20, D=1024, x_row=2 ** 22)):
+        assert _forward(sfx, **sizes) == RUNTIME, sizes
+    for sizes in (dict(R=2048, C=1024, D=600000), dict(R=2048, C=600000, D=1024), dict(R=2048, C=1024, D=4096, x_row=600000),
+                  dict(R=4096, C=1024, D=4096, dy_row=600000), dict(R=200, C=4096, D=4096, x_row=4096000),
+                  dict(R=2048, C=2 ** 20, D=1024, x_row=2 ** 22, dy_row=2 ** 22), dict(R=157, C=4096, D=4096, x_row=3000000)):
+        assert _backward(sfx, **sizes, dx=None) == RUNTIME, sizes
+        assert _backward(sfx, **sizes, dkernel=None) == RUNTIME, sizes
+
+
+def test_products_of_long_rows_are_taken():
+    """The float product by itself: short runs of a contraction, tiles whose rows are 2^22 apart."""
+    product = lib.entry("haste_hip_gemm_f32")
+    for trans_a, M, N, K, lda, ldb in ((0, 2048, 600000, 1024, 1024, 600000), (0, 2048, 4096, 1024, 2 ** 22, 4096), (0, 300, 2 ** 20, 4096, 4096, 2 ** 20),
+                                       (0, 128, 128, 2 ** 20, 2 ** 22, 128), (1, 1024, 4096, 200, 2 ** 22, 4096),
+                                       (1, 1024, 4096, 100000, 1024, 2 ** 22), (1, 600000, 64, 2048, 600000, 64)):
+        assert product(trans_a, M, N, K, 2 ** 12, lda, 2 ** 13, ldb, 2 ** 15, N, 0, None) == RUNTIME, (trans_a, M, N, K, lda, ldb)
+    assert product(0, 128, 128, 2 ** 20, 2 ** 12, 2 ** 22 + 2 ** 20, 2 ** 13, 128, 2 ** 15, 128, 0, None) == UNSUPPORTED

@@ -1,0 +1,47 @@
+"""Sizes, rows and values at which the operators of a gated linear recurrent block could go wrong, on the GPU against the formulas in
+float64 (gated_block_formulas.py), bounded as derived there."""
+import pytest
+import torch
+
+import gated_block_formulas as formulas
+from test_gpu_gated_block import compare_linear, exact_linear, linear_problem, run_linear
+
+pytestmark = pytest.mark.gpu
+
+
+def _far(t, distance, memory):
+    """The rows of t, `distance` elements apart."""
+    rows = memory.as_strided(t.shape, (distance, 1))
+    return rows.copy_(t)
+
+
+@pytest.mark.parametrize("R,C,D", [(200, 1028, 4096), (129, 4096, 4096)])
+def test_floats_of_rows_far_apart(R, C, D):
+    """The last steps of long sequences, one behind the other: the products' contractions over rows are cut into short runs.  Sums of
+    runs are added as pieces are, a rounding for 32 terms or more: the bound has room for one for 16 in each of two sums."""
+    distance = 2 ** 22
+    memory = torch.empty(R * distance, device="cuda")
+    q = linear_problem(R, torch.float32, (R,), C, D, "silu")
+    want = exact_linear(q)
+    for name in ("x", "residual", "dy"):
+        print("far", R, C, D, name, flush=True)
+        compare_linear(run_linear(dict(q.g, **{name: _far(q.g[name], distance, memory)})), want)
+
+
+@pytest.mark.parametrize("R,C,D", [(300, 1000, 600000), (1000, 600000, 64)])
+def test_floats_of_long_rows(R, C, D):
+    """More than 2^19 columns on either side of the kernel, where a contraction of the other two sizes is cut: the last columns of each."""
+    print("long", R, C, D, flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    normal = lambda *shape: torch.randn(*shape, generator=gen, device="cuda")  # noqa: E731
+    g = dict(x=normal(R, C), kernel=normal(C, D) * C ** -0.5, bias=normal(D), residual=None, dy=normal(R, D), activation="none")
+    got = run_linear(g)
+    part = lambda **cut: {"dtype": torch.float32, "activation": "none", "residual": None,  # noqa: E731
+                          **{k: g[k].double() if i is None else g[k][i].double() for k, i in cut.items()}}
+    last = (slice(None), slice(-24, None))
+    want = formulas.linear(part(x=None, kernel=last, bias=slice(-24, None), dy=last))  # all inputs, the last outputs
+    for k, at in (("y", last), ("dkernel", last), ("dbias", slice(-24, None))):
+        formulas.check_error(got[k][at], *want[k], k)
+    want = formulas.linear(part(x=last, kernel=slice(-24, None), bias=None, dy=None))  # the last inputs, all outputs
+    formulas.check_error(got["dx"][last], *want["dx"], "dx")
+    formulas.check_error(got["dkernel"][-24:], *want["dkernel"], "dkernel")
