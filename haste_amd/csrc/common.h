@@ -237,6 +237,8 @@ int gemm_f32_pieces(hipStream_t stream, int M, int N, int K, const float* A, int
 
 // Bytes of scratch gemm_f32 may use for this shape (0 when nothing is split).
 size_t gemm_f32_scratch_bytes(int M, int N, int K);
+// At least that, also where a contraction of K is cut into runs (rows of the operands far apart).
+size_t gemm_f32_scratch_bound(int M, int N, int K);
 
 // The product for M <= 128 with B streamed from HBM straight into the MFMA operands
 // (gemm_skinny.hip); gemm_f32 hands such shapes over when the operands are 16-byte aligned.
@@ -244,6 +246,7 @@ bool gemm_f32_skinny_shape(bool trans_a, int M, int N, int K);
 bool gemm_f32_skinny_applies(bool trans_a, int M, int N, int K, const float* A, int lda,
                              const float* B, int ldb, const float* C, int ldc);
 size_t gemm_f32_skinny_scratch_bytes(int M, int N, int K);
+size_t gemm_f32_skinny_scratch_bound(int M, int N, int K);
 int gemm_f32_skinny(hipStream_t stream, int M, int N, int K, const float* A, int lda,
                     const float* B, int ldb, float* C, int ldc, bool accumulate,
                     size_t scratch_offset);

@@ -712,6 +712,18 @@ size_t gemm_f32_scratch_bytes(int M, int N, int K) {
   return tiled > skinny ? tiled : skinny;
 }
 
+// Whatever runs gemm_f32() cuts a contraction of K into: that depends on the leading dimensions, and a shorter run may want more
+// pieces (of which plan_gemm() makes at most one for 64 k, 64, and four a CU together).
+size_t gemm_f32_scratch_bound(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const GemmPlan g = plan_gemm(M, N, K);
+  const long long each = g.rest > 0 ? 4LL * (device_cu_count() > 0 ? device_cu_count() : 256) / g.rest : 0;
+  const long long splits = each < K / 64 ? (each < 64 ? each : 64) : (K / 64 < 64 ? K / 64 : 64);
+  const size_t tiled = splits > 1 ? (size_t)g.rest * splits * g.bm * BN * sizeof(float) : 0;
+  const size_t skinny = gemm_f32_skinny_scratch_bound(M, N, K);
+  return tiled > skinny ? tiled : skinny;
+}
+
 namespace {
 int gemm_f32_once(hipStream_t stream, bool trans_a, int M, int N, int K,
                   const float* A, int lda, const float* B, int ldb,

@@ -161,18 +161,25 @@ struct SkinnyPlan {
   int mt, col_blocks, chunks, k_per_wg;  // mt: MFMA tile rows
 };
 
+// Enough workgroups for about three per CU (measured: four is no faster at 268 MB of B and
+// slower when B fits the memory-side cache), a workgroup keeping at least 128 of K.
+int wanted_chunks(int col_blocks, int K) {
+  const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  int chunks = (3 * cus + col_blocks - 1) / col_blocks;
+  const int most = (K + 127) / 128;
+  if (chunks > most) chunks = most;
+  return chunks < 1 ? 1 : chunks;
+}
+int col_blocks_of(int M, int N) {
+  const int cols = M <= 16 ? 64 : 128;
+  return (N + cols - 1) / cols;
+}
+
 SkinnyPlan plan_skinny(int M, int N, int K) {
   SkinnyPlan p;
   p.mt = M <= 16 ? 16 : 32;
-  const int cols = 4 * p.mt;
-  p.col_blocks = (N + cols - 1) / cols;
-  // Enough workgroups for about three per CU (measured: four is no faster at 268 MB of B and
-  // slower when B fits the memory-side cache), a workgroup keeping at least 128 of K.
-  const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  int chunks = (3 * cus + p.col_blocks - 1) / p.col_blocks;
-  const int most = (K + 127) / 128;
-  if (chunks > most) chunks = most;
-  if (chunks < 1) chunks = 1;
+  p.col_blocks = col_blocks_of(M, N);
+  const int chunks = wanted_chunks(p.col_blocks, K);
   p.k_per_wg = (K + chunks - 1) / chunks;
   p.k_per_wg = (p.k_per_wg + 31) / 32 * 32;  // four wavefronts x a multiple of 8
   p.chunks = (K + p.k_per_wg - 1) / p.k_per_wg;
@@ -201,6 +208,11 @@ bool gemm_f32_skinny_shape(bool trans_a, int M, int N, int K) {
 
 size_t gemm_f32_skinny_scratch_bytes(int M, int N, int K) {
   return (size_t)plan_skinny(M, N, K).chunks * M * N * sizeof(float);
+}
+
+// For any part of the contraction too: longer ones want as many chunks or more.
+size_t gemm_f32_skinny_scratch_bound(int M, int N, int K) {
+  return M <= 32 && N % 4 == 0 ? (size_t)wanted_chunks(col_blocks_of(M, N), K) * M * N * sizeof(float) : 0;
 }
 
 bool gemm_f32_skinny_applies(bool trans_a, int M, int N, int K, const float* A, int lda,

@@ -1051,14 +1051,6 @@ struct Layout {
   Plan plan, plan_kernel;  // of the product forward, or of dx and dkernel
 };
 
-size_t float_product_bytes(int M, int N, int K) {
-  // a contraction that exceeds the float product's panels is cut into runs, whose pieces are bounded by four tiles a CU
-  const size_t bytes = gemm_f32_scratch_bytes(M, N, K);
-  if ((long long)K * (M > N ? M : N) < (1ll << 28)) return bytes;
-  const size_t bound = (size_t)4 * cus() * 128 * 128 * sizeof(float);
-  return bytes > bound ? bytes : bound;
-}
-
 // What gemm.hip's product of M rows takes, ns: 190 TFLOP/s, and beside them less for few rows.  Products of floats go by tiles of the float
 // instruction where those cost less, which have no pass behind them.  us, tiles / gemm.hip: 512 x 512 x 512 (R, C, D) 10.9 / 15.7, both
 // gradients 16.2 / 33.8; 1024 x 1024 x 1024 27.7 / 31.7, 43 / 65; 1296 x 224 x 630 12.4 / 18.9; 3071 x 300 x 1001 28.5 / 28.8, 59 / 68;
@@ -1110,8 +1102,9 @@ Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) 
     l.product_kernel = l.product + whole(l.plan.floats * sizeof(float));
     need = l.product_kernel - l.product + l.plan_kernel.floats * sizeof(float);
   } else {
-    const size_t a = backward ? float_product_bytes(R, C, D) : float_product_bytes(R, D, C);
-    const size_t b = backward ? float_product_bytes(C, D, R) : 0;
+    // (how far apart rows are, by which a contraction may be cut into runs, is not known here)
+    const size_t a = backward ? gemm_f32_scratch_bound(R, C, D) : gemm_f32_scratch_bound(R, D, C);
+    const size_t b = backward ? gemm_f32_scratch_bound(C, D, R) : 0;
     need = a > b ? a : b;
   }
   l.total = at + whole(need);

@@ -1,6 +1,8 @@
 """Which sizes and rows the operators of a gated linear recurrent block take, without a GPU: a call that is taken gets as far as its
 first launch, which finds no device."""
 import ctypes
+import math
+import random
 
 import pytest
 import torch
@@ -17,14 +19,19 @@ def _bytes(name, *sizes):
     return fn(*sizes)
 
 
+def _linear_bytes(backward, sfx, R, C, D, x_row):
+    element = 4 if sfx == "_f32" else 2
+    return _bytes("haste_hip_linear_workspace_bytes", backward, element, R, C, D, int((x_row or C) * element % 16 == 0))
+
+
 def _forward(sfx, R, C, D, x_row=None, x=2 ** 12, kernel=2 ** 13, workspace=2 ** 14, size=None):
     """The code of a projection whose caller has as much scratch memory as is said to be needed (or `size` bytes)."""
-    size = _bytes("haste_hip_linear_workspace_bytes", 0, 4 if sfx == "_f32" else 2, R, C, D, 1) if size is None else size
+    size = _linear_bytes(0, sfx, R, C, D, x_row) if size is None else size
     return lib.entry("haste_hip_linear_forward" + sfx)(R, C, D, x, x_row or C, kernel, None, 0, None, 0, 2 ** 15, None, workspace, size, None)
 
 
 def _backward(sfx, R, C, D, x_row=None, dy_row=None, dx=2 ** 15, dkernel=2 ** 16, size=None):
-    size = _bytes("haste_hip_linear_workspace_bytes", 1, 4 if sfx == "_f32" else 2, R, C, D, 1) if size is None else size
+    size = _linear_bytes(1, sfx, R, C, D, x_row) if size is None else size
     return lib.entry("haste_hip_linear_backward" + sfx)(R, C, D, 2 ** 12, x_row or C, 2 ** 13, 0, None, 2 ** 17, dy_row or D, dx, dkernel, None,
                                                         2 ** 14, size, None)
 
@@ -51,3 +58,17 @@ def test_products_of_long_rows_are_taken():
                                        (1, 1024, 4096, 100000, 1024, 2 ** 22), (1, 600000, 64, 2048, 600000, 64)):
         assert product(trans_a, M, N, K, 2 ** 12, lda, 2 ** 13, ldb, 2 ** 15, N, 0, None) == RUNTIME, (trans_a, M, N, K, lda, ldb)
     assert product(0, 128, 128, 2 ** 20, 2 ** 12, 2 ** 22 + 2 ** 20, 2 ** 13, 128, 2 ** 15, 128, 0, None) == UNSUPPORTED
+
+
+def test_scratch_memory_is_enough_for_every_run():
+    """Rows so far apart that a contraction is cut: a run may want more pieces than the whole."""
+    for R, C, D, x_row, dy_row in ((2550, 192, 2700, 237495, 2700), (16427, 128, 2112, 37069, 2112), (2550, 2700, 192, 2700, 237495)):
+        assert _backward("_f32", R, C, D, x_row, dy_row, dx=None) == RUNTIME, (R, C, D, x_row, dy_row)
+    gen = random.Random(1)
+    size = lambda low, high: round(math.exp(gen.uniform(math.log(low), math.log(high))))  # noqa: E731
+    for _ in range(4000):
+        R, C, D = size(128, 40000), size(64, 4096), size(64, 4096)
+        x_row, dy_row = size(C, 2 ** 22), size(D, 2 ** 22)
+        if min(x_row, dy_row) * R < 2 ** 40:
+            assert _backward("_f32", R, C, D, x_row, dy_row, dx=None) == RUNTIME, (R, C, D, x_row, dy_row)
+            assert _forward("_f32", R, C, D, x_row) == RUNTIME, (R, C, D, x_row)

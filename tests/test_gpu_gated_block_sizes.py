@@ -45,3 +45,12 @@ def test_floats_of_long_rows(R, C, D):
     want = formulas.linear(part(x=last, kernel=slice(-24, None), bias=None, dy=None))  # the last inputs, all outputs
     formulas.check_error(got["dx"][last], *want["dx"], "dx")
     formulas.check_error(got["dkernel"][-24:], *want["dkernel"], "dkernel")
+
+
+def test_floats_cut_into_runs_of_more_pieces():
+    """Runs of a contraction over rows that are cut into more pieces than the whole would be."""
+    for R, C, D, distance in ((2550, 192, 2700, 237495), (16427, 128, 2112, 37069)):
+        print("runs", R, C, D, distance, flush=True)
+        q = linear_problem(R, torch.float32, (R,), C, D, "none")
+        memory = torch.empty(R * distance, device="cuda")
+        compare_linear(run_linear(dict(q.g, x=_far(q.g["x"], distance, memory))), exact_linear(q))
