@@ -1142,10 +1142,10 @@ int forward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kernel
   HASTE_HIP_PROPAGATE(check_sizes(R, C, D, sizeof(T)));
   HASTE_HIP_REQUIRE(x != nullptr && kernel != nullptr && y != nullptr && act >= kNone && act <= kSilu);
   HASTE_HIP_REQUIRE(R == 1 || x_row >= (size_t)C);
+  const bool aligned = in_pieces(x, R == 1 ? 8 : x_row, sizeof(T)) && in_pieces(kernel, 8, sizeof(T));
   if (R == 1) x_row = C;
   if (x_row > (size_t)(1 << 22)) return too_large("linear: rows of x more than 2^22 elements apart");
   hipStream_t stream = as_stream(stream_);
-  const bool aligned = in_pieces(x, x_row, sizeof(T)) && in_pieces(kernel, 8, sizeof(T));
   const Layout l = layout_of(false, sizeof(T), R, C, D, aligned);
   HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
   char* ws = static_cast<char*>(workspace);
@@ -1179,10 +1179,10 @@ int backward_entry(int R, int C, int D, const T* x, size_t x_row, const T* kerne
   HASTE_HIP_REQUIRE(x != nullptr && kernel != nullptr && dy != nullptr && act >= kNone && act <= kSilu);
   HASTE_HIP_REQUIRE(act == kNone || cache != nullptr);
   HASTE_HIP_REQUIRE(R == 1 || (x_row >= (size_t)C && dy_row >= (size_t)D));
+  const bool aligned = in_pieces(x, R == 1 ? 8 : x_row, sizeof(T)) && in_pieces(kernel, 8, sizeof(T));
   if (R == 1) x_row = C, dy_row = D;
   if (x_row > (size_t)(1 << 22) || dy_row > (size_t)(1 << 22)) return too_large("linear: rows more than 2^22 elements apart");
   hipStream_t stream = as_stream(stream_);
-  const bool aligned = in_pieces(x, x_row, sizeof(T)) && in_pieces(kernel, 8, sizeof(T));
   const Layout l = layout_of(true, sizeof(T), R, C, D, aligned);
   HASTE_HIP_REQUIRE(workspace_ok(workspace, workspace_bytes, l.total));
   char* ws = static_cast<char*>(workspace);

@@ -72,3 +72,12 @@ def test_scratch_memory_is_enough_for_every_run():
         if min(x_row, dy_row) * R < 2 ** 40:
             assert _backward("_f32", R, C, D, x_row, dy_row, dx=None) == RUNTIME, (R, C, D, x_row, dy_row)
             assert _forward("_f32", R, C, D, x_row) == RUNTIME, (R, C, D, x_row)
+
+
+@pytest.mark.parametrize("sfx", ["_f32", "_f16", "_bf16"])
+def test_scratch_memory_of_a_single_row(sfx):
+    """x and the kernel at 16 bytes: how far the next row would be makes no difference."""
+    for C, D, x_row in ((77, 992, 80), (80, 992, 80), (77, 992, 77), (77, 991, 88), (4097, 64, 4104)):
+        for backward, call in ((0, _forward), (1, _backward)):
+            size = _bytes("haste_hip_linear_workspace_bytes", backward, 4 if sfx == "_f32" else 2, 1, C, D, 1)
+            assert call(sfx, 1, C, D, x_row, size=size) == RUNTIME, (backward, C, D, x_row)

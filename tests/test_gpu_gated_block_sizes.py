@@ -3,8 +3,11 @@ float64 (gated_block_formulas.py), bounded as derived there."""
 import pytest
 import torch
 
+from haste_amd import lib, ops
+
 import gated_block_formulas as formulas
 from test_gpu_gated_block import compare_linear, exact_linear, linear_problem, run_linear
+from test_gpu_state_space import short
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +57,26 @@ def test_floats_cut_into_runs_of_more_pieces():
         q = linear_problem(R, torch.float32, (R,), C, D, "none")
         memory = torch.empty(R * distance, device="cuda")
         compare_linear(run_linear(dict(q.g, x=_far(q.g["x"], distance, memory))), exact_linear(q))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=short)
+def test_a_single_row_in_the_scratch_memory_it_asks_for(dtype):
+    """A row of a wider tensor whose rows are a multiple of 16 bytes apart, its own width is not: what lies behind the scratch memory stays."""
+    element, sfx = torch.finfo(dtype).bits // 8, {torch.float32: "_f32", torch.float16: "_f16", torch.bfloat16: "_bf16"}[dtype]
+    for C, D, x_row in ((77, 992, 80), (2049, 70, 2056)):
+        q = linear_problem(C, dtype, (1,), C, D, "none", True, False)
+        want, g = exact_linear(q), q.g
+        x = torch.full((1, x_row), float("nan"), device="cuda", dtype=dtype)
+        x[:, :C] = g["x"]
+        got = {k: torch.full(s, 7.0, device="cuda", dtype=dtype) for k, s in (("y", (1, D)), ("dx", (1, C)), ("dkernel", (C, D)), ("dbias", (D,)))}
+        for backward in (0, 1):
+            print("single", C, D, backward, dtype, flush=True)
+            size = ops._scratch_bytes("haste_hip_linear_workspace_bytes", x.device, backward, element, 1, C, D, 1)
+            scratch = torch.full((size + 256,), 77, device="cuda", dtype=torch.uint8)
+            if backward:
+                lib.call("haste_hip_linear_backward" + sfx, 1, C, D, x, x_row, g["kernel"], 0, None, g["dy"], D, got["dx"], got["dkernel"],
+                         got["dbias"], scratch, size)
+            else:
+                lib.call("haste_hip_linear_forward" + sfx, 1, C, D, x, x_row, g["kernel"], g["bias"], 0, None, 0, got["y"], None, scratch, size)
+            assert (scratch[size:] == 77).all()
+        compare_linear(got, want)
