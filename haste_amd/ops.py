@@ -1011,6 +1011,8 @@ def _linear_arguments(x, kernel, bias, activation):
     if not (_alike(x.dtype, device, kernel, bias) and kernel.shape[0] == C and (bias is None or bias.shape == (D,))):
         _activation("kernel", kernel, (C, D), x)  # one of these says what is wrong
         _activation("bias", bias, (D,), x)
+    if x.numel() // C > 2 ** 30:  # the entry points count them in 32 bits
+        raise ValueError("more than 2^30 rows are not implemented, got %s" % list(x.shape))
     suffix = _activation_suffix(x)
     rows, step = _linear_rows(x)
     return (x.numel() // C, C, D), rows, step, _contiguous(kernel), _contiguous(bias), number, device, suffix

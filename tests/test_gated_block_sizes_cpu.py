@@ -7,7 +7,7 @@ import random
 import pytest
 import torch
 
-from haste_amd import lib
+from haste_amd import lib, ops
 
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="calls with addresses of nothing, for machines on which nothing is launched")
 INVALID, UNSUPPORTED, RUNTIME = 1, 2, 3
@@ -81,3 +81,13 @@ def test_scratch_memory_of_a_single_row(sfx):
         for backward, call in ((0, _forward), (1, _backward)):
             size = _bytes("haste_hip_linear_workspace_bytes", backward, 4 if sfx == "_f32" else 2, 1, C, D, 1)
             assert call(sfx, 1, C, D, x_row, size=size) == RUNTIME, (backward, C, D, x_row)
+
+
+@pytest.mark.parametrize("shape", [(2 ** 30 + 1,), (2 ** 16 + 1, 2 ** 16), (2 ** 20, 2 ** 11), (5, 2 ** 32 // 5 + 1)])
+def test_more_rows_than_are_counted_are_refused(shape):
+    """Steps times batch rows, each of which is in range: not to be taken for what is left of their product in 32 bits."""
+    x, kernel = torch.zeros(1, 1).expand(*shape, 1), torch.zeros(1, 4)
+    with pytest.raises(ValueError, match="rows"):
+        ops.linear_forward(False, x, kernel)
+    with pytest.raises(ValueError, match="rows"):
+        ops.linear_backward(x, kernel, None, "none", None, x.expand(*shape, 4))
