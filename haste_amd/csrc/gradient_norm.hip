@@ -4,9 +4,9 @@
 // Bound: HBM, twice the gradients in (the norm comes first) and once out; where they fit the last-level cache the second reading is
 // cheap.  Tensors are cut into chunks of kChunk bytes; a workgroup takes chunks in turn, so that many small tensors and
 // few large ones fill the device alike.  Where tensors lie is an argument of the kernels (kTensors to a launch): nothing is copied to the
-// device, and a captured launch keeps it.  Squares are added in double, a lane's, a workgroup's and all: no gradient overflows or
-// vanishes by being squared, and an element costs two operations at a rate that the memory does not reach.  Sums
-// are parked per workgroup and added in order.
+// device, and a captured launch keeps it.  Squares are added in double, a lane's, a workgroup's and all: no gradient in float or half overflows
+// or vanishes by being squared, and an element costs two operations at a rate that the memory does not reach (those of doubles do from 1.4e154 on
+// and below 1.5e-162: the norm is infinite, or is without them).  Sums are parked per workgroup and added in order.
 //
 // The gradients are scaled from the last chunk to the first, and neither they nor the results are kept in the caches any more: what the norm
 // read last is then still in the last-level cache.  us, forwards / backwards / and so: 537 million gradients (1.07 GB) 611 / 608 / 560, 67
@@ -107,12 +107,11 @@ void gradient_squares_kernel(Tensors<MOST> list, double* __restrict__ partial) {
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// The norm from what the workgroups left, as it is handed out: in float, or in double.
-__device__ __forceinline__ double norm_of_parts(int parts, const double* partial, int in_double) {
+// The sum of what the workgroups left.
+__device__ __forceinline__ double sum_of_parts(int parts, const double* partial) {
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += kThreads) sum += partial[i];
-  sum = sqrt(workgroup_sum(sum));
-  return in_double ? sum : (double)(float)sum;
+  return workgroup_sum(sum);
 }
 
 __device__ __forceinline__ void store_norm(void* norm, int in_double, double value) {
@@ -121,9 +120,11 @@ __device__ __forceinline__ void store_norm(void* norm, int in_double, double val
 }
 
 __global__ __launch_bounds__(kThreads)
-void gradient_norm_kernel(int parts, const double* __restrict__ partial, void* __restrict__ norm, int in_double) {
-  const double value = norm_of_parts(parts, partial, in_double);
-  if (threadIdx.x == 0) store_norm(norm, in_double, value);
+void gradient_norm_kernel(int parts, const double* partial, double* total, void* __restrict__ norm, int in_double) {
+  const double sum = sum_of_parts(parts, partial);
+  if (threadIdx.x != 0) return;
+  store_norm(norm, in_double, sqrt(sum));
+  if (total != nullptr) *total = sum;
 }
 
 // parts: those of the norm, which every workgroup adds up for itself and the first hands out (a launch less: 2 us, and 4 of the host);
@@ -134,13 +135,19 @@ void gradient_scale_kernel(Tensors<MOST> list, void* __restrict__ norm, int in_d
                            const double* __restrict__ partial) {
   double length;
   if (parts > 0) {
-    length = norm_of_parts(parts, partial, in_double);
+    length = sqrt(sum_of_parts(parts, partial));
     if (blockIdx.x == 0 && threadIdx.x == 0) store_norm(norm, in_double, length);
+    // As it is handed out, so that the gradients are the same where it is given; beyond a float's range, where it is handed out as
+    // infinite, as it is: finite gradients of such a norm are not zeros.
+    const float rounded = (float)length;
+    if (!in_double && rounded <= 0x1.fffffep127f) length = rounded;
   } else {
     length = in_double ? *static_cast<const double*>(norm) : (double)*static_cast<const float*>(norm);
   }
   double factor = max_norm / (length + 1e-6);
   factor = factor > 1.0 ? 1.0 : factor;  // (a NaN stays)
+  // A factor below a float's normal range goes into the product in two: the first lifts it by a power of 2, which the product, below 4, has room for.
+  const double lift = factor < 0x1p-126 ? 0x1p120 : 1.0;
   for_chunks<true>(list, [&](auto zero, int tensor, size_t start, int n) {
     typedef decltype(zero) T;
     typedef typename std::conditional<sizeof(T) == 8, double, float>::type scale_t;
@@ -148,7 +155,7 @@ void gradient_scale_kernel(Tensors<MOST> list, void* __restrict__ norm, int in_d
     const T* p = static_cast<const T*>(list.in[tensor]) + start;
     T* to = static_cast<T*>(list.out[tensor]) + start;
     if (factor == 1.0 && p == to) return;
-    const scale_t by = (scale_t)factor;
+    const scale_t by = (scale_t)(factor * lift), down = (scale_t)(1.0 / lift);
     if (n == (int)(kChunk / sizeof(T))) {
       typename Packed<T, V>::type v[EACH];
 #pragma unroll
@@ -157,7 +164,7 @@ void gradient_scale_kernel(Tensors<MOST> list, void* __restrict__ norm, int in_d
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = (T)((scale_t)v[i][e] * by);
+        for (int e = 0; e < V; ++e) v[i][e] = (T)((scale_t)v[i][e] * by * down);
         __builtin_nontemporal_store(v[i], reinterpret_cast<typename Wide<T, V>::type*>(to + (i * kThreads + threadIdx.x) * V));
       }
     } else {
@@ -165,10 +172,10 @@ void gradient_scale_kernel(Tensors<MOST> list, void* __restrict__ norm, int in_d
       for (; i + V <= n; i += kThreads * V) {
         typename Packed<T, V>::type v = *reinterpret_cast<const typename Wide<T, V>::type*>(p + i);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = (T)((scale_t)v[e] * by);
+        for (int e = 0; e < V; ++e) v[e] = (T)((scale_t)v[e] * by * down);
         *reinterpret_cast<typename Wide<T, V>::type*>(to + i) = v;
       }
-      for (const int last = i + V < n ? i + V : n; i < last; ++i) to[i] = (T)((scale_t)p[i] * by);
+      for (const int last = i + V < n ? i + V : n; i < last; ++i) to[i] = (T)((scale_t)p[i] * by * down);
     }
   });
 }
@@ -284,9 +291,10 @@ int squares_of(const Call& call, int* parts, void* workspace, size_t workspace_b
   });
 }
 
-int norm_of(int parts, void* norm, int in_double, const void* workspace, hipStream_t stream) {
+// total: where the sum of the squares is left too, or null.
+int norm_of(int parts, double* total, void* norm, int in_double, const void* workspace, hipStream_t stream) {
   ScopedKernelTimer timer("gradient_norm", stream);
-  gradient_norm_kernel<<<1, kThreads, 0, stream>>>(parts, static_cast<const double*>(workspace), norm, in_double);
+  gradient_norm_kernel<<<1, kThreads, 0, stream>>>(parts, static_cast<const double*>(workspace), total, norm, in_double);
   HASTE_HIP_TRY(hipGetLastError());
   return HASTE_HIP_OK;
 }
@@ -313,7 +321,7 @@ int haste_hip_gradient_norm(int count, const void* const* gradients, const size_
   HASTE_HIP_REQUIRE(norm != nullptr);
   int parts = 0;
   HASTE_HIP_PROPAGATE(squares_of(call, &parts, workspace, workspace_bytes, as_stream(stream)));
-  return norm_of(parts, norm, norm_in_double, workspace, as_stream(stream));
+  return norm_of(parts, nullptr, norm, norm_in_double, workspace, as_stream(stream));
 }
 
 int haste_hip_clip_gradients(int count, const void* const* gradients, void* const* clipped, const size_t* elements, const int* types,
@@ -325,14 +333,15 @@ int haste_hip_clip_gradients(int count, const void* const* gradients, void* cons
   HASTE_HIP_REQUIRE(norm != nullptr && max_norm >= 0.0);
   HASTE_HIP_PROPAGATE(check_apart(call, norm, norm_in_double ? 8 : 4, norm_given != 0));
   int parts = 0;
+  double* partial = static_cast<double*>(workspace);
   if (!norm_given) {
     HASTE_HIP_PROPAGATE(squares_of(call, &parts, workspace, workspace_bytes, as_stream(stream)));
     if (parts == 0 || parts > kOwnParts) {  // none: there is nothing to scale behind it
-      HASTE_HIP_PROPAGATE(norm_of(parts, norm, norm_in_double, workspace, as_stream(stream)));
-      parts = 0;
+      HASTE_HIP_PROPAGATE(norm_of(parts, partial + parts, norm, norm_in_double, workspace, as_stream(stream)));
+      partial += parts;  // their sum, for which the workspace has room behind those of all lists
+      parts = 1;
     }
   }
-  const double* partial = static_cast<const double*>(workspace);
   ScopedKernelTimer timer("gradient_scale", as_stream(stream));
   return for_lists(call, workgroups(), [&](const auto& list, unsigned groups) {
     gradient_scale_kernel<<<groups, kThreads, 0, as_stream(stream)>>>(list, norm, norm_in_double, max_norm, parts, partial);

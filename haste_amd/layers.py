@@ -1210,8 +1210,9 @@ def clip_gradients_(parameters, max_norm):
         if not float(max_norm) >= 0:
             raise ValueError("max_norm must not be below 0, got %r" % max_norm)
         wide = torch.float64 if any(g.dtype == torch.float64 for g in grads) else torch.float32
-        norm = torch.sqrt(sum(g.double().square().sum() for g in grads)).to(wide)
-        factor = (float(max_norm) / (norm.double() + 1e-6)).clamp(max=1.0)
-        for g in grads:
-            g.copy_(g.double() * factor if g.dtype == torch.float64 else g.float() * factor.float())
+        whole = torch.sqrt(sum(g.double().square().sum() for g in grads))
+        norm = whole.to(wide)
+        factor = (float(max_norm) / ((norm.double() if norm.isfinite() else whole) + 1e-6)).clamp(max=1.0)
+        for g in grads:  # (a factor below a float's normal range would lose bits, or all, as one)
+            g.copy_(g.double() * factor if g.dtype == torch.float64 or factor < 2.0 ** -126 else g.float() * factor.float())
         return norm

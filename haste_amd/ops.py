@@ -1208,7 +1208,8 @@ def _gradient_arguments(grads):
 
 def gradient_norm(grads):
     """The norm of all elements of all tensors together, sqrt(sum g^2), without waiting for it: a tensor of no axes, float32
-    (float64 if a gradient is).  grads: a list of float32, float64, float16 or bfloat16 tensors on one device."""
+    (float64 if a gradient is), infinite beyond its range.  grads: a list of float32, float64, float16 or bfloat16 tensors on one device,
+    each filling its memory; squares of float64 are in range from 1.5e-162 to 1.4e154."""
     addresses, elements, types, device, wide = _gradient_arguments(grads)
     norm = torch.empty((), device=grads[0].device, dtype=wide)
     scratch = _scratch("haste_hip_gradient_norm_workspace_bytes", norm, len(grads))
@@ -1219,7 +1220,8 @@ def gradient_norm(grads):
 
 def clip_gradients(grads, max_norm, norm=None, out=None):
     """grads, a list as of gradient_norm() -> clipped, norm: each gradient times min(1, max_norm / (norm + 1e-6)).  norm: that of
-    gradient_norm(), or of more than these gradients (of the ranks that share a model); None: that of these.  out: the list of
+    gradient_norm(), or of more than these gradients (of the ranks that share a model), an infinite one makes them 0; None: that of
+    these, also where it is beyond a float32 and returned as infinite.  out: the list of
     tensors to write, alike in type and strides; its tensors may be the gradients, and may overlap nothing else."""
     addresses, elements, types, device, wide = _gradient_arguments(grads)
     max_norm = float(max_norm)

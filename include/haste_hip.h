@@ -899,7 +899,9 @@ int haste_hip_gated_recurrence_iterate_bf16(int batch_size, int channels, const 
  * during the call: device addresses, elements (each tensor contiguous; 0: left out), and types (0 float, 1 half, 2 bfloat16, 3
  * double).  norm: a float (norm_in_double: a double) on the device; norm_given: it is read (the gradients are a part
  * of what was normed), otherwise written.  A clipped tensor may be its gradient, and may overlap nothing else.  Squares are
- * added in double.  A norm that is no number makes all gradients none; an infinite one makes them 0, infinite ones NaN.
+ * added in double (those of doubles beyond 1.4e154 are infinite).  A norm beyond a float is handed out as infinite in one, and
+ * what it is where the same call clips by it.  A norm that is no number makes all gradients none; an infinite one makes them 0,
+ * infinite ones NaN.
  * Workspace (not used where the norm is given): aligned to 8 bytes. */
 size_t haste_hip_gradient_norm_workspace_bytes(int count);
 int haste_hip_gradient_norm(int count, const void* const* gradients, const size_t* elements, const int* types,

@@ -80,3 +80,51 @@ def test_a_single_row_in_the_scratch_memory_it_asks_for(dtype):
                 lib.call("haste_hip_linear_forward" + sfx, 1, C, D, x, x_row, g["kernel"], g["bias"], 0, None, 0, got["y"], None, scratch, size)
             assert (scratch[size:] == 77).all()
         compare_linear(got, want)
+
+
+# ---- clipping ---------------------------------------------------------------------------
+def check_scaled(got, grads, factor):
+    """The factor is rounded twice and the product once, to floats or among doubles to doubles."""
+    for a, g in zip(got, grads):
+        want = g.double() * factor
+        formulas.check_error(a, want, want.abs() * 4 * 2.0 ** (-50 if a.dtype == torch.float64 else -24), "clipped")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=short)
+def test_clip_by_a_norm_beyond_a_float(dtype):
+    """Finite gradients are brought to the length that is asked for, whether every workgroup adds the norm's parts up or one does."""
+    for count, size in ((1, 2), (3, 8192), (130, 300001)):
+        print("beyond", count, size, dtype, flush=True)
+        grads = [torch.full((size,), 3e38 if i % 2 else -2.5e38, device="cuda", dtype=dtype) for i in range(count)]
+        norm = float(sum(g[:1].double().square().sum() * size for g in grads).sqrt())
+        assert ops.gradient_norm(grads).isinf()
+        for max_norm in (1.0, 1e-6, 1e20):
+            clipped, n = ops.clip_gradients(grads, max_norm)
+            assert n.isinf() and n.dtype == torch.float32
+            check_scaled(clipped, grads, max_norm / norm)
+        same, _ = ops.clip_gradients(grads, 1.0, out=[g.clone() for g in grads])
+        check_scaled(same, grads, 1.0 / norm)
+        zeros, given = ops.clip_gradients(grads, 1.0, norm=n)
+        assert given is n and all((z == 0).all() for z in zeros)  # an infinite norm that is given is taken for infinite
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64], ids=short)
+def test_clip_by_factors_below_a_floats_range(dtype):
+    few, many = torch.tensor([3e37, -1e37, 1e20, 0.0], device="cuda", dtype=dtype), torch.linspace(-2e37, 2e37, 20001, device="cuda").to(dtype)
+    for grads in ([few], [few, many]):  # a norm of 3.2e37, and one of 2e37 sqrt(20001 / 3) = 1.6e39, which a float does not hold
+        norm = float(sum(g.double().square().sum() for g in grads).sqrt())
+        for max_norm in (1e-9, 1e-2, 0.5):
+            clipped, n = ops.clip_gradients(grads, max_norm)
+            assert n.isinf() if dtype != torch.float64 and norm > 3.41e38 else abs(float(n) - norm) <= norm * 2.0 ** -24
+            check_scaled(clipped, grads, max_norm / norm)
+
+
+def test_clip_of_doubles_in_range_and_beyond():
+    for scale in (1e150, 1e-150):
+        g = torch.randn(5001, device="cuda", dtype=torch.float64) * scale
+        norm = float((g / scale).square().sum().sqrt()) * scale
+        assert abs(float(ops.gradient_norm([g])) - norm) <= norm * 1e-14
+    clipped, _ = ops.clip_gradients([torch.full((4,), 1e150, device="cuda", dtype=torch.float64)], 1.0)
+    assert (clipped[0] - 0.5).abs().max() <= 1e-14
+    clipped, norm = ops.clip_gradients([torch.full((4,), 1e155, device="cuda", dtype=torch.float64)], 1.0)
+    assert norm.isinf() and (clipped[0] == 0).all()  # as documented: squares of doubles have a range
