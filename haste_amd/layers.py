@@ -1195,11 +1195,14 @@ class GatedRecurrence(_BlockLayer):
 
 
 def clip_gradients_(parameters, max_norm):
-    """Scales the gradients of `parameters` (a tensor or several; those without one are left out) in place so that their norm
-    together is at most max_norm: each times min(1, max_norm / (norm + 1e-6)).  Returns the norm before, a tensor of no axes; on the GPU
-    nothing is waited for.  Gradients of float32, float64, float16 and bfloat16 may be mixed, on one device."""
+    """Scales the gradients of `parameters` (a tensor or several; those without one are left out, and one that is listed more than
+    once, as tied weights may be, counts once) in place so that their norm together is at most max_norm: each times
+    min(1, max_norm / (norm + 1e-6)).  Returns the norm before, a tensor of no axes; on the GPU nothing is waited for.  Gradients of
+    float32, float64, float16 and bfloat16 may be mixed; they are on one device, and on the GPU each fills its memory, as those that
+    autograd makes do, and shares it with no other."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
+    grads = list({id(g): g for g in grads}.values())
     if not grads:
         return torch.zeros(())
     with torch.no_grad():

@@ -1,4 +1,4 @@
-"""Clipping of gradients on the host: norms beyond a float's range."""
+"""Clipping of gradients on the host: norms beyond a float's range, parameters listed twice."""
 import torch
 
 import haste_amd
@@ -34,3 +34,13 @@ def test_infinite_gradients_are_no_numbers():
     parameters = _parameters(torch.tensor([1.0, float("inf")]))
     assert haste_amd.clip_gradients_(parameters, 1.0).isinf()
     assert parameters[0].grad[0] == 0 and parameters[0].grad[1].isnan()
+
+
+def test_a_parameter_that_is_listed_twice_counts_once():
+    a, b = _parameters(torch.tensor([3.0, 0.0]), torch.tensor([4.0]))
+    assert haste_amd.clip_gradients_([a, b, a], 1.0) == 5
+    assert (a.grad - torch.tensor([0.6, 0.0])).abs().max() <= 1e-6 and (b.grad - 0.8).abs() <= 1e-6
+    shared = torch.nn.Parameter(torch.zeros(2))
+    shared.grad = a.grad  # the same gradient of two parameters
+    assert abs(float(haste_amd.clip_gradients_(iter([a, shared, a]), 0.3)) - 0.6) <= 1e-6
+    assert abs(float(a.grad[0]) - 0.3) <= 1e-6

@@ -3,6 +3,7 @@ float64 (gated_block_formulas.py), bounded as derived there."""
 import pytest
 import torch
 
+import haste_amd
 from haste_amd import lib, ops
 
 import gated_block_formulas as formulas
@@ -128,3 +129,16 @@ def test_clip_of_doubles_in_range_and_beyond():
     assert (clipped[0] - 0.5).abs().max() <= 1e-14
     clipped, norm = ops.clip_gradients([torch.full((4,), 1e155, device="cuda", dtype=torch.float64)], 1.0)
     assert norm.isinf() and (clipped[0] == 0).all()  # as documented: squares of doubles have a range
+
+
+def test_a_parameter_that_is_listed_twice_is_clipped_once():
+    """The parameters of two models that share a weight, one behind the other."""
+    tied = torch.nn.Parameter(torch.zeros(100, 70, device="cuda"))
+    own = [torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=t)) for n, t in ((5, torch.float32), (9001, torch.bfloat16))]
+    for p in (tied, *own):
+        p.grad = torch.randn(p.shape, device="cuda").to(p.dtype)
+    before = [p.grad.clone() for p in (tied, *own)]
+    norm = float(sum(g.double().square().sum() for g in before).sqrt())
+    got = haste_amd.clip_gradients_([tied, own[0], tied, own[1]], 0.25)
+    assert abs(float(got) - norm) <= norm * 2.0 ** -24
+    check_scaled([p.grad for p in (tied, *own)], before, 0.25 / norm)
