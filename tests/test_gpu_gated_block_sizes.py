@@ -7,7 +7,8 @@ import haste_amd
 from haste_amd import lib, ops
 
 import gated_block_formulas as formulas
-from test_gpu_gated_block import compare_linear, exact_linear, linear_problem, run_linear
+import state_space_bounds as bounds
+from test_gpu_gated_block import PARTS, compare_linear, exact_linear, gated_problem, linear_problem, run_gated, run_linear
 from test_gpu_state_space import short
 
 pytestmark = pytest.mark.gpu
@@ -142,3 +143,55 @@ def test_a_parameter_that_is_listed_twice_is_clipped_once():
     got = haste_amd.clip_gradients_([tied, own[0], tied, own[1]], 0.25)
     assert abs(float(got) - norm) <= norm * 2.0 ** -24
     check_scaled([p.grad for p in (tied, *own)], before, 0.25 / norm)
+
+
+# ---- the recurrence --------------------------------------------------------------------
+def test_every_gradient_of_extreme_gates():
+    """Gates that are shut or open beyond what a float tells from 0 and 1 under decays of nothing and of everything: all gradients.  Where
+    1 - a^2 is below a float's normal range it and its root's slope are 0: what enters, x sqrt(1 - a^2), is then off by 2^-63 |x| at most, and
+    what reaches forget through it, |x sqrt(decay r / 2)|, by half of that."""
+    T, N, D = 70, 2, 64
+    q = gated_problem(17, torch.float32, T, N, D)
+    forget = torch.randn(T, N, D, generator=q.gen, dtype=torch.float64)
+    forget[::3], forget[1::3] = 200.0, -200.0
+    q.put("forget", forget)
+    q.put("admit", forget.flip(0))
+    q.put("decay", torch.where(torch.arange(D) % 2 == 0, 1e-30, 1e30), torch.float32)
+    p = q.p
+    rate = 2 * p["decay"] * torch.sigmoid(p["forget"] + p["forget_bias"])
+    cut = rate < 2.0 ** -126
+    assert ((rate < 2.0 ** -140) | (rate > 2.0 ** -110)).all() and 0 < cut.sum() < cut.numel()  # none near the border
+    got, want, most = run_gated(q.g), formulas.gated(p), formulas.gated(p, True)
+    silu = (p["z"] * torch.sigmoid(p["z"])).abs()
+    most_g = ((p["dy"].abs() * silu).sum(0) + p["dh_last"].abs()).max()  # no a is above 1
+    off = cut * 2.0 ** -63 * most_g * (1 + p["x"].abs())
+    entered = 2.0 ** -63 * p["x"].abs().sum(0)
+    allowed = dict(dx=off, dforget=off, dadmit=off, dforget_bias=off.sum((0, 1)), dadmit_bias=off.sum((0, 1)), h_last=entered, y=entered * silu,
+                   dz=entered * p["dy"].abs() * (1 + p["z"].abs()))
+    roundings = 24 * T + N + 64
+    assert set(got) == set(want) == {"y", "h_last", "dx", "dforget", "dadmit", "dz", "ddecay", "dforget_bias", "dadmit_bias", "dh0"}
+    for k in want:
+        bounds.check(got[k], want[k], most[k] + allowed.get(k, 0.0) / (roundings * 2.0 ** -24), roundings, k)
+    assert (got["dforget"].cpu()[cut] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=short)
+def test_steps_are_what_the_whole_is(dtype):
+    for N, D, options in ((1, 1, {}), (3, 100, dict(decay=False)), (2, 33, dict(admit=False)), (4, 51, dict(decay=False, admit=False, z=False)),
+                          (70, 2000, {})):
+        print("steps", N, D, options, dtype, flush=True)
+        q = gated_problem(N + D, dtype, 5, N, D, **options)
+        full, want, most = run_gated(q.g), formulas.gated(q.p), formulas.gated(q.p, True)
+        state, ys = q.g["h0"], []
+        for t in range(5):
+            x, forget, admit, z = (None if q.g[k] is None else q.g[k][t] for k in ("x", "forget", "admit", "z"))
+            y, state = ops.gated_recurrence_iterate(x, forget, state, admit, z, *[q.g[k] for k in PARTS[2:]])
+            ys.append(y)
+        for k, stepped in (("y", torch.stack(ys)), ("h_last", state)):
+            for value in (full[k], stepped):
+                bounds.check(value, want[k], most[k], 24 * 5 + 64, k)
+            # both are so far from the same value at most
+            error = 2 * (24 * 5 + 64) * 2.0 ** -24 * most[k]
+            half_step = 0.0 if stepped.dtype == torch.float32 else torch.finfo(dtype).eps / 2
+            apart = (full[k].double() - stepped.double()).abs().cpu()
+            assert (apart <= error + 2 * half_step * (want[k].abs() + error) + 2 * torch.finfo(torch.float16).tiny).all(), k
