@@ -150,12 +150,16 @@ __device__ __forceinline__ uint4_t resource(const void* base, long long bytes) {
 }
 
 // 16 bytes a lane from the resource into LDS at `lds` and the 1008 bytes behind it, lane by lane.  The load has no register
-// to write; it is waited for by count, in tile_ready().
+// to write; it is waited for by count, in tile_ready().  m0 is named, so that the compiler does not take what it put there for what is there still
+// (its warning is that it does not save what the register holds, which is right).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(unsigned lds, unsigned offset, uint4_t from, unsigned shift) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(from),
                "s"(shift)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Waits until at most LEFT of this wavefront's loads are on their way and all its reads of LDS have returned, then for the others.
 template <int LEFT>
