@@ -865,8 +865,8 @@ constexpr double kStep[kTiles][3] = {{21.0}, {9.0, 13.9}, {4.2, 6.3, 8.4}}, kRou
 constexpr double kFloatStep[3] = {23.0, 38.0, 56.0};  // floats, 64 x 64
 double step_cost(int element, int kind, int on_a_cu) { return element == 4 ? kFloatStep[on_a_cu - 1] : kStep[kind][on_a_cu - 1]; }
 
-// Adding pieces up, 2500 ns and 1000 for a launch more, which the host bears; and writing and reading their elements at 4 TB/s. (The estimates
-// below are without the 1000.)
+// Adding pieces up, 2500 ns and 1000 for a launch more, which the host bears; and writing and reading their elements at 4 TB/s. (The 1000 is
+// in the estimates below and not in what the device was measured to take.)
 double join_cost(int pieces, int M, int N) { return pieces > 1 ? 3500 + (double)pieces * M * N * 8 / 4000 : 0.0; }
 
 // The cheapest of the tiles from `first` to `last` and of 1 to 32 pieces by cost(kind, workgroups, k of a workgroup), and its joins.
@@ -891,10 +891,10 @@ Plan cheapest(int cus, int first, int last, int M, int N, int K, Cost cost) {
 }
 
 // A product by itself: its steps in rounds of workgroups.  us, estimate / measured: 128 x 4096 x 4096 (M, K, N) in 4 / 8
-// pieces of 128 x 128 19.4 / 18.3, 19.0 / 18.8, in 8 of 256 x 256 26 / 24, in 2 / 4 of 64 x 64 16.7 / 16.8, 16.6 / 17.0; 1024 x 8192 x 2048 in 4 of
-// 128 x 128 51 / 48, in 8 of 256 x 256 63 / 51; 512 x 16384 x 512 in 16 of 128 x 128 24 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
+// pieces of 128 x 128 20.4 / 18.3, 20.0 / 18.8, in 8 of 256 x 256 28 / 24, in 2 / 4 of 64 x 64 17.7 / 16.8, 17.6 / 17.0; 1024 x 8192 x 2048 in 4 of
+// 128 x 128 52 / 48, in 8 of 256 x 256 64 / 51; 512 x 16384 x 512 in 16 of 128 x 128 25 / 26; 8192 x 2048 x 1024 whole, 128 x 128 / 256 x 256 32, 48 /
 // 34, 48; 512 x 2048 x 2048 whole of 64 x 64 12 / 13 (before there were those: 20.7), 1024 x 1024 x 1024 7.8 / 8.6 (14.0), 512 x 512 x 512 5.7 / 5.7
-// (9.1), 2048 x 2048 x 2048 whole of 128 x 128 / 64 x 64 32 / 24, 29 / 29.
+// (9.1), 2048 x 2048 x 2048 whole of 128 x 128 22 / 24, of 64 x 64 33 / 29.
 Plan plan_product(int cus, int element, int first, int last, int M, int N, int K) {
   return cheapest(cus, first, last, M, N, K, [=](int kind, long long workgroups, int per) {
     const unsigned slots = (unsigned)(kPerCu[kind] * cus), all = (unsigned)workgroups, rounds = all / slots, rest = all % slots;
@@ -905,8 +905,8 @@ Plan plan_product(int cus, int element, int first, int last, int M, int N, int K
 
 // One that is launched with `other`: all workgroups' shares of a full CU, which has as many as fit of the larger tiles, or the
 // longest's time where that is more.  us, estimate / measured: both gradients of
-// 8192 x 1024 x 2048 with that of the kernel in 2 / 3 / 4 pieces 73 / 76, 78 / 80, 83 / 81 (by itself 4 would be best), of 4096 x 2048 x 1024 in 2 / 4
-// 45 / 45, 52 / 49.
+// 8192 x 1024 x 2048 with that of the kernel in 2 / 3 / 4 pieces 74 / 76, 79 / 80, 84 / 81 (by itself 4 would be best), of 4096 x 2048 x 1024 in 2 / 4
+// 46 / 45, 56 / 49.
 Plan plan_product_beside(int cus, int element, const Plan& other, int M, int N, int K) {
   const double others = (double)other.tiles_m * other.tiles_n * other.pieces;
   return cheapest(cus, element == 4 ? kNarrow : kSmall, kNarrow, M, N, K, [&](int kind, long long workgroups, int per) {
