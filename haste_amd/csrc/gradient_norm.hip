@@ -275,9 +275,11 @@ int check_apart(const Call& call, const void* norm, size_t norm_bytes, bool norm
 }
 
 size_t lists_of(int count) { return ((size_t)count + kTensors - 1) / kTensors; }
+constexpr size_t kMostLists = 1u << 16;
 
 // Leaves the parts of the norm in the workspace.
 int squares_of(const Call& call, int* parts, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (lists_of(call.count) > kMostLists) return too_large("gradient_norm: more than 7340032 gradients");
   HASTE_HIP_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0 &&
                     workspace_bytes >= haste_hip_gradient_norm_workspace_bytes(call.count));
   double* partial = static_cast<double*>(workspace);
@@ -310,7 +312,7 @@ extern "C" {
 using namespace haste_hip;
 
 size_t haste_hip_gradient_norm_workspace_bytes(int count) {
-  if (count < 0 || lists_of(count) > (1u << 16)) return 0;
+  if (count < 0 || lists_of(count) > kMostLists) return 0;
   return (lists_of(count) + 1) * workgroups() * sizeof(double);
 }
 

@@ -91,3 +91,16 @@ def test_more_rows_than_are_counted_are_refused(shape):
         ops.linear_forward(False, x, kernel)
     with pytest.raises(ValueError, match="rows"):
         ops.linear_backward(x, kernel, None, "none", None, x.expand(*shape, 4))
+
+
+def test_more_gradients_than_the_norm_has_scratch_memory_for_are_refused():
+    """Where the size of the scratch memory is said to be 0.  (No gradient has elements: nothing would be written if it went on.)"""
+    size = lambda count: _bytes("haste_hip_gradient_norm_workspace_bytes", count)  # noqa: E731
+    most = 7340032
+    assert size(most) > 0 and size(most + 1) == 0
+    none = (ctypes.c_void_p * (most + 1))(), (ctypes.c_size_t * (most + 1))(), (ctypes.c_int * (most + 1))()
+    norm = lambda count: lib.entry("haste_hip_gradient_norm")(count, *none, 64, 0, 256, size(count), None)  # noqa: E731
+    clip = lambda count, given: lib.entry("haste_hip_clip_gradients")(count, none[0], *none, 1.0, given, 64, 0, 256, size(count), None)  # noqa: E731
+    assert norm(most) == RUNTIME and norm(most + 1) == UNSUPPORTED
+    assert clip(most, 0) == RUNTIME and clip(most + 1, 0) == UNSUPPORTED
+    assert clip(most + 1, 1) == 0  # the norm is there, and nothing to scale
