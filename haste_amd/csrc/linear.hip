@@ -1077,7 +1077,8 @@ Layout layout_of(bool backward, int element, int R, int C, int D, bool aligned) 
       const double here = plan_kernel.cost + join_cost(plan.pieces, R, C);
       if (here < cost) l.plan = plan, l.plan_kernel = plan_kernel, cost = here, l.together = true;
     };
-    const Plan small = l.plan.kind >= kSmall ? l.plan : plan_product(cus, element, kSmall, kNarrow, R, C, D);
+    // (floats have the narrow tiles alone; where those are too many for a grid there is no plan)
+    const Plan small = l.plan.kind >= kSmall || element == 4 ? l.plan : plan_product(cus, element, kSmall, kNarrow, R, C, D);
     if (small.cost < 1e300) consider(small, plan_product_beside(cus, element, small, C, D, R));
     if (element == 2) {
       Plan whole = plan_product(cus, element, kLarge, kLarge, R, C, D);
