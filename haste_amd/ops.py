@@ -1209,7 +1209,7 @@ def _gradient_arguments(grads):
 def gradient_norm(grads):
     """The norm of all elements of all tensors together, sqrt(sum g^2), without waiting for it: a tensor of no axes, float32
     (float64 if a gradient is), infinite beyond its range.  grads: a list of float32, float64, float16 or bfloat16 tensors on one device,
-    each filling its memory; squares of float64 are in range from 1.5e-162 to 1.4e154."""
+    each filling its memory; squares of float64 are in range from 1.5e-154 to 1.3e154."""
     addresses, elements, types, device, wide = _gradient_arguments(grads)
     norm = torch.empty((), device=grads[0].device, dtype=wide)
     scratch = _scratch("haste_hip_gradient_norm_workspace_bytes", norm, len(grads))

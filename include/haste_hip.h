@@ -810,7 +810,7 @@ int haste_hip_residual_norm_backward_bf16(int steps, int batch_size, int channel
  * _f16) or half (_bf16), or NULL; without an activation there is none.  Backward: dx[R,C], dW[C,D], dbias[D] from
  * dy[R,D], which is the residual's gradient too; each may be NULL (not wanted).  Workspace: aligned to 16 bytes; `aligned`
  * says that x and W start at, and (where there are several) rows of x are apart by, multiples of 16 bytes.  Up to 2^30 rows, 2^20
- * columns, rows 2^22 elements apart; in float the order of sums depends on alignment and on how far rows are apart too. */
+ * columns, rows 2^22 elements apart, and 2^22 tiles of 128 x 128 (float: 2^24) in each of the three products; in float the order of sums depends on alignment and on how far rows are apart too. */
 size_t haste_hip_linear_workspace_bytes(int backward, int element_bytes, int rows, int inputs, int outputs,
                                         int aligned);
 int haste_hip_linear_forward_f32(int rows, int inputs, int outputs, const void* x, size_t x_row,
